@@ -1,0 +1,428 @@
+// Beam search's selection: for each request the n best continuations over its W beams and the whole
+// vocabulary, by score[w] + x[w][v] - lse(x[w]).
+//
+// Two launches. k_beam_part: one workgroup a segment of a row, held in registers, so that a row is read
+// once. A lane's maximum gives a bound: the n-th largest of a wave's 64 lane maxima (n <= 64) is at most the
+// segment's n-th largest logit, and few elements reach the largest of the four waves' bounds (about
+// 64 ln(64 / (64 - n)) a wave where the logits come in any order). Those go to a list in LDS, ranked by
+// counting, and the list's first n are the segment's candidates in order. The others, all of them below the
+// bound, add their fp32 exponentials against the segment's maximum; the list's exponentials are taken in
+// fp64 and added in fixed point, so that neither the large terms lose precision nor the order of the list,
+// which varies, shows in the sum: the beams of a request are compared across their rows by these sums.
+// k_beam_merge: one workgroup a request. The rows' lse from the segments' sums; the n-th largest score of the
+// segments' first candidates bounds the request's n-th best; the few candidates that reach it are ranked.
+//
+// A row with a NaN, an infinite maximum or no finite logit has no candidates, nor have logits of -inf.
+// Rows of finished beams and of beams whose score is not finite are not read.
+#pragma once
+
+#include "rows.cuh"
+
+namespace vo {
+
+constexpr int kMaxBeams = 64;
+constexpr int kMaxPick = 64;        // most continuations a request: a lane each
+constexpr int kPartThreads = 256;
+constexpr int kPartWaves = kPartThreads / kWave;
+constexpr int kPartList = 512;      // a segment's candidates before they are ranked
+constexpr int kMergeList = 1024;    // a request's
+constexpr int kMergeMaxThreads = 1024;
+constexpr double kFix = 4503599627370496.0;  // 2^52
+
+struct BeamArgs {
+  const void* logits;  // row (b, w) at b * rstride + w * bstride
+  int64_t rstride, bstride;
+  int B, W, V, n;
+  int S;               // segments a row
+  const float* scores;      // [B, W]
+  const uint8_t* finished;  // [B, W] or null
+  int pad, keep;
+  u64* keys;           // [B W, S, n] the segments' candidates, descending (0: none)
+  double* sums;        // [B W, S] sums of exp(x - max)
+  float* maxs;         // [B W, S]
+  float* out_scores;   // [B, n]
+  int32_t* out_beams;
+  int32_t* out_tokens;
+};
+
+// The n-th largest of the wave's 64 keys with the bits below LOW cleared: at most the key itself. A step is
+// scalar but for its compare.
+template <int LOW>
+__device__ __forceinline__ uint32_t wave_nth_floor(uint32_t key, int n) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int b = 31; b >= LOW; --b) {
+    const uint32_t c = t | (1u << b);
+    if (__popcll(__ballot(key >= c)) >= n) t = c;
+  }
+  return t;
+}
+
+__device__ __forceinline__ u64 pack_key(float x, int id) {
+  return (static_cast<u64>(key_of(x)) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(id));
+}
+__device__ __forceinline__ float key_value(u64 k) { return val_of(static_cast<uint32_t>(k >> 32)); }
+__device__ __forceinline__ int key_id(u64 k) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(k)); }
+
+// A term e in [0, 1] of a sum whose order varies: rint(e 2^52).
+__device__ __forceinline__ u64 fix52(double e) { return static_cast<u64>(__builtin_rint(e * kFix)); }
+
+struct PartShared {
+  u64 list[kPartList];
+  u64 top[kMaxPick];
+  double wsum[kPartWaves];
+  u64 wfix[kPartWaves];
+  float wmax[kPartWaves];
+  uint32_t wtau[kPartWaves];
+  uint32_t wcnt[kPartWaves];
+  uint32_t count;
+};
+
+// f(x, id) for each element that this thread holds.
+template <class Tin, int NV, class F>
+__device__ __forceinline__ void each_held(const uint4* d, int first, F f) {
+  constexpr int E = Vec<Tin>::kElems;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float x[E];
+    Vec<Tin>::unpack(d[j], x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f(x[e], first + (j * kPartThreads + static_cast<int>(threadIdx.x)) * E + e);
+  }
+}
+
+// Segments with more elements at or above the bound than the list takes (equal logits, or few lanes with a
+// finite one): the n-th largest key, ids included, bit by bit over the registers (at most 52 counts), and
+// this thread's part of the whole segment's sum.
+template <class Tin, int NV>
+__device__ __forceinline__ double part_crowded(const uint4* d, int first, int n, float ref, PartShared& sh) {
+  const int w = threadIdx.x / kWave;
+  auto total = [&](uint32_t c) {
+    c = wave_sum(c);
+    __syncthreads();
+    if (lane_id() == 0) sh.wcnt[w] = c;
+    __syncthreads();
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < kPartWaves; ++i) t += sh.wcnt[i];
+    return t;
+  };
+  double s = 0.0;
+  uint32_t c = 0;
+  each_held<Tin, NV>(d, first, [&](float x, int) {
+    s += static_cast<double>(__builtin_amdgcn_exp2f((x - ref) * kLog2e));
+    c += finite_f(x);
+  });
+  const uint32_t live = total(c);
+  const uint32_t want = live < static_cast<uint32_t>(n) ? live : static_cast<uint32_t>(n);
+  u64 kn = 0xFFF00000ull;  // (ids are below 2^20: a key's lower word begins with twelve ones)
+  uint32_t have = live;
+  for (int b = 63; b >= 0 && have != want; b = b == 32 ? 19 : b - 1) {
+    const u64 cand = kn | (1ull << b);
+    c = 0;
+    each_held<Tin, NV>(d, first, [&](float x, int id) { c += finite_f(x) && pack_key(x, id) >= cand; });
+    c = total(c);
+    if (c >= want) {
+      kn = cand;
+      have = c;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  each_held<Tin, NV>(d, first, [&](float x, int id) {
+    if (finite_f(x) && pack_key(x, id) >= kn) {
+      const uint32_t at = atomicAdd(&sh.count, 1u);
+      if (at < kPartList) sh.list[at] = pack_key(x, id);
+    }
+  });
+  __syncthreads();
+  return s;
+}
+
+template <class Tin, int NV>
+__global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
+  constexpr int E = Vec<Tin>::kElems;
+  __shared__ PartShared sh;
+  const int tid = threadIdx.x, w = tid / kWave;
+  const int row = blockIdx.x / a.S, seg = blockIdx.x % a.S;
+  if (!finite_f(a.scores[row]) || (a.finished && a.finished[row])) return;  // (uniform)
+  const Tin* p = as_global(static_cast<const Tin*>(a.logits)) + (row / a.W) * a.rstride + (row % a.W) * a.bstride;
+  const int first = seg * NV * kPartThreads * E;
+  uint4 d[NV];
+  load_segment<Tin, NV, kPartThreads>(p, a.V, first, d);
+  if (tid == 0) sh.count = 0;
+  float lm = -__builtin_inff();
+  each_held<Tin, NV>(d, first, [&](float x, int) { lm = fmaxf(lm, x); });
+  const float wm = wave_max_f(lm);
+  const uint32_t tau = wave_nth_floor<16>(key_of(lm), a.n);
+  if (lane_id() == 0) {
+    sh.wmax[w] = wm;
+    sh.wtau[w] = tau;
+  }
+  __syncthreads();
+  float M = sh.wmax[0];
+  uint32_t tk = sh.wtau[0];
+#pragma unroll
+  for (int i = 1; i < kPartWaves; ++i) {
+    M = fmaxf(M, sh.wmax[i]);
+    tk = max(tk, sh.wtau[i]);
+  }
+  const float ref = M == -__builtin_inff() ? 0.0f : M;  // (no finite logit: exp(-inf - 0) = 0)
+  // (a bound below every finite number takes all of them, and never -inf)
+  constexpr float kLowest = -3.4028234663852886e38f;
+  const float bound = tk <= key_of(kLowest) ? kLowest : val_of(tk);
+  float s = 0.0f;
+  each_held<Tin, NV>(d, first, [&](float x, int id) {
+    const bool hit = x >= bound;
+    const float t = __builtin_amdgcn_exp2f((x - ref) * kLog2e);
+    s += hit ? 0.0f : t;
+    const u64 mask = __ballot(hit);
+    if (mask) {  // (uniform)
+      uint32_t at = 0;
+      if (lane_id() == 0) at = atomicAdd(&sh.count, static_cast<uint32_t>(__popcll(mask)));
+      at = uniform_u(at) + lanes_below(mask);
+      if (hit && at < kPartList) sh.list[at] = pack_key(x, id);
+    }
+  });
+  double sd = s;
+  __syncthreads();
+  uint32_t c = sh.count;
+  const bool crowded = c > kPartList;  // (uniform)
+  if (crowded) {
+    sd = part_crowded<Tin, NV>(d, first, a.n, ref, sh);
+    c = sh.count;
+  }
+  // ranks by counting (keys differ); the list's exponentials in fixed point
+  const uint32_t n = static_cast<uint32_t>(a.n);
+  u64 fx = 0;
+  u64* out = a.keys + static_cast<int64_t>(blockIdx.x) * a.n;
+  for (uint32_t i = tid; i < c; i += kPartThreads) {
+    const u64 k = sh.list[i];
+    uint32_t r = 0;
+    for (uint32_t j = 0; j < c; ++j) r += sh.list[j] > k;
+    if (r < n) out[r] = k;
+    if (!crowded) fx += fix52(exp(static_cast<double>(key_value(k)) - static_cast<double>(ref)));
+  }
+  for (uint32_t i = c + tid; i < n; i += kPartThreads) out[i] = 0;
+  sd = wave_sum(sd);
+  fx = wave_sum(fx);
+  if (lane_id() == 0) {
+    sh.wsum[w] = sd;
+    sh.wfix[w] = fx;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    double t = 0.0;
+    u64 f = 0;
+#pragma unroll
+    for (int i = 0; i < kPartWaves; ++i) {
+      t += sh.wsum[i];
+      f += sh.wfix[i];
+    }
+    a.sums[blockIdx.x] = t + static_cast<double>(f) * (1.0 / kFix);
+    a.maxs[blockIdx.x] = M;
+  }
+}
+
+// ---- the request's best ---------------------------------------------------------------------------
+struct MergeShared {
+  u64 sk[kMergeList];  // a candidate's score, ordered
+  u64 tb[kMergeList];  // what decides between equal scores
+  uint32_t head[kMergeMaxThreads];
+  double lse[kMaxBeams];
+  double score[kMaxBeams];
+  u64 rsk[kMergeMaxThreads / kWave], rtb[kMergeMaxThreads / kWave];
+  float ch_score[kMaxPick];
+  int32_t ch_beam[kMaxPick], ch_token[kMaxPick];
+  int32_t kind[kMaxBeams];  // 0: no candidates, 1: its row's, 2: finished
+  uint32_t count, bound;
+};
+
+__device__ __forceinline__ u64 ordered(double x) {
+  const u64 b = static_cast<u64>(__double_as_longlong(x + 0.0));
+  return (b >> 63) ? ~b : (b | (1ull << 63));
+}
+__device__ __forceinline__ double unordered(u64 k) {
+  return __longlong_as_double(static_cast<long long>((k >> 63) ? (k & ~(1ull << 63)) : ~k));
+}
+// Equal scores: the lower beam, then the larger logit, then the lower id.
+__device__ __forceinline__ u64 tie_word(int beam, u64 key) {
+  return (static_cast<u64>(kMaxBeams - 1 - beam) << 52) | ((key >> 32) << 20) | (key & 0xFFFFFull);
+}
+
+// The score of entry e of list l (of W S lists, S a beam), ordered, and its tie word; 0 where there is none.
+__device__ __forceinline__ u64 merge_entry(const BeamArgs& a, const MergeShared& sh, const u64* keys, int l, int e,
+                                           u64* tb) {
+  const int w = l / a.S;
+  const int kind = sh.kind[w];
+  if (kind == 1) {
+    const u64 k = keys[static_cast<int64_t>(l) * a.n + e];
+    if (!k) return 0;
+    *tb = tie_word(w, k);
+    const double c = (static_cast<double>(key_value(k)) - sh.lse[w]) + sh.score[w];
+    return ordered(c);
+  }
+  if (kind == 2 && e == 0 && l == w * a.S) {
+    *tb = tie_word(w, pack_key(0.0f, 0));
+    return ordered(sh.score[w]);
+  }
+  return 0;
+}
+
+// The upper words of ordered fp64 scores order them too, coarsely: the first launch's bound by lane maxima again.
+__global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
+  __shared__ MergeShared sh;
+  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id(), nt = blockDim.x, nw = nt / kWave;
+  const int b = blockIdx.x;
+  const int W = a.W, S = a.S, n = a.n;
+  for (int w = wave; w < W; w += nw) {
+    const int row = b * W + w;
+    const float sc = a.scores[row];
+    int kind = 0;
+    double l = 0.0;
+    if (finite_f(sc)) {
+      if (a.finished && a.finished[row]) {
+        kind = 2;
+      } else {
+        const float* ms = a.maxs + static_cast<int64_t>(row) * S;
+        const double* ss = a.sums + static_cast<int64_t>(row) * S;
+        float m = -__builtin_inff();
+        for (int s = lane; s < S; s += kWave) m = fmaxf(m, ms[s]);
+        const float M = wave_max_f(m);
+        double t = 0.0;
+        for (int s = lane; s < S; s += kWave) t += ss[s] * exp(static_cast<double>(ms[s]) - static_cast<double>(M));
+        t = wave_sum(t);
+        l = static_cast<double>(M) + log(t);
+        kind = finite_f(M) && l == l ? 1 : 0;
+      }
+    }
+    if (lane == 0) {
+      sh.kind[w] = kind;
+      sh.lse[w] = l;
+      sh.score[w] = sc;
+    }
+  }
+  if (tid < n) {
+    sh.ch_score[tid] = -__builtin_inff();
+    sh.ch_beam[tid] = -1;
+    sh.ch_token[tid] = -1;
+  }
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  const u64* keys = a.keys + static_cast<int64_t>(b) * W * S * n;
+  const int lists = W * S;
+  uint32_t h = 0;
+  u64 tb = 0;
+  for (int l = tid; l < lists; l += nt) h = max(h, static_cast<uint32_t>(merge_entry(a, sh, keys, l, 0, &tb) >> 32));
+  sh.head[tid] = h;
+  __syncthreads();
+  if (wave == 0) {
+    for (int i = lane + kWave; i < nt; i += kWave) h = max(h, sh.head[i]);
+    const uint32_t t = wave_nth_floor<4>(h, n);
+    if (lane == 0) sh.bound = max(t, 1u);
+  }
+  __syncthreads();
+  const uint32_t bound = sh.bound;
+  const int total = lists * n;
+  for (int i = tid; i < total; i += nt) {
+    const u64 sk = merge_entry(a, sh, keys, i / n, i % n, &tb);
+    if (static_cast<uint32_t>(sk >> 32) >= bound) {
+      const uint32_t at = atomicAdd(&sh.count, 1u);
+      if (at < kMergeList) {
+        sh.sk[at] = sk;
+        sh.tb[at] = tb;
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t c = sh.count;
+  auto choose = [&](uint32_t r, u64 sk, u64 t) {
+    const int w = kMaxBeams - 1 - static_cast<int>(t >> 52);
+    sh.ch_score[r] = static_cast<float>(unordered(sk));
+    sh.ch_beam[r] = w;
+    sh.ch_token[r] = sh.kind[w] == 2 ? a.pad : static_cast<int>(0xFFFFFu - static_cast<uint32_t>(t & 0xFFFFFull));
+  };
+  if (c <= kMergeList) {
+    for (uint32_t i = tid; i < c; i += nt) {
+      const u64 sk = sh.sk[i], t = sh.tb[i];
+      uint32_t r = 0;
+      for (uint32_t j = 0; j < c; ++j) r += sh.sk[j] > sk || (sh.sk[j] == sk && sh.tb[j] > t);
+      if (r < static_cast<uint32_t>(n)) choose(r, sk, t);
+    }
+  } else {
+    // (thousands of equal scores: the best one after the last, n times)
+    u64 psk = ~0ull, ptb = ~0ull;
+    for (int r = 0; r < n; ++r) {
+      u64 bsk = 0, btb = 0;
+      for (int i = tid; i < total; i += nt) {
+        const u64 sk = merge_entry(a, sh, keys, i / n, i % n, &tb);
+        if (!sk || !(sk < psk || (sk == psk && tb < ptb))) continue;
+        if (sk > bsk || (sk == bsk && tb > btb)) {
+          bsk = sk;
+          btb = tb;
+        }
+      }
+      u64 m = wave_max_u64(bsk);
+      u64 mt = wave_max_u64(bsk == m ? btb : 0);
+      if (lane == 0) {
+        sh.rsk[wave] = m;
+        sh.rtb[wave] = mt;
+      }
+      __syncthreads();
+      m = 0;
+      mt = 0;
+      for (int i = 0; i < nw; ++i) {
+        const u64 x = sh.rsk[i], y = sh.rtb[i];
+        if (x > m || (x == m && y > mt)) {
+          m = x;
+          mt = y;
+        }
+      }
+      if (!m) break;  // (uniform)
+      if (tid == 0) choose(r, m, mt);
+      psk = m;
+      ptb = mt;
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  // A lane a choice. keep_slots (n = W): the first child of each parent takes the parent's place, the others the
+  // free places in their order, the empty ones behind them.
+  const bool mine = lane < n;
+  const int beam = mine ? sh.ch_beam[lane] : -1;
+  int place = lane;
+  if (a.keep) {
+    u64 taken = 0;
+    bool stays = false;
+    for (int i = 0; i < n; ++i) {
+      const int bi = sh.ch_beam[i];
+      if (bi >= 0 && !((taken >> bi) & 1)) {
+        taken |= 1ull << bi;
+        stays = stays || i == lane;
+      }
+    }
+    const u64 others = __ballot(mine && !stays);
+    if (stays) {
+      place = beam;
+    } else {
+      int skip = static_cast<int>(lanes_below(others));
+      for (int i = 0; i < n; ++i) {
+        if ((taken >> i) & 1) continue;
+        if (skip-- == 0) {
+          place = i;
+          break;
+        }
+      }
+    }
+  }
+  if (mine) {
+    const int64_t at = static_cast<int64_t>(b) * n + place;
+    a.out_scores[at] = sh.ch_score[lane];
+    a.out_beams[at] = beam;
+    a.out_tokens[at] = sh.ch_token[lane];
+  }
+}
+
+}  // namespace vo

@@ -1,4 +1,5 @@
-"""Compile the sampler's HIP sources into ``vinfer_amd/libvsampler.so`` (gfx950 only).
+"""Compile the HIP sources (gfx950 only): the sampler into ``vinfer_amd/libvsampler.so``, the operators
+around it into ``vinfer_amd/libvops.so``.
 
 Run as ``python -m vinfer_amd.csrc.build``. The build is in-tree so the library travels with
 the source tree; there is no JIT cache.
@@ -10,12 +11,15 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parents[1]
 ROOT = PKG.parent
 LIB = PKG / "libvsampler.so"
 SOURCES = [PKG / "csrc" / "capi.hip"]
+OPS_LIB = PKG / "libvops.so"
+OPS_SOURCES = [PKG / "csrc" / "vops.hip"]
 
 # -ffp-contract=off: the penalty arithmetic rounds every operation on its own.
 # -fhip-fp32-correctly-rounded-divide-sqrt: x / T is IEEE division, as on the CPU.
@@ -40,12 +44,12 @@ def hipcc() -> str:
     for c in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
         if c and Path(c).exists():
             return c
-    raise RuntimeError("hipcc not found (ROCm is required to build the sampler library)")
+    raise RuntimeError("hipcc not found (ROCm is required to build the libraries)")
 
 
-def build(verbose: bool = False) -> Path:
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [hipcc(), *FLAGS, f"-I{ROOT / 'include'}", "-o", str(tmp), *map(str, SOURCES)]
+def _compile(lib: Path, sources: list[Path], verbose: bool) -> None:
+    tmp = lib.with_suffix(".so.tmp")
+    cmd = [hipcc(), *FLAGS, f"-I{ROOT / 'include'}", "-o", str(tmp), *map(str, sources)]
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -58,10 +62,18 @@ def build(verbose: bool = False) -> Path:
         raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{out}")
     if verbose and out.strip():
         print(out)
-    os.replace(tmp, LIB)
+    os.replace(tmp, lib)
+
+
+def build(verbose: bool = False) -> Path:
+    with ThreadPoolExecutor(2) as pool:
+        jobs = [pool.submit(_compile, lib, src, verbose) for lib, src in ((LIB, SOURCES), (OPS_LIB, OPS_SOURCES))]
+    for job in jobs:
+        job.result()
     return LIB
 
 
 if __name__ == "__main__":
     build(verbose="-v" in sys.argv)
     print(LIB)
+    print(OPS_LIB)

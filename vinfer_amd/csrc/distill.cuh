@@ -1,0 +1,297 @@
+// The distillation loss on a teacher's top entries, and its gradient in the student's logits x.
+//
+// With z = x / T, q = softmax(z) and the teacher's probabilities p_k of the entries' ids:
+//   loss = sum_k p_k (log p_k - log q_k)            (+ rest (log rest - log q_rest) where the rest counts)
+//   d loss / d z_j = mass q_j - p_j                 listed j, mass = sum_k p_k (+ rest)
+//                  = mass q_j (- rest q_j / q_rest) the others
+// rest = 1 - sum_k p_k and q_rest = 1 - sum_k q_k, each taken without that subtraction where it would cancel: the
+// ids' logits are left out of the vocabulary's sum, S = sum over the others of exp(z - m) with m their largest,
+// so that q_rest = S exp(m - lse) however small it is, and the others' gradient is exp(z_j - m) times one number
+// A = mass exp(m - lse) - rest / S a row.
+//
+// k_distill_part: a segment's m and S, its logits held in registers, the listed ones struck out by a bitmap of
+// the segment. k_distill_row: a wave a row, in fp64: the loss, m, A and the listed entries' gradients.
+// k_distill_grad: a segment's gradient. Rows of weight 0 are not read: their loss and gradient are 0.
+#pragma once
+
+#include "rows.cuh"
+
+namespace vo {
+
+constexpr int kDistillThreads = 256;
+constexpr int kDistillWaves = kDistillThreads / kWave;
+constexpr int kMaxEntries = 1024;
+
+struct DistillArgs {
+  const void* x;  // row t at t * stride
+  int64_t stride;
+  int T, V, K, S;
+  const int32_t* ids;     // [T, K]; outside [0, V): no entry
+  const float* teacher;   // [T, K]
+  const float* weights;   // [T] or null (1)
+  float temp;
+  int tail;
+  float* maxs;    // [T, S]
+  double* sums;   // [T, S]
+  float* states;  // [T, 2 + K] m, A, the entries' gradients
+  float* loss;    // [T]
+  void* grad;     // row t at t * gstride
+  int64_t gstride;
+};
+
+// The segment's listed ids as a bitmap, cleared and filled by the workgroup (a barrier at its end).
+template <int ELEMS>
+__device__ __forceinline__ void mark_listed(const int32_t* ids, int K, int V, int first, uint32_t* bits) {
+  for (int i = threadIdx.x; i < ELEMS / 32; i += kDistillThreads) bits[i] = 0;
+  __syncthreads();
+  for (int k = threadIdx.x; k < K; k += kDistillThreads) {
+    const int64_t i = static_cast<int64_t>(ld_global(ids + k)) - first;
+    if (i >= 0 && i < ELEMS && i < V - first) atomicOr(&bits[i >> 5], 1u << (i & 31));
+  }
+  __syncthreads();
+}
+
+// Strikes the marked elements out of the registers (-inf).
+template <class Tin, int NV>
+__device__ __forceinline__ void strike_listed(const uint32_t* bits, uint4* d) {
+  constexpr int E = Vec<Tin>::kElems;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const uint32_t at = (j * kDistillThreads + threadIdx.x) * E;
+    const uint32_t m = (bits[at >> 5] >> (at & 31)) & ((1u << E) - 1);
+    if (m) {
+      uint32_t w[4] = {d[j].x, d[j].y, d[j].z, d[j].w};
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (!((m >> e) & 1)) continue;
+        if constexpr (E == 8) w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xFFFFu) | 0xFF800000u : (w[e >> 1] & 0xFFFF0000u) | 0xFF80u;
+        else w[e] = 0xFF800000u;
+      }
+      d[j] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+template <class Tin, int NV>
+__global__ __launch_bounds__(kDistillThreads) void k_distill_part(DistillArgs a) {
+  constexpr int E = Vec<Tin>::kElems;
+  constexpr int kElems = NV * kDistillThreads * E;
+  __shared__ uint32_t bits[kElems / 32];
+  __shared__ float wmax[kDistillWaves];
+  __shared__ double wsum[kDistillWaves];
+  const int row = blockIdx.x / a.S, seg = blockIdx.x % a.S;
+  if (a.weights && a.weights[row] == 0.0f) return;  // (uniform)
+  const int first = seg * kElems;
+  uint4 d[NV];
+  load_segment<Tin, NV, kDistillThreads>(as_global(static_cast<const Tin*>(a.x)) + row * a.stride, a.V, first, d);
+  mark_listed<kElems>(a.ids + static_cast<int64_t>(row) * a.K, a.K, a.V, first, bits);
+  strike_listed<Tin, NV>(bits, d);
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float x[E];
+    Vec<Tin>::unpack(d[j], x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
+  }
+  m = wave_max_f(m);
+  const float ref = m == -__builtin_inff() ? 0.0f : m;
+  const float c = kLog2e / a.temp;
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float x[E];
+    Vec<Tin>::unpack(d[j], x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * c);
+  }
+  const double t = wave_sum(static_cast<double>(s));
+  if (lane_id() == 0) {
+    wmax[threadIdx.x / kWave] = m;
+    wsum[threadIdx.x / kWave] = t;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float M = wmax[0];
+    for (int i = 1; i < kDistillWaves; ++i) M = fmaxf(M, wmax[i]);
+    double S = 0.0;
+    // (a wave without a finite logit has the sum 0, or NaN for a NaN)
+    for (int i = 0; i < kDistillWaves; ++i)
+      S += wmax[i] == M ? wsum[i] : wsum[i] * exp((static_cast<double>(wmax[i]) - M) / a.temp);
+    a.maxs[blockIdx.x] = M;
+    a.sums[blockIdx.x] = S;
+  }
+}
+
+__device__ __forceinline__ double wave_max_d(double x) {
+  return dpp::reduce(x, [](double p, double q) { return p > q ? p : q; });
+}
+
+template <class Tin>
+__device__ __forceinline__ double logit(const Tin* p) {
+  if constexpr (sizeof(Tin) == 2) return bf16_to_f32(ld_global(p));
+  else return ld_global(p);
+}
+
+// A wave's row: the loss, m, A and the listed gradients, from the segments' sums.
+template <class Tin>
+__global__ __launch_bounds__(kDistillThreads) void k_distill_row(DistillArgs a) {
+  const int row = blockIdx.x * kDistillWaves + threadIdx.x / kWave;
+  if (row >= a.T) return;
+  const int lane = lane_id();
+  const float weight = a.weights ? as_global(a.weights)[row] : 1.0f;
+  float* st = as_global(a.states) + static_cast<int64_t>(row) * (2 + a.K);
+  if (weight == 0.0f) {
+    for (int k = lane; k < a.K; k += kWave) st[2 + k] = 0.0f;
+    if (lane == 0) {
+      a.loss[row] = 0.0f;
+      st[0] = 0.0f;
+      st[1] = 0.0f;
+    }
+    return;
+  }
+  const double inv = 1.0 / static_cast<double>(a.temp);
+  const double ninf = -static_cast<double>(__builtin_inff());
+  const float* ms = as_global(a.maxs) + static_cast<int64_t>(row) * a.S;
+  const double* ss = as_global(a.sums) + static_cast<int64_t>(row) * a.S;
+  const int32_t* ids = as_global(a.ids) + static_cast<int64_t>(row) * a.K;
+  const float* teacher = as_global(a.teacher) + static_cast<int64_t>(row) * a.K;
+  const Tin* x = as_global(static_cast<const Tin*>(a.x)) + row * a.stride;
+  float mf = -__builtin_inff();
+  for (int s = lane; s < a.S; s += kWave) mf = fmaxf(mf, ms[s]);
+  mf = wave_max_f(mf);
+  const double m = mf;
+  double S = 0.0;
+  for (int s = lane; s < a.S; s += kWave) S += ms[s] == mf ? ss[s] : ss[s] * exp((ms[s] - m) * inv);
+  S = wave_sum(S);
+  // the teacher's normaliser and the listed logits' largest
+  double tm = ninf, xm = m;
+  for (int k = lane; k < a.K; k += kWave) {
+    if (static_cast<uint32_t>(ids[k]) >= static_cast<uint32_t>(a.V)) continue;
+    const double v = teacher[k], z = logit(x + ids[k]);
+    tm = v > tm ? v : tm;
+    xm = z > xm ? z : xm;
+  }
+  tm = wave_max_d(tm);
+  xm = wave_max_d(xm);
+  double ts = 0.0, xs = 0.0;
+  for (int k = lane; k < a.K; k += kWave) {
+    if (static_cast<uint32_t>(ids[k]) >= static_cast<uint32_t>(a.V)) continue;
+    ts += exp(a.tail ? static_cast<double>(teacher[k]) : (teacher[k] - tm) * inv);
+    xs += exp((logit(x + ids[k]) - xm) * inv);
+  }
+  ts = wave_sum(ts);
+  xs = wave_sum(xs);
+  const bool none = tm == ninf;  // (no entry, or all of probability 0)
+  const double lts = a.tail ? 0.0 : tm * inv + log(ts);
+  const double lse = xm * inv + log((m == ninf ? S : S * exp((m - xm) * inv)) + xs);
+  const double rest = a.tail ? fmax(0.0, 1.0 - ts) : 0.0;
+  const double mass = a.tail ? ts + rest : (none ? 0.0 : 1.0);
+  double loss = 0.0;
+  for (int k = lane; k < a.K; k += kWave) {
+    float g = 0.0f;
+    if (static_cast<uint32_t>(ids[k]) < static_cast<uint32_t>(a.V)) {
+      const double lp = a.tail ? static_cast<double>(teacher[k]) : teacher[k] * inv - lts;
+      const double lq = logit(x + ids[k]) * inv - lse;
+      const double p = none ? 0.0 : exp(lp);
+      if (p != 0.0) loss += p * (lp - lq);
+      g = static_cast<float>(exp(lq) * mass - p);
+    }
+    st[2 + k] = g;
+  }
+  loss = wave_sum(loss);
+  if (lane == 0) {
+    if (rest > 0.0) loss += rest * (log(rest) - (m * inv + log(S) - lse));
+    double A = 0.0;
+    if (m != ninf || S != 0.0) A = mass * exp(m * inv - lse) - (rest > 0.0 ? rest / S : 0.0);
+    a.loss[row] = static_cast<float>(weight * loss);
+    st[0] = mf;
+    st[1] = static_cast<float>(A);
+  }
+}
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+// Two fp32 values rounded to bf16 (to nearest, ties to even: one v_cvt_pk_bf16_f32).
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, bf16x2_t));
+}
+
+typedef u32x4_t u32x4_row_t __attribute__((aligned(2)));
+__device__ __forceinline__ void st_row16(void* p, uint4 v) {
+  *(__attribute__((address_space(1))) u32x4_row_t*)p = u32x4_t{v.x, v.y, v.z, v.w};
+}
+
+// A vector's gradients, factor exp2((x - ref) c), packed.
+template <class Tin>
+__device__ __forceinline__ uint4 grad_vector(const uint4& d, float ref, float c, float factor) {
+  constexpr int E = Vec<Tin>::kElems;
+  float x[E];
+  Vec<Tin>::unpack(d, x);
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = factor * __builtin_amdgcn_exp2f((x[e] - ref) * c);
+  if constexpr (E == 8)
+    return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+  else
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+}
+
+template <class Tin>
+__device__ __forceinline__ void store_elem(Tin* p, float v) {
+  if constexpr (sizeof(Tin) == 2) *(__attribute__((address_space(1))) uint16_t*)p = static_cast<uint16_t>(pack_bf16(v, v));
+  else *(__attribute__((address_space(1))) float*)p = v;
+}
+
+// Stores vector v at element i of a row of V.
+template <class Tin>
+__device__ __forceinline__ void store_vector(Tin* row, int V, int i, const uint4& v) {
+  constexpr int E = Vec<Tin>::kElems;
+  if (i + E <= V) {
+    st_row16(row + i, v);
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (i + e >= V) continue;
+    if constexpr (E == 8)
+      *(__attribute__((address_space(1))) uint16_t*)(row + i + e) = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+    else
+      *(__attribute__((address_space(1))) uint32_t*)(row + i + e) = w[e];
+  }
+}
+
+template <class Tin, int NV>
+__global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a) {
+  constexpr int E = Vec<Tin>::kElems;
+  constexpr int kElems = NV * kDistillThreads * E;
+  const int row = blockIdx.x / a.S, seg = blockIdx.x % a.S;
+  const int first = seg * kElems;
+  const float weight = a.weights ? a.weights[row] : 1.0f;
+  Tin* g = as_global(static_cast<Tin*>(a.grad)) + row * a.gstride;
+  const int at = first + static_cast<int>(threadIdx.x) * E;
+  if (weight == 0.0f) {  // (uniform)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) store_vector<Tin>(g, a.V, at + j * kDistillThreads * E, make_uint4(0, 0, 0, 0));
+    return;
+  }
+  uint4 d[NV];
+  load_segment<Tin, NV, kDistillThreads>(as_global(static_cast<const Tin*>(a.x)) + row * a.stride, a.V, first, d);
+  const float* st = as_global(a.states) + static_cast<int64_t>(row) * (2 + a.K);
+  const float ref = st[0] == -__builtin_inff() ? 0.0f : st[0];
+  const float scale = weight / a.temp;
+  const float factor = scale * st[1];
+  const float c = kLog2e / a.temp;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    store_vector<Tin>(g, a.V, at + j * kDistillThreads * E, grad_vector<Tin>(d[j], ref, c, factor));
+  __syncthreads();  // (the workgroup's stores have landed: the listed ones go over them)
+  const int32_t* ids = a.ids + static_cast<int64_t>(row) * a.K;
+  for (int k = threadIdx.x; k < a.K; k += kDistillThreads) {
+    const int id = ld_global(ids + k);
+    if (id >= first && id < a.V && id - first < kElems)
+      store_elem<Tin>(g + id, scale * st[2 + k]);
+  }
+}
+
+}  // namespace vo

@@ -1,0 +1,81 @@
+// Rows of logits in segments held in registers, for the operators over whole vocabularies.
+#pragma once
+
+#include "common.cuh"
+
+namespace vo {
+
+using namespace vs;
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+__device__ __forceinline__ bool finite_f(float x) { return fabsf(x) < __builtin_inff(); }
+
+// One 16-byte vector's elements as fp32.
+template <class Tin>
+struct Vec;
+template <>
+struct Vec<uint16_t> {
+  static constexpr int kElems = 8;
+  static constexpr uint32_t kNegInf = 0xFF80FF80u;
+  static __device__ __forceinline__ void unpack(const uint4& d, float* x) {
+    const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = __uint_as_float(w[j] << 16);
+      x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    }
+  }
+};
+template <>
+struct Vec<float> {
+  static constexpr int kElems = 4;
+  static constexpr uint32_t kNegInf = 0xFF800000u;
+  static __device__ __forceinline__ void unpack(const uint4& d, float* x) {
+    x[0] = __uint_as_float(d.x);
+    x[1] = __uint_as_float(d.y);
+    x[2] = __uint_as_float(d.z);
+    x[3] = __uint_as_float(d.w);
+  }
+};
+
+// NV vectors a thread of the segment that starts at element `first`: vector j of thread t holds the elements
+// from first + (j * threads + t) * kElems. What lies past V reads as -inf.
+template <class Tin, int NV, int THREADS>
+__device__ __forceinline__ void load_segment(const Tin* row, int V, int first, uint4* d) {
+  constexpr int E = Vec<Tin>::kElems;
+  const int at = first + static_cast<int>(threadIdx.x) * E;
+  if (first + NV * THREADS * E <= V) {  // (uniform)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) d[j] = ld_row16(row + at + j * THREADS * E);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int i = at + j * THREADS * E;
+    uint4 v = make_uint4(Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf);
+    if (i + E <= V) {
+      v = ld_row16(row + i);
+    } else if (i < V) {  // (the row's last vector)
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (i + e >= V) continue;
+        if constexpr (sizeof(Tin) == 2) {
+          const uint32_t h = ld_global(reinterpret_cast<const uint16_t*>(row) + i + e);
+          w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xFFFFu) | (h << 16) : (w[e >> 1] & 0xFFFF0000u) | h;
+        } else {
+          w[e] = __float_as_uint(ld_global(reinterpret_cast<const float*>(row) + i + e));
+        }
+      }
+      v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    d[j] = v;
+  }
+}
+
+__device__ __forceinline__ float wave_max_f(float x) {
+  return dpp::reduce(x, [](float p, float q) { return fmaxf(p, q); });
+}
+
+}  // namespace vo

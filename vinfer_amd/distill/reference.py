@@ -1,0 +1,76 @@
+"""The ``reference`` distillation backend: the definition in torch, in fp64, on any device."""
+
+from __future__ import annotations
+
+import torch
+
+from vinfer_amd.distill.base import DISTILL, check, check_states
+from vinfer_amd.registry import BackendContext
+
+
+@DISTILL.register("reference")
+class ReferenceDistill:
+    def __init__(self, ctx: BackendContext) -> None:
+        self.ctx = ctx
+
+    @staticmethod
+    def _rows(student, ids, teacher, temperature, tail):
+        """Losses and the rows' states without their weights: the ids' gradients, then the largest of the other
+        logits and their gradients' factor."""
+        T, V = student.shape
+        x = student.double()
+        there = (ids >= 0) & (ids < V)
+        at = torch.where(there, ids, 0).long()
+        member = torch.zeros(T, V, dtype=torch.int32, device=x.device).scatter_add_(1, at, there.int()) > 0
+        logp = teacher.double() if tail else teacher.double() / temperature
+        logp = torch.where(there, logp, -torch.inf)
+        none = (logp == -torch.inf).all(1, keepdim=True)
+        if not tail:
+            logp = logp - torch.where(none, 0.0, torch.logsumexp(logp, 1, keepdim=True))
+        p = torch.exp(logp)
+        rest = (1 - p.sum(1)).clamp(min=0) if tail else torch.zeros(T, dtype=torch.float64, device=x.device)
+        mass = p.sum(1) + rest
+        z = x / temperature
+        lse = torch.logsumexp(z, 1)
+        logq = torch.gather(z, 1, at) - lse[:, None]
+        loss = torch.where(p != 0, p * (logp - logq), 0.0).sum(1)
+        others = torch.where(member, -torch.inf, z)
+        m = others.amax(1)
+        lse_others = torch.logsumexp(others, 1)
+        loss = loss + torch.where(rest > 0, rest * (torch.log(rest) - (lse_others - lse)), 0.0)
+        # the others' gradient: exp(z - m) times this
+        factor = mass * torch.exp(m - lse) - torch.where(rest > 0, rest * torch.exp(m - lse_others), 0.0)
+        factor = torch.where(m == -torch.inf, 0.0, factor)
+        listed = torch.where(there, torch.exp(logq) * mass[:, None] - p, 0.0)
+        return loss, torch.cat([m[:, None] * temperature, factor[:, None], listed], 1)
+
+    def loss_and_states(self, student, ids, teacher, weights=None, *, temperature=1.0, tail=False):
+        check(student, ids, teacher, weights, temperature)
+        loss, states = self._rows(student, ids, teacher, temperature, tail)
+        if weights is not None:
+            loss = torch.where(weights == 0, 0.0, weights.double() * loss)
+            states = torch.where(weights[:, None] == 0, 0.0, states)
+        return loss.float(), states.float()
+
+    def grad(self, student, ids, states, weights=None, *, temperature=1.0):
+        check(student, ids, None, weights, temperature)
+        check_states(states, ids, student)
+        T, V = student.shape
+        m, factor, listed = states[:, :1].double(), states[:, 1:2].double(), states[:, 2:].double()
+        m = torch.where(m == -torch.inf, 0.0, m)
+        w = torch.ones(T, 1, dtype=torch.float64, device=student.device) if weights is None else weights.double()[:, None]
+        g = torch.exp((student.double() - m) / temperature) * factor
+        there = (ids >= 0) & (ids < V)
+        rows = torch.arange(T, device=ids.device)[:, None].expand_as(ids)
+        g[rows[there], ids[there].long()] = listed[there]
+        return torch.where(w == 0, 0.0, w / temperature * g).to(student.dtype)
+
+    def loss(self, student, ids, teacher, weights=None, *, temperature=1.0, tail=False):
+        return self.loss_and_states(student, ids, teacher, weights, temperature=temperature, tail=tail)[0]
+
+    def loss_and_grad(self, student, ids, teacher, weights=None, *, temperature=1.0, tail=False):
+        loss, states = self.loss_and_states(student, ids, teacher, weights, temperature=temperature, tail=tail)
+        return loss, self.grad(student, ids, states, weights, temperature=temperature)
+
+
+__all__ = ["ReferenceDistill"]

@@ -15,6 +15,7 @@ from typing import Protocol
 import torch
 
 from vinfer_amd.registry import BackendRegistry
+from vinfer_amd.sampler.beams import BeamState
 from vinfer_amd.sampling import PackedParams, SamplingParams, penalized
 
 
@@ -106,6 +107,35 @@ class SamplerBackend(Protocol):
         hist_offsets: torch.Tensor | None = None,
     ) -> tuple[torch.Tensor, torch.Tensor]:
         """Penalised fp32 logits ``[B, V]`` and the history count of every id (int32 ``[B, V]``)."""
+        ...
+
+    def beam_select(
+        self,
+        logits: torch.Tensor,
+        scores: torch.Tensor,
+        n: int,
+        finished: torch.Tensor | None = None,
+        pad_id: int = 0,
+        keep_slots: bool = False,
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """One step of a beam search: each request's ``n`` (1 .. 64) best continuations over its beams and
+        the whole vocabulary, by ``scores[b, w] + log_softmax(logits[b, w])[v]``. ``logits`` ``[B, W, V]``
+        (bf16 or fp32, unit stride along V; rows may be shared, as by ``expand``), ``scores`` fp32
+        ``[B, W]``, W up to 64. Equal scores go by ascending beam, then descending logit, then ascending
+        id. A beam marked in ``finished`` (bool ``[B, W]``) has one continuation: ``pad_id``, at its own
+        score. A beam whose score is not finite has none (the first step: all scores but one -inf), nor has
+        a row with a NaN, a +inf or no finite logit, nor a logit of -inf. With ``keep_slots`` (n = W) the
+        best child of each parent is placed where the parent is, the others in the free places in their
+        order, so that few states move. Returns ``(scores fp32, beams int32, tokens int32)``, ``[B, n]``
+        each; where there are fewer continuations, -inf, -1 and -1."""
+        ...
+
+    def prepare_reorder(self, states: Sequence[BeamState], requests: int, beams: int):
+        """A reusable reordering, in place, of the ``requests * beams`` slots (beams up to 32) of every
+        state: ``launch(parents int32 [requests, beams], lengths int32 [requests] or None)`` on the result
+        gives slot ``b * beams + w`` what slot ``b * beams + parents[b, w]`` held, up to ``lengths[b]``
+        positions (clamped to the state's) in states with a ``length_dim``; a parent outside
+        ``[0, beams)`` (the -1 of ``beam_select``) leaves its slot as it is."""
         ...
 
 

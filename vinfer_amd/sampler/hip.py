@@ -23,6 +23,7 @@ import torch
 from vinfer_amd import _lib
 from vinfer_amd.registry import BackendContext
 from vinfer_amd.sampler.base import SAMPLER, require_history
+from vinfer_amd.sampler.beams import HipBeams, HipReorder
 from vinfer_amd.sampling import PackedParams, SamplingParams, field, pack_params, penalized, uniform
 
 _DTYPES = {torch.bfloat16: _lib.VSAMP_BF16, torch.float32: _lib.VSAMP_F32}
@@ -62,6 +63,7 @@ class HipSampler:
         # Small batches take the tile pass in one launch (vsamp_sample_tile_pass), whose rows the
         # tile maxima decide from a few tiles; identical results. False: the row passes only.
         self.tile_pass = True
+        self._beams: HipBeams | None = None
 
     # ---- argument checks ---------------------------------------------------------------------
     def _device(self, logits: torch.Tensor) -> torch.device:
@@ -460,6 +462,14 @@ class HipSampler:
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         _lib.check(self._lib.vsamp_spec_advance(inputs.data_ptr(), n, K, ptr(tokens), ptr(counts), seeds.data_ptr(),
                                                 uniforms.data_ptr(), self._stream(dev)))
+
+    def beam_select(self, logits, scores, n, finished=None, pad_id=0, keep_slots=False):
+        if self._beams is None:  # (libvops.so: loaded by its first use)
+            self._beams = HipBeams()
+        return self._beams.select(logits, scores, n, finished, pad_id, keep_slots)
+
+    def prepare_reorder(self, states, requests, beams):
+        return HipReorder(states, requests, beams)
 
     def verify(self, target_logits, draft_logits, draft_tokens, params, u_accept, u_residual, u_bonus,
                draft_params=None, draft_states=None):

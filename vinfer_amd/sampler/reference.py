@@ -18,6 +18,7 @@ import torch
 
 from vinfer_amd.registry import BackendContext
 from vinfer_amd.sampler.base import SAMPLER, require_history
+from vinfer_amd.sampler.beams import ReorderReference, select_reference
 from vinfer_amd.sampling import SamplingParams, pack_params, penalized, uniform
 
 
@@ -159,6 +160,11 @@ class ReferenceSampler:
         ids[:, :k] = order.int()
         lps[:, :k] = lp.gather(1, order).float()
         return out_tok, ids, lps
+
+    beam_select = staticmethod(select_reference)
+
+    def prepare_reorder(self, states, requests, beams):
+        return ReorderReference(states, requests, beams)
 
     def verify(self, target_logits, draft_logits, draft_tokens, params, u_accept, u_residual, u_bonus,
                draft_params=None, draft_states=None):
