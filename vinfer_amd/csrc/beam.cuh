@@ -78,24 +78,28 @@ struct PartShared {
   uint32_t count;
 };
 
-// f(x, id) for each element that this thread holds.
+// f(x, id) for each of this thread's elements of the segment, read again.
 template <class Tin, int NV, class F>
-__device__ __forceinline__ void each_held(const uint4* d, int first, F f) {
+__device__ __forceinline__ void each_again(const Tin* row, int V, int first, F f) {
   constexpr int E = Vec<Tin>::kElems;
-#pragma unroll
+#pragma unroll 1
   for (int j = 0; j < NV; ++j) {
+    const int at = first + j * kPartThreads * E;
+    uint4 d;
+    load_segment<Tin, 1, kPartThreads>(row, V, at, &d);
     float x[E];
-    Vec<Tin>::unpack(d[j], x);
+    Vec<Tin>::unpack(d, x);
 #pragma unroll
-    for (int e = 0; e < E; ++e) f(x[e], first + (j * kPartThreads + static_cast<int>(threadIdx.x)) * E + e);
+    for (int e = 0; e < E; ++e) f(x[e], at + static_cast<int>(threadIdx.x) * E + e);
   }
 }
 
 // Segments with more elements at or above the bound than the list takes (equal logits, or few lanes with a
-// finite one): the n-th largest key, ids included, bit by bit over the registers (at most 52 counts), and
-// this thread's part of the whole segment's sum.
+// finite one): the n-th largest key, ids included, bit by bit (at most 52 counts of the segment, read again from
+// the cache: held in registers, its keys would take 238 a lane, and the ordinary segments' occupancy), and this
+// thread's part of the whole segment's sum.
 template <class Tin, int NV>
-__device__ __forceinline__ double part_crowded(const uint4* d, int first, int n, float ref, PartShared& sh) {
+__device__ __forceinline__ double part_crowded(const Tin* row, int V, int first, int n, float ref, PartShared& sh) {
   const int w = threadIdx.x / kWave;
   auto total = [&](uint32_t c) {
     c = wave_sum(c);
@@ -109,7 +113,7 @@ __device__ __forceinline__ double part_crowded(const uint4* d, int first, int n,
   };
   double s = 0.0;
   uint32_t c = 0;
-  each_held<Tin, NV>(d, first, [&](float x, int) {
+  each_again<Tin, NV>(row, V, first, [&](float x, int) {
     s += static_cast<double>(__builtin_amdgcn_exp2f((x - ref) * kLog2e));
     c += finite_f(x);
   });
@@ -117,10 +121,11 @@ __device__ __forceinline__ double part_crowded(const uint4* d, int first, int n,
   const uint32_t want = live < static_cast<uint32_t>(n) ? live : static_cast<uint32_t>(n);
   u64 kn = 0xFFF00000ull;  // (ids are below 2^20: a key's lower word begins with twelve ones)
   uint32_t have = live;
+#pragma unroll 1
   for (int b = 63; b >= 0 && have != want; b = b == 32 ? 19 : b - 1) {
     const u64 cand = kn | (1ull << b);
     c = 0;
-    each_held<Tin, NV>(d, first, [&](float x, int id) { c += finite_f(x) && pack_key(x, id) >= cand; });
+    each_again<Tin, NV>(row, V, first, [&](float x, int id) { c += finite_f(x) && pack_key(x, id) >= cand; });
     c = total(c);
     if (c >= want) {
       kn = cand;
@@ -130,7 +135,7 @@ __device__ __forceinline__ double part_crowded(const uint4* d, int first, int n,
   __syncthreads();
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
-  each_held<Tin, NV>(d, first, [&](float x, int id) {
+  each_again<Tin, NV>(row, V, first, [&](float x, int id) {
     if (finite_f(x) && pack_key(x, id) >= kn) {
       const uint32_t at = atomicAdd(&sh.count, 1u);
       if (at < kPartList) sh.list[at] = pack_key(x, id);
@@ -153,7 +158,17 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   load_segment<Tin, NV, kPartThreads>(p, a.V, first, d);
   if (tid == 0) sh.count = 0;
   float lm = -__builtin_inff();
-  each_held<Tin, NV>(d, first, [&](float x, int) { lm = fmaxf(lm, x); });
+  float vm[NV];  // each vector's largest
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float x[E];
+    Vec<Tin>::unpack(d[j], x);
+    vm[j] = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) vm[j] = fmaxf(vm[j], x[e]);
+    lm = fmaxf(lm, vm[j]);
+  }
+  forget<NV>(d);
   const float wm = wave_max_f(lm);
   const uint32_t tau = wave_nth_floor<16>(key_of(lm), a.n);
   if (lane_id() == 0) {
@@ -172,25 +187,42 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   // (a bound below every finite number takes all of them, and never -inf)
   constexpr float kLowest = -3.4028234663852886e38f;
   const float bound = tk <= key_of(kLowest) ? kLowest : val_of(tk);
-  float s = 0.0f;
-  each_held<Tin, NV>(d, first, [&](float x, int id) {
-    const bool hit = x >= bound;
-    const float t = __builtin_amdgcn_exp2f((x - ref) * kLog2e);
-    s += hit ? 0.0f : t;
-    const u64 mask = __ballot(hit);
-    if (mask) {  // (uniform)
-      uint32_t at = 0;
-      if (lane_id() == 0) at = atomicAdd(&sh.count, static_cast<uint32_t>(__popcll(mask)));
-      at = uniform_u(at) + lanes_below(mask);
-      if (hit && at < kPartList) sh.list[at] = pack_key(x, id);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (!(vm[j] >= bound)) continue;
+    // (a few vectors a wave: their elements from the bound up go to the list, and out of the sum; a word at a
+    // time, the words passing through the first one's place, so that the code stays small)
+    uint4 v = d[j];
+    int id = first + (j * kPartThreads + tid) * E;
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+      uint32_t word = v.x;
+#pragma unroll
+      for (int h = 0; h < E / 4; ++h, ++id) {
+        const float x = word_value<E>(word, h);
+        if (!(x >= bound)) continue;
+        const uint32_t at = atomicAdd(&sh.count, 1u);
+        if (at < kPartList) sh.list[at] = pack_key(x, id);
+        word = strike_word<E>(word, h);
+      }
+      v = make_uint4(v.y, v.z, v.w, word);
     }
-  });
+    d[j] = v;
+  }
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float x[E];
+    Vec<Tin>::unpack(d[j], x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * kLog2e);
+  }
   double sd = s;
   __syncthreads();
   uint32_t c = sh.count;
   const bool crowded = c > kPartList;  // (uniform)
   if (crowded) {
-    sd = part_crowded<Tin, NV>(d, first, a.n, ref, sh);
+    sd = part_crowded<Tin, NV>(p, a.V, first, a.n, ref, sh);
     c = sh.count;
   }
   // ranks by counting (keys differ); the list's exponentials in fixed point

@@ -62,11 +62,8 @@ __device__ __forceinline__ void strike_listed(const uint32_t* bits, uint4* d) {
     if (m) {
       uint32_t w[4] = {d[j].x, d[j].y, d[j].z, d[j].w};
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (!((m >> e) & 1)) continue;
-        if constexpr (E == 8) w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xFFFFu) | 0xFF800000u : (w[e >> 1] & 0xFFFF0000u) | 0xFF80u;
-        else w[e] = 0xFF800000u;
-      }
+      for (int e = 0; e < E; ++e)
+        if ((m >> e) & 1) w[e * 4 / E] = strike_word<E>(w[e * 4 / E], e & 1);
       d[j] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
@@ -94,6 +91,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_part(DistillArgs a)
 #pragma unroll
     for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
   }
+  forget<NV>(d);
   m = wave_max_f(m);
   const float ref = m == -__builtin_inff() ? 0.0f : m;
   const float c = kLog2e / a.temp;

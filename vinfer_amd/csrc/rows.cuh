@@ -39,6 +39,23 @@ struct Vec<float> {
   }
 };
 
+// Element h of a word, and the word with -inf in its place (E elements a vector: two or one a word).
+template <int E>
+__device__ __forceinline__ float word_value(uint32_t w, int h) {
+  return __uint_as_float(E == 4 ? w : h ? w & 0xFFFF0000u : w << 16);
+}
+template <int E>
+__device__ __forceinline__ uint32_t strike_word(uint32_t w, int h) {
+  return E == 4 ? 0xFF800000u : h ? (w & 0xFFFFu) | 0xFF800000u : (w & 0xFFFF0000u) | 0xFF80u;
+}
+
+// New registers to the compiler: it unpacks a vector again in the next pass rather than keep its elements.
+template <int NV>
+__device__ __forceinline__ void forget(uint4* d) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(d[j].x), "+v"(d[j].y), "+v"(d[j].z), "+v"(d[j].w));
+}
+
 // NV vectors a thread of the segment that starts at element `first`: vector j of thread t holds the elements
 // from first + (j * threads + t) * kElems. What lies past V reads as -inf.
 template <class Tin, int NV, int THREADS>
