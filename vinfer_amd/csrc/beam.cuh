@@ -4,11 +4,11 @@
 // Two launches. k_beam_part: one workgroup a segment of a row, held in registers, so that a row is read
 // once. A lane's maximum gives a bound: the n-th largest of a wave's 64 lane maxima (n <= 64) is at most the
 // segment's n-th largest logit, and few elements reach the largest of the four waves' bounds (about
-// 64 ln(64 / (64 - n)) a wave where the logits come in any order). Those go to a list in LDS, ranked by
-// counting, and the list's first n are the segment's candidates in order. The others, all of them below the
-// bound, add their fp32 exponentials against the segment's maximum; the list's exponentials are taken in
-// fp64 and added in fixed point, so that neither the large terms lose precision nor the order of the list,
-// which varies, shows in the sum: the beams of a request are compared across their rows by these sums.
+// 64 ln(64 / (64 - n)) a wave where the logits come in any order). The vectors that hold one go to LDS, their
+// elements' exponentials are taken in fp64 and added in fixed point, and those that reach the bound are ranked by
+// counting: the first n are the segment's candidates in order. The other vectors, all below the bound, add their
+// fp32 exponentials. So neither do the large terms lose precision nor does the order of the list, which varies,
+// show in the sum: the beams of a request are compared across their rows by these sums.
 // k_beam_merge: one workgroup a request. The rows' lse from the segments' sums; the n-th largest score of the
 // segments' first candidates bounds the request's n-th best; the few candidates that reach it are ranked.
 //
@@ -24,16 +24,18 @@ constexpr int kMaxBeams = 64;
 constexpr int kMaxPick = 64;        // most continuations a request: a lane each
 constexpr int kPartThreads = 256;
 constexpr int kPartWaves = kPartThreads / kWave;
-constexpr int kPartList = 512;      // a segment's candidates before they are ranked
+constexpr int kPartVecs = 512;      // a segment's vectors that hold candidates
+constexpr int kPartList = 512;      // its candidates before they are ranked
 constexpr int kMergeList = 1024;    // a request's
 constexpr int kMergeMaxThreads = 1024;
+constexpr int kAhead = 4;           // entries of a list that are loaded at once
 constexpr double kFix = 4503599627370496.0;  // 2^52
 
 struct BeamArgs {
   const void* logits;  // row (b, w) at b * rstride + w * bstride
   int64_t rstride, bstride;
   int B, W, V, n;
-  int S;               // segments a row
+  int S;               // segments a row, at most 64
   const float* scores;      // [B, W]
   const uint8_t* finished;  // [B, W] or null
   int pad, keep;
@@ -46,7 +48,7 @@ struct BeamArgs {
 };
 
 // The n-th largest of the wave's 64 keys with the bits below LOW cleared: at most the key itself. A step is
-// scalar but for its compare.
+// scalar but for its compare. The second form: of 128 keys, two a lane.
 template <int LOW>
 __device__ __forceinline__ uint32_t wave_nth_floor(uint32_t key, int n) {
   uint32_t t = 0;
@@ -54,6 +56,17 @@ __device__ __forceinline__ uint32_t wave_nth_floor(uint32_t key, int n) {
   for (int b = 31; b >= LOW; --b) {
     const uint32_t c = t | (1u << b);
     if (__popcll(__ballot(key >= c)) >= n) t = c;
+  }
+  return t;
+}
+
+template <int LOW>
+__device__ __forceinline__ uint32_t wave_nth_floor2(uint32_t k0, uint32_t k1, int n) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int b = 31; b >= LOW; --b) {
+    const uint32_t c = t | (1u << b);
+    if (__popcll(__ballot(k0 >= c)) + __popcll(__ballot(k1 >= c)) >= n) t = c;
   }
   return t;
 }
@@ -68,14 +81,15 @@ __device__ __forceinline__ int key_id(u64 k) { return static_cast<int>(0xFFFFFFF
 __device__ __forceinline__ u64 fix52(double e) { return static_cast<u64>(__builtin_rint(e * kFix)); }
 
 struct PartShared {
-  u64 list[kPartList];
-  u64 top[kMaxPick];
+  uint4 vec[kPartVecs];  // the vectors with an element at or above the bound
+  int32_t vid[kPartVecs];  // their first ids
+  u64 list[kPartList];   // those elements
   double wsum[kPartWaves];
   u64 wfix[kPartWaves];
   float wmax[kPartWaves];
   uint32_t wtau[kPartWaves];
   uint32_t wcnt[kPartWaves];
-  uint32_t count;
+  uint32_t vecs, count;
 };
 
 // f(x, id) for each of this thread's elements of the segment, read again.
@@ -145,32 +159,52 @@ __device__ __forceinline__ double part_crowded(const Tin* row, int V, int first,
   return s;
 }
 
-template <class Tin, int NV>
+// MANY: more than half a wave's lanes of continuations.
+template <class Tin, int NV, bool MANY>
 __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   constexpr int E = Vec<Tin>::kElems;
   __shared__ PartShared sh;
   const int tid = threadIdx.x, w = tid / kWave;
   const int row = blockIdx.x / a.S, seg = blockIdx.x % a.S;
-  if (!finite_f(a.scores[row]) || (a.finished && a.finished[row])) return;  // (uniform)
+  const float score = a.scores[row];
+  const int finished = a.finished ? a.finished[row] : 0;  // (both loads at once)
+  if (!finite_f(score) || finished) return;  // (uniform)
   const Tin* p = as_global(static_cast<const Tin*>(a.logits)) + (row / a.W) * a.rstride + (row % a.W) * a.bstride;
   const int first = seg * NV * kPartThreads * E;
   uint4 d[NV];
   load_segment<Tin, NV, kPartThreads>(p, a.V, first, d);
-  if (tid == 0) sh.count = 0;
+  if (tid == 0) sh.vecs = sh.count = 0;
+  exp_table_init();
   float lm = -__builtin_inff();
   float vm[NV];  // each vector's largest
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    float x[E];
-    Vec<Tin>::unpack(d[j], x);
-    vm[j] = x[0];
+    vm[j] = Vec<Tin>::largest(d[j]);
+    lm = max_nan(lm, vm[j]);
+    __builtin_amdgcn_sched_barrier(0);  // (a vector at a time: 64 registers)
+  }
+  const float wm = wave_max_f(lm);
+  uint32_t tau;
+  if constexpr (!MANY) {
+    tau = wave_nth_floor<16>(key_of(lm), a.n);
+  } else {
+    // (nearly all lanes' maxima would be asked for, and the least of them bounds little: two values a lane)
+    forget<NV>(d);
+    float l0 = -__builtin_inff(), l1 = l0;
 #pragma unroll
-    for (int e = 1; e < E; ++e) vm[j] = fmaxf(vm[j], x[e]);
-    lm = fmaxf(lm, vm[j]);
+    for (int j = 0; j < NV; ++j) {
+      float x[E];
+      Vec<Tin>::unpack(d[j], x);
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) {
+        l0 = max_nan(l0, x[e]);
+        l1 = max_nan(l1, x[E / 2 + e]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    tau = wave_nth_floor2<16>(key_of(l0), key_of(l1), a.n);
   }
   forget<NV>(d);
-  const float wm = wave_max_f(lm);
-  const uint32_t tau = wave_nth_floor<16>(key_of(lm), a.n);
   if (lane_id() == 0) {
     sh.wmax[w] = wm;
     sh.wtau[w] = tau;
@@ -187,54 +221,57 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   // (a bound below every finite number takes all of them, and never -inf)
   constexpr float kLowest = -3.4028234663852886e38f;
   const float bound = tk <= key_of(kLowest) ? kLowest : val_of(tk);
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (!(vm[j] >= bound)) continue;
-    // (a few vectors a wave: their elements from the bound up go to the list, and out of the sum; a word at a
-    // time, the words passing through the first one's place, so that the code stays small)
-    uint4 v = d[j];
-    int id = first + (j * kPartThreads + tid) * E;
-#pragma unroll 1
-    for (int k = 0; k < 4; ++k) {
-      uint32_t word = v.x;
-#pragma unroll
-      for (int h = 0; h < E / 4; ++h, ++id) {
-        const float x = word_value<E>(word, h);
-        if (!(x >= bound)) continue;
-        const uint32_t at = atomicAdd(&sh.count, 1u);
-        if (at < kPartList) sh.list[at] = pack_key(x, id);
-        word = strike_word<E>(word, h);
-      }
-      v = make_uint4(v.y, v.z, v.w, word);
-    }
-    d[j] = v;
-  }
+  // The few vectors that reach the bound go to the list, and out of this thread's sum. (A NaN reaches none, and
+  // stays in the sum.)
+  const float refl = ref * kLog2e;
   float s = 0.0f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
+    if (vm[j] >= bound) {
+      const uint32_t at = atomicAdd(&sh.vecs, 1u);
+      if (at < kPartVecs) {
+        sh.vec[at] = d[j];
+        sh.vid[at] = first + (j * kPartThreads + tid) * E;
+      }
+      d[j] = make_uint4(Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf);
+    }
     float x[E];
     Vec<Tin>::unpack(d[j], x);
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * kLog2e);
+    for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], kLog2e, -refl));
+    __builtin_amdgcn_sched_barrier(0);
   }
   double sd = s;
   __syncthreads();
+  const uint32_t nv = sh.vecs;
+  u64 fx = 0;
+  if (nv <= kPartVecs) {  // (uniform)
+    for (uint32_t i = tid; i < nv * E; i += kPartThreads) {
+      const int e = i % E;
+      const float x = word_value<E>(reinterpret_cast<const uint32_t*>(&sh.vec[i / E])[e * 4 / E], e & 1);
+      if (x >= bound) {
+        const uint32_t at = atomicAdd(&sh.count, 1u);
+        if (at < kPartList) sh.list[at] = pack_key(x, sh.vid[i / E] + e);
+      }
+      fx += fix52(exp_nonpos(static_cast<double>(x) - static_cast<double>(ref)));
+    }
+  }
+  __syncthreads();
   uint32_t c = sh.count;
-  const bool crowded = c > kPartList;  // (uniform)
+  const bool crowded = nv > kPartVecs || c > kPartList;  // (uniform)
   if (crowded) {
     sd = part_crowded<Tin, NV>(p, a.V, first, a.n, ref, sh);
+    fx = 0;
     c = sh.count;
   }
-  // ranks by counting (keys differ); the list's exponentials in fixed point
+  // ranks by counting (keys differ)
   const uint32_t n = static_cast<uint32_t>(a.n);
-  u64 fx = 0;
   u64* out = a.keys + static_cast<int64_t>(blockIdx.x) * a.n;
   for (uint32_t i = tid; i < c; i += kPartThreads) {
     const u64 k = sh.list[i];
     uint32_t r = 0;
     for (uint32_t j = 0; j < c; ++j) r += sh.list[j] > k;
     if (r < n) out[r] = k;
-    if (!crowded) fx += fix52(exp(static_cast<double>(key_value(k)) - static_cast<double>(ref)));
   }
   for (uint32_t i = c + tid; i < n; i += kPartThreads) out[i] = 0;
   sd = wave_sum(sd);
@@ -252,6 +289,8 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
       t += sh.wsum[i];
       f += sh.wfix[i];
     }
+    // (x kLog2e - refl = (x - ref) kLog2e + (ref kLog2e - refl): the latter, refl's rounding, is exact in fp64)
+    if (!crowded) t *= exp((refl - static_cast<double>(ref) * static_cast<double>(kLog2e)) * 0.6931471805599453);
     a.sums[blockIdx.x] = t + static_cast<double>(f) * (1.0 / kFix);
     a.maxs[blockIdx.x] = M;
   }
@@ -283,23 +322,20 @@ __device__ __forceinline__ u64 tie_word(int beam, u64 key) {
   return (static_cast<u64>(kMaxBeams - 1 - beam) << 52) | ((key >> 32) << 20) | (key & 0xFFFFFull);
 }
 
-// The score of entry e of list l (of W S lists, S a beam), ordered, and its tie word; 0 where there is none.
-__device__ __forceinline__ u64 merge_entry(const BeamArgs& a, const MergeShared& sh, const u64* keys, int l, int e,
-                                           u64* tb) {
-  const int w = l / a.S;
+// The score of entry e, whose key is k, of list l (of W S lists, S a beam), ordered, and its tie word; 0 where
+// there is none.
+__device__ __forceinline__ u64 merge_score(const MergeShared& sh, int w, bool first, u64 k, u64* tb) {
   const int kind = sh.kind[w];
   if (kind == 1) {
-    const u64 k = keys[static_cast<int64_t>(l) * a.n + e];
-    if (!k) return 0;
     *tb = tie_word(w, k);
-    const double c = (static_cast<double>(key_value(k)) - sh.lse[w]) + sh.score[w];
-    return ordered(c);
+    return k ? ordered((static_cast<double>(key_value(k)) - sh.lse[w]) + sh.score[w]) : 0;
   }
-  if (kind == 2 && e == 0 && l == w * a.S) {
-    *tb = tie_word(w, pack_key(0.0f, 0));
-    return ordered(sh.score[w]);
-  }
-  return 0;
+  *tb = tie_word(w, pack_key(0.0f, 0));
+  return kind == 2 && first ? ordered(sh.score[w]) : 0;
+}
+__device__ __forceinline__ u64 merge_entry(const BeamArgs& a, const MergeShared& sh, const u64* keys, int l, int e, u64* tb) {
+  const int w = l / a.S;
+  return merge_score(sh, w, e == 0 && l == w * a.S, ld_global(keys + static_cast<int64_t>(l) * a.n + e), tb);
 }
 
 // The upper words of ordered fp64 scores order them too, coarsely: the first launch's bound by lane maxima again.
@@ -308,25 +344,28 @@ __global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
   const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id(), nt = blockDim.x, nw = nt / kWave;
   const int b = blockIdx.x;
   const int W = a.W, S = a.S, n = a.n;
+  // A thread a list (the first of its lists is loaded ahead of the rows' sums).
+  const u64* keys = a.keys + static_cast<int64_t>(b) * W * S * n;
+  const int lists = W * S;
+  u64 ahead[kAhead];
+#pragma unroll
+  for (int e = 0; e < kAhead; ++e) ahead[e] = tid < lists && e < n ? ld_global(keys + static_cast<int64_t>(tid) * n + e) : 0;
   for (int w = wave; w < W; w += nw) {
     const int row = b * W + w;
+    // (all loads at once; a row that was not read has left whatever the workspace held)
     const float sc = a.scores[row];
+    const int finished = a.finished ? a.finished[row] : 0;
+    const float m = lane < S ? ld_global(a.maxs + static_cast<int64_t>(row) * S + lane) : -__builtin_inff();
+    const double sum = lane < S ? ld_global(a.sums + static_cast<int64_t>(row) * S + lane) : 0.0;
     int kind = 0;
     double l = 0.0;
     if (finite_f(sc)) {
-      if (a.finished && a.finished[row]) {
+      if (finished) {
         kind = 2;
       } else {
-        const float* ms = a.maxs + static_cast<int64_t>(row) * S;
-        const double* ss = a.sums + static_cast<int64_t>(row) * S;
-        float m = -__builtin_inff();
-        for (int s = lane; s < S; s += kWave) m = fmaxf(m, ms[s]);
         const float M = wave_max_f(m);
-        double t = 0.0;
-        for (int s = lane; s < S; s += kWave) t += ss[s] * exp(static_cast<double>(ms[s]) - static_cast<double>(M));
-        t = wave_sum(t);
-        l = static_cast<double>(M) + log(t);
-        kind = finite_f(M) && l == l ? 1 : 0;
+        l = static_cast<double>(M) + log(wave_sum(sum * exp(static_cast<double>(m) - static_cast<double>(M))));
+        kind = finite_f(M) && l - l == 0.0 ? 1 : 0;
       }
     }
     if (lane == 0) {
@@ -342,31 +381,46 @@ __global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
   }
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  const u64* keys = a.keys + static_cast<int64_t>(b) * W * S * n;
-  const int lists = W * S;
   uint32_t h = 0;
   u64 tb = 0;
-  for (int l = tid; l < lists; l += nt) h = max(h, static_cast<uint32_t>(merge_entry(a, sh, keys, l, 0, &tb) >> 32));
+  const int own = tid / S;  // (the first list's beam)
+  if (tid < lists) h = static_cast<uint32_t>(merge_score(sh, own, tid == own * S, ahead[0], &tb) >> 32);
+  for (int l = tid + nt; l < lists; l += nt) h = max(h, static_cast<uint32_t>(merge_entry(a, sh, keys, l, 0, &tb) >> 32));
   sh.head[tid] = h;
   __syncthreads();
   if (wave == 0) {
     for (int i = lane + kWave; i < nt; i += kWave) h = max(h, sh.head[i]);
-    const uint32_t t = wave_nth_floor<4>(h, n);
+    const uint32_t t = wave_nth_floor<8>(h, n);
     if (lane == 0) sh.bound = max(t, 1u);
   }
   __syncthreads();
   const uint32_t bound = sh.bound;
-  const int total = lists * n;
-  for (int i = tid; i < total; i += nt) {
-    const u64 sk = merge_entry(a, sh, keys, i / n, i % n, &tb);
-    if (static_cast<uint32_t>(sk >> 32) >= bound) {
-      const uint32_t at = atomicAdd(&sh.count, 1u);
-      if (at < kMergeList) {
-        sh.sk[at] = sk;
-        sh.tb[at] = tb;
-      }
+  // (a list's entries descend: the first one below the bound ends it)
+  auto take = [&](u64 sk, u64 t) {
+    if (static_cast<uint32_t>(sk >> 32) < bound) return false;
+    const uint32_t at = atomicAdd(&sh.count, 1u);
+    if (at < kMergeList) {
+      sh.sk[at] = sk;
+      sh.tb[at] = t;
     }
+    return true;
+  };
+  bool more = tid < lists;
+#pragma unroll
+  for (int e = 0; e < kAhead; ++e)
+    if (more && e < n) {
+      const u64 sk = merge_score(sh, own, e == 0 && tid == own * S, ahead[e], &tb);
+      more = take(sk, tb);
+    }
+  for (int e = kAhead; more && e < n; ++e) {
+    const u64 sk = merge_entry(a, sh, keys, tid, e, &tb);
+    more = take(sk, tb);
   }
+  for (int l = tid + nt; l < lists; l += nt)
+    for (int e = 0; e < n; ++e) {
+      const u64 sk = merge_entry(a, sh, keys, l, e, &tb);
+      if (!take(sk, tb)) break;
+    }
   __syncthreads();
   const uint32_t c = sh.count;
   auto choose = [&](uint32_t r, u64 sk, u64 t) {
@@ -387,7 +441,7 @@ __global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
     u64 psk = ~0ull, ptb = ~0ull;
     for (int r = 0; r < n; ++r) {
       u64 bsk = 0, btb = 0;
-      for (int i = tid; i < total; i += nt) {
+      for (int i = tid; i < lists * n; i += nt) {
         const u64 sk = merge_entry(a, sh, keys, i / n, i % n, &tb);
         if (!sk || !(sk < psk || (sk == psk && tb < ptb))) continue;
         if (sk > bsk || (sk == bsk && tb > btb)) {

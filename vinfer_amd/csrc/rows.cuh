@@ -11,6 +11,13 @@ constexpr float kLog2e = 1.44269504088896341f;
 
 __device__ __forceinline__ bool finite_f(float x) { return fabsf(x) < __builtin_inff(); }
 
+// One v_maximum3_f32: a NaN is the result of any NaN. (fmaxf costs an instruction more for each operand that may be
+// a signalling NaN.)
+__device__ __forceinline__ float max3_nan(float x, float y, float z) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(x, y), z);
+}
+__device__ __forceinline__ float max_nan(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+
 // One 16-byte vector's elements as fp32.
 template <class Tin>
 struct Vec;
@@ -26,6 +33,12 @@ struct Vec<uint16_t> {
       x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
     }
   }
+  // The largest element; NaN if there is one.
+  static __device__ __forceinline__ float largest(const uint4& d) {
+    float x[kElems];
+    unpack(d, x);
+    return max3_nan(max3_nan(x[0], x[1], x[2]), max3_nan(x[3], x[4], x[5]), max_nan(x[6], x[7]));
+  }
 };
 template <>
 struct Vec<float> {
@@ -36,6 +49,11 @@ struct Vec<float> {
     x[1] = __uint_as_float(d.y);
     x[2] = __uint_as_float(d.z);
     x[3] = __uint_as_float(d.w);
+  }
+  static __device__ __forceinline__ float largest(const uint4& d) {
+    float x[kElems];
+    unpack(d, x);
+    return max_nan(max3_nan(x[0], x[1], x[2]), x[3]);
   }
 };
 

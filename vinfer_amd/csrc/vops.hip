@@ -256,10 +256,13 @@ int vops_beam_select(const vops_beam_args* a, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(parts));
   with_nv(L.nv, [&](auto nv) {
-    if (a->dtype == VOPS_BF16)
-      hipLaunchKernelGGL((vo::k_beam_part<uint16_t, decltype(nv)::value>), grid, dim3(vo::kPartThreads), 0, st, k);
-    else
-      hipLaunchKernelGGL((vo::k_beam_part<float, decltype(nv)::value>), grid, dim3(vo::kPartThreads), 0, st, k);
+    constexpr int N = decltype(nv)::value;
+    const bool bf = a->dtype == VOPS_BF16, many = a->n > VOPS_MAX_CONTINUATIONS / 2;
+    const dim3 block(vo::kPartThreads);
+    if (bf && many) hipLaunchKernelGGL((vo::k_beam_part<uint16_t, N, true>), grid, block, 0, st, k);
+    else if (bf) hipLaunchKernelGGL((vo::k_beam_part<uint16_t, N, false>), grid, block, 0, st, k);
+    else if (many) hipLaunchKernelGGL((vo::k_beam_part<float, N, true>), grid, block, 0, st, k);
+    else hipLaunchKernelGGL((vo::k_beam_part<float, N, false>), grid, block, 0, st, k);
   });
   if (int rc = launched("launch k_beam_part")) return rc;
   // (a wave a beam, 4 to 16 waves)
