@@ -147,7 +147,9 @@ def test_random_rows(device, size, dtype, T, tail):
 @pytest.mark.gpu
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("size", [(2, 524288, 64, torch.float32), (700, 3001, 16, torch.bfloat16), (300, 9000, 40, torch.float32),
-                                  (270, 151936, 64, torch.bfloat16), (260, 40009, 50, torch.float32)], ids=str)
+                                  (270, 151936, 64, torch.bfloat16), (260, 40009, 50, torch.float32),
+                                  (1600, 4101, 512, torch.bfloat16), (900, 60001, 7, torch.bfloat16), (210, 90001, 600, torch.bfloat16),
+                                  (200, 75003, 70, torch.float32)], ids=str)
 def test_large_rows_and_batches(size, tail):
     x, ids, teacher, w = make(9, *size[:3], size[3], tail=tail, zeros=True)
     compare(GPU, x, ids, teacher, w, 1.0, tail)

@@ -38,6 +38,9 @@ FLAGS = [
     "-packed-fp32-ops",
     "-Wno-unused-command-line-argument",
 ]
+# The operators keep rows in registers across loops: constants that were kept in registers beside them would not fit
+# (the compiler moves each one's load out of the loop, fp64 polynomials' coefficients above all).
+OPS_FLAGS = [*FLAGS, "-mllvm", "-disable-machine-licm"]
 
 
 def hipcc() -> str:
@@ -47,9 +50,9 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (ROCm is required to build the libraries)")
 
 
-def _compile(lib: Path, sources: list[Path], verbose: bool) -> None:
+def _compile(lib: Path, sources: list[Path], flags: list[str], verbose: bool) -> None:
     tmp = lib.with_suffix(".so.tmp")
-    cmd = [hipcc(), *FLAGS, f"-I{ROOT / 'include'}", "-o", str(tmp), *map(str, sources)]
+    cmd = [hipcc(), *flags, f"-I{ROOT / 'include'}", "-o", str(tmp), *map(str, sources)]
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -67,7 +70,7 @@ def _compile(lib: Path, sources: list[Path], verbose: bool) -> None:
 
 def build(verbose: bool = False) -> Path:
     with ThreadPoolExecutor(2) as pool:
-        jobs = [pool.submit(_compile, lib, src, verbose) for lib, src in ((LIB, SOURCES), (OPS_LIB, OPS_SOURCES))]
+        jobs = [pool.submit(_compile, *job, verbose) for job in ((LIB, SOURCES, FLAGS), (OPS_LIB, OPS_SOURCES, OPS_FLAGS))]
     for job in jobs:
         job.result()
     return LIB

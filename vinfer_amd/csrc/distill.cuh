@@ -283,12 +283,233 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
 #pragma unroll
   for (int j = 0; j < NV; ++j)
     store_vector<Tin>(g, a.V, at + j * kDistillThreads * E, grad_vector<Tin>(d[j], ref, c, factor));
-  __syncthreads();  // (the workgroup's stores have landed: the listed ones go over them)
+  __syncthreads();  // (the listed gradients go over what the vectors stored there)
   const int32_t* ids = a.ids + static_cast<int64_t>(row) * a.K;
   for (int k = threadIdx.x; k < a.K; k += kDistillThreads) {
     const int id = ld_global(ids + k);
     if (id >= first && id < a.V && id - first < kElems)
       store_elem<Tin>(g + id, scale * st[2 + k]);
+  }
+}
+
+// ---- loss and gradient of many rows in one pass -----------------------------------------------------------
+// A workgroup holds a whole row: NS vectors a thread in registers, and a row's last V % E elements one a thread. Rows
+// follow one another (grid-strided); as a row's gradients are stored, the next row's logits are loaded into the
+// registers that become free, so that a CU reads and writes at once and a row is read once. Per row two barriers:
+// the listed ids' bits (LDS only: the loads stay in flight), and the waves' sums, after which
+// the last row's listed gradients go over what its vectors stored there.
+template <int WAVES>
+struct HeldShared {
+  float m[2][WAVES];   // a wave's largest unlisted logit, and its sum
+  double s[2][WAVES];
+  double tm[2][WAVES], ts[2][WAVES];  // its entries': the teacher's largest and sum,
+  double xm[2][WAVES], xs[2][WAVES];  // the listed logits' largest and sum
+  double loss[2][WAVES];
+};
+
+template <class Tin, int THREADS, int NS, int ROWS>  // ROWS workgroups a CU
+__global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(DistillArgs a) {
+  constexpr int E = Vec<Tin>::kElems;
+  constexpr int kWavesHere = THREADS / kWave;
+  constexpr int kBits = (THREADS * NS * E + E + 31) / 32;
+  __shared__ uint32_t bits[2][kBits];
+  __shared__ HeldShared<kWavesHere> sh;
+  const int tid = threadIdx.x, lane = lane_id(), w = uniform_i(tid / kWave);
+  const int V = a.V, K = a.K, nvec = V / E;
+  const int left = nvec * E + tid;  // this thread's element of the row's end, if below V
+  const double inv = 1.0 / static_cast<double>(a.temp);
+  const double ninf = -static_cast<double>(__builtin_inff());
+  const float c = kLog2e / a.temp;
+  for (int i = tid; i < kBits; i += THREADS) bits[0][i] = bits[1][i] = 0;
+
+  auto weight_of = [&](int r) { return a.weights ? as_global(a.weights)[r] : 1.0f; };
+  auto row_of = [&](int r) { return as_global(static_cast<const Tin*>(a.x)) + r * a.stride; };
+  // (byte offsets of 32 bits from a uniform row; made anew each time, or the loop would keep them all in registers)
+  const uint32_t most = (nvec - 1) * 16;
+  auto offset = [&](int j) {
+    uint32_t t = tid;
+    asm volatile("" : "+v"(t));
+    return (j * THREADS + t) * 16;
+  };
+  auto vector_at = [&](const Tin* p, int j) { return ld_row16(reinterpret_cast<const char*>(p) + min(offset(j), most)); };
+  auto element = [&](const Tin* p) { return static_cast<float>(logit(p)); };
+
+  int r = blockIdx.x;  // (the grid has at most T workgroups)
+  float weight = weight_of(r);
+  uint4 d[NS];
+  float end = -__builtin_inff();  // the row's end's element
+  int id = -1;
+  float tv = 0.0f, xv = 0.0f;
+  if (weight != 0.0f) {
+    const Tin* p = row_of(r);
+    if (tid < K) {
+      id = ld_global(a.ids + static_cast<int64_t>(r) * K + tid);
+      tv = ld_global(a.teacher + static_cast<int64_t>(r) * K + tid);
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) d[j] = vector_at(p, j);
+    if (left < V) end = element(p + left);
+    if (static_cast<uint32_t>(id) < static_cast<uint32_t>(V)) xv = element(p + id);
+  }
+  // the row before: what is stored once its gradients have landed
+  int last = -1, last_id = -1;
+  float last_g = 0.0f, last_weight = 0.0f;
+  double last_rest = 0.0;
+  __syncthreads();
+
+  int par = 0;  // which of each pair of buffers is this row's
+  for (;; par ^= 1) {
+    const bool live = weight != 0.0f;  // (uniform)
+    const bool has = live && static_cast<uint32_t>(id) < static_cast<uint32_t>(V);
+    if (has) atomicOr(&bits[par][id >> 5], 1u << (id & 31));
+    lds_barrier();
+    if (live) {
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const uint32_t v = offset(j);  // (of element v / sizeof(Tin))
+        const uint32_t at = v / sizeof(Tin);
+        uint32_t marks = (bits[par][at >> 5] >> (at & 31)) & ((1u << E) - 1);
+        if (v > most) marks = (1u << E) - 1;
+        if (marks) {
+          uint32_t q[4] = {d[j].x, d[j].y, d[j].z, d[j].w};
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if ((marks >> e) & 1) q[e * 4 / E] = strike_word<E>(q[e * 4 / E], e & 1);
+          d[j] = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+        m = max_nan(m, Vec<Tin>::largest(d[j]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (left < V && (bits[par][left >> 5] >> (left & 31)) & 1) end = -__builtin_inff();
+      forget<NS>(d);
+      m = wave_max_f(max_nan(m, end));
+      const float ref = m == -__builtin_inff() ? 0.0f : m;
+      float s = __builtin_amdgcn_exp2f((end - ref) * c);
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        float x[E];
+        Vec<Tin>::unpack(d[j], x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * c);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      forget<NS>(d);
+      const double sd = wave_sum(static_cast<double>(s));
+      double tm = ninf, ts = 0.0, xm = ninf, xs = 0.0;
+      if (w * kWave < K) {  // (uniform)
+        tm = wave_max_d(has ? static_cast<double>(tv) : ninf);
+        xm = wave_max_d(has ? static_cast<double>(xv) : ninf);
+      __builtin_amdgcn_sched_barrier(0);
+        ts = wave_sum(!has ? 0.0 : exp(a.tail ? static_cast<double>(tv) : (tv - tm) * inv));
+      __builtin_amdgcn_sched_barrier(0);
+        xs = wave_sum(has ? exp((xv - xm) * inv) : 0.0);
+      }
+      if (lane == 0) {
+        sh.m[par][w] = m;
+        sh.s[par][w] = sd;
+        sh.tm[par][w] = tm;
+        sh.ts[par][w] = ts;
+        sh.xm[par][w] = xm;
+        sh.xs[par][w] = xs;
+      }
+    }
+    __syncthreads();
+    if (last >= 0) {
+      if (last_id >= 0) store_elem<Tin>(as_global(static_cast<Tin*>(a.grad)) + last * a.gstride + last_id, last_g);
+      if (tid == 0) {
+        double t = last_rest;
+        for (int i = 0; i < kWavesHere; ++i) t += sh.loss[par ^ 1][i];
+        a.loss[last] = static_cast<float>(last_weight * t);
+      }
+    }
+    float ref = 0.0f, factor = 0.0f;
+    last = -1;
+    if (live) {
+      if (has) bits[par][id >> 5] = 0;
+      // the row's numbers, in every wave: a lane a wave's part
+      const bool part = lane < kWavesHere;
+      const float mw = part ? sh.m[par][lane] : -__builtin_inff();
+      const float mf = wave_max_f(mw);
+      const double m = mf;
+      double S = part ? sh.s[par][lane] : 0.0;
+      __builtin_amdgcn_sched_barrier(0);
+      S = wave_sum(mw == mf ? S : S * exp((mw - m) * inv));
+      const double tw = part ? sh.tm[par][lane] : ninf, xw = part ? sh.xm[par][lane] : ninf;
+      const double tm = wave_max_d(tw), xmax = wave_max_d(xw), xm = xmax > m ? xmax : m;
+      double ts = part ? sh.ts[par][lane] : 0.0, xs = part ? sh.xs[par][lane] : 0.0;
+      __builtin_amdgcn_sched_barrier(0);
+      ts = wave_sum(a.tail || tw == tm ? ts : ts * exp((tw - tm) * inv));
+      __builtin_amdgcn_sched_barrier(0);
+      xs = wave_sum(xw == xm ? xs : xs * exp((xw - xm) * inv));
+      __builtin_amdgcn_sched_barrier(0);
+      const bool none = tm == ninf;
+      const double lts = a.tail ? 0.0 : tm * inv + log(ts);
+      __builtin_amdgcn_sched_barrier(0);
+      const double lse = xm * inv + log((m == ninf ? S : S * exp((m - xm) * inv)) + xs);
+      const double rest = a.tail ? fmax(0.0, 1.0 - ts) : 0.0;
+      const double mass = a.tail ? ts + rest : (none ? 0.0 : 1.0);
+      __builtin_amdgcn_sched_barrier(0);
+      double A = 0.0;
+      if (m != ninf || S != 0.0) A = mass * exp(m * inv - lse) - (rest > 0.0 ? rest / S : 0.0);
+      __builtin_amdgcn_sched_barrier(0);
+      const float scale = weight / a.temp;
+      ref = uniform_f(mf == -__builtin_inff() ? 0.0f : mf);
+      factor = uniform_f(scale * static_cast<float>(A));
+      double loss = 0.0;
+      float g = 0.0f;
+      if (w * kWave < K && has) {
+        const double lp = a.tail ? static_cast<double>(tv) : tv * inv - lts;
+        const double lq = xv * inv - lse;
+        const double p = none ? 0.0 : exp(lp);
+        if (p != 0.0) loss = p * (lp - lq);
+        g = scale * static_cast<float>(exp(lq) * mass - p);
+      }
+      if (w * kWave < K) loss = wave_sum(loss);
+      __builtin_amdgcn_sched_barrier(0);
+      if (lane == 0) sh.loss[par][w] = loss;
+      last = r;
+      last_id = has ? id : -1;
+      last_g = g;
+      last_weight = weight;
+      last_rest = rest > 0.0 ? rest * (log(rest) - (m * inv + log(S) - lse)) : 0.0;
+    } else if (tid == 0) {
+      a.loss[r] = 0.0f;
+    }
+    // the gradients out, the next row in
+    Tin* g = as_global(static_cast<Tin*>(a.grad)) + r * a.gstride;
+    const int next = r + gridDim.x;
+    const bool more = next < a.T;
+    weight = more ? weight_of(next) : 0.0f;
+    const bool load = weight != 0.0f;
+    const Tin* p = row_of(more ? next : r);
+    id = -1;
+    if (load && tid < K) {
+      id = ld_global(a.ids + static_cast<int64_t>(next) * K + tid);
+      tv = ld_global(a.teacher + static_cast<int64_t>(next) * K + tid);
+    }
+    if (left < V) store_elem<Tin>(g + left, live ? factor * __builtin_amdgcn_exp2f((end - ref) * c) : 0.0f);
+    if (load && left < V) end = element(p + left);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const uint32_t at = offset(j);
+      const uint4 q = live ? grad_vector<Tin>(d[j], ref, c, factor) : make_uint4(0, 0, 0, 0);
+      if (at <= most) st_row16(reinterpret_cast<char*>(g) + at, q);
+      if (load) d[j] = vector_at(p, j);
+      __builtin_amdgcn_sched_barrier(0);
+      if (j == NS / 2 && load && static_cast<uint32_t>(id) < static_cast<uint32_t>(V)) xv = element(p + id);
+    }
+    if (!more) break;
+    r = next;
+  }
+  __syncthreads();
+  if (last >= 0) {
+    if (last_id >= 0) store_elem<Tin>(as_global(static_cast<Tin*>(a.grad)) + last * a.gstride + last_id, last_g);
+    if (tid == 0) {
+      double t = last_rest;
+      for (int i = 0; i < kWavesHere; ++i) t += sh.loss[par][i];
+      a.loss[last] = static_cast<float>(last_weight * t);
+    }
   }
 }
 

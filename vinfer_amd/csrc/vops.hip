@@ -143,6 +143,11 @@ template <int N>
 struct Nv {
   static constexpr int value = N;
 };
+// Loss and gradient of at least this many rows, of at least that many ids, are taken with whole rows held.
+constexpr int kHeldRows = 192;
+constexpr int kHeldVocab = 4096;
+constexpr int kHeldEntries = 512;  // (a thread each)
+
 template <class F>
 void with_nv(int nv, F f) {
   if (nv == 8) f(Nv<8>{});
@@ -188,6 +193,26 @@ vo::DistillArgs distill_args(const vops_distill_args* a, int S) {
   d.grad = a->out_grad;
   d.gstride = a->grad_stride;
   return d;
+}
+
+// The held form's launch, if a row of the call fits a workgroup's registers.
+template <class Tin>
+bool launch_held(const vo::DistillArgs& k, hipStream_t st) {
+  const int nvec = k.V / vo::Vec<Tin>::kElems;
+#define VO_HELD(THREADS, NS, ROWS_A_CU)                                                                  \
+  if (nvec <= THREADS * NS) {                                                                            \
+    const int grid = k.T < 256 * ROWS_A_CU ? k.T : 256 * ROWS_A_CU;                                      \
+    hipLaunchKernelGGL((vo::k_distill_held<Tin, THREADS, NS, ROWS_A_CU>), dim3(grid), dim3(THREADS), 0, st, k);     \
+    return true;                                                                                         \
+  }
+  VO_HELD(512, 8, 3)
+  VO_HELD(512, 16, 2)
+  VO_HELD(512, 20, 2)
+  VO_HELD(1024, 13, 1)
+  VO_HELD(1024, 16, 1)
+  VO_HELD(1024, 20, 1)
+#undef VO_HELD
+  return false;
 }
 
 int grid_ok(int64_t workgroups) {
@@ -338,6 +363,10 @@ int vops_distill(const vops_distill_args* a, void* stream) {
   const dim3 grid(static_cast<unsigned>(parts)), block(vo::kDistillThreads);
   const dim3 rows((a->rows + vo::kDistillWaves - 1) / vo::kDistillWaves);
   const bool bf = a->dtype == VOPS_BF16;
+  if (a->out_grad && !a->states && a->rows >= kHeldRows && a->vocab >= kHeldVocab &&
+      a->entries <= kHeldEntries &&
+      (bf ? launch_held<uint16_t>(k, st) : launch_held<float>(k, st)))
+    return launched("launch k_distill_held");
   with_nv(L.nv, [&](auto nv) {
     constexpr int N = decltype(nv)::value;
     if (bf) hipLaunchKernelGGL((vo::k_distill_part<uint16_t, N>), grid, block, 0, st, k);
