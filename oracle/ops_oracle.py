@@ -23,9 +23,9 @@ def beam_select(logits, scores, n, finished=None, pad_id=0, keep_slots=False):
             m = np.max(x)  # (NaN for a row with one)
             if not np.isfinite(m):
                 continue
-            lse = m + np.log(np.sum(np.exp(x - m)))
+            logs = np.log(np.sum(np.exp(x - m)))
             order = np.lexsort((np.arange(V), -x))[:n]
-            cand += [((x[v] - lse) + s, w, x[v], int(v), int(v)) for v in order if x[v] > -np.inf]
+            cand += [((x[v] - m) - logs + s, w, x[v], int(v), int(v)) for v in order if x[v] > -np.inf]
         cand.sort(key=lambda c: (-c[0], c[1], -c[2], c[3]))
         cand = cand[:n]
         place = list(range(n))
@@ -54,9 +54,12 @@ def reorder(state, parents, lengths=None):
     return new
 
 
-def _lse(x):
-    m = np.max(x, initial=-np.inf)
-    return m if not np.isfinite(m) else m + np.log(np.sum(np.exp(x - m)))
+def _log_softmax(x):
+    """(The largest is taken off first: beside values of 1e38 a log of the sum would be lost.)"""
+    if not np.any(x > -np.inf) and not np.any(np.isnan(x)):
+        return x
+    d = x - np.max(x)
+    return d - np.log(np.sum(np.exp(d)))
 
 
 def distill(student, ids, teacher, weights, temperature=1.0, tail=False):
@@ -75,9 +78,9 @@ def distill(student, ids, teacher, weights, temperature=1.0, tail=False):
             a = a / temperature
             if not np.any(a > -np.inf):
                 continue
-            a = a - _lse(a)
+            a = _log_softmax(a)
         p = np.exp(a)
-        logq = z - _lse(z)
+        logq = _log_softmax(z)
         q = np.exp(logq)
         hot = p > 0
         total = np.sum(p[hot] * (a[hot] - logq[at][hot]))
@@ -86,9 +89,13 @@ def distill(student, ids, teacher, weights, temperature=1.0, tail=False):
         others = np.ones(V, bool)
         others[at] = False
         if rest > 0.0:
-            log_rest = _lse(z[others]) - _lse(z)
+            with np.errstate(divide="ignore"):
+                log_rest = np.max(logq[others], initial=-np.inf)
+                if log_rest > -np.inf:
+                    log_rest += np.log(np.sum(np.exp(logq[others] - log_rest)))
             total += rest * (np.log(rest) - log_rest)
-            g[others] -= rest * np.exp(logq[others] - log_rest)
+            if log_rest > -np.inf:
+                g[others] -= rest * np.exp(_log_softmax(z[others]))
         g[at] -= p
         loss[t], grad[t] = w * total, w / temperature * g
     return loss, grad

@@ -155,6 +155,32 @@ def test_large_rows_and_batches(size, tail):
     compare(GPU, x, ids, teacher, w, 1.0, tail)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_large_batches_of_uneven_and_odd_rows(dtype, tail):
+    # rows whose beginning says nothing of the rest, and every kind of row that is not read, in turn
+    x, ids, teacher, w = make(61, 620, 9003, 20, dtype, tail=tail, ragged=True)
+    x[0::7, :8500] = -torch.inf  # nothing but the end is left
+    x[1::7, :9000] -= 300.0
+    x[2::7, 4000:] += 250.0
+    x[3::7, 1::2] = -torch.inf
+    x[4::7, :] = torch.finfo(dtype).min
+    w[5::7], x[5::7, :] = 0.0, float("nan")
+    ids[6::14] = -1
+    w[300:420] = 0.0
+    w[-1] = w[0] = 0.0
+    compare(GPU, x, ids, teacher, w, 1.0, tail)
+    x, ids, teacher, w = make(62, 200, 9003, 300, dtype, tail=tail)
+    teacher[::2, 60:250] = -torch.inf  # whole waves of entries of probability 0, and of ids that are masked
+    for t in range(0, 200, 3):
+        x[t, ids[t, 100:260].long()] = -torch.inf
+        teacher[t, 100:260] = -torch.inf
+    compare(GPU, x, ids, teacher, w, 1.0, tail)
+    x, ids, teacher, w = make(63, 620, 9003, 20, dtype, tail=tail, ragged=True)
+    compare(GPU, x[:, 1:], torch.where(ids < 9002, ids, -1), teacher, w, 1.7, tail)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
 @pytest.mark.parametrize("device", DEVICES, ids=str)
 def test_masks_and_empty_rows(device, dtype):

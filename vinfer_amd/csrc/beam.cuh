@@ -301,7 +301,7 @@ struct MergeShared {
   u64 sk[kMergeList];  // a candidate's score, ordered
   u64 tb[kMergeList];  // what decides between equal scores
   uint32_t head[kMergeMaxThreads];
-  double lse[kMaxBeams];
+  double top[kMaxBeams], logs[kMaxBeams];  // a row's largest logit, and the log of its sum against it
   double score[kMaxBeams];
   u64 rsk[kMergeMaxThreads / kWave], rtb[kMergeMaxThreads / kWave];
   float ch_score[kMaxPick];
@@ -328,7 +328,7 @@ __device__ __forceinline__ u64 merge_score(const MergeShared& sh, int w, bool fi
   const int kind = sh.kind[w];
   if (kind == 1) {
     *tb = tie_word(w, k);
-    return k ? ordered((static_cast<double>(key_value(k)) - sh.lse[w]) + sh.score[w]) : 0;
+    return k ? ordered((static_cast<double>(key_value(k)) - sh.top[w]) - sh.logs[w] + sh.score[w]) : 0;
   }
   *tb = tie_word(w, pack_key(0.0f, 0));
   return kind == 2 && first ? ordered(sh.score[w]) : 0;
@@ -359,18 +359,19 @@ __global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
     const double sum = lane < S ? ld_global(a.sums + static_cast<int64_t>(row) * S + lane) : 0.0;
     int kind = 0;
     double l = 0.0;
+    const float M = wave_max_f(m);
     if (finite_f(sc)) {
       if (finished) {
         kind = 2;
       } else {
-        const float M = wave_max_f(m);
-        l = static_cast<double>(M) + log(wave_sum(sum * exp(static_cast<double>(m) - static_cast<double>(M))));
+        l = log(wave_sum(sum * exp(static_cast<double>(m) - static_cast<double>(M))));
         kind = finite_f(M) && l - l == 0.0 ? 1 : 0;
       }
     }
     if (lane == 0) {
       sh.kind[w] = kind;
-      sh.lse[w] = l;
+      sh.top[w] = M;
+      sh.logs[w] = l;
       sh.score[w] = sc;
     }
   }

@@ -181,16 +181,19 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_row(DistillArgs a) 
   ts = wave_sum(ts);
   xs = wave_sum(xs);
   const bool none = tm == ninf;  // (no entry, or all of probability 0)
-  const double lts = a.tail ? 0.0 : tm * inv + log(ts);
-  const double lse = xm * inv + log((m == ninf ? S : S * exp((m - xm) * inv)) + xs);
+  // (differences of logits before anything else: beside logits of 1e38 an lse would lose log S)
+  const double lts = a.tail ? 0.0 : log(ts);
+  const double em = m == ninf ? 0.0 : exp((m - xm) * inv);
+  const double total = (m == ninf ? S : S * em) + xs;
+  const double ltotal = log(total);
   const double rest = a.tail ? fmax(0.0, 1.0 - ts) : 0.0;
   const double mass = a.tail ? ts + rest : (none ? 0.0 : 1.0);
   double loss = 0.0;
   for (int k = lane; k < a.K; k += kWave) {
     float g = 0.0f;
     if (static_cast<uint32_t>(ids[k]) < static_cast<uint32_t>(a.V)) {
-      const double lp = a.tail ? static_cast<double>(teacher[k]) : teacher[k] * inv - lts;
-      const double lq = logit(x + ids[k]) * inv - lse;
+      const double lp = a.tail ? static_cast<double>(teacher[k]) : (teacher[k] - tm) * inv - lts;
+      const double lq = (logit(x + ids[k]) - xm) * inv - ltotal;
       const double p = none ? 0.0 : exp(lp);
       if (p != 0.0) loss += p * (lp - lq);
       g = static_cast<float>(exp(lq) * mass - p);
@@ -199,9 +202,9 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_row(DistillArgs a) 
   }
   loss = wave_sum(loss);
   if (lane == 0) {
-    if (rest > 0.0) loss += rest * (log(rest) - (m * inv + log(S) - lse));
+    if (rest > 0.0) loss += rest * (log(rest) - ((m == ninf ? ninf : (m - xm) * inv) + log(S) - ltotal));
     double A = 0.0;
-    if (m != ninf || S != 0.0) A = mass * exp(m * inv - lse) - (rest > 0.0 ? rest / S : 0.0);
+    if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
     a.loss[row] = static_cast<float>(weight * loss);
     st[0] = mf;
     st[1] = static_cast<float>(A);
@@ -225,7 +228,7 @@ template <class Tin>
 __device__ __forceinline__ uint4 grad_vector(const uint4& d, float ref, float c, float factor) {
   constexpr int E = Vec<Tin>::kElems;
   float x[E];
-  Vec<Tin>::unpack(d, x);
+  Vec<Tin>::unpack_again(d, x);
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] = factor * __builtin_amdgcn_exp2f((x[e] - ref) * c);
   if constexpr (E == 8)
@@ -294,13 +297,19 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
 
 // ---- loss and gradient of many rows in one pass -----------------------------------------------------------
 // A workgroup holds a whole row: NS vectors a thread in registers, and a row's last V % E elements one a thread. Rows
-// follow one another (grid-strided); as a row's gradients are stored, the next row's logits are loaded into the
-// registers that become free, so that a CU reads and writes at once and a row is read once. Per row two barriers:
-// the listed ids' bits (LDS only: the loads stay in flight), and the waves' sums, after which
-// the last row's listed gradients go over what its vectors stored there.
+// follow one another (grid-strided). As a row's gradients are stored, the next row's logits are loaded into the
+// registers that become free, and kBehind vectors later they are added to the next row's sum: a row is read once,
+// and a CU reads, writes and computes at once. One barrier a row: the waves' sums, and the next row's listed ids'
+// bits (three bitmaps take turns, so that one is cleared a barrier before it is used again). After it the last row's
+// listed gradients go over what its vectors stored there.
+//
+// A wave's sum is against the largest of its first vectors, not of its row: nothing has to be known of a vector
+// before it is added. Where that was far off (a sum outside 2^-40 .. 2^60) the wave adds up again against its largest.
+constexpr int kBehind = 4;
+
 template <int WAVES>
 struct HeldShared {
-  float m[2][WAVES];   // a wave's largest unlisted logit, and its sum
+  float m[2][WAVES];  // a wave's reference, and its sum
   double s[2][WAVES];
   double tm[2][WAVES], ts[2][WAVES];  // its entries': the teacher's largest and sum,
   double xm[2][WAVES], xs[2][WAVES];  // the listed logits' largest and sum
@@ -312,7 +321,7 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
   constexpr int E = Vec<Tin>::kElems;
   constexpr int kWavesHere = THREADS / kWave;
   constexpr int kBits = (THREADS * NS * E + E + 31) / 32;
-  __shared__ uint32_t bits[2][kBits];
+  __shared__ uint32_t bits[3][kBits];
   __shared__ HeldShared<kWavesHere> sh;
   const int tid = threadIdx.x, lane = lane_id(), w = uniform_i(tid / kWave);
   const int V = a.V, K = a.K, nvec = V / E;
@@ -320,10 +329,15 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
   const double inv = 1.0 / static_cast<double>(a.temp);
   const double ninf = -static_cast<double>(__builtin_inff());
   const float c = kLog2e / a.temp;
-  for (int i = tid; i < kBits; i += THREADS) bits[0][i] = bits[1][i] = 0;
+  for (int i = tid; i < kBits; i += THREADS) bits[0][i] = bits[1][i] = bits[2][i] = 0;
 
-  auto weight_of = [&](int r) { return a.weights ? as_global(a.weights)[r] : 1.0f; };
-  auto row_of = [&](int r) { return as_global(static_cast<const Tin*>(a.x)) + r * a.stride; };
+  // A row's weight; 0 for none.
+  auto weight_of = [&](int r) { return r >= a.T ? 0.0f : a.weights ? as_global(a.weights)[r] : 1.0f; };
+  auto row_of = [&](int r) { return as_global(static_cast<const Tin*>(a.x)) + (r < a.T ? r : 0) * a.stride; };
+  auto element = [&](const Tin* p) { return static_cast<float>(logit(p)); };
+  auto listed = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(V); };
+  auto id_of = [&](int r) { return ld_global(a.ids + static_cast<int64_t>(r) * K + tid); };
+  auto teacher_of = [&](int r) { return ld_global(a.teacher + static_cast<int64_t>(r) * K + tid); };
   // (byte offsets of 32 bits from a uniform row; made anew each time, or the loop would keep them all in registers)
   const uint32_t most = (nvec - 1) * 16;
   auto offset = [&](int j) {
@@ -332,81 +346,133 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
     return (j * THREADS + t) * 16;
   };
   auto vector_at = [&](const Tin* p, int j) { return ld_row16(reinterpret_cast<const char*>(p) + min(offset(j), most)); };
-  auto element = [&](const Tin* p) { return static_cast<float>(logit(p)); };
 
-  int r = blockIdx.x;  // (the grid has at most T workgroups)
-  float weight = weight_of(r);
-  uint4 d[NS];
+  uint4 d[NS];  // (a row that is not read: -inf throughout)
+#pragma unroll
+  for (int j = 0; j < NS; ++j) d[j] = make_uint4(Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf);
   float end = -__builtin_inff();  // the row's end's element
-  int id = -1;
-  float tv = 0.0f, xv = 0.0f;
+  float ref = 0.0f, s = 0.0f;     // a wave's reference, a thread's sum
+  // Strikes the listed elements, and what lies past the row, out of the row's vector j of this thread.
+  auto strike_marked = [&](uint4& v, int j, const uint32_t* marked) {
+    const uint32_t o = offset(j);
+    const uint32_t at = o / sizeof(Tin);
+    uint32_t marks = (marked[at >> 5] >> (at & 31)) & ((1u << E) - 1);
+    if (o > most) marks = (1u << E) - 1;
+    if (marks) {
+      uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if ((marks >> e) & 1) q[e * 4 / E] = strike_word<E>(q[e * 4 / E], e & 1);
+      v = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+  };
+  // Vector j without its listed elements joins the sum.
+  auto add = [&](int j, const uint32_t* marked) {
+    strike_marked(d[j], j, marked);
+    if (j == 0) {
+      const float m = wave_max_f(Vec<Tin>::largest(d[j]));
+      ref = finite_f(m) ? m : 0.0f;
+      s = 0.0f;
+    }
+    float x[E];
+    Vec<Tin>::unpack(d[j], x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * c);
+  };
+  auto add_end = [&](const uint32_t* marked) {
+    if (left < V && (marked[left >> 5] >> (left & 31)) & 1) end = -__builtin_inff();
+    s += __builtin_amdgcn_exp2f((end - ref) * c);
+  };
+
+  // the first row, and the second one's entries
+  int r = blockIdx.x, now = 0, next_bits = 1, free_bits = 2;
+  float weight = weight_of(r), weight1 = weight_of(r + gridDim.x);
+  int id = -1, id1 = -1;
+  float tv = 0.0f, xv = 0.0f, tv1 = 0.0f;
+  __syncthreads();
   if (weight != 0.0f) {
     const Tin* p = row_of(r);
     if (tid < K) {
-      id = ld_global(a.ids + static_cast<int64_t>(r) * K + tid);
-      tv = ld_global(a.teacher + static_cast<int64_t>(r) * K + tid);
+      id = id_of(r);
+      tv = teacher_of(r);
     }
 #pragma unroll
     for (int j = 0; j < NS; ++j) d[j] = vector_at(p, j);
     if (left < V) end = element(p + left);
-    if (static_cast<uint32_t>(id) < static_cast<uint32_t>(V)) xv = element(p + id);
+    if (listed(id)) {
+      xv = element(p + id);
+      atomicOr(&bits[0][id >> 5], 1u << (id & 31));
+    }
   }
-  // the row before: what is stored once its gradients have landed
-  int last = -1, last_id = -1;
+  if (weight1 != 0.0f && tid < K) {
+    id1 = id_of(r + gridDim.x);
+    tv1 = teacher_of(r + gridDim.x);
+  }
+  lds_barrier();
+  if (weight != 0.0f) {
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      add(j, bits[0]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    add_end(bits[0]);
+  }
+  // the row before: what is stored once its gradients are
+  int last = -1, last_id = -1, par = 0;
   float last_g = 0.0f, last_weight = 0.0f;
   double last_rest = 0.0;
-  __syncthreads();
 
-  int par = 0;  // which of each pair of buffers is this row's
   for (;; par ^= 1) {
     const bool live = weight != 0.0f;  // (uniform)
-    const bool has = live && static_cast<uint32_t>(id) < static_cast<uint32_t>(V);
-    if (has) atomicOr(&bits[par][id >> 5], 1u << (id & 31));
-    lds_barrier();
+    const bool has = live && listed(id);
+    const bool load = weight1 != 0.0f;
+    const int next = r + gridDim.x;
+    const Tin* p = row_of(next);
+    // the next row's listed ids, and their logits
+    float xv1 = 0.0f;
+    if (load && listed(id1)) {
+      atomicOr(&bits[next_bits][id1 >> 5], 1u << (id1 & 31));
+      xv1 = element(p + id1);
+    }
     if (live) {
-      float m = -__builtin_inff();
-#pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        const uint32_t v = offset(j);  // (of element v / sizeof(Tin))
-        const uint32_t at = v / sizeof(Tin);
-        uint32_t marks = (bits[par][at >> 5] >> (at & 31)) & ((1u << E) - 1);
-        if (v > most) marks = (1u << E) - 1;
-        if (marks) {
-          uint32_t q[4] = {d[j].x, d[j].y, d[j].z, d[j].w};
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if ((marks >> e) & 1) q[e * 4 / E] = strike_word<E>(q[e * 4 / E], e & 1);
-          d[j] = make_uint4(q[0], q[1], q[2], q[3]);
+      double sd = wave_sum(static_cast<double>(s));
+      if (!(sd > 0x1p-40 && sd < 0x1p60)) {  // (uniform over the wave)
+        // (read again: a rolled loop, no registers)
+        const Tin* own = row_of(r);
+        float m = end;
+#pragma unroll 1
+        for (int j = 0; j < NS; ++j) {
+          uint4 v = vector_at(own, j);
+          strike_marked(v, j, bits[now]);
+          m = max_nan(m, Vec<Tin>::largest(v));
         }
-        m = max_nan(m, Vec<Tin>::largest(d[j]));
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if (left < V && (bits[par][left >> 5] >> (left & 31)) & 1) end = -__builtin_inff();
-      forget<NS>(d);
-      m = wave_max_f(max_nan(m, end));
-      const float ref = m == -__builtin_inff() ? 0.0f : m;
-      float s = __builtin_amdgcn_exp2f((end - ref) * c);
+        ref = wave_max_f(m);
+        const float z = ref == -__builtin_inff() ? 0.0f : ref;
+        s = __builtin_amdgcn_exp2f((end - z) * c);
+#pragma unroll 1
+        for (int j = 0; j < NS; ++j) {
+          uint4 v = vector_at(own, j);
+          strike_marked(v, j, bits[now]);
+          float x[E];
+          Vec<Tin>::unpack(v, x);
 #pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        float x[E];
-        Vec<Tin>::unpack(d[j], x);
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * c);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - z) * c);
+        }
+        sd = wave_sum(static_cast<double>(s));
       }
-      forget<NS>(d);
-      const double sd = wave_sum(static_cast<double>(s));
       double tm = ninf, ts = 0.0, xm = ninf, xs = 0.0;
       if (w * kWave < K) {  // (uniform)
         tm = wave_max_d(has ? static_cast<double>(tv) : ninf);
         xm = wave_max_d(has ? static_cast<double>(xv) : ninf);
-      __builtin_amdgcn_sched_barrier(0);
-        ts = wave_sum(!has ? 0.0 : exp(a.tail ? static_cast<double>(tv) : (tv - tm) * inv));
-      __builtin_amdgcn_sched_barrier(0);
-        xs = wave_sum(has ? exp((xv - xm) * inv) : 0.0);
+        __builtin_amdgcn_sched_barrier(0);
+        // (-inf adds nothing, also where a wave's entries have nothing else)
+        ts = wave_sum(!has || tv == ninf ? 0.0 : exp(a.tail ? static_cast<double>(tv) : (tv - tm) * inv));
+        __builtin_amdgcn_sched_barrier(0);
+        xs = wave_sum(!has || xv == ninf ? 0.0 : exp((xv - xm) * inv));
       }
+      __builtin_amdgcn_sched_barrier(0);
       if (lane == 0) {
-        sh.m[par][w] = m;
+        sh.m[par][w] = ref;
         sh.s[par][w] = sd;
         sh.tm[par][w] = tm;
         sh.ts[par][w] = ts;
@@ -423,10 +489,10 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
         a.loss[last] = static_cast<float>(last_weight * t);
       }
     }
-    float ref = 0.0f, factor = 0.0f;
+    float zero = 0.0f, factor = 0.0f;  // the row's reference, and its gradients' factor
     last = -1;
     if (live) {
-      if (has) bits[par][id >> 5] = 0;
+      if (has) bits[now][id >> 5] = 0;
       // the row's numbers, in every wave: a lane a wave's part
       const bool part = lane < kWavesHere;
       const float mw = part ? sh.m[par][lane] : -__builtin_inff();
@@ -444,63 +510,77 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
       xs = wave_sum(xw == xm ? xs : xs * exp((xw - xm) * inv));
       __builtin_amdgcn_sched_barrier(0);
       const bool none = tm == ninf;
-      const double lts = a.tail ? 0.0 : tm * inv + log(ts);
+      const double lts = a.tail ? 0.0 : log(ts);
       __builtin_amdgcn_sched_barrier(0);
-      const double lse = xm * inv + log((m == ninf ? S : S * exp((m - xm) * inv)) + xs);
+      const double em = m == ninf ? 0.0 : exp((m - xm) * inv);
+      const double total = (m == ninf ? S : S * em) + xs;
+      __builtin_amdgcn_sched_barrier(0);
+      const double ltotal = log(total);
       const double rest = a.tail ? fmax(0.0, 1.0 - ts) : 0.0;
       const double mass = a.tail ? ts + rest : (none ? 0.0 : 1.0);
       __builtin_amdgcn_sched_barrier(0);
       double A = 0.0;
-      if (m != ninf || S != 0.0) A = mass * exp(m * inv - lse) - (rest > 0.0 ? rest / S : 0.0);
+      if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
       __builtin_amdgcn_sched_barrier(0);
       const float scale = weight / a.temp;
-      ref = uniform_f(mf == -__builtin_inff() ? 0.0f : mf);
+      zero = uniform_f(mf == -__builtin_inff() ? 0.0f : mf);
       factor = uniform_f(scale * static_cast<float>(A));
       double loss = 0.0;
       float g = 0.0f;
       if (w * kWave < K && has) {
-        const double lp = a.tail ? static_cast<double>(tv) : tv * inv - lts;
-        const double lq = xv * inv - lse;
-        const double p = none ? 0.0 : exp(lp);
-        if (p != 0.0) loss = p * (lp - lq);
-        g = scale * static_cast<float>(exp(lq) * mass - p);
+        const double lp = a.tail ? static_cast<double>(tv) : (tv - tm) * inv - lts;
+        const double lq = (xv - xm) * inv - ltotal;
+        const double q = none ? 0.0 : exp(lp);
+        if (q != 0.0) loss = q * (lp - lq);
+        g = scale * static_cast<float>(exp(lq) * mass - q);
       }
       if (w * kWave < K) loss = wave_sum(loss);
-      __builtin_amdgcn_sched_barrier(0);
       if (lane == 0) sh.loss[par][w] = loss;
       last = r;
       last_id = has ? id : -1;
       last_g = g;
       last_weight = weight;
-      last_rest = rest > 0.0 ? rest * (log(rest) - (m * inv + log(S) - lse)) : 0.0;
+      last_rest = rest > 0.0 ? rest * (log(rest) - ((m == ninf ? ninf : (m - xm) * inv) + log(S) - ltotal)) : 0.0;
     } else if (tid == 0) {
       a.loss[r] = 0.0f;
     }
-    // the gradients out, the next row in
+    // the gradients out, the next row in, and its sum
     Tin* g = as_global(static_cast<Tin*>(a.grad)) + r * a.gstride;
-    const int next = r + gridDim.x;
-    const bool more = next < a.T;
-    weight = more ? weight_of(next) : 0.0f;
-    const bool load = weight != 0.0f;
-    const Tin* p = row_of(more ? next : r);
-    id = -1;
-    if (load && tid < K) {
-      id = ld_global(a.ids + static_cast<int64_t>(next) * K + tid);
-      tv = ld_global(a.teacher + static_cast<int64_t>(next) * K + tid);
+    const float weight2 = weight_of(next + gridDim.x);
+    id = load ? id1 : -1;
+    tv = tv1;
+    xv = xv1;
+    if (weight2 != 0.0f && tid < K) {
+      id1 = id_of(next + gridDim.x);
+      tv1 = teacher_of(next + gridDim.x);
     }
-    if (left < V) store_elem<Tin>(g + left, live ? factor * __builtin_amdgcn_exp2f((end - ref) * c) : 0.0f);
-    if (load && left < V) end = element(p + left);
+    if (left < V) {
+      store_elem<Tin>(g + left, factor * __builtin_amdgcn_exp2f((end - zero) * c));
+      end = load ? element(p + left) : -__builtin_inff();
+    }
+    const uint32_t* marked = bits[next_bits];
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      const uint32_t at = offset(j);
-      const uint4 q = live ? grad_vector<Tin>(d[j], ref, c, factor) : make_uint4(0, 0, 0, 0);
-      if (at <= most) st_row16(reinterpret_cast<char*>(g) + at, q);
-      if (load) d[j] = vector_at(p, j);
+    for (int j = 0; j < NS + kBehind; ++j) {
+      if (j < NS) {
+        const uint32_t at = offset(j);
+        const uint4 q = grad_vector<Tin>(d[j], zero, c, factor);
+        if (at <= most) st_row16(reinterpret_cast<char*>(g) + at, q);
+        d[j] = make_uint4(Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf);
+        if (load) d[j] = vector_at(p, j);
+      }
       __builtin_amdgcn_sched_barrier(0);
-      if (j == NS / 2 && load && static_cast<uint32_t>(id) < static_cast<uint32_t>(V)) xv = element(p + id);
+      if (j >= kBehind) add(j - kBehind, marked);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (!more) break;
+    add_end(marked);
+    if (next >= a.T) break;
     r = next;
+    weight = weight1;
+    weight1 = weight2;
+    const int t = now;
+    now = next_bits;
+    next_bits = free_bits;
+    free_bits = t;
   }
   __syncthreads();
   if (last >= 0) {

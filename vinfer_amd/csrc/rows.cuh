@@ -33,6 +33,15 @@ struct Vec<uint16_t> {
       x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
     }
   }
+  // The same by byte permutes: to the compiler other values, which it does not keep from an earlier unpack on.
+  static __device__ __forceinline__ void unpack_again(const uint4& d, float* x) {
+    const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = __uint_as_float(__builtin_amdgcn_perm(w[j], 0u, 0x05040C0Cu));
+      x[2 * j + 1] = __uint_as_float(__builtin_amdgcn_perm(w[j], 0u, 0x07060C0Cu));
+    }
+  }
   // The largest element; NaN if there is one.
   static __device__ __forceinline__ float largest(const uint4& d) {
     float x[kElems];
@@ -50,6 +59,7 @@ struct Vec<float> {
     x[2] = __uint_as_float(d.z);
     x[3] = __uint_as_float(d.w);
   }
+  static __device__ __forceinline__ void unpack_again(const uint4& d, float* x) { unpack(d, x); }
   static __device__ __forceinline__ float largest(const uint4& d) {
     float x[kElems];
     unpack(d, x);
@@ -71,7 +81,11 @@ __device__ __forceinline__ uint32_t strike_word(uint32_t w, int h) {
 template <int NV>
 __device__ __forceinline__ void forget(uint4* d) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(d[j].x), "+v"(d[j].y), "+v"(d[j].z), "+v"(d[j].w));
+  for (int j = 0; j < NV; ++j) {
+    u32x4_t v = __builtin_bit_cast(u32x4_t, d[j]);
+    asm volatile("" : "+v"(v));
+    d[j] = make_uint4(v.x, v.y, v.z, v.w);
+  }
 }
 
 // NV vectors a thread of the segment that starts at element `first`: vector j of thread t holds the elements

@@ -210,7 +210,7 @@ bool launch_held(const vo::DistillArgs& k, hipStream_t st) {
   VO_HELD(512, 20, 2)
   VO_HELD(1024, 13, 1)
   VO_HELD(1024, 16, 1)
-  VO_HELD(1024, 20, 1)
+  VO_HELD(1024, 19, 1)
 #undef VO_HELD
   return false;
 }

@@ -31,18 +31,19 @@ class ReferenceDistill:
         rest = (1 - p.sum(1)).clamp(min=0) if tail else torch.zeros(T, dtype=torch.float64, device=x.device)
         mass = p.sum(1) + rest
         z = x / temperature
-        lse = torch.logsumexp(z, 1)
-        logq = torch.gather(z, 1, at) - lse[:, None]
+        logq = torch.log_softmax(z, 1)
+        others = torch.where(member, -torch.inf, logq)
+        log_rest = torch.logsumexp(others, 1)
+        largest = others.amax(1)
+        m = torch.where(member, -torch.inf, x).amax(1)
+        logq = torch.gather(logq, 1, at)
         loss = torch.where(p != 0, p * (logp - logq), 0.0).sum(1)
-        others = torch.where(member, -torch.inf, z)
-        m = others.amax(1)
-        lse_others = torch.logsumexp(others, 1)
-        loss = loss + torch.where(rest > 0, rest * (torch.log(rest) - (lse_others - lse)), 0.0)
-        # the others' gradient: exp(z - m) times this
-        factor = mass * torch.exp(m - lse) - torch.where(rest > 0, rest * torch.exp(m - lse_others), 0.0)
+        loss = loss + torch.where(rest > 0, rest * (torch.log(rest) - log_rest), 0.0)
+        # the others' gradient: exp((x - m) / temperature) times this
+        factor = mass * torch.exp(largest) - torch.where(rest > 0, rest * torch.exp(largest - log_rest), 0.0)
         factor = torch.where(m == -torch.inf, 0.0, factor)
         listed = torch.where(there, torch.exp(logq) * mass[:, None] - p, 0.0)
-        return loss, torch.cat([m[:, None] * temperature, factor[:, None], listed], 1)
+        return loss, torch.cat([m[:, None], factor[:, None], listed], 1)
 
     def loss_and_states(self, student, ids, teacher, weights=None, *, temperature=1.0, tail=False):
         check(student, ids, teacher, weights, temperature)

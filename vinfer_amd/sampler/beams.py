@@ -159,10 +159,10 @@ def select_reference(logits, scores, n, finished=None, pad_id=0, keep_slots=Fals
             m = x.max()  # (NaN where there is one)
             if not bool(torch.isfinite(m)):
                 continue
-            lse = m + torch.log(torch.exp(x - m).sum())
+            logs = torch.log(torch.exp(x - m).sum())
             order = torch.sort(x + 0.0, descending=True, stable=True).indices[:n]
             entries += [(float(c), -w, float(x[v]) + 0.0, -int(v), int(v))
-                        for v, c in zip(order, (x[order] - lse) + score) if float(c) > -math.inf]
+                        for v, c in zip(order, (x[order] - m) - logs + score) if float(c) > -math.inf]
         entries.sort(reverse=True)
         chosen = entries[:n]
         places = list(range(n))
