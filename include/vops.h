@@ -131,7 +131,7 @@ typedef struct vops_distill_args {
   float temperature;    /* > 0 */
   uint32_t flags;
   float* out_loss; /* [rows] */
-  void* out_grad;  /* `dtype`, row t at t * grad_stride; NULL: the loss alone */
+  void* out_grad;  /* `dtype`, row t at t * grad_stride, not over the student; NULL: the loss alone */
   int64_t grad_stride;
   float* states; /* NULL, or [rows, 2 + entries]: what vops_distill_grad takes */
   void* workspace;

@@ -136,6 +136,19 @@ def test_masks_infinities_and_nan(device, dtype):
         compare(device, x[:, w : w + 1], scores[:, w : w + 1], 40)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_rows_of_the_lowest_value(device, dtype):
+    # masked by the type's lowest value throughout, or but for a few ids: whole segments hold nothing else, and few of them
+    low = torch.finfo(dtype).min
+    for V in (300, 4196, 8492):
+        x, scores = rows(8, 2, 3, V, dtype)
+        x[:, 0] = low
+        x[:, 1, 7:] = low
+        x[:, 2, : V - 5] = low
+        compare(device, x, scores, 6)
+
+
 @pytest.mark.parametrize("device", DEVICES, ids=str)
 def test_equal_rows_and_scores_go_by_beam(device):
     # every beam has the same row and score: whole lists of equal scores, in the order beam, logit, id

@@ -258,7 +258,8 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   }
   __syncthreads();
   uint32_t c = sh.count;
-  const bool crowded = nv > kPartVecs || c > kPartList;  // (uniform)
+  // (or logits so large that the products would overflow: masks of the type's lowest value alone, say)
+  const bool crowded = nv > kPartVecs || c > kPartList || (finite_f(M) && fabsf(M) > 1e30f);  // (uniform)
   if (crowded) {
     sd = part_crowded<Tin, NV>(p, a.V, first, a.n, ref, sh);
     fx = 0;

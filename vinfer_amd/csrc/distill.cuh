@@ -223,6 +223,11 @@ __device__ __forceinline__ void st_row16(void* p, uint4 v) {
   *(__attribute__((address_space(1))) u32x4_row_t*)p = u32x4_t{v.x, v.y, v.z, v.w};
 }
 
+// (past the cache: gradients of a batch larger than it)
+__device__ __forceinline__ void st_row16_nt(void* p, uint4 v) {
+  __builtin_nontemporal_store(u32x4_t{v.x, v.y, v.z, v.w}, (__attribute__((address_space(1))) u32x4_row_t*)p);
+}
+
 // A vector's gradients, factor exp2((x - ref) c), packed.
 template <class Tin>
 __device__ __forceinline__ uint4 grad_vector(const uint4& d, float ref, float c, float factor) {
@@ -297,15 +302,19 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
 
 // ---- loss and gradient of many rows in one pass -----------------------------------------------------------
 // A workgroup holds a whole row: NS vectors a thread in registers, and a row's last V % E elements one a thread. Rows
-// follow one another (grid-strided). As a row's gradients are stored, the next row's logits are loaded into the
-// registers that become free, and kBehind vectors later they are added to the next row's sum: a row is read once,
-// and a CU reads, writes and computes at once. One barrier a row: the waves' sums, and the next row's listed ids'
-// bits (three bitmaps take turns, so that one is cleared a barrier before it is used again). After it the last row's
-// listed gradients go over what its vectors stored there.
+// follow one another (grid-strided, those of weight 0 passed over). As a row's gradients are stored, the next row's
+// logits are loaded into the registers that become free, and kBehind vectors later they are added to the next row's
+// sum: a row is read once, and a CU reads, writes and computes at once. Loads and stores there are unconditional (the
+// lanes past the row's end repeat its last vector), so that the waits count them. One barrier a row: the waves' sums,
+// and the next row's listed ids' bits (three bitmaps take turns: one is cleared a barrier before it is used again).
+// After it the last row's listed gradients go over what its vectors stored there.
 //
-// A wave's sum is against the largest of its first vectors, not of its row: nothing has to be known of a vector
-// before it is added. Where that was far off (a sum outside 2^-40 .. 2^60) the wave adds up again against its largest.
-constexpr int kBehind = 4;
+// A wave's sum is against the largest of its first vectors, not of its row: nothing has to be known of a vector before
+// it is added. Where that was far off (a sum outside 2^-40 .. 2^60) the wave adds up again against its largest.
+// exp(x / T - ref / T) is one fma and v_exp_f32: 2^(x c - fl(ref c)), c = fl(log2(e) / T); the rounding of ref c is
+// put right in the sum, in fp64. A bf16 gradient's factor goes into the exponent too (off by 2^-19 at most).
+constexpr int kBehind = 8;
+constexpr float kHugeLogit = 1e30f;  // (past it x c may overflow: differences first)
 
 template <int WAVES>
 struct HeldShared {
@@ -321,6 +330,7 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
   constexpr int E = Vec<Tin>::kElems;
   constexpr int kWavesHere = THREADS / kWave;
   constexpr int kBits = (THREADS * NS * E + E + 31) / 32;
+  constexpr double kLn2 = 0.6931471805599453;
   __shared__ uint32_t bits[3][kBits];
   __shared__ HeldShared<kWavesHere> sh;
   const int tid = threadIdx.x, lane = lane_id(), w = uniform_i(tid / kWave);
@@ -328,36 +338,49 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
   const int left = nvec * E + tid;  // this thread's element of the row's end, if below V
   const double inv = 1.0 / static_cast<double>(a.temp);
   const double ninf = -static_cast<double>(__builtin_inff());
-  const float c = kLog2e / a.temp;
-  for (int i = tid; i < kBits; i += THREADS) bits[0][i] = bits[1][i] = bits[2][i] = 0;
+  const float c = uniform_f(kLog2e / a.temp);
 
-  // A row's weight; 0 for none.
-  auto weight_of = [&](int r) { return r >= a.T ? 0.0f : a.weights ? as_global(a.weights)[r] : 1.0f; };
-  auto row_of = [&](int r) { return as_global(static_cast<const Tin*>(a.x)) + (r < a.T ? r : 0) * a.stride; };
+  auto row_of = [&](int r) { return as_global(static_cast<const Tin*>(a.x)) + r * a.stride; };
+  auto grad_of = [&](int r) { return as_global(static_cast<Tin*>(a.grad)) + r * a.gstride; };
+  auto weight_of = [&](int r) { return a.weights ? as_global(a.weights)[r] : 1.0f; };
   auto element = [&](const Tin* p) { return static_cast<float>(logit(p)); };
   auto listed = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(V); };
   auto id_of = [&](int r) { return ld_global(a.ids + static_cast<int64_t>(r) * K + tid); };
   auto teacher_of = [&](int r) { return ld_global(a.teacher + static_cast<int64_t>(r) * K + tid); };
-  // (byte offsets of 32 bits from a uniform row; made anew each time, or the loop would keep them all in registers)
-  const uint32_t most = (nvec - 1) * 16;
-  auto offset = [&](int j) {
-    uint32_t t = tid;
+  // Vector j of this thread: bytes from a uniform base, and the offset of the lane (made anew each time, or the loops
+  // would keep them all in registers).
+  const uint32_t most = (nvec - 1) * 16, t16 = tid * 16;
+  auto anew = [&]() {
+    uint32_t t = t16;
     asm volatile("" : "+v"(t));
-    return (j * THREADS + t) * 16;
+    return t;
   };
-  auto vector_at = [&](const Tin* p, int j) { return ld_row16(reinterpret_cast<const char*>(p) + min(offset(j), most)); };
+  auto base = [&](int j) { return min(static_cast<uint32_t>(j * THREADS * 16), most); };
+  auto offset = [&](int j) { return min(anew(), most - base(j)); };
+  auto own = [&](int j) { return anew() + j * THREADS * 16 <= most; };  // (not a repetition)
+  auto vector_at = [&](const Tin* p, int j) { return ld_row16(reinterpret_cast<const char*>(p) + base(j) + offset(j)); };
 
-  uint4 d[NS];  // (a row that is not read: -inf throughout)
-#pragma unroll
-  for (int j = 0; j < NS; ++j) d[j] = make_uint4(Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf);
+  // The first row from r on (in steps of the grid) whose weight is not 0, T for none; the ones passed over get their
+  // zeros.
+  auto live_from = [&](int r) {
+    for (; r < a.T && weight_of(r) == 0.0f; r += gridDim.x) {
+      char* g = reinterpret_cast<char*>(grad_of(r));
+#pragma unroll 1
+      for (uint32_t o = t16; o <= most; o += THREADS * 16) st_row16_nt(g + o, make_uint4(0, 0, 0, 0));
+      if (left < V) store_elem<Tin>(grad_of(r) + left, 0.0f);
+      if (tid == 0) a.loss[r] = 0.0f;
+    }
+    return min(r, a.T);
+  };
+
+  uint4 d[NS];
   float end = -__builtin_inff();  // the row's end's element
-  float ref = 0.0f, s = 0.0f;     // a wave's reference, a thread's sum
-  // Strikes the listed elements, and what lies past the row, out of the row's vector j of this thread.
+  float ref = 0.0f, refc = 0.0f, s = 0.0f;  // a wave's reference, a thread's sum
+  // Strikes the listed elements out of the row's vector j of this thread.
   auto strike_marked = [&](uint4& v, int j, const uint32_t* marked) {
-    const uint32_t o = offset(j);
-    const uint32_t at = o / sizeof(Tin);
-    uint32_t marks = (marked[at >> 5] >> (at & 31)) & ((1u << E) - 1);
-    if (o > most) marks = (1u << E) - 1;
+    const uint32_t at = (base(j) + offset(j)) / 16;
+    const uint8_t* bytes = reinterpret_cast<const uint8_t*>(marked);
+    const uint32_t marks = E == 8 ? bytes[at] : (bytes[at >> 1] >> ((at & 1) * 4)) & 15u;
     if (marks) {
       uint32_t q[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -371,26 +394,31 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
     strike_marked(d[j], j, marked);
     if (j == 0) {
       const float m = wave_max_f(Vec<Tin>::largest(d[j]));
-      ref = finite_f(m) ? m : 0.0f;
+      ref = fabsf(m) < kHugeLogit ? m : 0.0f;
+      refc = uniform_f(ref * c);
       s = 0.0f;
     }
-    float x[E];
+    float x[E], t = 0.0f;
     Vec<Tin>::unpack(d[j], x);
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - ref) * c);
+    for (int e = 0; e < E; ++e) t += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -refc));
+    s += own(j) ? t : 0.0f;
+    asm volatile("" : "+v"(s));  // (here, not where the sum is used)
   };
   auto add_end = [&](const uint32_t* marked) {
     if (left < V && (marked[left >> 5] >> (left & 31)) & 1) end = -__builtin_inff();
-    s += __builtin_amdgcn_exp2f((end - ref) * c);
+    s += __builtin_amdgcn_exp2f(__builtin_fmaf(end, c, -refc));
   };
 
-  // the first row, and the second one's entries
-  int r = blockIdx.x, now = 0, next_bits = 1, free_bits = 2;
-  float weight = weight_of(r), weight1 = weight_of(r + gridDim.x);
+  int r = live_from(blockIdx.x);
+  if (r >= a.T) return;  // (uniform)
+  for (int i = tid; i < kBits; i += THREADS) bits[0][i] = bits[1][i] = bits[2][i] = 0;
+  __syncthreads();
+  int next = live_from(r + gridDim.x);
+  int now = 0, next_bits = 1, free_bits = 2;
   int id = -1, id1 = -1;
   float tv = 0.0f, xv = 0.0f, tv1 = 0.0f;
-  __syncthreads();
-  if (weight != 0.0f) {
+  {
     const Tin* p = row_of(r);
     if (tid < K) {
       id = id_of(r);
@@ -404,193 +432,233 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
       atomicOr(&bits[0][id >> 5], 1u << (id & 31));
     }
   }
-  if (weight1 != 0.0f && tid < K) {
-    id1 = id_of(r + gridDim.x);
-    tv1 = teacher_of(r + gridDim.x);
+  if (next < a.T && tid < K) {
+    id1 = id_of(next);
+    tv1 = teacher_of(next);
   }
   lds_barrier();
-  if (weight != 0.0f) {
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      add(j, bits[0]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    add_end(bits[0]);
+  for (int j = 0; j < NS; ++j) {
+    add(j, bits[0]);
+    __builtin_amdgcn_sched_barrier(0);
   }
+  add_end(bits[0]);
   // the row before: what is stored once its gradients are
   int last = -1, last_id = -1, par = 0;
-  float last_g = 0.0f, last_weight = 0.0f;
+  float last_g = 0.0f;
   double last_rest = 0.0;
+  auto finish_last = [&](int buffer) {
+    if (last_id >= 0) store_elem<Tin>(grad_of(last) + last_id, last_g);
+    if (tid == 0) {
+      double t = last_rest;
+      for (int i = 0; i < kWavesHere; ++i) t += sh.loss[buffer][i];
+      a.loss[last] = static_cast<float>(weight_of(last) * t);
+    }
+  };
 
   for (;; par ^= 1) {
-    const bool live = weight != 0.0f;  // (uniform)
-    const bool has = live && listed(id);
-    const bool load = weight1 != 0.0f;
-    const int next = r + gridDim.x;
-    const Tin* p = row_of(next);
+    const bool has = listed(id);
+    const bool more = next < a.T;  // (uniform)
     // the next row's listed ids, and their logits
     float xv1 = 0.0f;
-    if (load && listed(id1)) {
+    if (more && listed(id1)) {
       atomicOr(&bits[next_bits][id1 >> 5], 1u << (id1 & 31));
-      xv1 = element(p + id1);
+      xv1 = element(row_of(next) + id1);
     }
-    if (live) {
-      double sd = wave_sum(static_cast<double>(s));
-      if (!(sd > 0x1p-40 && sd < 0x1p60)) {  // (uniform over the wave)
-        // (read again: a rolled loop, no registers)
-        const Tin* own = row_of(r);
-        float m = end;
+    double sd = wave_sum(static_cast<double>(s));
+    if (sd > 0x1p-40 && sd < 0x1p60) {  // (uniform over the wave)
+      sd *= 1.0 + kLn2 * (refc - static_cast<double>(ref) * static_cast<double>(c));
+    } else {
+      // (read again: rolled loops, no registers)
+      const Tin* p = row_of(r);
+      float m = end;
 #pragma unroll 1
-        for (int j = 0; j < NS; ++j) {
-          uint4 v = vector_at(own, j);
-          strike_marked(v, j, bits[now]);
-          m = max_nan(m, Vec<Tin>::largest(v));
-        }
-        ref = wave_max_f(m);
-        const float z = ref == -__builtin_inff() ? 0.0f : ref;
-        s = __builtin_amdgcn_exp2f((end - z) * c);
+      for (int j = 0; j < NS; ++j) {
+        uint4 v = vector_at(p, j);
+        strike_marked(v, j, bits[now]);
+        m = max_nan(m, Vec<Tin>::largest(v));
+      }
+      ref = wave_max_f(m);
+      const float z = ref == -__builtin_inff() ? 0.0f : ref;
+      s = __builtin_amdgcn_exp2f((end - z) * c);
 #pragma unroll 1
-        for (int j = 0; j < NS; ++j) {
-          uint4 v = vector_at(own, j);
-          strike_marked(v, j, bits[now]);
-          float x[E];
-          Vec<Tin>::unpack(v, x);
+      for (int j = 0; j < NS; ++j) {
+        uint4 v = vector_at(p, j);
+        strike_marked(v, j, bits[now]);
+        float x[E], t = 0.0f;
+        Vec<Tin>::unpack(v, x);
 #pragma unroll
-          for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - z) * c);
-        }
-        sd = wave_sum(static_cast<double>(s));
+        for (int e = 0; e < E; ++e) t += __builtin_amdgcn_exp2f((x[e] - z) * c);
+        s += own(j) ? t : 0.0f;
       }
-      double tm = ninf, ts = 0.0, xm = ninf, xs = 0.0;
-      if (w * kWave < K) {  // (uniform)
-        tm = wave_max_d(has ? static_cast<double>(tv) : ninf);
-        xm = wave_max_d(has ? static_cast<double>(xv) : ninf);
-        __builtin_amdgcn_sched_barrier(0);
-        // (-inf adds nothing, also where a wave's entries have nothing else)
-        ts = wave_sum(!has || tv == ninf ? 0.0 : exp(a.tail ? static_cast<double>(tv) : (tv - tm) * inv));
-        __builtin_amdgcn_sched_barrier(0);
-        xs = wave_sum(!has || xv == ninf ? 0.0 : exp((xv - xm) * inv));
-      }
+      sd = wave_sum(static_cast<double>(s));
+    }
+    if (w * kWave < K) {  // (uniform)
+      const double tm = wave_max_d(has ? static_cast<double>(tv) : ninf);
+      const double xm = wave_max_d(has ? static_cast<double>(xv) : ninf);
+      __builtin_amdgcn_sched_barrier(0);
+      // (-inf adds nothing, also where a wave's entries have nothing else)
+      const double ts = wave_sum(!has || tv == ninf ? 0.0 : exp(a.tail ? static_cast<double>(tv) : (tv - tm) * inv));
+      __builtin_amdgcn_sched_barrier(0);
+      const double xs = wave_sum(!has || xv == ninf ? 0.0 : exp((xv - xm) * inv));
       __builtin_amdgcn_sched_barrier(0);
       if (lane == 0) {
-        sh.m[par][w] = ref;
-        sh.s[par][w] = sd;
         sh.tm[par][w] = tm;
         sh.ts[par][w] = ts;
         sh.xm[par][w] = xm;
         sh.xs[par][w] = xs;
       }
     }
-    __syncthreads();
-    if (last >= 0) {
-      if (last_id >= 0) store_elem<Tin>(as_global(static_cast<Tin*>(a.grad)) + last * a.gstride + last_id, last_g);
-      if (tid == 0) {
-        double t = last_rest;
-        for (int i = 0; i < kWavesHere; ++i) t += sh.loss[par ^ 1][i];
-        a.loss[last] = static_cast<float>(last_weight * t);
-      }
+    if (lane == 0) {
+      sh.m[par][w] = ref;
+      sh.s[par][w] = sd;
     }
-    float zero = 0.0f, factor = 0.0f;  // the row's reference, and its gradients' factor
-    last = -1;
-    if (live) {
-      if (has) bits[now][id >> 5] = 0;
-      // the row's numbers, in every wave: a lane a wave's part
-      const bool part = lane < kWavesHere;
-      const float mw = part ? sh.m[par][lane] : -__builtin_inff();
-      const float mf = wave_max_f(mw);
-      const double m = mf;
-      double S = part ? sh.s[par][lane] : 0.0;
-      __builtin_amdgcn_sched_barrier(0);
-      S = wave_sum(mw == mf ? S : S * exp((mw - m) * inv));
-      const double tw = part ? sh.tm[par][lane] : ninf, xw = part ? sh.xm[par][lane] : ninf;
-      const double tm = wave_max_d(tw), xmax = wave_max_d(xw), xm = xmax > m ? xmax : m;
-      double ts = part ? sh.ts[par][lane] : 0.0, xs = part ? sh.xs[par][lane] : 0.0;
+    const int after = more ? live_from(next + gridDim.x) : a.T;
+    __syncthreads();
+    if (last >= 0) finish_last(par ^ 1);
+    if (has) bits[now][id >> 5] = 0;
+    // the row's numbers, in every wave: a lane a wave's part
+    const bool part = lane < kWavesHere;
+    const float mw = part ? sh.m[par][lane] : -__builtin_inff();
+    const float mf = wave_max_f(mw);
+    const double m = mf;
+    double S = part ? sh.s[par][lane] : 0.0;
+    __builtin_amdgcn_sched_barrier(0);
+    S = wave_sum(mw == mf ? S : S * exp((mw - m) * inv));
+    __builtin_amdgcn_sched_barrier(0);
+    double tm = sh.tm[par][0], ts = sh.ts[par][0], xm = sh.xm[par][0], xs = sh.xs[par][0];
+    if (K > kWave) {  // (uniform)
+      const bool entries = lane * kWave < K;  // (waves that have some)
+      const double tw = entries ? sh.tm[par][lane] : ninf, xw = entries ? sh.xm[par][lane] : ninf;
+      tm = wave_max_d(tw);
+      xm = wave_max_d(xw);
+      ts = entries ? sh.ts[par][lane] : 0.0;
+      xs = entries ? sh.xs[par][lane] : 0.0;
       __builtin_amdgcn_sched_barrier(0);
       ts = wave_sum(a.tail || tw == tm ? ts : ts * exp((tw - tm) * inv));
       __builtin_amdgcn_sched_barrier(0);
       xs = wave_sum(xw == xm ? xs : xs * exp((xw - xm) * inv));
-      __builtin_amdgcn_sched_barrier(0);
-      const bool none = tm == ninf;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // (against the larger of the two largest)
+    double em = 1.0;
+    if (xm > m) {
+      em = m == ninf ? 0.0 : exp((m - xm) * inv);
+    } else {
+      xs = xm == ninf ? xs : xs * exp((xm - m) * inv);
+      xm = m;
+    }
+    const double total = (m == ninf ? S : S * em) + xs;
+    __builtin_amdgcn_sched_barrier(0);
+    const bool none = tm == ninf;
+    const double rest = a.tail ? fmax(0.0, 1.0 - ts) : 0.0;
+    const double mass = a.tail ? ts + rest : (none ? 0.0 : 1.0);
+    double A = 0.0;
+    if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
+    __builtin_amdgcn_sched_barrier(0);
+    const float scale = weight_of(r) / a.temp;
+    const bool huge = !(fabsf(mf) < kHugeLogit) && mf != -__builtin_inff();  // (uniform)
+    const float zero = uniform_f(huge || mf == -__builtin_inff() ? 0.0f : mf);
+    float factor = uniform_f(scale * static_cast<float>(A));
+    // the gradients out, the next row in, and its sum
+    {
+      Tin* g = grad_of(r);
+      char* gb = reinterpret_cast<char*>(g);
+      float zeroc = uniform_f(zero * c);
+      uint32_t sign = 0;
+      if constexpr (E == 8) {
+        sign = __float_as_uint(factor) & 0x80000000u;
+        sign = uniform_u(sign | (sign >> 16));
+        zeroc = uniform_f(zeroc - __builtin_amdgcn_logf(fabsf(factor)));
+      } else {
+        factor = uniform_f(factor * static_cast<float>(1.0 + kLn2 * (zeroc - static_cast<double>(zero) * static_cast<double>(c))));
+      }
+      auto gradient = [&](const uint4& v) {
+        float x[E];
+        Vec<Tin>::unpack_again(v, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -zeroc));
+        if constexpr (E == 8) {
+          return make_uint4(pack_bf16(x[0], x[1]) ^ sign, pack_bf16(x[2], x[3]) ^ sign, pack_bf16(x[4], x[5]) ^ sign,
+                            pack_bf16(x[6], x[7]) ^ sign);
+        } else {
+          return make_uint4(__float_as_uint(factor * x[0]), __float_as_uint(factor * x[1]),
+                            __float_as_uint(factor * x[2]), __float_as_uint(factor * x[3]));
+        }
+      };
+      if (left < V) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(end, c, -zeroc));
+        store_elem<Tin>(g + left, E == 8 ? __uint_as_float(__float_as_uint(e) ^ (sign & 0x80000000u)) : factor * e);
+      }
+      if (more) {
+        const Tin* p = row_of(next);
+        if (left < V) end = element(p + left);
+        const uint32_t* marked = bits[next_bits];
+#pragma unroll
+        for (int j = 0; j < NS + kBehind; ++j) {
+          if (j < NS) {
+            const uint32_t at = offset(j);
+            st_row16_nt(gb + base(j) + at, gradient(d[j]));
+            d[j] = ld_row16(reinterpret_cast<const char*>(p) + base(j) + at);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if (j >= kBehind) add(j - kBehind, marked);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        add_end(marked);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          st_row16_nt(gb + base(j) + offset(j), gradient(d[j]));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (huge) {  // (the gradients again, from differences)
+        const float f = scale * static_cast<float>(A);
+#pragma unroll 1
+        for (int j = 0; j < NS; ++j)
+          st_row16_nt(gb + base(j) + offset(j), grad_vector<Tin>(vector_at(row_of(r), j), mf, c, f));
+        if (left < V) store_elem<Tin>(g + left, f * __builtin_amdgcn_exp2f((element(row_of(r) + left) - mf) * c));
+      }
+    }
+    // the listed gradients and the loss, stored after the next barrier
+    last = r;
+    last_id = has ? id : -1;
+    if (w * kWave < K) {  // (uniform)
       const double lts = a.tail ? 0.0 : log(ts);
-      __builtin_amdgcn_sched_barrier(0);
-      const double em = m == ninf ? 0.0 : exp((m - xm) * inv);
-      const double total = (m == ninf ? S : S * em) + xs;
-      __builtin_amdgcn_sched_barrier(0);
       const double ltotal = log(total);
-      const double rest = a.tail ? fmax(0.0, 1.0 - ts) : 0.0;
-      const double mass = a.tail ? ts + rest : (none ? 0.0 : 1.0);
-      __builtin_amdgcn_sched_barrier(0);
-      double A = 0.0;
-      if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
-      __builtin_amdgcn_sched_barrier(0);
-      const float scale = weight / a.temp;
-      zero = uniform_f(mf == -__builtin_inff() ? 0.0f : mf);
-      factor = uniform_f(scale * static_cast<float>(A));
       double loss = 0.0;
-      float g = 0.0f;
-      if (w * kWave < K && has) {
+      if (has) {
         const double lp = a.tail ? static_cast<double>(tv) : (tv - tm) * inv - lts;
         const double lq = (xv - xm) * inv - ltotal;
         const double q = none ? 0.0 : exp(lp);
         if (q != 0.0) loss = q * (lp - lq);
-        g = scale * static_cast<float>(exp(lq) * mass - q);
+        last_g = scale * static_cast<float>(exp(lq) * mass - q);
       }
-      if (w * kWave < K) loss = wave_sum(loss);
+      loss = wave_sum(loss);
       if (lane == 0) sh.loss[par][w] = loss;
-      last = r;
-      last_id = has ? id : -1;
-      last_g = g;
-      last_weight = weight;
       last_rest = rest > 0.0 ? rest * (log(rest) - ((m == ninf ? ninf : (m - xm) * inv) + log(S) - ltotal)) : 0.0;
-    } else if (tid == 0) {
-      a.loss[r] = 0.0f;
+    } else if (lane == 0) {
+      sh.loss[par][w] = 0.0;
     }
-    // the gradients out, the next row in, and its sum
-    Tin* g = as_global(static_cast<Tin*>(a.grad)) + r * a.gstride;
-    const float weight2 = weight_of(next + gridDim.x);
-    id = load ? id1 : -1;
+    if (!more) break;
+    id = id1;
     tv = tv1;
     xv = xv1;
-    if (weight2 != 0.0f && tid < K) {
-      id1 = id_of(next + gridDim.x);
-      tv1 = teacher_of(next + gridDim.x);
-    }
-    if (left < V) {
-      store_elem<Tin>(g + left, factor * __builtin_amdgcn_exp2f((end - zero) * c));
-      end = load ? element(p + left) : -__builtin_inff();
-    }
-    const uint32_t* marked = bits[next_bits];
-#pragma unroll
-    for (int j = 0; j < NS + kBehind; ++j) {
-      if (j < NS) {
-        const uint32_t at = offset(j);
-        const uint4 q = grad_vector<Tin>(d[j], zero, c, factor);
-        if (at <= most) st_row16(reinterpret_cast<char*>(g) + at, q);
-        d[j] = make_uint4(Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf, Vec<Tin>::kNegInf);
-        if (load) d[j] = vector_at(p, j);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (j >= kBehind) add(j - kBehind, marked);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    add_end(marked);
-    if (next >= a.T) break;
     r = next;
-    weight = weight1;
-    weight1 = weight2;
+    next = after;
+    id1 = -1;
+    if (next < a.T && tid < K) {
+      id1 = id_of(next);
+      tv1 = teacher_of(next);
+    }
     const int t = now;
     now = next_bits;
     next_bits = free_bits;
     free_bits = t;
   }
   __syncthreads();
-  if (last >= 0) {
-    if (last_id >= 0) store_elem<Tin>(as_global(static_cast<Tin*>(a.grad)) + last * a.gstride + last_id, last_g);
-    if (tid == 0) {
-      double t = last_rest;
-      for (int i = 0; i < kWavesHere; ++i) t += sh.loss[par][i];
-      a.loss[last] = static_cast<float>(last_weight * t);
-    }
-  }
+  finish_last(par);
 }
 
 }  // namespace vo
