@@ -1,10 +1,10 @@
 // The states of a beam search's slots in their parents' order, in place: slot b W + w takes what slot
 // b W + parents[b][w] held before, up to lengths[b] positions.
 //
-// A thread owns a 16-byte column of a request's slots: it loads the column from the parent of every slot that
-// changes, then stores them all. Whatever the permutation, nothing is overwritten before it is read, with no
-// second buffer, no order of copies and no barrier, and a parent with several children is read once from
-// memory (the other loads of the column hit the cache). Slots that are their own parent are left alone.
+// A thread owns a 16-byte column of a request's slots: it loads the column from every slot that becomes a parent,
+// then stores it to their children. Whatever the permutation, nothing is overwritten before it is read, with no
+// second buffer, no order of copies and no barrier, and a parent with several children is read once. Slots that
+// are their own parent are left alone.
 #pragma once
 
 #include "common.cuh"
@@ -15,7 +15,7 @@ using namespace vs;
 
 constexpr int kMaxReorderBeams = 32;
 constexpr int kReorderThreads = 256;
-constexpr int kReorderColumns = 1024;  // a workgroup's step
+constexpr int kReorderColumns = 512;  // a workgroup's step
 constexpr int kOuterDims = 3;
 
 // One tensor: `rows` (the outer dimensions' product) runs of contiguous bytes a slot. The lengths limit the run
@@ -44,16 +44,18 @@ __device__ __forceinline__ void st_col(char* p, T v) {
   *(__attribute__((address_space(1))) T*)p = v;
 }
 
-// Columns of type T at p in every slot of the request.
-template <int WMAX, class T>
-__device__ __forceinline__ void move_column(char* p, int64_t slot_stride, const int* parents, uint32_t moved) {
-  T v[WMAX];
-#pragma unroll
-  for (int w = 0; w < WMAX; ++w)
-    if ((moved >> w) & 1) v[w] = ld_col<T>(p + parents[w] * slot_stride);
-#pragma unroll
-  for (int w = 0; w < WMAX; ++w)
-    if ((moved >> w) & 1) st_col<T>(p + w * slot_stride, v[w]);
+// A column of type T at p in every slot of the request from slot Q on: loaded from the parents, all the loads ahead of
+// the first store, then stored to each one's children (bits of slots; all of it uniform). By recursion: an array that
+// a loop fills under conditions stays one value of all its registers to the compiler, copied at each of them.
+template <int Q, int WMAX, class T>
+__device__ __forceinline__ void move_column(char* p, int64_t slot_stride, const uint32_t* children) {
+  if constexpr (Q < WMAX) {
+    T v;
+    if (children[Q]) v = ld_col<T>(p + Q * slot_stride);
+    move_column<Q + 1, WMAX, T>(p, slot_stride, children);
+#pragma unroll 1
+    for (uint32_t m = children[Q]; m; m &= m - 1) st_col<T>(p + (__ffs(m) - 1) * slot_stride, v);
+  }
 }
 
 template <int WMAX>
@@ -61,18 +63,14 @@ __global__ __launch_bounds__(kReorderThreads) void k_reorder(const StateDesc* de
                                                              const int32_t* lengths, int W) {
   const StateDesc& s = as_global(descs)[blockIdx.y];
   const int b = blockIdx.z;
-  int par[WMAX];
+  uint32_t children[WMAX] = {};
   uint32_t moved = 0;
+  for (int w = 0; w < W; ++w) {
+    const int q = as_global(parents)[b * W + w];
+    if (q == w) continue;  // (and of any other value than a slot: the slot keeps its state)
 #pragma unroll
-  for (int w = 0; w < WMAX; ++w) {
-    par[w] = w;
-    if (w < W) {
-      const int q = as_global(parents)[b * W + w];
-      if (q >= 0 && q < W && q != w) {  // (any other value: the slot keeps its state)
-        par[w] = q;
-        moved |= 1u << w;
-      }
-    }
+    for (int k = 0; k < WMAX; ++k) children[k] |= k < W && q == k ? 1u << w : 0u;
+    moved |= q >= 0 && q < W;
   }
   if (!moved) return;
   uint32_t n0 = s.size[0], n1 = s.size[1], n2 = s.size[2];
@@ -89,7 +87,9 @@ __global__ __launch_bounds__(kReorderThreads) void k_reorder(const StateDesc* de
   const uint32_t rows = n0 * n1 * n2;
   const uint32_t all = rows * cols;
   char* base = as_global(s.base) + static_cast<int64_t>(b) * W * s.slot_stride;
+#pragma unroll 1
   for (uint32_t t = blockIdx.x * kReorderColumns; t < all; t += gridDim.x * kReorderColumns) {
+#pragma unroll 1
     for (uint32_t i = t + threadIdx.x; i < min(t + kReorderColumns, all); i += kReorderThreads) {
       uint32_t row = 0, col = i;
       int64_t off = 0;
@@ -104,11 +104,13 @@ __global__ __launch_bounds__(kReorderThreads) void k_reorder(const StateDesc* de
       char* p = base + off + (static_cast<int64_t>(col) << 4);
       const int64_t left = run - (static_cast<int64_t>(col) << 4);
       if (left >= 16) {
-        move_column<WMAX, u32x4_byte_t>(p, s.slot_stride, par, moved);
+        move_column<0, WMAX, u32x4_byte_t>(p, s.slot_stride, children);
       } else {  // (a run's end)
         int k = 0;
-        for (; k + 4 <= left; k += 4) move_column<WMAX, u32_byte_t>(p + k, s.slot_stride, par, moved);
-        for (; k < left; ++k) move_column<WMAX, uint8_t>(p + k, s.slot_stride, par, moved);
+#pragma unroll 1
+        for (; k + 4 <= left; k += 4) move_column<0, WMAX, u32_byte_t>(p + k, s.slot_stride, children);
+#pragma unroll 1
+        for (; k < left; ++k) move_column<0, WMAX, uint8_t>(p + k, s.slot_stride, children);
       }
     }
   }

@@ -324,9 +324,10 @@ int vops_reorder(const vops_state* states, int32_t n_states, int64_t max_columns
   if (!states || !parents) return fail(VOPS_E_ARG, "states and parents must be set");
   if (int rc = check_current_device()) return rc;
   static_assert(sizeof(vo::StateDesc) == sizeof(vops_state), "one layout");
-  // (as many workgroups a state and request as its columns need, while the launch has about 16 thousand)
+  // (as many workgroups a state and request as its columns need, up to 65536 in all: with 16384, caches of 16 x 4
+  // beams take 434 us against 411, 16 x 8 beams' matrices 306 against 285)
   int64_t x = (max_columns + vo::kReorderColumns - 1) / vo::kReorderColumns;
-  const int64_t most = 16384 / (static_cast<int64_t>(n_states) * requests);
+  const int64_t most = 65536 / (static_cast<int64_t>(n_states) * requests);
   if (x > most) x = most < 1 ? 1 : most;
   const dim3 grid(static_cast<unsigned>(x), n_states, requests);
   const auto* d = reinterpret_cast<const vo::StateDesc*>(states);
