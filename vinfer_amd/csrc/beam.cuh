@@ -1,5 +1,5 @@
 // Beam search's selection: for each request the n best continuations over its W beams and the whole
-// vocabulary, by score[w] + x[w][v] - lse(x[w]).
+// vocabulary, by score[w] + log_softmax(x[w])[v].
 //
 // Two launches. k_beam_part: one workgroup a segment of a row, held in registers, so that a row is read
 // once. A lane's maximum gives a bound: the n-th largest of a wave's 64 lane maxima (n <= 64) is at most the
@@ -9,8 +9,8 @@
 // counting: the first n are the segment's candidates in order. The other vectors, all below the bound, add their
 // fp32 exponentials. So neither do the large terms lose precision nor does the order of the list, which varies,
 // show in the sum: the beams of a request are compared across their rows by these sums.
-// k_beam_merge: one workgroup a request. The rows' lse from the segments' sums; the n-th largest score of the
-// segments' first candidates bounds the request's n-th best; the few candidates that reach it are ranked.
+// k_beam_merge: one workgroup a request. The rows' normalisers from the segments' sums; lane maxima of the segments'
+// candidates' scores bound the request's n-th best in the same way; the few candidates that reach it are ranked.
 //
 // A row with a NaN, an infinite maximum or no finite logit has no candidates, nor have logits of -inf.
 // Rows of finished beams and of beams whose score is not finite are not read.
@@ -28,7 +28,8 @@ constexpr int kPartVecs = 512;      // a segment's vectors that hold candidates
 constexpr int kPartList = 512;      // its candidates before they are ranked
 constexpr int kMergeList = 1024;    // a request's
 constexpr int kMergeMaxThreads = 1024;
-constexpr int kAhead = 4;           // entries of a list that are loaded at once
+constexpr int kMergeHeads = 512;
+constexpr int kAhead = 4;           // entries that a thread loads at once
 constexpr double kFix = 4503599627370496.0;  // 2^52
 
 struct BeamArgs {
@@ -39,6 +40,7 @@ struct BeamArgs {
   const float* scores;      // [B, W]
   const uint8_t* finished;  // [B, W] or null
   int pad, keep;
+  uint32_t row_magic, list_magic;  // for divisions by S n and n
   u64* keys;           // [B W, S, n] the segments' candidates, descending (0: none)
   double* sums;        // [B W, S] sums of exp(x - max)
   float* maxs;         // [B W, S]
@@ -71,6 +73,26 @@ __device__ __forceinline__ uint32_t wave_nth_floor2(uint32_t k0, uint32_t k1, in
   return t;
 }
 
+// How many of the first c words are larger than k, and how many equal it; the words behind them, up to a multiple of
+// kRankStep, are 0. (kRankStep words a step: one at a time each read would wait for the last.)
+constexpr int kRankStep = 8;
+__device__ __forceinline__ uint32_t rank_of(const u64* words, uint32_t c, u64 k, uint32_t* equal) {
+  uint32_t r = 0, e = 0;
+#pragma unroll 1
+  for (uint32_t j = 0; j < c; j += kRankStep) {
+    u64 x[kRankStep];
+#pragma unroll
+    for (int i = 0; i < kRankStep; ++i) x[i] = words[j + i];
+#pragma unroll
+    for (int i = 0; i < kRankStep; ++i) {
+      r += x[i] > k;
+      e += x[i] == k;
+    }
+  }
+  *equal = e;
+  return r;
+}
+
 __device__ __forceinline__ u64 pack_key(float x, int id) {
   return (static_cast<u64>(key_of(x)) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(id));
 }
@@ -83,7 +105,7 @@ __device__ __forceinline__ u64 fix52(double e) { return static_cast<u64>(__built
 struct PartShared {
   uint4 vec[kPartVecs];  // the vectors with an element at or above the bound
   int32_t vid[kPartVecs];  // their first ids
-  u64 list[kPartList];   // those elements
+  u64 list[kPartList + kRankStep];  // those elements
   double wsum[kPartWaves];
   u64 wfix[kPartWaves];
   float wmax[kPartWaves];
@@ -268,10 +290,12 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   // ranks by counting (keys differ)
   const uint32_t n = static_cast<uint32_t>(a.n);
   u64* out = a.keys + static_cast<int64_t>(blockIdx.x) * a.n;
+  if (tid < kRankStep) sh.list[c + tid] = 0;
+  __syncthreads();
   for (uint32_t i = tid; i < c; i += kPartThreads) {
     const u64 k = sh.list[i];
-    uint32_t r = 0;
-    for (uint32_t j = 0; j < c; ++j) r += sh.list[j] > k;
+    uint32_t equal = 0;
+    const uint32_t r = rank_of(sh.list, c, k, &equal);
     if (r < n) out[r] = k;
   }
   for (uint32_t i = c + tid; i < n; i += kPartThreads) out[i] = 0;
@@ -299,9 +323,9 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
 
 // ---- the request's best ---------------------------------------------------------------------------
 struct MergeShared {
-  u64 sk[kMergeList];  // a candidate's score, ordered
+  u64 sk[kMergeList + kRankStep];  // a candidate's score, ordered
   u64 tb[kMergeList];  // what decides between equal scores
-  uint32_t head[kMergeMaxThreads];
+  uint32_t head[kMergeHeads];  // the upper words of the lists' first scores, lists that share one by their largest
   double top[kMaxBeams], logs[kMaxBeams];  // a row's largest logit, and the log of its sum against it
   double score[kMaxBeams];
   u64 rsk[kMergeMaxThreads / kWave], rtb[kMergeMaxThreads / kWave];
@@ -310,6 +334,11 @@ struct MergeShared {
   int32_t kind[kMaxBeams];  // 0: no candidates, 1: its row's, 2: finished
   uint32_t count, bound;
 };
+
+// i / d for i d < 2^32, with magic = 2^32 / d + 1 (host).
+__device__ __forceinline__ int quotient(int i, int d, uint32_t magic) {
+  return d == 1 ? i : static_cast<int>(__umulhi(static_cast<uint32_t>(i), magic));
+}
 
 __device__ __forceinline__ u64 ordered(double x) {
   const u64 b = static_cast<u64>(__double_as_longlong(x + 0.0));
@@ -334,23 +363,24 @@ __device__ __forceinline__ u64 merge_score(const MergeShared& sh, int w, bool fi
   *tb = tie_word(w, pack_key(0.0f, 0));
   return kind == 2 && first ? ordered(sh.score[w]) : 0;
 }
-__device__ __forceinline__ u64 merge_entry(const BeamArgs& a, const MergeShared& sh, const u64* keys, int l, int e, u64* tb) {
-  const int w = l / a.S;
-  return merge_score(sh, w, e == 0 && l == w * a.S, ld_global(keys + static_cast<int64_t>(l) * a.n + e), tb);
-}
-
 // The upper words of ordered fp64 scores order them too, coarsely: the first launch's bound by lane maxima again.
 __global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
   __shared__ MergeShared sh;
   const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id(), nt = blockDim.x, nw = nt / kWave;
   const int b = blockIdx.x;
   const int W = a.W, S = a.S, n = a.n;
-  // A thread a list (the first of its lists is loaded ahead of the rows' sums).
+  // A thread an entry of the segments' lists, kAhead of them at once, and the first ones ahead of the rows' sums.
   const u64* keys = a.keys + static_cast<int64_t>(b) * W * S * n;
-  const int lists = W * S;
-  u64 ahead[kAhead];
+  const int total = W * S * n;
+  auto load = [&](int i) { return i < total ? ld_global(keys + i) : 0; };
+  auto score_of = [&](int i, u64 k, u64* tb) -> u64 {
+    if (i >= total) return 0;
+    const int w = quotient(i, S * n, a.row_magic);
+    return merge_score(sh, w, i == w * S * n, k, tb);
+  };
+  u64 ahead[kAhead], sk[kAhead], tb[kAhead];
 #pragma unroll
-  for (int e = 0; e < kAhead; ++e) ahead[e] = tid < lists && e < n ? ld_global(keys + static_cast<int64_t>(tid) * n + e) : 0;
+  for (int e = 0; e < kAhead; ++e) ahead[e] = load(tid + e * nt);
   for (int w = wave; w < W; w += nw) {
     const int row = b * W + w;
     // (all loads at once; a row that was not read has left whatever the workspace held)
@@ -382,47 +412,55 @@ __global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
     sh.ch_token[tid] = -1;
   }
   if (tid == 0) sh.count = 0;
+  for (int i = tid; i < kMergeHeads; i += nt) sh.head[i] = 0;
   __syncthreads();
-  uint32_t h = 0;
-  u64 tb = 0;
-  const int own = tid / S;  // (the first list's beam)
-  if (tid < lists) h = static_cast<uint32_t>(merge_score(sh, own, tid == own * S, ahead[0], &tb) >> 32);
-  for (int l = tid + nt; l < lists; l += nt) h = max(h, static_cast<uint32_t>(merge_entry(a, sh, keys, l, 0, &tb) >> 32));
-  sh.head[tid] = h;
+  // the lists' first entries bound the n-th best: the n-th largest of 64 lane maxima over them
+  auto head = [&](int i, u64 score) {
+    const int l = quotient(i, n, a.list_magic);
+    if (score && l * n == i) atomicMax(&sh.head[l % kMergeHeads], static_cast<uint32_t>(score >> 32));
+  };
+#pragma unroll
+  for (int e = 0; e < kAhead; ++e) {
+    sk[e] = score_of(tid + e * nt, ahead[e], &tb[e]);
+    head(tid + e * nt, sk[e]);
+  }
+  for (int i = tid + kAhead * nt; i < total; i += kAhead * nt) {
+    u64 k[kAhead], t;
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) k[e] = load(i + e * nt);
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) head(i + e * nt, score_of(i + e * nt, k[e], &t));
+  }
   __syncthreads();
   if (wave == 0) {
-    for (int i = lane + kWave; i < nt; i += kWave) h = max(h, sh.head[i]);
-    const uint32_t t = wave_nth_floor<8>(h, n);
-    if (lane == 0) sh.bound = max(t, 1u);
+    uint32_t h = 0;
+#pragma unroll
+    for (int i = 0; i < kMergeHeads / kWave; ++i) h = max(h, sh.head[lane + i * kWave]);
+    h = wave_nth_floor<8>(h, n);
+    if (lane == 0) sh.bound = max(h, 1u);
   }
   __syncthreads();
   const uint32_t bound = sh.bound;
-  // (a list's entries descend: the first one below the bound ends it)
-  auto take = [&](u64 sk, u64 t) {
-    if (static_cast<uint32_t>(sk >> 32) < bound) return false;
+  auto take = [&](u64 score, u64 t) {
+    if (static_cast<uint32_t>(score >> 32) < bound) return;
     const uint32_t at = atomicAdd(&sh.count, 1u);
     if (at < kMergeList) {
-      sh.sk[at] = sk;
+      sh.sk[at] = score;
       sh.tb[at] = t;
     }
-    return true;
   };
-  bool more = tid < lists;
 #pragma unroll
-  for (int e = 0; e < kAhead; ++e)
-    if (more && e < n) {
-      const u64 sk = merge_score(sh, own, e == 0 && tid == own * S, ahead[e], &tb);
-      more = take(sk, tb);
+  for (int e = 0; e < kAhead; ++e) take(sk[e], tb[e]);
+  for (int i = tid + kAhead * nt; i < total; i += kAhead * nt) {
+    u64 k[kAhead], t;
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) k[e] = load(i + e * nt);
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const u64 score = score_of(i + e * nt, k[e], &t);
+      take(score, t);
     }
-  for (int e = kAhead; more && e < n; ++e) {
-    const u64 sk = merge_entry(a, sh, keys, tid, e, &tb);
-    more = take(sk, tb);
   }
-  for (int l = tid + nt; l < lists; l += nt)
-    for (int e = 0; e < n; ++e) {
-      const u64 sk = merge_entry(a, sh, keys, l, e, &tb);
-      if (!take(sk, tb)) break;
-    }
   __syncthreads();
   const uint32_t c = sh.count;
   auto choose = [&](uint32_t r, u64 sk, u64 t) {
@@ -431,24 +469,40 @@ __global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
     sh.ch_beam[r] = w;
     sh.ch_token[r] = sh.kind[w] == 2 ? a.pad : static_cast<int>(0xFFFFFu - static_cast<uint32_t>(t & 0xFFFFFull));
   };
-  if (c <= kMergeList) {
+  if (c <= kWave) {
+    // (the first wave alone, a candidate a lane)
+    if (wave != 0) return;
+    const u64 score = lane < static_cast<int>(c) ? sh.sk[lane] : 0;
+    const u64 t = lane < static_cast<int>(c) ? sh.tb[lane] : 0;
+    uint32_t r = 0;
+    for (uint32_t j = 0; j < c; ++j) {
+      const u64 other = readlane64(score, j);
+      r += other > score || (other == score && readlane64(t, j) > t);
+    }
+    if (score && r < static_cast<uint32_t>(n)) choose(r, score, t);
+    wave_lds_sync();
+  } else if (c <= kMergeList) {
+    if (tid < kRankStep) sh.sk[c + tid] = 0;  // (below every score)
+    __syncthreads();
     for (uint32_t i = tid; i < c; i += nt) {
-      const u64 sk = sh.sk[i], t = sh.tb[i];
-      uint32_t r = 0;
-      for (uint32_t j = 0; j < c; ++j) r += sh.sk[j] > sk || (sh.sk[j] == sk && sh.tb[j] > t);
-      if (r < static_cast<uint32_t>(n)) choose(r, sk, t);
+      const u64 score = sh.sk[i], t = sh.tb[i];
+      uint32_t equal = 0, r = rank_of(sh.sk, c, score, &equal);
+      if (equal > 1)
+        for (uint32_t j = 0; j < c; ++j) r += sh.sk[j] == score && sh.tb[j] > t;
+      if (r < static_cast<uint32_t>(n)) choose(r, score, t);
     }
   } else {
     // (thousands of equal scores: the best one after the last, n times)
     u64 psk = ~0ull, ptb = ~0ull;
     for (int r = 0; r < n; ++r) {
       u64 bsk = 0, btb = 0;
-      for (int i = tid; i < lists * n; i += nt) {
-        const u64 sk = merge_entry(a, sh, keys, i / n, i % n, &tb);
-        if (!sk || !(sk < psk || (sk == psk && tb < ptb))) continue;
-        if (sk > bsk || (sk == bsk && tb > btb)) {
-          bsk = sk;
-          btb = tb;
+      for (int i = tid; i < total; i += nt) {
+        u64 t;
+        const u64 score = score_of(i, load(i), &t);
+        if (!score || !(score < psk || (score == psk && t < ptb))) continue;
+        if (score > bsk || (score == bsk && t > btb)) {
+          bsk = score;
+          btb = t;
         }
       }
       u64 m = wave_max_u64(bsk);
@@ -474,42 +528,38 @@ __global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
       __syncthreads();
     }
   }
-  __syncthreads();
-  if (wave != 0) return;
+  if (c > kWave) {
+    __syncthreads();
+    if (wave != 0) return;
+  }
   // A lane a choice. keep_slots (n = W): the first child of each parent takes the parent's place, the others the
   // free places in their order, the empty ones behind them.
   const bool mine = lane < n;
-  const int beam = mine ? sh.ch_beam[lane] : -1;
+  const int beam = mine ? lds_peek(&sh.ch_beam[lane]) : -1;
   int place = lane;
   if (a.keep) {
     u64 taken = 0;
     bool stays = false;
     for (int i = 0; i < n; ++i) {
-      const int bi = sh.ch_beam[i];
+      const int bi = __builtin_amdgcn_readlane(beam, i);
       if (bi >= 0 && !((taken >> bi) & 1)) {
         taken |= 1ull << bi;
         stays = stays || i == lane;
       }
     }
-    const u64 others = __ballot(mine && !stays);
-    if (stays) {
-      place = beam;
-    } else {
-      int skip = static_cast<int>(lanes_below(others));
-      for (int i = 0; i < n; ++i) {
-        if ((taken >> i) & 1) continue;
-        if (skip-- == 0) {
-          place = i;
-          break;
-        }
-      }
+    const uint32_t skip = lanes_below(__ballot(mine && !stays));
+    uint32_t free = 0;
+    for (int i = 0; i < n; ++i) {
+      if ((taken >> i) & 1) continue;
+      if (free++ == skip) place = i;
     }
+    if (stays) place = beam;
   }
   if (mine) {
     const int64_t at = static_cast<int64_t>(b) * n + place;
-    a.out_scores[at] = sh.ch_score[lane];
+    a.out_scores[at] = lds_peek(&sh.ch_score[lane]);
     a.out_beams[at] = beam;
-    a.out_tokens[at] = sh.ch_token[lane];
+    a.out_tokens[at] = lds_peek(&sh.ch_token[lane]);
   }
 }
 

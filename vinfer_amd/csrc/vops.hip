@@ -272,6 +272,8 @@ int vops_beam_select(const vops_beam_args* a, void* stream) {
   k.finished = a->finished;
   k.pad = a->pad_id;
   k.keep = (a->flags & VOPS_BEAM_KEEP_SLOTS) != 0;
+  k.row_magic = static_cast<uint32_t>((uint64_t(1) << 32) / (static_cast<uint64_t>(L.S) * a->n)) + 1u;
+  k.list_magic = static_cast<uint32_t>((uint64_t(1) << 32) / static_cast<uint64_t>(a->n)) + 1u;
   k.keys = reinterpret_cast<vs::u64*>(ws + L.keys);
   k.sums = reinterpret_cast<double*>(ws + L.sums);
   k.maxs = reinterpret_cast<float*>(ws + L.maxs);
@@ -290,8 +292,9 @@ int vops_beam_select(const vops_beam_args* a, void* stream) {
     else hipLaunchKernelGGL((vo::k_beam_part<float, N, false>), grid, block, 0, st, k);
   });
   if (int rc = launched("launch k_beam_part")) return rc;
-  // (a wave a beam, 4 to 16 waves)
-  const int threads = a->beams <= 4 ? 256 : a->beams <= 8 ? 512 : 1024;
+  // (4 entries a thread, if 16 waves have as many)
+  const int64_t entries = static_cast<int64_t>(a->beams) * L.S * a->n;
+  const int threads = entries <= 1024 ? 256 : entries <= 2048 ? 512 : 1024;
   hipLaunchKernelGGL(vo::k_beam_merge, dim3(a->requests), dim3(threads), 0, st, k);
   return launched("launch k_beam_merge");
 }
