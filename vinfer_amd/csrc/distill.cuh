@@ -131,8 +131,91 @@ __device__ __forceinline__ double logit(const Tin* p) {
   else return ld_global(p);
 }
 
-// A wave's row: the loss, m, A and the listed gradients, from the segments' sums.
-template <class Tin>
+// A wave's row from the segments' sums: m and A (in every lane), the loss (lane 0) and the listed entries' gradients
+// (to `listed`, K of them). ONE: at most an entry a lane, loaded once and ahead of the rest.
+struct RowNumbers {
+  float m, A;
+  double loss;
+};
+template <class Tin, bool ONE>
+__device__ __forceinline__ RowNumbers row_numbers(const DistillArgs& a, int row, float* listed) {
+  const int lane = lane_id();
+  const double inv = 1.0 / static_cast<double>(a.temp);
+  const double ninf = -static_cast<double>(__builtin_inff());
+  const float* ms = as_global(a.maxs) + static_cast<int64_t>(row) * a.S;
+  const double* ss = as_global(a.sums) + static_cast<int64_t>(row) * a.S;
+  const int32_t* ids = as_global(a.ids) + static_cast<int64_t>(row) * a.K;
+  const float* teacher = as_global(a.teacher) + static_cast<int64_t>(row) * a.K;
+  const Tin* x = as_global(static_cast<const Tin*>(a.x)) + row * a.stride;
+  // f(k, is there an entry, the teacher's value, the logit)
+  int id = -1;
+  double tv = 0.0, xv = 0.0;
+  auto load = [&](int k) {
+    id = k < a.K ? ld_global(ids + k) : -1;
+    tv = k < a.K ? ld_global(teacher + k) : 0.0f;
+    const bool has = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.V);
+    xv = has ? logit(x + id) : 0.0;
+    return has;
+  };
+  const float m1 = lane < a.S ? ms[lane] : -__builtin_inff();  // (at most 64 segments)
+  const double s1 = lane < a.S ? ss[lane] : 0.0;
+  bool has1 = false;
+  if constexpr (ONE) has1 = load(lane);
+  auto each = [&](auto f) {
+    if constexpr (ONE) {
+      f(lane, has1);
+    } else {
+      for (int k = lane; k < a.K; k += kWave) f(k, load(k));
+    }
+  };
+  const float mf = wave_max_f(m1);
+  const double m = mf;
+  const double S = wave_sum(m1 == mf ? s1 : s1 * exp((m1 - m) * inv));
+  // the teacher's normaliser and the listed logits' largest
+  double tm = ninf, xm = m;
+  each([&](int, bool has) {
+    if (!has) return;
+    tm = tv > tm ? tv : tm;
+    xm = xv > xm ? xv : xm;
+  });
+  tm = wave_max_d(tm);
+  xm = wave_max_d(xm);
+  double ts = 0.0, xs = 0.0;
+  each([&](int, bool has) {
+    if (!has) return;
+    ts += exp(a.tail ? tv : (tv - tm) * inv);
+    xs += exp((xv - xm) * inv);
+  });
+  ts = wave_sum(ts);
+  xs = wave_sum(xs);
+  const bool none = tm == ninf;  // (no entry, or all of probability 0)
+  // (differences of logits before anything else: beside logits of 1e38 an lse would lose log S)
+  const double lts = a.tail ? 0.0 : log(ts);
+  const double em = m == ninf ? 0.0 : exp((m - xm) * inv);
+  const double total = (m == ninf ? S : S * em) + xs;
+  const double ltotal = log(total);
+  const double rest = a.tail ? fmax(0.0, 1.0 - ts) : 0.0;
+  const double mass = a.tail ? ts + rest : (none ? 0.0 : 1.0);
+  double loss = 0.0;
+  each([&](int k, bool has) {
+    float g = 0.0f;
+    if (has) {
+      const double lp = a.tail ? tv : (tv - tm) * inv - lts;
+      const double lq = (xv - xm) * inv - ltotal;
+      const double p = none ? 0.0 : exp(lp);
+      if (p != 0.0) loss += p * (lp - lq);
+      g = static_cast<float>(exp(lq) * mass - p);
+    }
+    if (k < a.K) listed[k] = g;
+  });
+  loss = wave_sum(loss);
+  if (rest > 0.0) loss += rest * (log(rest) - ((m == ninf ? ninf : (m - xm) * inv) + log(S) - ltotal));
+  double A = 0.0;
+  if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
+  return RowNumbers{mf, static_cast<float>(A), loss};
+}
+
+template <class Tin, bool ONE>
 __global__ __launch_bounds__(kDistillThreads) void k_distill_row(DistillArgs a) {
   const int row = blockIdx.x * kDistillWaves + threadIdx.x / kWave;
   if (row >= a.T) return;
@@ -148,66 +231,11 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_row(DistillArgs a) 
     }
     return;
   }
-  const double inv = 1.0 / static_cast<double>(a.temp);
-  const double ninf = -static_cast<double>(__builtin_inff());
-  const float* ms = as_global(a.maxs) + static_cast<int64_t>(row) * a.S;
-  const double* ss = as_global(a.sums) + static_cast<int64_t>(row) * a.S;
-  const int32_t* ids = as_global(a.ids) + static_cast<int64_t>(row) * a.K;
-  const float* teacher = as_global(a.teacher) + static_cast<int64_t>(row) * a.K;
-  const Tin* x = as_global(static_cast<const Tin*>(a.x)) + row * a.stride;
-  float mf = -__builtin_inff();
-  for (int s = lane; s < a.S; s += kWave) mf = fmaxf(mf, ms[s]);
-  mf = wave_max_f(mf);
-  const double m = mf;
-  double S = 0.0;
-  for (int s = lane; s < a.S; s += kWave) S += ms[s] == mf ? ss[s] : ss[s] * exp((ms[s] - m) * inv);
-  S = wave_sum(S);
-  // the teacher's normaliser and the listed logits' largest
-  double tm = ninf, xm = m;
-  for (int k = lane; k < a.K; k += kWave) {
-    if (static_cast<uint32_t>(ids[k]) >= static_cast<uint32_t>(a.V)) continue;
-    const double v = teacher[k], z = logit(x + ids[k]);
-    tm = v > tm ? v : tm;
-    xm = z > xm ? z : xm;
-  }
-  tm = wave_max_d(tm);
-  xm = wave_max_d(xm);
-  double ts = 0.0, xs = 0.0;
-  for (int k = lane; k < a.K; k += kWave) {
-    if (static_cast<uint32_t>(ids[k]) >= static_cast<uint32_t>(a.V)) continue;
-    ts += exp(a.tail ? static_cast<double>(teacher[k]) : (teacher[k] - tm) * inv);
-    xs += exp((logit(x + ids[k]) - xm) * inv);
-  }
-  ts = wave_sum(ts);
-  xs = wave_sum(xs);
-  const bool none = tm == ninf;  // (no entry, or all of probability 0)
-  // (differences of logits before anything else: beside logits of 1e38 an lse would lose log S)
-  const double lts = a.tail ? 0.0 : log(ts);
-  const double em = m == ninf ? 0.0 : exp((m - xm) * inv);
-  const double total = (m == ninf ? S : S * em) + xs;
-  const double ltotal = log(total);
-  const double rest = a.tail ? fmax(0.0, 1.0 - ts) : 0.0;
-  const double mass = a.tail ? ts + rest : (none ? 0.0 : 1.0);
-  double loss = 0.0;
-  for (int k = lane; k < a.K; k += kWave) {
-    float g = 0.0f;
-    if (static_cast<uint32_t>(ids[k]) < static_cast<uint32_t>(a.V)) {
-      const double lp = a.tail ? static_cast<double>(teacher[k]) : (teacher[k] - tm) * inv - lts;
-      const double lq = (logit(x + ids[k]) - xm) * inv - ltotal;
-      const double p = none ? 0.0 : exp(lp);
-      if (p != 0.0) loss += p * (lp - lq);
-      g = static_cast<float>(exp(lq) * mass - p);
-    }
-    st[2 + k] = g;
-  }
-  loss = wave_sum(loss);
+  const RowNumbers n = row_numbers<Tin, ONE>(a, row, st + 2);
   if (lane == 0) {
-    if (rest > 0.0) loss += rest * (log(rest) - ((m == ninf ? ninf : (m - xm) * inv) + log(S) - ltotal));
-    double A = 0.0;
-    if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
-    a.loss[row] = static_cast<float>(weight * loss);
-    st[0] = mf;
-    st[1] = static_cast<float>(A);
+    a.loss[row] = static_cast<float>(weight * n.loss);
+    st[0] = n.m;
+    st[1] = n.A;
   }
 }
 
@@ -267,10 +295,13 @@ __device__ __forceinline__ void store_vector(Tin* row, int V, int i, const uint4
   }
 }
 
-template <class Tin, int NV>
+// ROW: the row's numbers are worked out here, by each segment's first wave while the logits are on their way (at most
+// an entry a lane), and the first segment writes the loss: a launch less, for few rows.
+template <class Tin, int NV, bool ROW>
 __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a) {
   constexpr int E = Vec<Tin>::kElems;
   constexpr int kElems = NV * kDistillThreads * E;
+  __shared__ float listed[kWave], numbers[2];
   const int row = blockIdx.x / a.S, seg = blockIdx.x % a.S;
   const int first = seg * kElems;
   const float weight = a.weights ? a.weights[row] : 1.0f;
@@ -279,14 +310,32 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
   if (weight == 0.0f) {  // (uniform)
 #pragma unroll
     for (int j = 0; j < NV; ++j) store_vector<Tin>(g, a.V, at + j * kDistillThreads * E, make_uint4(0, 0, 0, 0));
+    if (ROW && seg == 0 && threadIdx.x == 0) a.loss[row] = 0.0f;
     return;
   }
   uint4 d[NV];
   load_segment<Tin, NV, kDistillThreads>(as_global(static_cast<const Tin*>(a.x)) + row * a.stride, a.V, first, d);
   const float* st = as_global(a.states) + static_cast<int64_t>(row) * (2 + a.K);
-  const float ref = st[0] == -__builtin_inff() ? 0.0f : st[0];
+  float m, A;
+  if constexpr (ROW) {
+    if (threadIdx.x < kWave) {
+      const RowNumbers n = row_numbers<Tin, true>(a, row, listed);
+      if (threadIdx.x == 0) {
+        numbers[0] = n.m;
+        numbers[1] = n.A;
+        if (seg == 0) a.loss[row] = static_cast<float>(weight * n.loss);
+      }
+    }
+    lds_barrier();
+    m = numbers[0];
+    A = numbers[1];
+  } else {
+    m = st[0];
+    A = st[1];
+  }
+  const float ref = m == -__builtin_inff() ? 0.0f : m;
   const float scale = weight / a.temp;
-  const float factor = scale * st[1];
+  const float factor = scale * A;
   const float c = kLog2e / a.temp;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -295,8 +344,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
   const int32_t* ids = a.ids + static_cast<int64_t>(row) * a.K;
   for (int k = threadIdx.x; k < a.K; k += kDistillThreads) {
     const int id = ld_global(ids + k);
-    if (id >= first && id < a.V && id - first < kElems)
-      store_elem<Tin>(g + id, scale * st[2 + k]);
+    if (id >= first && id < a.V && id - first < kElems) store_elem<Tin>(g + id, scale * (ROW ? listed[k] : st[2 + k]));
   }
 }
 

@@ -377,14 +377,23 @@ int vops_distill(const vops_distill_args* a, void* stream) {
     else hipLaunchKernelGGL((vo::k_distill_part<float, N>), grid, block, 0, st, k);
   });
   if (int rc = launched("launch k_distill_part")) return rc;
-  if (bf) hipLaunchKernelGGL(vo::k_distill_row<uint16_t>, rows, block, 0, st, k);
-  else hipLaunchKernelGGL(vo::k_distill_row<float>, rows, block, 0, st, k);
-  if (int rc = launched("launch k_distill_row")) return rc;
+  const bool one = a->entries <= vs::kWave;
+  // (few rows: their numbers in the gradient's launch; 16 rows of 151936 XX us against YY)
+  const bool in_grad = a->out_grad && !a->states && one && a->rows < kHeldRows;
+  if (!in_grad) {
+    if (bf && one) hipLaunchKernelGGL((vo::k_distill_row<uint16_t, true>), rows, block, 0, st, k);
+    else if (bf) hipLaunchKernelGGL((vo::k_distill_row<uint16_t, false>), rows, block, 0, st, k);
+    else if (one) hipLaunchKernelGGL((vo::k_distill_row<float, true>), rows, block, 0, st, k);
+    else hipLaunchKernelGGL((vo::k_distill_row<float, false>), rows, block, 0, st, k);
+    if (int rc = launched("launch k_distill_row")) return rc;
+  }
   if (!a->out_grad) return VOPS_OK;
   with_nv(L.nv, [&](auto nv) {
     constexpr int N = decltype(nv)::value;
-    if (bf) hipLaunchKernelGGL((vo::k_distill_grad<uint16_t, N>), grid, block, 0, st, k);
-    else hipLaunchKernelGGL((vo::k_distill_grad<float, N>), grid, block, 0, st, k);
+    if (bf && in_grad) hipLaunchKernelGGL((vo::k_distill_grad<uint16_t, N, true>), grid, block, 0, st, k);
+    else if (bf) hipLaunchKernelGGL((vo::k_distill_grad<uint16_t, N, false>), grid, block, 0, st, k);
+    else if (in_grad) hipLaunchKernelGGL((vo::k_distill_grad<float, N, true>), grid, block, 0, st, k);
+    else hipLaunchKernelGGL((vo::k_distill_grad<float, N, false>), grid, block, 0, st, k);
   });
   return launched("launch k_distill_grad");
 }
@@ -404,8 +413,8 @@ int vops_distill_grad(const vops_distill_args* a, void* stream) {
   const dim3 grid(static_cast<unsigned>(parts)), block(vo::kDistillThreads);
   with_nv(L.nv, [&](auto nv) {
     constexpr int N = decltype(nv)::value;
-    if (a->dtype == VOPS_BF16) hipLaunchKernelGGL((vo::k_distill_grad<uint16_t, N>), grid, block, 0, st, k);
-    else hipLaunchKernelGGL((vo::k_distill_grad<float, N>), grid, block, 0, st, k);
+    if (a->dtype == VOPS_BF16) hipLaunchKernelGGL((vo::k_distill_grad<uint16_t, N, false>), grid, block, 0, st, k);
+    else hipLaunchKernelGGL((vo::k_distill_grad<float, N, false>), grid, block, 0, st, k);
   });
   return launched("launch k_distill_grad");
 }

@@ -21,6 +21,7 @@ class HipDistill:
     def __init__(self, ctx: BackendContext) -> None:
         self.ctx = ctx
         self._lib = _vops.load()
+        self._need: dict[tuple, int] = {}  # workspace bytes by sizes
 
     def _args(self, student, ids, weights, temperature, tail):
         if student.device.type != "cuda":
@@ -54,9 +55,12 @@ class HipDistill:
         if states:
             out = torch.empty(a.rows, 2 + a.entries, dtype=torch.float32, device=dev)
             a.states = out.data_ptr()
-        need = self._lib.vops_distill_workspace_bytes(a.dtype, a.rows, a.vocab, a.entries)
-        ws = torch.empty(need + 256, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = (ws.data_ptr() + 255) & ~255, need
+        sizes = a.dtype, a.rows, a.vocab, a.entries
+        need = self._need.get(sizes)
+        if need is None:
+            need = self._need[sizes] = self._lib.vops_distill_workspace_bytes(*sizes)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)  # (torch aligns to 512 bytes)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
         _vops.call(self._lib.vops_distill, dev, ctypes.byref(a))
         del keep
         return loss, out

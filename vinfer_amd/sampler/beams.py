@@ -212,6 +212,7 @@ class HipBeams:
 
     def __init__(self) -> None:
         self._lib = _vops.load()
+        self._need: dict[tuple, int] = {}  # workspace bytes by sizes
 
     def select(self, logits, scores, n, finished=None, pad_id=0, keep_slots=False):
         check_select(logits, scores, n, finished, pad_id, keep_slots)
@@ -234,9 +235,12 @@ class HipBeams:
         a.n, a.pad_id = n, pad_id
         a.flags = _vops.VOPS_BEAM_KEEP_SLOTS if keep_slots else 0
         a.out_scores, a.out_beams, a.out_tokens = out_scores.data_ptr(), out_beams.data_ptr(), out_tokens.data_ptr()
-        need = self._lib.vops_beam_workspace_bytes(a.dtype, B, W, V, n)
-        ws = torch.empty(need + 256, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = (ws.data_ptr() + 255) & ~255, need
+        sizes = a.dtype, B, W, V, n
+        need = self._need.get(sizes)
+        if need is None:
+            need = self._need[sizes] = self._lib.vops_beam_workspace_bytes(*sizes)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)  # (torch aligns to 512 bytes)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
         _vops.call(self._lib.vops_beam_select, dev, ctypes.byref(a))
         return out_scores, out_beams, out_tokens
 
