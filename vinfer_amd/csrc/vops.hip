@@ -143,10 +143,15 @@ template <int N>
 struct Nv {
   static constexpr int value = N;
 };
-// Loss and gradient of at least this many rows, of at least that many ids, are taken with whole rows held.
-constexpr int kHeldRows = 192;
+// Loss and gradient with whole rows held: from this many rows, or where a row is short enough for one workgroup to be
+// no slower than the segments' launches. Measured, held against segments (us): bf16 rows of 151936, 32 of them
+// 22.7 / 17.4, 64 23.0 / 23.2, 128 28.7 / 30.2, 512 72.8 / 98.2; of 32000, 32 10.1 / 16.2, 1024 34.8 / 46.0; fp32 rows
+// of 50257, 32 12.7 / 14.5, 256 25.7 / 30.9.
+constexpr int kHeldRows = 64;
+constexpr int kHeldVectors = 8192;  // (16-byte vectors of a row)
 constexpr int kHeldVocab = 4096;
 constexpr int kHeldEntries = 512;  // (a thread each)
+constexpr int kFewRows = 192;      // (their numbers are worked out by each segment of the gradient: 16 rows of 151936 15.4 -> 11.2 us)
 
 template <class F>
 void with_nv(int nv, F f) {
@@ -367,7 +372,7 @@ int vops_distill(const vops_distill_args* a, void* stream) {
   const dim3 grid(static_cast<unsigned>(parts)), block(vo::kDistillThreads);
   const dim3 rows((a->rows + vo::kDistillWaves - 1) / vo::kDistillWaves);
   const bool bf = a->dtype == VOPS_BF16;
-  if (a->out_grad && !a->states && a->rows >= kHeldRows && a->vocab >= kHeldVocab &&
+  if (a->out_grad && !a->states && (a->rows >= kHeldRows || a->vocab <= kHeldVectors * kVecElems[a->dtype]) && a->vocab >= kHeldVocab &&
       a->entries <= kHeldEntries &&
       (bf ? launch_held<uint16_t>(k, st) : launch_held<float>(k, st)))
     return launched("launch k_distill_held");
@@ -378,8 +383,7 @@ int vops_distill(const vops_distill_args* a, void* stream) {
   });
   if (int rc = launched("launch k_distill_part")) return rc;
   const bool one = a->entries <= vs::kWave;
-  // (few rows: their numbers in the gradient's launch; 16 rows of 151936 XX us against YY)
-  const bool in_grad = a->out_grad && !a->states && one && a->rows < kHeldRows;
+  const bool in_grad = a->out_grad && !a->states && one && a->rows < kFewRows;
   if (!in_grad) {
     if (bf && one) hipLaunchKernelGGL((vo::k_distill_row<uint16_t, true>), rows, block, 0, st, k);
     else if (bf) hipLaunchKernelGGL((vo::k_distill_row<uint16_t, false>), rows, block, 0, st, k);
