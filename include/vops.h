@@ -58,7 +58,7 @@ int vops_query(int device, char* why, size_t n);
 typedef struct vops_beam_args {
   const void* logits; /* `dtype`; row (b, w) at element b * request_stride + w * beam_stride */
   int32_t dtype;
-  int32_t requests; /* >= 0 */
+  int32_t requests; /* 0 .. 65535 */
   int32_t beams;    /* 1 .. VOPS_MAX_BEAMS */
   int32_t vocab;    /* 1 .. VOPS_MAX_VOCAB */
   int64_t request_stride; /* elements, >= 0 (0: one row for all) */

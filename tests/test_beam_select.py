@@ -220,6 +220,7 @@ BAD = [
     (dict(logits=torch.zeros(2, 3, 8).transpose(1, 2)), "logits must be"),
     (dict(logits=torch.zeros(2, 3, 8, dtype=torch.float16)), "bf16 and fp32"),
     (dict(logits=torch.zeros(2, 65, 8)), "beams must be"),
+    (dict(logits=torch.zeros(1, 3, 8).expand(65536, 3, 8)), "65535 requests"),
     (dict(logits=torch.zeros(2, 3, 0)), "vocab must be"),
     (dict(n=0), "n must be"),
     (dict(n=65), "n must be"),
@@ -252,6 +253,7 @@ def test_no_requests(device):
     [
         ({"dtype": 5}, 2, b"dtype"),
         ({"requests": -1}, 1, b"requests"),
+        ({"requests": 65536}, 1, b"requests"),
         ({"beams": 65}, 1, b"beams"),
         ({"vocab": 600000}, 1, b"vocab"),
         ({"n": 0}, 1, b"n in"),

@@ -187,11 +187,13 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   constexpr int E = Vec<Tin>::kElems;
   __shared__ PartShared sh;
   const int tid = threadIdx.x, w = tid / kWave;
-  const int row = blockIdx.x / a.S, seg = blockIdx.x % a.S;
+  // (a grid of segments, beams and requests)
+  const int seg = blockIdx.x, row = blockIdx.z * a.W + blockIdx.y;
+  const int64_t part = static_cast<int64_t>(row) * a.S + seg;
   const float score = a.scores[row];
   const int finished = a.finished ? a.finished[row] : 0;  // (both loads at once)
   if (!finite_f(score) || finished) return;  // (uniform)
-  const Tin* p = as_global(static_cast<const Tin*>(a.logits)) + (row / a.W) * a.rstride + (row % a.W) * a.bstride;
+  const Tin* p = as_global(static_cast<const Tin*>(a.logits)) + blockIdx.z * a.rstride + blockIdx.y * a.bstride;
   const int first = seg * NV * kPartThreads * E;
   uint4 d[NV];
   load_segment<Tin, NV, kPartThreads>(p, a.V, first, d);
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   }
   // ranks by counting (keys differ)
   const uint32_t n = static_cast<uint32_t>(a.n);
-  u64* out = a.keys + static_cast<int64_t>(blockIdx.x) * a.n;
+  u64* out = a.keys + part * a.n;
   if (tid < kRankStep) sh.list[c + tid] = 0;
   __syncthreads();
   for (uint32_t i = tid; i < c; i += kPartThreads) {
@@ -316,8 +318,8 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
     }
     // (x kLog2e - refl = (x - ref) kLog2e + (ref kLog2e - refl): the latter, refl's rounding, is exact in fp64)
     if (!crowded) t *= exp((refl - static_cast<double>(ref) * static_cast<double>(kLog2e)) * 0.6931471805599453);
-    a.sums[blockIdx.x] = t + static_cast<double>(f) * (1.0 / kFix);
-    a.maxs[blockIdx.x] = M;
+    a.sums[part] = t + static_cast<double>(f) * (1.0 / kFix);
+    a.maxs[part] = M;
   }
 }
 

@@ -129,7 +129,7 @@ DistillLayout distill_layout(int dtype, int64_t T, int64_t V, int64_t K) {
 }
 
 bool beam_sizes_ok(int32_t dtype, int32_t B, int32_t W, int32_t V, int32_t n) {
-  return (dtype == VOPS_BF16 || dtype == VOPS_F32) && B >= 0 && W >= 1 && W <= VOPS_MAX_BEAMS && V >= 1 &&
+  return (dtype == VOPS_BF16 || dtype == VOPS_F32) && B >= 0 && B <= 65535 && W >= 1 && W <= VOPS_MAX_BEAMS && V >= 1 &&
          V <= VOPS_MAX_VOCAB && n >= 1 && n <= VOPS_MAX_CONTINUATIONS;
 }
 
@@ -247,7 +247,7 @@ int vops_beam_select(const vops_beam_args* a, void* stream) {
   if (a->dtype != VOPS_BF16 && a->dtype != VOPS_F32)
     return fail(VOPS_E_DTYPE, "unsupported logits dtype %d (VOPS_BF16=0, VOPS_F32=1)", a->dtype);
   if (!beam_sizes_ok(a->dtype, a->requests, a->beams, a->vocab, a->n))
-    return fail(VOPS_E_ARG, "requests must be >= 0, beams in [1, %d], vocab in [1, %d], n in [1, %d], got %d, %d, %d, %d",
+    return fail(VOPS_E_ARG, "requests must be in [0, 65535], beams in [1, %d], vocab in [1, %d], n in [1, %d], got %d, %d, %d, %d",
                 VOPS_MAX_BEAMS, VOPS_MAX_VOCAB, VOPS_MAX_CONTINUATIONS, a->requests, a->beams, a->vocab, a->n);
   if (a->flags & ~VOPS_BEAM_KEEP_SLOTS) return fail(VOPS_E_ARG, "flags must be 0 or VOPS_BEAM_KEEP_SLOTS, got %u", a->flags);
   if ((a->flags & VOPS_BEAM_KEEP_SLOTS) && a->n != a->beams)
@@ -260,8 +260,6 @@ int vops_beam_select(const vops_beam_args* a, void* stream) {
     return fail(VOPS_E_ARG, "logits must be aligned to their elements");
   const BeamLayout L = beam_layout(a->dtype, a->requests, a->beams, a->vocab, a->n);
   if (int rc = check_workspace(a->workspace, a->workspace_bytes, L.total)) return rc;
-  const int64_t parts = static_cast<int64_t>(a->requests) * a->beams * L.S;
-  if (int rc = grid_ok(parts)) return rc;
   if (int rc = check_current_device()) return rc;
   char* ws = static_cast<char*>(a->workspace);
   vo::BeamArgs k;
@@ -286,7 +284,7 @@ int vops_beam_select(const vops_beam_args* a, void* stream) {
   k.out_beams = a->out_beams;
   k.out_tokens = a->out_tokens;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(parts));
+  const dim3 grid(L.S, a->beams, a->requests);
   with_nv(L.nv, [&](auto nv) {
     constexpr int N = decltype(nv)::value;
     const bool bf = a->dtype == VOPS_BF16, many = a->n > VOPS_MAX_CONTINUATIONS / 2;

@@ -39,6 +39,8 @@ def check_select(logits, scores, n, finished, pad_id, keep_slots) -> None:
     if logits.dtype not in _DTYPES:
         raise ValueError(f"beam_select supports bf16 and fp32 logits, got {logits.dtype}")
     B, W, V = logits.shape
+    if B > 65535:
+        raise ValueError(f"at most 65535 requests, got {B}")
     if not 1 <= W <= _vops.MAX_BEAMS:
         raise ValueError(f"beams must be in [1, {_vops.MAX_BEAMS}], got {W}")
     if not 1 <= V <= _vops.MAX_VOCAB:
