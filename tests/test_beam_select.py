@@ -150,6 +150,15 @@ def test_rows_of_the_lowest_value(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_logits_of_any_size(device):
+    for size in (1e3, 1e5, 1e8, 1e20, 1e37):
+        x, scores = rows(9, 2, 3, 5003, torch.float32, scale=1.0)
+        compare(device, x + size, scores, 6)
+        compare(device, x - size, scores, 6)
+        compare(device, x * (size / 8), scores, 6)
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
 def test_equal_rows_and_scores_go_by_beam(device):
     # every beam has the same row and score: whole lists of equal scores, in the order beam, logit, id
     x = torch.zeros(2, 9, 6000, dtype=torch.bfloat16)

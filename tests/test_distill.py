@@ -228,6 +228,31 @@ def test_infinite_losses_and_nan_rows(device, tail):
     np.testing.assert_allclose(grad[0].cpu().numpy(), want[0], rtol=1e-4, atol=1e-7)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_large_batches_of_large_logits(dtype, tail):
+    for size in (100.0, 1e4, 1e20):
+        x, ids, teacher, w = make(72, 70, 5003, 9, dtype, tail=tail)
+        x[::2] += size
+        x[1::2] -= size
+        compare(GPU, x, ids, teacher, w, 1.0, tail)
+
+
+@pytest.mark.parametrize("T", [1e-6, 1e-3, 1e6])
+@pytest.mark.parametrize("size", [(3, 700, 8), (70, 5001, 8)], ids=str)
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_extreme_temperatures_stay_finite(device, size, T):
+    # (cold: one entry and one logit hold everything; hot: all are equal. The values go by the scale of 1 / T, so only what
+    # does not depend on roundings of z is asked for)
+    x, ids, teacher, w = make(71, *size)
+    w[:] = 1.0
+    loss, grad = backend(device, torch.float32).loss_and_grad(*(t.to(device) for t in (x, ids, teacher, w)), temperature=T)
+    assert bool(torch.isfinite(loss).all()) and bool(torch.isfinite(grad).all())
+    total = grad.double().sum(1).cpu().abs() * T  # q and p sum to 1 each
+    assert float(total.max()) <= 1e-4
+
+
 @pytest.mark.parametrize("device", DEVICES, ids=str)
 def test_no_rows(device):
     x, ids, teacher, w = (t.to(device) for t in make(1, 0, 50, 3))
@@ -336,6 +361,8 @@ BAD = [
     (dict(teacher=torch.zeros(4, 3, dtype=torch.bfloat16)), "teacher must be"),
     (dict(weights=torch.zeros(3)), "weights must be"),
     (dict(temperature=0.0), "temperature"),
+    (dict(temperature=1e-7), "temperature"),
+    (dict(temperature=2e6), "temperature"),
     (dict(temperature=float("inf")), "temperature"),
     (dict(temperature=float("nan")), "temperature"),
 ]

@@ -25,6 +25,7 @@ MAX_BEAMS = 64
 MAX_CONTINUATIONS = 64
 MAX_REORDER_BEAMS = 32
 MAX_ENTRIES = 1024
+TEMPERATURES = (1e-6, 1e6)
 
 STATUS = {0: "ok", 1: "VOPS_E_ARG", 2: "VOPS_E_DTYPE", 3: "VOPS_E_HIP", 4: "VOPS_E_WORKSPACE", 5: "VOPS_E_DEVICE"}
 

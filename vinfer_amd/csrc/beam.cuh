@@ -282,8 +282,8 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   }
   __syncthreads();
   uint32_t c = sh.count;
-  // (or logits so large that the products would overflow: masks of the type's lowest value alone, say)
-  const bool crowded = nv > kPartVecs || c > kPartList || (finite_f(M) && fabsf(M) > 1e30f);  // (uniform)
+  // (or logits so large that the reference's rounding would be all of the sum: masks of the type's lowest value, say)
+  const bool crowded = nv > kPartVecs || c > kPartList || (finite_f(M) && fabsf(M) > 65536.0f);  // (uniform)
   if (crowded) {
     sd = part_crowded<Tin, NV>(p, a.V, first, a.n, ref, sh);
     fx = 0;

@@ -360,9 +360,10 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
 // A wave's sum is against the largest of its first vectors, not of its row: nothing has to be known of a vector before
 // it is added. Where that was far off (a sum outside 2^-40 .. 2^60) the wave adds up again against its largest.
 // exp(x / T - ref / T) is one fma and v_exp_f32: 2^(x c - fl(ref c)), c = fl(log2(e) / T); the rounding of ref c is
-// put right in the sum, in fp64. A bf16 gradient's factor goes into the exponent too (off by 2^-19 at most).
+// put right in the sum, in fp64. A bf16 gradient's factor goes into the exponent too (off by 2^-16 at most). Where
+// ref c is past 2^8 (logits in the hundreds, or a cold temperature) differences are taken first, in slower loops.
 constexpr int kBehind = 8;
-constexpr float kHugeLogit = 1e30f;  // (past it x c may overflow: differences first)
+constexpr float kMostExponent = 256.0f;
 
 template <int WAVES>
 struct HeldShared {
@@ -442,7 +443,7 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
     strike_marked(d[j], j, marked);
     if (j == 0) {
       const float m = wave_max_f(Vec<Tin>::largest(d[j]));
-      ref = fabsf(m) < kHugeLogit ? m : 0.0f;
+      ref = fabsf(m) * c < kMostExponent ? m : 0.0f;  // (0: far off, mostly)
       refc = uniform_f(ref * c);
       s = 0.0f;
     }
@@ -605,7 +606,7 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
     if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
     __builtin_amdgcn_sched_barrier(0);
     const float scale = weight_of(r) / a.temp;
-    const bool huge = !(fabsf(mf) < kHugeLogit) && mf != -__builtin_inff();  // (uniform)
+    const bool huge = !(fabsf(mf) * c < kMostExponent) && mf != -__builtin_inff();  // (uniform)
     const float zero = uniform_f(huge || mf == -__builtin_inff() ? 0.0f : mf);
     float factor = uniform_f(scale * static_cast<float>(A));
     // the gradients out, the next row in, and its sum

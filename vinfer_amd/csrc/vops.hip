@@ -2,7 +2,6 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
-#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -171,8 +170,9 @@ int distill_common(const vops_distill_args* a) {
                 VOPS_MAX_ENTRIES, a->rows, a->vocab, a->entries);
   if (a->row_stride < a->vocab || (a->out_grad && a->grad_stride < a->vocab))
     return fail(VOPS_E_ARG, "row_stride and grad_stride must be >= vocab");
-  if (!(a->temperature > 0.0f) || !std::isfinite(a->temperature))
-    return fail(VOPS_E_ARG, "temperature must be positive and finite, got %g", static_cast<double>(a->temperature));
+  if (!(a->temperature >= VOPS_MIN_TEMPERATURE && a->temperature <= VOPS_MAX_TEMPERATURE))
+    return fail(VOPS_E_ARG, "temperature must be in [%g, %g], got %g", static_cast<double>(VOPS_MIN_TEMPERATURE),
+                static_cast<double>(VOPS_MAX_TEMPERATURE), static_cast<double>(a->temperature));
   if (a->rows > 0 && (!a->student || !a->ids)) return fail(VOPS_E_ARG, "student and ids must be set");
   const uintptr_t mask = a->dtype == VOPS_BF16 ? 1u : 3u;
   if ((reinterpret_cast<uintptr_t>(a->student) | reinterpret_cast<uintptr_t>(a->out_grad)) & mask)

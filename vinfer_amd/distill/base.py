@@ -11,14 +11,16 @@ For each row t, with z = student / temperature, q = softmax(z) and the teacher's
 
 ``student`` is ``[T, V]`` (bf16 or fp32, unit stride along V), ``ids`` int32 ``[T, K]`` (K up to 1024,
 distinct in a row; an id outside ``[0, V)``, as -1, is no entry), ``teacher`` fp32 ``[T, K]``, ``weights``
-fp32 ``[T]`` or None (1). A row of weight 0 is not read: its loss and gradient are 0. So are those of a row
+fp32 ``[T]`` or None (1), the temperature between 1e-6 and 1e6. A row of weight 0 is not read: its loss and gradient are 0. So are those of a row
 without entries. An entry of probability 0 adds nothing to the loss; an id of q 0 with p > 0 makes it
 infinite.
+
+A row's numbers are sums of fp32 exponentials in an order of their own route: ``loss``, ``loss_and_grad`` and
+``loss_and_states`` may differ in their last bits, each of them gives the same bits every time.
 """
 
 from __future__ import annotations
 
-import math
 from typing import Protocol
 
 import torch
@@ -73,8 +75,9 @@ def check(student, ids, teacher, weights, temperature) -> None:
         raise ValueError(f"teacher must be a float32 [{T}, {K}] tensor on {dev}")
     if weights is not None and (weights.dtype != torch.float32 or weights.shape != (T,) or weights.device != dev):
         raise ValueError(f"weights must be a float32 [{T}] tensor on {dev}")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    low, high = _vops.TEMPERATURES
+    if not low <= temperature <= high:
+        raise ValueError(f"temperature must be in [{low}, {high}], got {temperature}")
 
 
 def check_states(states, ids, student) -> None:
