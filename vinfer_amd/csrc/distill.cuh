@@ -12,6 +12,8 @@
 // k_distill_part: a segment's m and S, its logits held in registers, the listed ones struck out by a bitmap of
 // the segment. k_distill_row: a wave a row, in fp64: the loss, m, A and the listed entries' gradients.
 // k_distill_grad: a segment's gradient. Rows of weight 0 are not read: their loss and gradient are 0.
+// Measured on an MI355X: 2048 rows of 151936 bf16 logits, 64 entries: the segments 106.9 us, 5.8 TB/s; the rows 8.6, a chain of
+// dependent loads and fp64 functions.
 #pragma once
 
 #include "rows.cuh"
@@ -362,6 +364,10 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
 // exp(x / T - ref / T) is one fma and v_exp_f32: 2^(x c - fl(ref c)), c = fl(log2(e) / T); the rounding of ref c is
 // put right in the sum, in fp64. A bf16 gradient's factor goes into the exponent too (off by 2^-16 at most). Where
 // ref c is past 2^8 (logits in the hundreds, or a cold temperature) differences are taken first, in slower loops.
+//
+// 4096 rows of 151936 bf16 logits, an eighth of weight 0: 499 us, 4.7 TB/s of logits and gradients (in segments, which read
+// the logits twice, 660); 1000 fp32 rows of 50257: 87 us. Vector issue takes 20 of a row's 31 us on its CU. A wave's sums
+// 4 vectors behind the loads: 10 us more. Gradients stored through the cache: 23 us more of the 87.
 constexpr int kBehind = 8;
 constexpr float kMostExponent = 256.0f;
 

@@ -80,7 +80,8 @@ int check_workspace(const void* p, size_t given, size_t need) {
 constexpr int kVecElems[2] = {8, 4};  // elements of a 16-byte vector, by dtype
 
 // The 16-byte vectors a thread of 256 holds (a power of two up to 8): as many as leave the launch `fill`
-// workgroups, and at least what keeps a row's segments to 64 (a lane each where they are joined).
+// workgroups, and at least what keeps a row's segments to 64 (a lane each where they are joined). Where the chip is
+// full, longer segments are faster: 2048 rows' losses (151936 ids) 107 us with 8 vectors, 140 with 4, 181 with 2.
 int segment_vectors(int dtype, int64_t rows, int64_t V, int64_t fill) {
   const int64_t unit = 256 * kVecElems[dtype];
   int nv = 8;
