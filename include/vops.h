@@ -126,7 +126,7 @@ typedef struct vops_distill_args {
   int32_t rows;    /* >= 0 */
   int32_t vocab;   /* 1 .. VOPS_MAX_VOCAB */
   int32_t entries; /* 1 .. VOPS_MAX_ENTRIES */
-  int64_t row_stride; /* elements, >= vocab */
+  int64_t row_stride; /* elements, >= 0 (0: one row for all) */
   const int32_t* ids;   /* [rows, entries] */
   const float* teacher; /* [rows, entries] */
   const float* weights; /* [rows]; NULL: 1 */

@@ -271,6 +271,25 @@ def test_rows_at_any_offset_and_stride(dtype):
     compare(GPU, x[::2, :4003], ids[::2], teacher[::2], w[::2])
 
 
+@pytest.mark.parametrize("T", [5, 80])
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_one_row_for_all(device, T):
+    # a broadcast student: its gradient is the rows' sum
+    x, ids, teacher, w = make(43, T, 5003, 9)
+    want = ops_oracle.distill(x[:1].expand(T, 5003).numpy(), ids.numpy(), teacher.numpy(), w.numpy(), 1.0, False)
+    s = backend(device, torch.float32)
+    leaf = x[:1].clone().to(device).requires_grad_()
+    loss = distill_loss(leaf.expand(T, 5003), ids.to(device), teacher.to(device), w.to(device), backend=s)
+    loss.sum().backward()
+    tol_loss, tol_grad = tolerance(x[:1].expand(T, 5003), ids, teacher, w, *want, 1.0, False, torch.float32)
+    assert np.all(np.abs(loss.detach().cpu().double().numpy() - want[0]) <= tol_loss)
+    # (summed by torch in fp32: half a step of the running sum a row)
+    size = np.abs(want[1]).sum(0)
+    assert np.all(np.abs(leaf.grad[0].cpu().double().numpy() - want[1].sum(0)) <= tol_grad.sum(0) + T * 2.0**-24 * size)
+    both = s.loss_and_grad(leaf.detach().expand(T, 5003), ids.to(device), teacher.to(device), w.to(device))[1]
+    assert np.all(np.abs(both.cpu().double().numpy() - want[1]) <= tol_grad)
+
+
 @pytest.mark.parametrize("device", DEVICES, ids=str)
 def test_incoming_gradients_weigh_the_rows(device):
     x, ids, teacher, w = make(41, 6, 700, 9)
@@ -399,7 +418,7 @@ def test_states_of_another_shape_and_gradients_of_constants_are_refused(device):
         ({"vocab": 0}, 1, b"vocab"),
         ({"entries": 1025}, 1, b"entries"),
         ({"flags": 2}, 1, b"flags"),
-        ({"row_stride": 99}, 1, b"row_stride"),
+        ({"row_stride": -1}, 1, b"row_stride"),
         ({"grad_stride": 99}, 1, b"grad_stride"),
         ({"temperature": -1.0}, 1, b"temperature"),
         ({"student": None}, 1, b"must be set"),

@@ -113,6 +113,19 @@ def test_lengths_are_clamped_and_a_plan_is_reused(device):
         plan = check(device, states, B, W, parents_of("any", B, W, rng), torch.tensor(lengths, dtype=torch.int32), plan)
 
 
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_nothing_to_move(device):
+    empty = torch.zeros(0, 7, device=device)
+    backend(device).prepare_reorder([BeamState(empty, 0, 1)], 0, 4).launch(
+        torch.zeros(0, 4, dtype=torch.int32, device=device), torch.zeros(0, dtype=torch.int32, device=device))
+    t = fill(torch.empty(6, 0, 3, device=device), 1)
+    u = fill(torch.empty(6, 5, device=device), 2)
+    old = u.cpu()
+    plan = backend(device).prepare_reorder([BeamState(t, 0, 1), BeamState(u)], 2, 3)
+    plan.launch(torch.full((2, 3), -1, dtype=torch.int32, device=device), torch.zeros(2, dtype=torch.int32, device=device))
+    assert torch.equal(u.cpu(), old)
+
+
 @pytest.mark.gpu
 def test_many_columns_and_workgroups():
     # several steps a workgroup, a run that ends inside a column, rows of many runs

@@ -366,8 +366,9 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
 // ref c is past 2^8 (logits in the hundreds, or a cold temperature) differences are taken first, in slower loops.
 //
 // 4096 rows of 151936 bf16 logits, an eighth of weight 0: 499 us, 4.7 TB/s of logits and gradients (in segments, which read
-// the logits twice, 660); 1000 fp32 rows of 50257: 87 us. Vector issue takes 20 of a row's 31 us on its CU. A wave's sums
-// 4 vectors behind the loads: 10 us more. Gradients stored through the cache: 23 us more of the 87.
+// the logits twice, 660); 1000 fp32 rows of 50257: 87 us. Vector issue takes 20 of a row's 31 us on its CU. Of the choices, in an
+// earlier form: the sum 8 vectors behind the loads 551 us, 4 570, 2 587; gradients stored past the cache 70 us for 1000 fp32
+// rows whose logits are partly in it, through it 93.
 constexpr int kBehind = 8;
 constexpr float kMostExponent = 256.0f;
 

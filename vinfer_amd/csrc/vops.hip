@@ -169,8 +169,8 @@ int distill_common(const vops_distill_args* a) {
   if (!distill_sizes_ok(a->dtype, a->rows, a->vocab, a->entries))
     return fail(VOPS_E_ARG, "rows must be >= 0, vocab in [1, %d], entries in [1, %d], got %d, %d, %d", VOPS_MAX_VOCAB,
                 VOPS_MAX_ENTRIES, a->rows, a->vocab, a->entries);
-  if (a->row_stride < a->vocab || (a->out_grad && a->grad_stride < a->vocab))
-    return fail(VOPS_E_ARG, "row_stride and grad_stride must be >= vocab");
+  if (a->row_stride < 0 || (a->out_grad && a->grad_stride < a->vocab))
+    return fail(VOPS_E_ARG, "row_stride must be >= 0 and grad_stride >= vocab");
   if (!(a->temperature >= VOPS_MIN_TEMPERATURE && a->temperature <= VOPS_MAX_TEMPERATURE))
     return fail(VOPS_E_ARG, "temperature must be in [%g, %g], got %g", static_cast<double>(VOPS_MIN_TEMPERATURE),
                 static_cast<double>(VOPS_MAX_TEMPERATURE), static_cast<double>(a->temperature));
