@@ -4,7 +4,8 @@
 // Two launches. k_beam_part: one workgroup a segment of a row, held in registers, so that a row is read
 // once. A lane's maximum gives a bound: the n-th largest of a wave's 64 lane maxima (n <= 64) is at most the
 // segment's n-th largest logit, and few elements reach the largest of the four waves' bounds (about
-// 64 ln(64 / (64 - n)) a wave where the logits come in any order). The vectors that hold one go to LDS, their
+// 64 ln(64 / (64 - n)) a wave where the logits come in any order); above n = 8 the n-th largest of the workgroup's 256
+// lane maxima is taken, with about as many elements above it as n. The vectors that hold one go to LDS, their
 // elements' exponentials are taken in fp64 and added in fixed point, and those that reach the bound are ranked by
 // counting: the first n are the segment's candidates in order. The other vectors, all below the bound, add their
 // fp32 exponentials. So neither do the large terms lose precision nor does the order of the list, which varies,
@@ -12,9 +13,9 @@
 // k_beam_merge: one workgroup a request. The rows' normalisers from the segments' sums; lane maxima of the segments'
 // candidates' scores bound the request's n-th best in the same way; the few candidates that reach it are ranked.
 //
-// Measured on an MI355X: 64 x 4 rows of 151936 bf16 logits, n = 8: 20.6 us, 3.8 TB/s; 24 x 16 rows of 262144, n = 16: 45.0,
-// 4.5 TB/s: vector issue, 700 to 833 instructions a wave of which 324 are an element's own (8 vectors a thread: fewer leave more
-// waves with the same overhead, 23 and 56 us with 4). The merges 5.4 and 10.2; n = 32 and 64 of the former in all 39 and 71 us.
+// Measured on an MI355X: 64 x 4 rows of 151936 bf16 logits, n = 8: 21.1 us, 3.7 TB/s; 24 x 16 rows of 262144, n = 16: 39.4,
+// 5.1 TB/s: vector issue, 700 to 713 instructions a wave of which 324 are an element's own (8 vectors a thread: fewer leave more
+// waves with the same overhead, 23 and 56 us with 4). The merges 5.4 and 10.0; n = 32 and 64 of the former in all 30 and 37 us.
 //
 // A row with a NaN, an infinite maximum or no finite logit has no candidates, nor have logits of -inf.
 // Rows of finished beams and of beams whose score is not finite are not read.
@@ -53,28 +54,24 @@ struct BeamArgs {
   int32_t* out_tokens;
 };
 
-// The n-th largest of the wave's 64 keys with the bits below LOW cleared: at most the key itself. A step is
-// scalar but for its compare. The second form: of 128 keys, two a lane.
-template <int LOW>
-__device__ __forceinline__ uint32_t wave_nth_floor(uint32_t key, int n) {
+// The n-th largest of the wave's 64 N keys, N a lane, with the bits below LOW cleared: at most the key itself. A step
+// is scalar but for its compares.
+template <int LOW, int N>
+__device__ __forceinline__ uint32_t wave_nth_floor_of(const uint32_t* keys, int n) {
   uint32_t t = 0;
 #pragma unroll
   for (int b = 31; b >= LOW; --b) {
     const uint32_t c = t | (1u << b);
-    if (__popcll(__ballot(key >= c)) >= n) t = c;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) count += __popcll(__ballot(keys[i] >= c));
+    if (count >= n) t = c;
   }
   return t;
 }
-
 template <int LOW>
-__device__ __forceinline__ uint32_t wave_nth_floor2(uint32_t k0, uint32_t k1, int n) {
-  uint32_t t = 0;
-#pragma unroll
-  for (int b = 31; b >= LOW; --b) {
-    const uint32_t c = t | (1u << b);
-    if (__popcll(__ballot(k0 >= c)) + __popcll(__ballot(k1 >= c)) >= n) t = c;
-  }
-  return t;
+__device__ __forceinline__ uint32_t wave_nth_floor(uint32_t key, int n) {
+  return wave_nth_floor_of<LOW, 1>(&key, n);
 }
 
 // How many of the first c words are larger than k, and how many equal it; the words behind them, up to a multiple of
@@ -114,6 +111,7 @@ struct PartShared {
   u64 wfix[kPartWaves];
   float wmax[kPartWaves];
   uint32_t wtau[kPartWaves];
+  uint32_t lane_max[kPartThreads];
   uint32_t wcnt[kPartWaves];
   uint32_t vecs, count;
 };
@@ -211,7 +209,7 @@ __device__ __forceinline__ double part_crowded(const Tin* row, int V, int first,
   return s;
 }
 
-// MANY: more than half a wave's lanes of continuations.
+// MANY: the n-th largest of all the workgroup's lane maxima, not of a wave's: fewer elements reach it.
 template <class Tin, int NV, bool MANY>
 __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   constexpr int E = Vec<Tin>::kElems;
@@ -238,38 +236,27 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
     __builtin_amdgcn_sched_barrier(0);  // (a vector at a time: 64 registers)
   }
   const float wm = wave_max_f(lm);
-  uint32_t tau;
-  if constexpr (!MANY) {
-    tau = wave_nth_floor<16>(key_of(lm), a.n);
-  } else {
-    // (nearly all lanes' maxima would be asked for, and the least of them bounds little: two values a lane)
-    forget<NV>(d);
-    float l0 = -__builtin_inff(), l1 = l0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float x[E];
-      Vec<Tin>::unpack(d[j], x);
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        l0 = max_nan(l0, x[e]);
-        l1 = max_nan(l1, x[E / 2 + e]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    tau = wave_nth_floor2<16>(key_of(l0), key_of(l1), a.n);
-  }
   forget<NV>(d);
-  if (lane_id() == 0) {
-    sh.wmax[w] = wm;
-    sh.wtau[w] = tau;
+  if constexpr (MANY) {
+    sh.lane_max[tid] = key_of(lm);
+  } else {
+    const uint32_t tau = wave_nth_floor<16>(key_of(lm), a.n);
+    if (lane_id() == 0) sh.wtau[w] = tau;
   }
+  if (lane_id() == 0) sh.wmax[w] = wm;
   __syncthreads();
   float M = sh.wmax[0];
-  uint32_t tk = sh.wtau[0];
 #pragma unroll
-  for (int i = 1; i < kPartWaves; ++i) {
-    M = fmaxf(M, sh.wmax[i]);
-    tk = max(tk, sh.wtau[i]);
+  for (int i = 1; i < kPartWaves; ++i) M = fmaxf(M, sh.wmax[i]);
+  uint32_t tk = 0;
+  if constexpr (MANY) {
+    uint32_t k[kPartWaves];
+#pragma unroll
+    for (int i = 0; i < kPartWaves; ++i) k[i] = sh.lane_max[i * kWave + lane_id()];
+    tk = wave_nth_floor_of<16, kPartWaves>(k, a.n);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPartWaves; ++i) tk = max(tk, sh.wtau[i]);
   }
   const float ref = M == -__builtin_inff() ? 0.0f : M;  // (no finite logit: exp(-inf - 0) = 0)
   // (a bound below every finite number takes all of them, and never -inf)
@@ -475,7 +462,8 @@ __global__ __launch_bounds__(kMergeMaxThreads) void k_beam_merge(BeamArgs a) {
       h1 = max(h1, min(h, x));
       h = max(h, x);
     }
-    h = wave_nth_floor2<8>(h, h1, n);
+    const uint32_t two[2] = {h, h1};
+    h = wave_nth_floor_of<8, 2>(two, n);
     if (lane == 0) sh.bound = max(h, 1u);
   }
   __syncthreads();

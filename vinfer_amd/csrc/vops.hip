@@ -95,6 +95,10 @@ int segments(int dtype, int nv, int64_t V) {
 }
 
 constexpr int64_t kFillWorkgroups = 1024;
+// Above this many continuations a segment's bound is taken over its whole workgroup, at and below it over each wave.
+// (64 x 4 x 151936 bf16 logits in all, per wave and per workgroup: n = 1 22.9 and 24.0 us, 4 23.5 and 24.0, 8 25.4 and
+// 25.0; bounds of a wave alone 39 us at n = 32 and 71 at 64, of the workgroup 30 and 37)
+constexpr int kManyContinuations = 8;
 
 struct BeamLayout {
   int nv, S;
@@ -288,7 +292,7 @@ int vops_beam_select(const vops_beam_args* a, void* stream) {
   const dim3 grid(L.S, a->beams, a->requests);
   with_nv(L.nv, [&](auto nv) {
     constexpr int N = decltype(nv)::value;
-    const bool bf = a->dtype == VOPS_BF16, many = a->n > VOPS_MAX_CONTINUATIONS / 2;
+    const bool bf = a->dtype == VOPS_BF16, many = a->n > kManyContinuations;
     const dim3 block(vo::kPartThreads);
     if (bf && many) hipLaunchKernelGGL((vo::k_beam_part<uint16_t, N, true>), grid, block, 0, st, k);
     else if (bf) hipLaunchKernelGGL((vo::k_beam_part<uint16_t, N, false>), grid, block, 0, st, k);
