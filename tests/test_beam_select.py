@@ -87,6 +87,21 @@ def test_large_rows_and_batches(size):
     compare(GPU, x, scores, n)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("n", [1, 8, 9, 33])
+def test_a_waves_bound_and_a_workgroups(n, dtype):
+    """Requests enough for the longest segments; rows whose best logits lie in one lane's, one wave's or all places."""
+    x, scores = rows(n, 72, 5, 20011, dtype)
+    x[:, 0] = x[:, 0].sort(-1).values
+    x[:, 1, :600] += 20.0
+    x[:, 2, 64:] = -torch.inf
+    x[:, 3] = -torch.inf
+    x[:, 3, 1024:1032] = torch.arange(8).to(dtype)  # a single vector's or two
+    x[:, 4] = x[:, 4].round()
+    compare(GPU, x, scores, n)
+
+
 @pytest.mark.parametrize("device", DEVICES, ids=str)
 def test_finished_dead_and_kept_places(device):
     x, scores = rows(5, 4, 6, 3001)
