@@ -152,6 +152,28 @@ def test_masks_infinities_and_nan(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("n", [8, 64])
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_nans_among_equal_logits(device, n, dtype):
+    # Equal logits crowd a segment's list. In the first beams some of each wave's lanes (8 or 4 elements every 2048 or
+    # 1024) hold a NaN, and logits above the others', so that no maximum of a lane tells what the segment holds: such rows
+    # have no candidates, whatever else is in them.
+    g = torch.Generator().manual_seed(n)
+    B, V = (72, 33001) if device.type == "cuda" else (2, 5000)
+    e = 8 if dtype == torch.bfloat16 else 4
+    x = torch.ones(B, 6, V, dtype=dtype)
+    lane = torch.arange(V) // e % 64
+    for w, (lanes, top) in enumerate([(7, 2.0), (40, 2.0), (63, 70000.0), (64, 2.0)]):
+        x[:, w, lane < lanes] = top
+        x[:, w, (torch.arange(V) % (256 * e) < lanes * e) & (torch.arange(V) % e == 1)] = float("nan")
+    x[:, 3, 3] = torch.inf
+    x[:, 4] = 70000.0
+    x[:, 4, V // 3] = -float("nan")
+    compare(device, x, -3.0 - 2.0 * torch.rand(B, 6, generator=g), n)
+    compare(device, x[:, :4], torch.zeros(B, 4), n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
 @pytest.mark.parametrize("device", DEVICES, ids=str)
 def test_rows_of_the_lowest_value(device, dtype):
     # masked by the type's lowest value throughout, or but for a few ids: whole segments hold nothing else, and few of them

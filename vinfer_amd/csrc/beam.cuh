@@ -235,7 +235,8 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
     lm = max_nan(lm, vm[j]);
     __builtin_amdgcn_sched_barrier(0);  // (a vector at a time: 64 registers)
   }
-  const float wm = wave_max_f(lm);
+  // (NaN where the wave holds one: wave_max_f passes NaNs over)
+  const float wm = __ballot(lm != lm) ? __builtin_nanf("") : wave_max_f(lm);
   forget<NV>(d);
   if constexpr (MANY) {
     sh.lane_max[tid] = key_of(lm);
@@ -247,7 +248,7 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
   __syncthreads();
   float M = sh.wmax[0];
 #pragma unroll
-  for (int i = 1; i < kPartWaves; ++i) M = fmaxf(M, sh.wmax[i]);
+  for (int i = 1; i < kPartWaves; ++i) M = max_nan(M, sh.wmax[i]);
   uint32_t tk = 0;
   if constexpr (MANY) {
     uint32_t k[kPartWaves];
@@ -298,13 +299,16 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
     }
   }
   __syncthreads();
-  uint32_t c = sh.count;
+  // A segment with a NaN or an infinite largest has no candidates (nor has its row), and its lane maxima bound nothing: it never
+  // counts as crowded, and its list is dropped.
+  const bool live = finite_f(M);  // (uniform, as all here)
+  uint32_t c = live ? sh.count : 0;
   // (or logits so large that the reference's rounding would be all of the sum: masks of the type's lowest value, say)
-  const bool crowded = nv > kPartVecs || c > kPartList || (finite_f(M) && fabsf(M) > 65536.0f);  // (uniform)
+  const bool crowded = live && (nv > kPartVecs || c > kPartList || fabsf(M) > 65536.0f);
   if (crowded) {
     sd = part_crowded<Tin, NV>(p, a.V, first, a.n, ref, tk, sh);
     fx = 0;
-    c = sh.count;
+    c = min(sh.count, static_cast<uint32_t>(kPartList));  // (n at most)
   }
   // ranks by counting (keys differ)
   const uint32_t n = static_cast<uint32_t>(a.n);
