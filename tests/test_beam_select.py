@@ -235,6 +235,20 @@ def test_large_terms_keep_their_precision():
         compare(GPU, x, s, 2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("V", [4096, 32768, 151936, 262144])
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_segments_whose_listed_terms_are_all_one(device, V, dtype):
+    # one logit of each 8 just above 0, the others 0: up to 512 listed vectors of 8 elements, each element's exponential 1
+    x = torch.zeros(1, 4, V, dtype=dtype)
+    x[..., ::8] = 1e-30
+    x[:, 2, ::16] = -torch.inf
+    x[:, 3] = -x[:, 3]
+    scores = torch.tensor([[-1.0, -1.5, -2.0, -1.25]])
+    for n in (4, 9):
+        compare(device, x, scores, n)
+
+
 @pytest.mark.gpu
 def test_repeats_graphs_and_other_streams_agree():
     x, scores = rows(13, 5, 4, 151936)

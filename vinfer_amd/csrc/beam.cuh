@@ -35,7 +35,8 @@ constexpr int kMergeList = 1024;    // a request's
 constexpr int kMergeMaxThreads = 1024;
 constexpr int kMergeHeads = 512;
 constexpr int kAhead = 4;           // entries that a thread loads at once
-constexpr double kFix = 4503599627370496.0;  // 2^52
+constexpr double kFix = 2251799813685248.0;  // 2^51
+static_assert(kPartVecs * 8 * kFix < 18446744073709551616.0, "a sum of all listed elements' terms holds in 64 bits");
 
 struct BeamArgs {
   const void* logits;  // row (b, w) at b * rstride + w * bstride
@@ -100,8 +101,8 @@ __device__ __forceinline__ u64 pack_key(float x, int id) {
 __device__ __forceinline__ float key_value(u64 k) { return val_of(static_cast<uint32_t>(k >> 32)); }
 __device__ __forceinline__ int key_id(u64 k) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(k)); }
 
-// A term e in [0, 1] of a sum whose order varies: rint(e 2^52).
-__device__ __forceinline__ u64 fix52(double e) { return static_cast<u64>(__builtin_rint(e * kFix)); }
+// A term e in [0, 1] of a sum whose order varies: rint(e 2^51).
+__device__ __forceinline__ u64 fixed(double e) { return static_cast<u64>(__builtin_rint(e * kFix)); }
 
 struct PartShared {
   uint4 vec[kPartVecs];  // the vectors with an element at or above the bound
@@ -295,7 +296,7 @@ __global__ __launch_bounds__(kPartThreads) void k_beam_part(BeamArgs a) {
         const uint32_t at = atomicAdd(&sh.count, 1u);
         if (at < kPartList) sh.list[at] = pack_key(x, sh.vid[i / E] + e);
       }
-      fx += fix52(exp_nonpos(static_cast<double>(x) - static_cast<double>(ref)));
+      fx += fixed(exp_nonpos(static_cast<double>(x) - static_cast<double>(ref)));
     }
   }
   __syncthreads();
