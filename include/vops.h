@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define VOPS_ABI_VERSION 1
+#define VOPS_ABI_VERSION 2 /* 2: vops_distill_args.temperature is a double */
 
 enum vops_dtype { VOPS_BF16 = 0, VOPS_F32 = 1 };
 
@@ -38,8 +38,8 @@ enum vops_status {
 #define VOPS_MAX_CONTINUATIONS 64 /* its n */
 #define VOPS_MAX_REORDER_BEAMS 32
 #define VOPS_MAX_ENTRIES 1024     /* vops_distill */
-#define VOPS_MIN_TEMPERATURE 1e-6f
-#define VOPS_MAX_TEMPERATURE 1e6f
+#define VOPS_MIN_TEMPERATURE 1e-6
+#define VOPS_MAX_TEMPERATURE 1e6
 
 int vops_abi_version(void);
 
@@ -130,7 +130,7 @@ typedef struct vops_distill_args {
   const int32_t* ids;   /* [rows, entries] */
   const float* teacher; /* [rows, entries] */
   const float* weights; /* [rows]; NULL: 1 */
-  float temperature;    /* VOPS_MIN_TEMPERATURE .. VOPS_MAX_TEMPERATURE */
+  double temperature;   /* VOPS_MIN_TEMPERATURE .. VOPS_MAX_TEMPERATURE */
   uint32_t flags;
   float* out_loss; /* [rows] */
   void* out_grad;  /* `dtype`, row t at t * grad_stride, not over the student; NULL: the loss alone */

@@ -253,6 +253,16 @@ def test_extreme_temperatures_stay_finite(device, size, T):
     assert float(total.max()) <= 1e-4
 
 
+@pytest.mark.parametrize("T", [0.1, 1.0 / 3.0])
+@pytest.mark.parametrize("size", [(5, 33, 4), (3, 5003, 70), (80, 5003, 9)], ids=str)
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_temperatures_that_fp32_does_not_hold(device, size, T):
+    # (0.1 in fp32 is off by 2^-26 of itself, and the teacher's logits lie 100 apart when divided by it)
+    x, ids, teacher, w = make(73, *size)
+    for tail in (False, True):
+        compare(device, x, ids, teacher if not tail else torch.log_softmax(teacher, 1) - 0.1, w, T, tail)
+
+
 @pytest.mark.parametrize("device", DEVICES, ids=str)
 def test_no_rows(device):
     x, ids, teacher, w = (t.to(device) for t in make(1, 0, 50, 3))

@@ -13,7 +13,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libvops.so"
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 VOPS_BF16 = 0
 VOPS_F32 = 1
@@ -98,7 +98,7 @@ class VopsDistillArgs(ctypes.Structure):
         ("ids", ctypes.c_void_p),
         ("teacher", ctypes.c_void_p),
         ("weights", ctypes.c_void_p),
-        ("temperature", ctypes.c_float),
+        ("temperature", ctypes.c_double),
         ("flags", ctypes.c_uint32),
         ("out_loss", ctypes.c_void_p),
         ("out_grad", ctypes.c_void_p),

@@ -31,7 +31,8 @@ struct DistillArgs {
   const int32_t* ids;     // [T, K]; outside [0, V): no entry
   const float* teacher;   // [T, K]
   const float* weights;   // [T] or null (1)
-  float temp;
+  double inv;  // 1 / temperature
+  float c;     // log2(e) / temperature
   int tail;
   float* maxs;    // [T, S]
   double* sums;   // [T, S]
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_part(DistillArgs a)
   forget<NV>(d);
   m = wave_max_f(m);
   const float ref = m == -__builtin_inff() ? 0.0f : m;
-  const float c = kLog2e / a.temp;
+  const float c = a.c;
   float s = 0.0f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_part(DistillArgs a)
     double S = 0.0;
     // (a wave without a finite logit has the sum 0, or NaN for a NaN)
     for (int i = 0; i < kDistillWaves; ++i)
-      S += wmax[i] == M ? wsum[i] : wsum[i] * exp((static_cast<double>(wmax[i]) - M) / a.temp);
+      S += wmax[i] == M ? wsum[i] : wsum[i] * exp((static_cast<double>(wmax[i]) - M) * a.inv);
     a.maxs[blockIdx.x] = M;
     a.sums[blockIdx.x] = S;
   }
@@ -142,7 +143,7 @@ struct RowNumbers {
 template <class Tin, bool ONE>
 __device__ __forceinline__ RowNumbers row_numbers(const DistillArgs& a, int row, float* listed) {
   const int lane = lane_id();
-  const double inv = 1.0 / static_cast<double>(a.temp);
+  const double inv = a.inv;
   const double ninf = -static_cast<double>(__builtin_inff());
   const float* ms = as_global(a.maxs) + static_cast<int64_t>(row) * a.S;
   const double* ss = as_global(a.sums) + static_cast<int64_t>(row) * a.S;
@@ -336,9 +337,9 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
     A = st[1];
   }
   const float ref = m == -__builtin_inff() ? 0.0f : m;
-  const float scale = weight / a.temp;
+  const float scale = static_cast<float>(weight * a.inv);
   const float factor = scale * A;
-  const float c = kLog2e / a.temp;
+  const float c = a.c;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
     store_vector<Tin>(g, a.V, at + j * kDistillThreads * E, grad_vector<Tin>(d[j], ref, c, factor));
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
 //
 // A wave's sum is against the largest of its first vectors, not of its row: nothing has to be known of a vector before
 // it is added. Where that was far off (a sum outside 2^-40 .. 2^60) the wave adds up again against its largest.
-// exp(x / T - ref / T) is one fma and v_exp_f32: 2^(x c - fl(ref c)), c = fl(log2(e) / T); the rounding of ref c is
+// exp(x / T - ref / T) is one fma and v_exp_f32: 2^(x c - fl(ref c)), c = fl(log2(e) / T) (host); the rounding of ref c is
 // put right in the sum, in fp64. A bf16 gradient's factor goes into the exponent too (off by 2^-16 at most). Where
 // ref c is past 2^8 (logits in the hundreds, or a cold temperature) differences are taken first, in slower loops.
 //
@@ -392,9 +393,9 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
   const int tid = threadIdx.x, lane = lane_id(), w = uniform_i(tid / kWave);
   const int V = a.V, K = a.K, nvec = V / E;
   const int left = nvec * E + tid;  // this thread's element of the row's end, if below V
-  const double inv = 1.0 / static_cast<double>(a.temp);
+  const double inv = a.inv;
   const double ninf = -static_cast<double>(__builtin_inff());
-  const float c = uniform_f(kLog2e / a.temp);
+  const float c = a.c;
 
   auto row_of = [&](int r) { return as_global(static_cast<const Tin*>(a.x)) + r * a.stride; };
   auto grad_of = [&](int r) { return as_global(static_cast<Tin*>(a.grad)) + r * a.gstride; };
@@ -612,7 +613,7 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
     double A = 0.0;
     if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
     __builtin_amdgcn_sched_barrier(0);
-    const float scale = weight_of(r) / a.temp;
+    const float scale = static_cast<float>(weight_of(r) * inv);
     const bool huge = !(fabsf(mf) * c < kMostExponent) && mf != -__builtin_inff();  // (uniform)
     const float zero = uniform_f(huge || mf == -__builtin_inff() ? 0.0f : mf);
     float factor = uniform_f(scale * static_cast<float>(A));

@@ -176,8 +176,8 @@ int distill_common(const vops_distill_args* a) {
   if (a->row_stride < 0 || (a->out_grad && a->grad_stride < a->vocab))
     return fail(VOPS_E_ARG, "row_stride must be >= 0 and grad_stride >= vocab");
   if (!(a->temperature >= VOPS_MIN_TEMPERATURE && a->temperature <= VOPS_MAX_TEMPERATURE))
-    return fail(VOPS_E_ARG, "temperature must be in [%g, %g], got %g", static_cast<double>(VOPS_MIN_TEMPERATURE),
-                static_cast<double>(VOPS_MAX_TEMPERATURE), static_cast<double>(a->temperature));
+    return fail(VOPS_E_ARG, "temperature must be in [%g, %g], got %g", VOPS_MIN_TEMPERATURE,
+                VOPS_MAX_TEMPERATURE, a->temperature);
   if (a->rows > 0 && (!a->student || !a->ids)) return fail(VOPS_E_ARG, "student and ids must be set");
   const uintptr_t mask = a->dtype == VOPS_BF16 ? 1u : 3u;
   if ((reinterpret_cast<uintptr_t>(a->student) | reinterpret_cast<uintptr_t>(a->out_grad)) & mask)
@@ -197,7 +197,8 @@ vo::DistillArgs distill_args(const vops_distill_args* a, int S) {
   d.ids = a->ids;
   d.teacher = a->teacher;
   d.weights = a->weights;
-  d.temp = a->temperature;
+  d.inv = 1.0 / a->temperature;
+  d.c = static_cast<float>(1.4426950408889634 / a->temperature);
   d.tail = (a->flags & VOPS_DISTILL_TAIL) != 0;
   d.loss = a->out_loss;
   d.grad = a->out_grad;
