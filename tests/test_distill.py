@@ -315,6 +315,32 @@ def test_incoming_gradients_weigh_the_rows(device):
         assert not distill_loss(leaf, *rest, backend=s).requires_grad
 
 
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("T", [1.0, 0.1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_rows_of_weight_0_have_gradient_0_under_any_later_weights(device, dtype, T, tail):
+    x, ids, teacher, w = make(45, 12, 5003, 9, dtype, tail=tail)
+    w[:] = 1.0
+    w[[1, 3, 4, 8, 11]] = 0.0
+    x[1] = 120.0  # (exp(x) and exp(x / 0.1) are infinite in fp32)
+    x[3] = float("nan")
+    x[4] = torch.inf
+    x[8] = torch.finfo(dtype).max
+    x[11, ::2] = -torch.inf
+    s = backend(device, dtype)
+    xd, *rest = (t.to(device) for t in (x, ids, teacher, w))
+    loss, states = s.loss_and_states(xd, *rest, temperature=T, tail=tail)
+    other = torch.linspace(-1.5, 2.5, 12)
+    for later in (None, other):
+        grad = s.grad(xd, rest[0], states, None if later is None else later.to(device), temperature=T)
+        eff = (torch.ones(12) if later is None else later) * (w != 0)
+        want = ops_oracle.distill(x.float().numpy(), ids.numpy(), teacher.numpy(), eff.numpy(), T, tail)
+        _, tol = tolerance(x, ids, teacher, eff, *want, T, tail, dtype)
+        assert not loss[w == 0].any() and not grad[w == 0].any()
+        assert np.all(np.abs(grad.cpu().double().numpy() - want[1]) <= tol)
+
+
 @pytest.mark.gpu
 def test_calls_are_deterministic_on_any_stream_and_in_graphs():
     x, ids, teacher, w = (t.to(GPU) for t in make(51, 300, 20011, 30, torch.bfloat16, zeros=True))

@@ -11,7 +11,9 @@
 //
 // k_distill_part: a segment's m and S, its logits held in registers, the listed ones struck out by a bitmap of
 // the segment. k_distill_row: a wave a row, in fp64: the loss, m, A and the listed entries' gradients.
-// k_distill_grad: a segment's gradient. Rows of weight 0 are not read: their loss and gradient are 0.
+// k_distill_grad: a segment's gradient. Rows of weight 0 are not read: their loss and gradient are 0. So is their A, and a
+// row whose A is 0 has zeros for all but its listed gradients, whatever its logits hold (0 times an infinite or NaN exponential
+// would be NaN, and the m of a row that was not read says nothing of it).
 // Measured on an MI355X: 2048 rows of 151936 bf16 logits, 64 entries: the segments 106.9 us, 5.8 TB/s; the rows 8.6, a chain of
 // dependent loads and fp64 functions.
 #pragma once
@@ -340,9 +342,11 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
   const float scale = static_cast<float>(weight * a.inv);
   const float factor = scale * A;
   const float c = a.c;
+  const bool zero = A == 0.0f;  // (uniform)
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    store_vector<Tin>(g, a.V, at + j * kDistillThreads * E, grad_vector<Tin>(d[j], ref, c, factor));
+    store_vector<Tin>(g, a.V, at + j * kDistillThreads * E,
+                      zero ? make_uint4(0, 0, 0, 0) : grad_vector<Tin>(d[j], ref, c, factor));
   __syncthreads();  // (the listed gradients go over what the vectors stored there)
   const int32_t* ids = a.ids + static_cast<int64_t>(row) * a.K;
   for (int k = threadIdx.x; k < a.K; k += kDistillThreads) {

@@ -60,7 +60,8 @@ class ReferenceDistill:
         m, factor, listed = states[:, :1].double(), states[:, 1:2].double(), states[:, 2:].double()
         m = torch.where(m == -torch.inf, 0.0, m)
         w = torch.ones(T, 1, dtype=torch.float64, device=student.device) if weights is None else weights.double()[:, None]
-        g = torch.exp((student.double() - m) / temperature) * factor
+        # (a factor of 0: nothing of the row's logits counts, which a row of weight 0 in the forward pass was not asked for)
+        g = torch.where(factor == 0, 0.0, torch.exp((student.double() - m) / temperature) * factor)
         there = (ids >= 0) & (ids < V)
         rows = torch.arange(T, device=ids.device)[:, None].expand_as(ids)
         g[rows[there], ids[there].long()] = listed[there]
