@@ -315,6 +315,23 @@ def test_incoming_gradients_weigh_the_rows(device):
         assert not distill_loss(leaf, *rest, backend=s).requires_grad
 
 
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_rows_of_weight_0_take_no_incoming_gradient(device):
+    x, ids, teacher, w = make(46, 6, 700, 9)
+    w[:] = 0.5
+    w[[0, 2, 3]] = 0.0
+    g = torch.tensor([torch.inf, 2.0, float("nan"), -torch.inf, 1.0, -3.0])
+    x[0] = float("nan")
+    leaf = x.clone().to(device).requires_grad_()
+    loss = distill_loss(leaf, *(t.to(device) for t in (ids, teacher, w)), backend=backend(device, torch.float32))
+    loss.backward(g.to(device))
+    assert not leaf.grad[w == 0].any()
+    eff = torch.where(w == 0, 0.0, w * g)
+    want = ops_oracle.distill(x.numpy(), ids.numpy(), teacher.numpy(), eff.numpy(), 1.0, False)
+    _, tol = tolerance(x, ids, teacher, eff, *want, 1.0, False, torch.float32)
+    assert np.all(np.abs(leaf.grad.cpu().double().numpy() - want[1]) <= tol)
+
+
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("T", [1.0, 0.1])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)

@@ -22,7 +22,8 @@ class _DistillLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         student, ids, states, weights = ctx.saved_tensors
-        w = g.float() if weights is None else weights * g
+        # (a row of weight 0 has gradient 0, also where what comes in is infinite or NaN)
+        w = g.float() if weights is None else torch.where(weights == 0, 0.0, weights * g)
         return ctx.backend.grad(student, ids, states, w.contiguous(), temperature=ctx.temperature), *([None] * 6)
 
 
