@@ -181,6 +181,29 @@ def test_graph_replays_and_other_streams():
         np.testing.assert_array_equal(t.cpu().view(torch.int16).numpy().reshape(want.shape), want)
 
 
+@pytest.mark.gpu
+def test_a_plan_may_be_dropped_behind_a_launch_on_another_stream():
+    # its descriptions stay allocated until that launch has read them
+    B, W, L = 2, 4, 50
+    t = fill(torch.empty(B * W, L, 64, dtype=torch.bfloat16, device=GPU), 1)
+    p = parents_of("cycle", B, W, np.random.default_rng(6))
+    n = torch.tensor([L, 7], dtype=torch.int32)
+    want = ops_oracle.reorder(t.cpu().view(torch.int16).numpy().reshape(B, W, L, 64), p.numpy(), n.numpy())
+    pd, nd = p.to(GPU), n.to(GPU)
+    plan = backend(GPU).prepare_reorder([BeamState(t, 0, 1)], B, W)
+    at, size = plan._descs.data_ptr(), plan._descs.numel()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        plan.launch(pd, nd)
+    del plan
+    others = [torch.empty(size, dtype=torch.uint8, device=GPU) for _ in range(8)]
+    assert all(o.data_ptr() != at for o in others)
+    side.synchronize()
+    np.testing.assert_array_equal(t.cpu().view(torch.int16).numpy().reshape(want.shape), want)
+
+
 # ---- what the kernel is told, checked on the CPU ----------------------------------------------------------
 def addresses(d, W, slot, length):
     """The bytes of one slot that the kernel moves, by its own arithmetic."""

@@ -135,7 +135,8 @@ class SamplerBackend(Protocol):
         state: ``launch(parents int32 [requests, beams], lengths int32 [requests] or None)`` on the result
         gives slot ``b * beams + w`` what slot ``b * beams + parents[b, w]`` held, up to ``lengths[b]``
         positions (clamped to the state's) in states with a ``length_dim``; a parent outside
-        ``[0, beams)`` (the -1 of ``beam_select``) leaves its slot as it is."""
+        ``[0, beams)`` (the -1 of ``beam_select``) leaves its slot as it is. A HIP graph that captured a launch holds
+        addresses: the plan and the states have to outlive it."""
         ...
 
 

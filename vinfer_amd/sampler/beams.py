@@ -248,7 +248,8 @@ class HipBeams:
 
 
 class HipReorder:
-    """A reusable reordering of fixed states (``prepare_reorder`` of the ``hip`` sampler backend)."""
+    """A reusable reordering of fixed states (``prepare_reorder`` of the ``hip`` sampler backend). It may be dropped as
+    soon as its launches are enqueued, on whatever streams; only graphs that captured one need it to live on."""
 
     def __init__(self, states: Sequence[BeamState], requests: int, beams: int) -> None:
         self._lib = _vops.load()
@@ -269,12 +270,15 @@ class HipReorder:
         self._n = len(descs)
         blob = b"".join(bytes(d) for d in descs)
         self._descs = torch.frombuffer(bytearray(blob), dtype=torch.uint8).to(dev) if blob else None
+        self._stream = torch._C._cuda_getCurrentRawStream(dev.index)  # (whose memory the descriptions are in)
 
     def launch(self, parents: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
         """Enqueue one reordering on torch's current stream of the states' device."""
         check_reorder(parents, lengths, self.requests, self.beams, self.device, self._has_length)
         if self._descs is None:
             return
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._stream:
+            self._descs.record_stream(torch.cuda.current_stream(self.device))
         parents = parents.contiguous()
         if lengths is not None:
             lengths = lengths.contiguous()
