@@ -264,6 +264,58 @@ def test_one_memory_twice_is_refused():
         backend(torch.device("cpu")).prepare_reorder([BeamState(t), BeamState(t.view(6, 2, 2))], 2, 3)
 
 
+def test_states_that_share_some_memory_are_refused():
+    c = torch.zeros(6, 8, 10)
+    pool = torch.zeros(6, 2, 8, 10)
+    shared = [
+        (c, c[:, 1:]), (c[:, :5], c[:, 4:]), (c[..., :6], c[..., 5:]), (c, c[:, :, 3]), (c[:, ::2], c[:, ::3]),
+        (pool, pool[:, 1]), (pool[:, 0, 2:], pool[:, 0, :3]), (c[:, ::2, :4], c[:, 2:, 3:]),
+        (c.view(-1)[1:337].view(6, 56), c), (c.view(torch.uint8)[..., 3:], c.view(torch.uint8)[..., :4]),
+    ]
+    for a, b in shared:
+        for s in ((a, b), (b, a), (torch.zeros(6, 3), a, torch.zeros(6, 3), b)):
+            with pytest.raises(ValueError, match="same memory"):
+                backend(torch.device("cpu")).prepare_reorder([BeamState(t) for t in s], 2, 3)
+
+
+def test_states_side_by_side_in_one_buffer_are_taken():
+    c = torch.zeros(6, 8, 10)
+    pool = torch.zeros(4, 6, 2, 8, 5, 12)  # layers, slots, keys and values, positions, heads, numbers
+    record = torch.zeros(6, 100)  # of a slot: a matrix, a window, a few numbers; a gap behind them
+    wide = torch.zeros(6, 8, 3, 10)[:, :7]
+    apart = [
+        (c[:, :5], c[:, 5:]), (c[..., :6], c[..., 6:]), (c[..., 0], c[..., 7]), (c[:, ::2], c[:, 1::2]), (c[:3].repeat(2, 1, 1), c),
+        tuple(pool[i, :, j] for i in range(4) for j in range(2)),
+        tuple(pool.transpose(0, 3)[i, :, j] for i in range(8) for j in range(2)),
+        tuple(pool[0, :, :, :, :, 3 * i : 3 * i + 3] for i in range(4)),
+        (record[:, :64].view(6, 8, 8), record[:, 64:80].view(6, 4, 4), record[:, 80:83]),
+        (wide[:, :, 0], wide[:, :, 2, :4], wide[:, :, 2, 4:], wide[:, :, 1]),
+        (c[:, :0], c),
+    ]
+    for s in apart:
+        for t in (s, s[::-1]):
+            backend(torch.device("cpu")).prepare_reorder([BeamState(x) for x in t], 2, 3)
+    rng = np.random.default_rng(8)
+    for _ in range(300):  # what is taken shares nothing, in layouts of any kind
+        base = torch.zeros(2000, dtype=torch.uint8)
+        s, held = [], []
+        for _ in range(2):
+            dims = [(1, int(rng.integers(1, 5)))]
+            for _ in range(int(rng.integers(1, 4))):
+                st, n = dims[-1]
+                dims.append((st * n + int(rng.integers(0, 4)) * int(rng.integers(0, 9)), int(rng.integers(1, 4))))
+            dims[-1] = (dims[-1][0], 6)
+            off = int(rng.integers(0, 40))
+            t = base.as_strided([n for _, n in dims[::-1]], [st for st, _ in dims[::-1]], off)
+            s.append(t)
+            held.append(set(np.ravel(off + sum(np.ix_(*[np.arange(n) * st for st, n in dims]))).tolist()))
+        try:
+            backend(torch.device("cpu")).prepare_reorder([BeamState(t) for t in s], 2, 3)
+        except ValueError:
+            continue
+        assert not held[0] & held[1]
+
+
 def test_too_many_strided_dimensions_are_refused():
     t = torch.zeros(4, 4, 4, 4, 4)[:, ::2, ::2, ::2, ::2]
     with pytest.raises(ValueError, match="strided dimensions"):

@@ -24,7 +24,8 @@ _DTYPES = {torch.bfloat16: _vops.VOPS_BF16, torch.float32: _vops.VOPS_F32}
 class BeamState:
     """One tensor of states that a search's beams carry: ``slot_dim`` indexes the ``requests * beams`` slots
     (request b's beam w in slot ``b * beams + w``); with ``length_dim`` (a cache's or a history's positions)
-    only a request's first positions count. Any dtype, any strides without overlap."""
+    only a request's first positions count. Any dtype, any strides without overlap, and no memory that another state
+    of the same plan holds."""
 
     tensor: torch.Tensor
     slot_dim: int = 0
@@ -58,6 +59,25 @@ def check_select(logits, scores, n, finished, pad_id, keep_slots) -> None:
         raise ValueError(f"finished must be a bool [{B}, {W}] tensor on {logits.device}")
 
 
+def _apart(a: int, da: list[tuple[int, int]], b: int, db: list[tuple[int, int]]) -> bool:
+    """Whether the bytes at ``a + sum(i * stride)`` over the (stride, extent) pairs ``da`` are shown to be none of
+    ``b``'s: their ranges do not meet, or they do not within one period of a stride that the outer dimensions of both
+    are multiples of."""
+    end_a, end_b = (x + sum(st * (n - 1) for st, n in d) + 1 for x, d in ((a, da), (b, db)))
+    if end_a <= b or end_b <= a:
+        return True
+    for period in sorted({st for st, _ in da + db if st > 1}, reverse=True):
+        inner = [[(st, n) for st, n in d if st % period] for d in (da, db)]
+        if len(inner[0]) + len(inner[1]) == len(da) + len(db):
+            continue
+        for origin in {a, b}:
+            at = [(x - origin) % period for x in (a, b)]
+            if all(x + sum(st * (n - 1) for st, n in d) < period for x, d in zip(at, inner)) \
+                    and _apart(at[0], inner[0], at[1], inner[1]):
+                return True
+    return False
+
+
 def check_states(states: Sequence[BeamState], requests: int, beams: int) -> torch.device:
     """``ValueError`` for states that ``prepare_reorder`` cannot take; the states' device."""
     if not states:
@@ -84,11 +104,17 @@ def check_states(states: Sequence[BeamState], requests: int, beams: int) -> torc
             if st < end:
                 raise ValueError(f"state {i}: elements of a tensor with strides {t.stride()} may overlap")
             end = st * (n - 1) + end
-        spans.append((t.data_ptr(), i))
+        size = t.element_size()
+        d = [(st * size, n) for st, n in dims] + [(1, size)]
+        spans.append((t.data_ptr(), i, d, t.data_ptr() + end * size))
+    # (one launch moves all states, in no order: what two of them held would be read and written at once)
     spans.sort()
-    for (p, i), (q, j) in zip(spans, spans[1:]):
-        if p == q:
-            raise ValueError(f"states {min(i, j)} and {max(i, j)} are the same memory")
+    for k, (p, i, d, end) in enumerate(spans):
+        for q, j, e, _ in spans[k + 1 :]:
+            if q >= end:
+                break
+            if not _apart(p, d, q, e):
+                raise ValueError(f"states {min(i, j)} and {max(i, j)} may hold the same memory")
     return dev
 
 
