@@ -38,6 +38,7 @@ enum vops_status {
 #define VOPS_MAX_CONTINUATIONS 64 /* its n */
 #define VOPS_MAX_REORDER_BEAMS 32
 #define VOPS_MAX_ENTRIES 1024     /* vops_distill */
+#define VOPS_MAX_DISTILL_SEGMENTS 16777215 /* rows times a row's segments (1 to 64) in a call that goes by segments */
 #define VOPS_MIN_TEMPERATURE 1e-6
 #define VOPS_MAX_TEMPERATURE 1e6
 
@@ -123,7 +124,8 @@ int vops_reorder(const vops_state* states, int32_t n_states, int64_t max_columns
 typedef struct vops_distill_args {
   const void* student; /* `dtype`, row t at t * row_stride */
   int32_t dtype;
-  int32_t rows;    /* >= 0 */
+  int32_t rows;    /* >= 0; refused where they make more than VOPS_MAX_DISTILL_SEGMENTS segments (16 million rows
+                    * of up to 16384 bf16 or 8192 fp32 logits) */
   int32_t vocab;   /* 1 .. VOPS_MAX_VOCAB */
   int32_t entries; /* 1 .. VOPS_MAX_ENTRIES */
   int64_t row_stride; /* elements, >= 0 (0: one row for all) */

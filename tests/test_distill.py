@@ -412,6 +412,24 @@ def test_forward_and_backward_in_one_graph():
         assert torch.equal(loss, want) and torch.equal(x.grad, grad)
 
 
+@pytest.mark.parametrize("rows,vocab,dtype,ok", [
+    ((1 << 24) - 1, 200, 0, True), (1 << 24, 200, 0, False), ((1 << 31) - 1, 1, 1, False), (1 << 23, 16385, 0, False),
+    ((1 << 23) - 1, 16384, 1, True), (1 << 23, 8193, 1, False), (1 << 18, 524288, 1, False)], ids=str)
+def test_more_segments_than_a_launch_takes_are_refused(rows, vocab, dtype, ok):
+    # a launch has fewer than 2^32 threads in a dimension (refused before any device is looked for)
+    lib = _vops.load()
+    a = _vops.VopsDistillArgs()
+    a.student, a.dtype, a.rows, a.vocab, a.entries, a.row_stride = 0x1000, dtype, rows, vocab, 8, vocab
+    a.ids, a.teacher, a.temperature, a.out_loss, a.states = 0x2000, 0x3000, 1.0, 0x4000, 0x7000
+    a.workspace, a.workspace_bytes = 0x5000, 1 << 60
+    if torch.cuda.is_available() and ok:
+        pytest.skip("would run")
+    for entry in (lib.vops_distill, lib.vops_distill_grad):
+        a.out_grad, a.grad_stride = (0x6000, vocab) if entry is lib.vops_distill_grad else (None, 0)
+        code = entry(ctypes.byref(a), None)
+        assert (code == 1 and b"too many rows" in lib.vops_last_error()) == (not ok)
+
+
 def test_the_family_has_both_backends():
     assert DISTILL.names() == ["hip", "reference"]
     with pytest.raises(ValueError, match="distill backend 'hip' does not run on cpu"):

@@ -206,15 +206,23 @@ vo::DistillArgs distill_args(const vops_distill_args* a, int S) {
   return d;
 }
 
-// The held form's launch, if a row of the call fits a workgroup's registers.
+constexpr int kHeldMostVectors = 1024 * 19;  // (of the last VO_HELD below)
+
+// Whether loss and gradient go by the held form.
+bool held(const vops_distill_args* a) {
+  return a->out_grad && !a->states && (a->rows >= kHeldRows || a->vocab <= kHeldVectors * kVecElems[a->dtype]) &&
+         a->vocab >= kHeldVocab && a->entries <= kHeldEntries && a->vocab / kVecElems[a->dtype] <= kHeldMostVectors;
+}
+
+// Its launch: the first of these whose registers take a row.
 template <class Tin>
-bool launch_held(const vo::DistillArgs& k, hipStream_t st) {
+void launch_held(const vo::DistillArgs& k, hipStream_t st) {
   const int nvec = k.V / vo::Vec<Tin>::kElems;
 #define VO_HELD(THREADS, NS, ROWS_A_CU)                                                                  \
   if (nvec <= THREADS * NS) {                                                                            \
     const int grid = k.T < 256 * ROWS_A_CU ? k.T : 256 * ROWS_A_CU;                                      \
     hipLaunchKernelGGL((vo::k_distill_held<Tin, THREADS, NS, ROWS_A_CU>), dim3(grid), dim3(THREADS), 0, st, k);     \
-    return true;                                                                                         \
+    return;                                                                                              \
   }
   VO_HELD(512, 8, 3)
   VO_HELD(512, 16, 2)
@@ -223,11 +231,15 @@ bool launch_held(const vo::DistillArgs& k, hipStream_t st) {
   VO_HELD(1024, 16, 1)
   VO_HELD(1024, 19, 1)
 #undef VO_HELD
-  return false;
 }
 
+// (a launch has fewer than 2^32 threads in a dimension, and a segment has a workgroup)
 int grid_ok(int64_t workgroups) {
-  return workgroups < (int64_t(1) << 31) ? VOPS_OK : fail(VOPS_E_ARG, "too many rows for one call");
+  static_assert(VOPS_MAX_DISTILL_SEGMENTS * int64_t(vo::kDistillThreads) < (int64_t(1) << 32), "");
+  return workgroups <= VOPS_MAX_DISTILL_SEGMENTS
+             ? VOPS_OK
+             : fail(VOPS_E_ARG, "too many rows for one call: %lld segments, at most %d", static_cast<long long>(workgroups),
+                    VOPS_MAX_DISTILL_SEGMENTS);
 }
 
 }  // namespace
@@ -365,7 +377,8 @@ int vops_distill(const vops_distill_args* a, void* stream) {
   const DistillLayout L = distill_layout(a->dtype, a->rows, a->vocab, a->entries);
   if (int rc = check_workspace(a->workspace, a->workspace_bytes, L.total)) return rc;
   const int64_t parts = static_cast<int64_t>(a->rows) * L.S;
-  if (int rc = grid_ok(parts)) return rc;
+  const bool in_one = held(a);  // (in strides over the rows)
+  if (int rc = in_one ? VOPS_OK : grid_ok(parts)) return rc;
   if (int rc = check_current_device()) return rc;
   char* ws = static_cast<char*>(a->workspace);
   vo::DistillArgs k = distill_args(a, L.S);
@@ -373,13 +386,14 @@ int vops_distill(const vops_distill_args* a, void* stream) {
   k.maxs = reinterpret_cast<float*>(ws + L.maxs);
   k.states = a->states ? a->states : reinterpret_cast<float*>(ws + L.states);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool bf = a->dtype == VOPS_BF16;
+  if (in_one) {
+    if (bf) launch_held<uint16_t>(k, st);
+    else launch_held<float>(k, st);
+    return launched("launch k_distill_held");
+  }
   const dim3 grid(static_cast<unsigned>(parts)), block(vo::kDistillThreads);
   const dim3 rows((a->rows + vo::kDistillWaves - 1) / vo::kDistillWaves);
-  const bool bf = a->dtype == VOPS_BF16;
-  if (a->out_grad && !a->states && (a->rows >= kHeldRows || a->vocab <= kHeldVectors * kVecElems[a->dtype]) && a->vocab >= kHeldVocab &&
-      a->entries <= kHeldEntries &&
-      (bf ? launch_held<uint16_t>(k, st) : launch_held<float>(k, st)))
-    return launched("launch k_distill_held");
   with_nv(L.nv, [&](auto nv) {
     constexpr int N = decltype(nv)::value;
     if (bf) hipLaunchKernelGGL((vo::k_distill_part<uint16_t, N>), grid, block, 0, st, k);
