@@ -24,7 +24,6 @@ namespace vo {
 
 constexpr int kDistillThreads = 256;
 constexpr int kDistillWaves = kDistillThreads / kWave;
-constexpr int kMaxEntries = 1024;
 
 struct DistillArgs {
   const void* x;  // row t at t * stride

@@ -16,7 +16,7 @@ namespace vo {
 
 using namespace vs;
 
-constexpr int kMaxReorderBeams = 32;
+constexpr int kMaxReorderBeams = 32;  // (a parent's children are bits of a word)
 constexpr int kReorderThreads = 256;
 constexpr int kReorderColumns = 512;  // a workgroup's step
 constexpr int kOuterDims = 3;

@@ -77,6 +77,10 @@ int check_workspace(const void* p, size_t given, size_t need) {
   return VOPS_OK;
 }
 
+static_assert(VOPS_MAX_BEAMS <= vo::kMaxBeams && VOPS_MAX_CONTINUATIONS <= vo::kMaxPick && VOPS_MAX_VOCAB <= 1 << 20 &&
+                  VOPS_MAX_REORDER_BEAMS <= vo::kMaxReorderBeams,
+              "what is checked here is what the kernels hold (an id takes 20 bits of a selection's tie word)");
+
 constexpr int kVecElems[2] = {8, 4};  // elements of a 16-byte vector, by dtype
 
 // The 16-byte vectors a thread of 256 holds (a power of two up to 8): as many as leave the launch `fill`
