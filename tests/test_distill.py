@@ -481,6 +481,21 @@ def test_states_of_another_shape_and_gradients_of_constants_are_refused(device):
         distill_loss(x, ids, teacher.requires_grad_(), w, backend=s)
 
 
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_tangents_of_forward_mode_are_refused(device):
+    x, ids, teacher, w = (t.to(device) for t in make(2, 4, 9, 3))
+    s = backend(device, torch.float32)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(x), ids, teacher, w), (dual(x.clone().requires_grad_()), ids, teacher, w), (x, ids, dual(teacher), w),
+                     (x, ids, teacher, dual(w))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                distill_loss(*args, backend=s)
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            distill_loss(dual(x), ids, teacher, backend=s)
+        assert distill_loss(x, ids, teacher, w, backend=s).shape == (4,)
+
+
 @pytest.mark.parametrize(
     "kw,code,msg",
     [

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from vinfer_amd.distill.base import DISTILL, DistillBackend
 from vinfer_amd.registry import BackendContext
@@ -38,9 +39,12 @@ def distill_loss(
     backend: str | DistillBackend = "hip",
 ) -> torch.Tensor:
     """The rows' losses (fp32 ``[T]``; see ``DistillBackend``), differentiable in ``student``. ``teacher``
-    and ``weights`` are constants. ``backend``: a name of the ``distill`` family, or a resolved backend."""
+    and ``weights`` are constants. Backward mode alone: an argument with a tangent (forward mode) is refused. ``backend``:
+    a name of the ``distill`` family, or a resolved backend."""
     if teacher.requires_grad or (weights is not None and weights.requires_grad):
         raise ValueError("distill_loss differentiates in the student's logits only")
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (student, teacher, weights)):
+        raise ValueError("distill_loss has no forward-mode derivative")
     if isinstance(backend, str):
         backend = DISTILL.resolve(backend, BackendContext(student.device, student.dtype))
     if not (student.requires_grad and torch.is_grad_enabled()):
