@@ -119,7 +119,7 @@ int vops_reorder(const vops_state* states, int32_t n_states, int64_t max_columns
  *   of the ids that are not listed.
  * loss[t] = weights[t] (sum p (log p - log q) + rest (log rest - log q_rest)), q_rest = 1 - the listed q.
  * grad[t] = d loss[t] / d student[t], rounded to the student's dtype. A row of weight 0 is not read; its
- * loss and gradient are 0. A row without entries has loss 0 and gradient 0. */
+ * loss and gradient are 0. A row without entries has loss 0 and gradient 0, whatever its logits hold. */
 #define VOPS_DISTILL_TAIL 1u
 typedef struct vops_distill_args {
   const void* student; /* `dtype`, row t at t * row_stride */

@@ -214,6 +214,33 @@ def test_tail_of_rows_with_little_or_nothing_beside_the_list(device):
 
 
 @pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("size", [(9, 700, 8), (9, 5003, 70), (81, 5003, 8), (81, 5003, 70)], ids=str)
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_rows_without_entries_have_loss_and_gradient_0(device, size, dtype, tail):
+    x, ids, teacher, w = make(24, *size, dtype, tail=tail)
+    w[:] = torch.linspace(-1.0, 2.0, size[0])
+    kinds = [lambda r: None, lambda r: r.fill_(float("nan")), lambda r: r.fill_(-torch.inf), lambda r: r[5:6].fill_(float("nan")),
+             lambda r: r[-1:].fill_(torch.inf), lambda r: r.fill_(torch.finfo(dtype).max)]
+    for t in range(size[0]):
+        if t % 4 != 1:
+            ids[t] = -1 if t % 2 else size[1]
+            kinds[t % len(kinds)](x[t])
+    bare = (ids < 0).all(1) | (ids >= size[1]).all(1)
+    s = backend(device, dtype)
+    xd, *rest = (t.to(device) for t in (x, ids, teacher, w))
+    loss = s.loss(xd, *rest, tail=tail)
+    both, grad = s.loss_and_grad(xd, *rest, tail=tail)
+    leaf = xd.clone().requires_grad_()
+    last = distill_loss(leaf, *rest, tail=tail, backend=s)
+    last.sum().backward()
+    for v in (loss, both, last.detach(), grad, leaf.grad):
+        assert not v[bare].any()
+    live = ~bare
+    compare(device, x[live], ids[live], teacher[live], w[live], 1.0, tail)
+
+
+@pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("device", DEVICES, ids=str)
 def test_infinite_losses_and_nan_rows(device, tail):
     x, ids, teacher, w = make(23, 3, 600, 8, tail=tail)

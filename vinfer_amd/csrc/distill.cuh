@@ -176,14 +176,15 @@ __device__ __forceinline__ RowNumbers row_numbers(const DistillArgs& a, int row,
   const double m = mf;
   const double S = wave_sum(m1 == mf ? s1 : s1 * exp((m1 - m) * inv));
   // the teacher's normaliser and the listed logits' largest
-  double tm = ninf, xm = m;
+  double tm = ninf, lm = ninf;
   each([&](int, bool has) {
     if (!has) return;
     tm = tv > tm ? tv : tm;
-    xm = xv > xm ? xv : xm;
+    lm = xv > lm ? xv : lm;
   });
   tm = wave_max_d(tm);
-  xm = wave_max_d(xm);
+  lm = wave_max_d(lm);
+  const double xm = lm > m ? lm : m;
   double ts = 0.0, xs = 0.0;
   each([&](int, bool has) {
     if (!has) return;
@@ -193,6 +194,8 @@ __device__ __forceinline__ RowNumbers row_numbers(const DistillArgs& a, int row,
   ts = wave_sum(ts);
   xs = wave_sum(xs);
   const bool none = tm == ninf;  // (no entry, or all of probability 0)
+  // Nothing to learn from: no entry, or (tail) none that either side gives a probability. Its numbers are 0 whatever its logits hold.
+  const bool empty = none && (!a.tail || (lm == ninf && xs == 0.0));
   // (differences of logits before anything else: beside logits of 1e38 an lse would lose log S)
   const double lts = a.tail ? 0.0 : log(ts);
   const double em = m == ninf ? 0.0 : exp((m - xm) * inv);
@@ -203,7 +206,7 @@ __device__ __forceinline__ RowNumbers row_numbers(const DistillArgs& a, int row,
   double loss = 0.0;
   each([&](int k, bool has) {
     float g = 0.0f;
-    if (has) {
+    if (has && !empty) {
       const double lp = a.tail ? tv : (tv - tm) * inv - lts;
       const double lq = (xv - xm) * inv - ltotal;
       const double p = none ? 0.0 : exp(lp);
@@ -213,9 +216,9 @@ __device__ __forceinline__ RowNumbers row_numbers(const DistillArgs& a, int row,
     if (k < a.K) listed[k] = g;
   });
   loss = wave_sum(loss);
-  if (rest > 0.0) loss += rest * (log(rest) - ((m == ninf ? ninf : (m - xm) * inv) + log(S) - ltotal));
+  if (rest > 0.0 && !empty) loss += rest * (log(rest) - ((m == ninf ? ninf : (m - xm) * inv) + log(S) - ltotal));
   double A = 0.0;
-  if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
+  if ((m != ninf || S != 0.0) && !empty) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
   return RowNumbers{mf, static_cast<float>(A), loss};
 }
 
@@ -600,6 +603,7 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
       xs = wave_sum(xw == xm ? xs : xs * exp((xw - xm) * inv));
     }
     __builtin_amdgcn_sched_barrier(0);
+    const bool empty = tm == ninf && (!a.tail || (xm == ninf && xs == 0.0));  // (as in row_numbers)
     // (against the larger of the two largest)
     double em = 1.0;
     if (xm > m) {
@@ -614,10 +618,11 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
     const double rest = a.tail ? fmax(0.0, 1.0 - ts) : 0.0;
     const double mass = a.tail ? ts + rest : (none ? 0.0 : 1.0);
     double A = 0.0;
-    if (m != ninf || S != 0.0) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
+    if ((m != ninf || S != 0.0) && !empty) A = mass * em / total - (rest > 0.0 ? rest / S : 0.0);
     __builtin_amdgcn_sched_barrier(0);
     const float scale = static_cast<float>(weight_of(r) * inv);
     const bool huge = !(fabsf(mf) * c < kMostExponent) && mf != -__builtin_inff();  // (uniform)
+    const bool clear = empty && S - S != 0.0;  // (an infinite or NaN logit, whose 0 it is to be as well)
     const float zero = uniform_f(huge || mf == -__builtin_inff() ? 0.0f : mf);
     float factor = uniform_f(scale * static_cast<float>(A));
     // the gradients out, the next row in, and its sum
@@ -673,12 +678,14 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (huge) {  // (the gradients again, from differences)
+      if (huge || clear) {  // (the gradients again, from differences)
         const float f = scale * static_cast<float>(A);
 #pragma unroll 1
         for (int j = 0; j < NS; ++j)
-          st_row16_nt(gb + base(j) + offset(j), grad_vector<Tin>(vector_at(row_of(r), j), mf, c, f));
-        if (left < V) store_elem<Tin>(g + left, f * __builtin_amdgcn_exp2f((element(row_of(r) + left) - mf) * c));
+          st_row16_nt(gb + base(j) + offset(j),
+                      clear ? make_uint4(0, 0, 0, 0) : grad_vector<Tin>(vector_at(row_of(r), j), mf, c, f));
+        if (left < V)
+          store_elem<Tin>(g + left, clear ? 0.0f : f * __builtin_amdgcn_exp2f((element(row_of(r) + left) - mf) * c));
       }
     }
     // the listed gradients and the loss, stored after the next barrier
@@ -693,11 +700,11 @@ __global__ __launch_bounds__(THREADS, ROWS * THREADS / 256) void k_distill_held(
         const double lq = (xv - xm) * inv - ltotal;
         const double q = none ? 0.0 : exp(lp);
         if (q != 0.0) loss = q * (lp - lq);
-        last_g = scale * static_cast<float>(exp(lq) * mass - q);
+        last_g = empty ? 0.0f : scale * static_cast<float>(exp(lq) * mass - q);
       }
       loss = wave_sum(loss);
       if (lane == 0) sh.loss[par][w] = loss;
-      last_rest = rest > 0.0 ? rest * (log(rest) - ((m == ninf ? ninf : (m - xm) * inv) + log(S) - ltotal)) : 0.0;
+      last_rest = rest > 0.0 && !empty ? rest * (log(rest) - ((m == ninf ? ninf : (m - xm) * inv) + log(S) - ltotal)) : 0.0;
     } else if (lane == 0) {
       sh.loss[par][w] = 0.0;
     }

@@ -36,6 +36,8 @@ class ReferenceDistill:
         log_rest = torch.logsumexp(others, 1)
         largest = others.amax(1)
         m = torch.where(member, -torch.inf, x).amax(1)
+        # (no entry, or none that either side gives a probability: nothing to learn from, whatever the logits hold)
+        empty = none[:, 0] & ((torch.gather(x, 1, at) == -torch.inf) | ~there).all(1) if tail else none[:, 0]
         logq = torch.gather(logq, 1, at)
         loss = torch.where(p != 0, p * (logp - logq), 0.0).sum(1)
         loss = loss + torch.where(rest > 0, rest * (torch.log(rest) - log_rest), 0.0)
@@ -43,7 +45,8 @@ class ReferenceDistill:
         factor = mass * torch.exp(largest) - torch.where(rest > 0, rest * torch.exp(largest - log_rest), 0.0)
         factor = torch.where(m == -torch.inf, 0.0, factor)
         listed = torch.where(there, torch.exp(logq) * mass[:, None] - p, 0.0)
-        return loss, torch.cat([m[:, None], factor[:, None], listed], 1)
+        states = torch.cat([m[:, None], factor[:, None], listed], 1)
+        return torch.where(empty, 0.0, loss), torch.where(empty[:, None], 0.0, states)
 
     def loss_and_states(self, student, ids, teacher, weights=None, *, temperature=1.0, tail=False):
         check(student, ids, teacher, weights, temperature)
