@@ -147,7 +147,7 @@ int vops_distill(const vops_distill_args* args, void* stream);
 
 /* out_grad alone, from the states that vops_distill wrote for the same student, ids, temperature and flags;
  * weights may be others (a backward pass: the weights times the incoming gradients; a row whose weight was 0
- * there has gradient 0). teacher, out_loss and the workspace are not used. */
+ * there has gradient 0 under any, NaN among them). teacher, out_loss and the workspace are not used. */
 int vops_distill_grad(const vops_distill_args* args, void* stream);
 
 const char* vops_last_error(void);

@@ -23,8 +23,8 @@ class _DistillLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         student, ids, states, weights = ctx.saved_tensors
-        # (a row of weight 0 has gradient 0, also where what comes in is infinite or NaN)
-        w = g.float() if weights is None else torch.where(weights == 0, 0.0, weights * g)
+        # (a row of weight 0 has states of 0, and gradient 0 also where what comes in is infinite or NaN)
+        w = g.float() if weights is None else weights * g
         return ctx.backend.grad(student, ids, states, w.contiguous(), temperature=ctx.temperature), *([None] * 6)
 
 
@@ -43,7 +43,9 @@ def distill_loss(
     a name of the ``distill`` family, or a resolved backend."""
     if teacher.requires_grad or (weights is not None and weights.requires_grad):
         raise ValueError("distill_loss differentiates in the student's logits only")
-    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (student, teacher, weights)):
+    # (a level is entered: 1.3 us a tensor otherwise)
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (student, teacher, weights)):
         raise ValueError("distill_loss has no forward-mode derivative")
     if isinstance(backend, str):
         backend = DISTILL.resolve(backend, BackendContext(student.device, student.dtype))

@@ -63,12 +63,13 @@ class ReferenceDistill:
         m, factor, listed = states[:, :1].double(), states[:, 1:2].double(), states[:, 2:].double()
         m = torch.where(m == -torch.inf, 0.0, m)
         w = torch.ones(T, 1, dtype=torch.float64, device=student.device) if weights is None else weights.double()[:, None]
-        # (a factor of 0: nothing of the row's logits counts, which a row of weight 0 in the forward pass was not asked for)
+        # (a factor of 0: nothing of the row's logits counts, which a row of weight 0 in the forward pass was not asked for; and
+        # what is 0 there is 0 under any weight)
         g = torch.where(factor == 0, 0.0, torch.exp((student.double() - m) / temperature) * factor)
         there = (ids >= 0) & (ids < V)
         rows = torch.arange(T, device=ids.device)[:, None].expand_as(ids)
         g[rows[there], ids[there].long()] = listed[there]
-        return torch.where(w == 0, 0.0, w / temperature * g).to(student.dtype)
+        return torch.where((w == 0) | (g == 0), 0.0, w / temperature * g).to(student.dtype)
 
     def loss(self, student, ids, teacher, weights=None, *, temperature=1.0, tail=False):
         return self.loss_and_states(student, ids, teacher, weights, temperature=temperature, tail=tail)[0]
