@@ -144,6 +144,20 @@ def test_random_rows(device, size, dtype, T, tail):
     compare(device, x, ids, teacher, w, T, tail)
 
 
+@pytest.mark.parametrize("T", [1.0, 0.7, 3.0])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("size", [(3, 7), (5, 40), (4, 1000)], ids=str)
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_lists_that_leave_one_or_two_ids_out(device, size, dtype, T):
+    n, V = size
+    x, ids, teacher, w = make(25, n, V, V, dtype)
+    for t in range(n):
+        ids[t, t % V] = -1
+        ids[t, (3 * t + 1) % V] = V
+    compare(device, x, ids, teacher, w, T, False)
+    compare(device, x, ids, torch.log_softmax(teacher, 1) - 0.05, w, T, True)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("size", [(2, 524288, 64, torch.float32), (700, 3001, 16, torch.bfloat16), (300, 9000, 40, torch.float32),
