@@ -54,8 +54,11 @@ int vops_query(int device, char* why, size_t n);
  * in descending order, equal scores by ascending beam, then descending logit, then ascending id. A finished
  * beam has one continuation, pad_id with the beam's own score. A beam whose score is not finite has none
  * (its row is not read), nor has a row with a NaN, a +inf or no finite logit, nor a logit of -inf. Where
- * there are fewer than n, the rest is score -inf, beam -1, token -1. Log-probabilities and comparisons are
- * in fp64. */
+ * there are fewer than n, the rest is score -inf, beam -1, token -1. Scores are worked out
+ * and compared in fp64, equal ones being equal there. A row's sum of exponentials has fp64 terms near its
+ * largest and fp32 terms (sums of up to 64) below: its log is off by at most 46 2^-23, for all continuations of
+ * the row alike, so that only continuations of different rows that lie nearer than twice that may change
+ * places. */
 #define VOPS_BEAM_KEEP_SLOTS 1u /* the order of the outputs: a parent's best child takes the parent's place, \
                                  * the others the free places in their order (needs n = beams) */
 typedef struct vops_beam_args {

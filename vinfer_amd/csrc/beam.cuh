@@ -9,13 +9,15 @@
 // elements' exponentials are taken in fp64 and added in fixed point, and those that reach the bound are ranked by
 // counting: the first n are the segment's candidates in order. The other vectors, all below the bound, add their
 // fp32 exponentials. So neither do the large terms lose precision nor does the order of the list, which varies,
-// show in the sum: the beams of a request are compared across their rows by these sums.
+// show in the sum: the beams of a request are compared across their rows by these sums. (The fp32 terms: two roundings of
+// the exponent, v_exp_f32's ulp and a thread's sum of at most 64 are 46 2^-23 of the sum at most, 13.2 being the mean
+// distance from the maximum that 524288 ids allow. In fp32, because their issue bounds the launch.)
 // k_beam_merge: one workgroup a request. The rows' normalisers from the segments' sums; lane maxima of the segments'
 // candidates' scores bound the request's n-th best in the same way; the few candidates that reach it are ranked.
 //
-// Measured on an MI355X: 64 x 4 rows of 151936 bf16 logits, n = 8: 21.1 us, 3.7 TB/s; 24 x 16 rows of 262144, n = 16: 39.4,
+// Measured on an MI355X: 64 x 4 rows of 151936 bf16 logits, n = 8: 20.7 us, 3.8 TB/s; 24 x 16 rows of 262144, n = 16: 39.5,
 // 5.1 TB/s: vector issue, 700 to 713 instructions a wave of which 324 are an element's own (8 vectors a thread: fewer leave more
-// waves with the same overhead, 23 and 56 us with 4). The merges 5.4 and 10.0; n = 32 and 64 of the former in all 30 and 37 us.
+// waves with the same overhead, 23 and 56 us with 4). The merges 5.4 and 10.0; n = 32 and 64 of the former in all 29 and 36 us.
 //
 // A row with a NaN, an infinite maximum or no finite logit has no candidates, nor have logits of -inf.
 // Rows of finished beams and of beams whose score is not finite are not read.
@@ -136,7 +138,7 @@ __device__ __forceinline__ void each_again(const Tin* row, int V, int first, F f
 // Segments with more elements at or above the bound than the list takes (equal logits, or few lanes with a
 // finite one): the n-th largest key, ids included, bit by bit between the bound and the largest key (a count of the
 // segment each, read again from the cache: held in registers, its keys would take 238 a lane, and the ordinary segments'
-// occupancy; 256 constant rows of 151936 bf16 logits 224 us in all, random ones 25), and this thread's part of the whole segment's sum.
+// occupancy; 256 constant rows of 151936 bf16 logits 215 us in all, random ones 24), and this thread's part of the whole segment's sum.
 template <class Tin, int NV>
 __device__ __forceinline__ double part_crowded(const Tin* row, int V, int first, int n, float ref, uint32_t bound,
                                                PartShared& sh) {

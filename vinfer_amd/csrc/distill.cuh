@@ -14,7 +14,7 @@
 // k_distill_grad: a segment's gradient. Rows of weight 0 are not read: their loss and gradient are 0. So are their A and listed
 // gradients, and what is 0 there stays 0 in a backward pass, whatever the row's logits and later weight hold (0 times an
 // infinite or NaN exponential would be NaN, and the m of a row that was not read says nothing of it).
-// Measured on an MI355X: 2048 rows of 151936 bf16 logits, 64 entries: the segments 106.9 us, 5.8 TB/s; the rows 8.6, a chain of
+// Measured on an MI355X: 2048 rows of 151936 bf16 logits, 64 entries: the segments 105.4 us, 5.9 TB/s; the rows 8.6, a chain of
 // dependent loads and fp64 functions.
 #pragma once
 
@@ -375,8 +375,8 @@ __global__ __launch_bounds__(kDistillThreads) void k_distill_grad(DistillArgs a)
 // put right in the sum, in fp64. A bf16 gradient's factor goes into the exponent too (off by 2^-16 at most). Where
 // ref c is past 2^8 (logits in the hundreds, or a cold temperature) differences are taken first, in slower loops.
 //
-// 4096 rows of 151936 bf16 logits, an eighth of weight 0: 499 us, 4.7 TB/s of logits and gradients (in segments, which read
-// the logits twice, 660); 1000 fp32 rows of 50257: 87 us. Vector issue takes 20 of a row's 31 us on its CU. Of the choices, in an
+// 4096 rows of 151936 bf16 logits, an eighth of weight 0: 496 us, 4.7 TB/s of logits and gradients (in segments, which read
+// the logits twice, 660); 1000 fp32 rows of 50257: 86 us. Vector issue takes 20 of a row's 31 us on its CU. Of the choices, in an
 // earlier form: the sum 8 vectors behind the loads 551 us, 4 570, 2 587; gradients stored past the cache 70 us for 1000 fp32
 // rows whose logits are partly in it, through it 93.
 constexpr int kBehind = 8;

@@ -14,7 +14,8 @@ distinct in a row; an id outside ``[0, V)``, as -1, is no entry), ``teacher`` fp
 fp32 ``[T]`` or None (1), the temperature between 1e-6 and 1e6. The hip backend refuses a call of more than 2^24 - 1 segments
 (16384 bf16 or 8192 fp32 logits of a row each, fewer in small calls). A row of weight 0 is not read: its loss and gradient are 0. So
 are those of a row without entries, whatever its logits hold. An entry of probability 0 adds nothing to the loss; an id of q 0 with p > 0 makes it
-infinite.
+infinite. So does, with ``tail``, a rest above 0 (a rounding of the teacher's log-probabilities is enough) where the student allows no
+unlisted id: such lists are complete, and ``tail=False`` is theirs.
 
 A row's numbers are sums of fp32 exponentials in an order of their own route: ``loss``, ``loss_and_grad`` and
 ``loss_and_states`` may differ in their last bits, each of them gives the same bits every time.

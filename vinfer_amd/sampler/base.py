@@ -121,7 +121,8 @@ class SamplerBackend(Protocol):
         """One step of a beam search: each request's ``n`` (1 .. 64) best continuations over its beams and
         the whole vocabulary, by ``scores[b, w] + log_softmax(logits[b, w])[v]``. ``logits`` ``[B, W, V]``
         (bf16 or fp32, unit stride along V; rows may be shared, as by ``expand``), ``scores`` fp32
-        ``[B, W]``, W up to 64. Equal scores go by ascending beam, then descending logit, then ascending
+        ``[B, W]``, W up to 64. Scores are compared in fp64 (on the hip backend the small terms of a row's sum of
+        exponentials are fp32: its log is off by at most 46 2^-23). Equal scores go by ascending beam, then descending logit, then ascending
         id. A beam marked in ``finished`` (bool ``[B, W]``) has one continuation: ``pad_id``, at its own
         score. A beam whose score is not finite has none (the first step: all scores but one -inf), nor has
         a row with a NaN, a +inf or no finite logit, nor a logit of -inf. With ``keep_slots`` (n = W) the
