@@ -59,14 +59,14 @@ def check_select(logits, scores, n, finished, pad_id, keep_slots) -> None:
         raise ValueError(f"finished must be a bool [{B}, {W}] tensor on {logits.device}")
 
 
-def _apart(a: int, da: list[tuple[int, int]], b: int, db: list[tuple[int, int]]) -> bool:
+def _apart(a: int, da: Sequence[tuple[int, int]], b: int, db: Sequence[tuple[int, int]]) -> bool:
     """Whether the bytes at ``a + sum(i * stride)`` over the (stride, extent) pairs ``da`` are shown to be none of
     ``b``'s: their ranges do not meet, or they do not within one period of a stride that the outer dimensions of both
     are multiples of."""
     end_a, end_b = (x + sum(st * (n - 1) for st, n in d) + 1 for x, d in ((a, da), (b, db)))
     if end_a <= b or end_b <= a:
         return True
-    for period in sorted({st for st, _ in da + db if st > 1}, reverse=True):
+    for period in sorted({st for d in (da, db) for st, _ in d if st > 1}, reverse=True):
         inner = [[(st, n) for st, n in d if st % period] for d in (da, db)]
         if len(inner[0]) + len(inner[1]) == len(da) + len(db):
             continue
@@ -85,7 +85,7 @@ def check_states(states: Sequence[BeamState], requests: int, beams: int) -> torc
     if requests < 0 or not 1 <= beams <= _vops.MAX_REORDER_BEAMS:
         raise ValueError(f"requests must be >= 0 and beams in [1, {_vops.MAX_REORDER_BEAMS}], got {requests} and {beams}")
     dev = states[0].tensor.device
-    spans = []
+    spans, layouts = [], {}
     for i, s in enumerate(states):
         t = s.tensor
         if t.device != dev:
@@ -105,15 +105,20 @@ def check_states(states: Sequence[BeamState], requests: int, beams: int) -> torc
                 raise ValueError(f"state {i}: elements of a tensor with strides {t.stride()} may overlap")
             end = st * (n - 1) + end
         size = t.element_size()
-        d = [(st * size, n) for st, n in dims] + [(1, size)]
-        spans.append((t.data_ptr(), i, d, t.data_ptr() + end * size))
-    # (one launch moves all states, in no order: what two of them held would be read and written at once)
+        d = tuple((st * size, n) for st, n in dims) + ((1, size),)
+        spans.append((t.data_ptr(), i, layouts.setdefault(d, len(layouts)), t.data_ptr() + end * size))
+    # One launch moves all states, in no order: what two of them held would be read and written at once. (Views of one
+    # buffer differ by few offsets: each is looked at once.)
     spans.sort()
+    layout, known = list(layouts), {}
     for k, (p, i, d, end) in enumerate(spans):
         for q, j, e, _ in spans[k + 1 :]:
             if q >= end:
                 break
-            if not _apart(p, d, q, e):
+            apart = known.get((q - p, d, e))
+            if apart is None:
+                apart = known[q - p, d, e] = _apart(0, layout[d], q - p, layout[e])
+            if not apart:
                 raise ValueError(f"states {min(i, j)} and {max(i, j)} may hold the same memory")
     return dev
 
