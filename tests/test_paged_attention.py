@@ -1,0 +1,280 @@
+"""Attention of sequences behind shared prefixes (``plan``, ``attend``): the reference backend and the hip kernels
+against softmaxes in 64 bits, a row at a time."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_oracle
+from vinfer_amd.paged import PAGED
+from vinfer_amd.registry import BackendContext
+
+GPU = torch.device("cuda", 0)
+DEVICES = [torch.device("cpu"), pytest.param(GPU, marks=pytest.mark.gpu)]
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def backend(device, dtype):
+    return PAGED.resolve("hip" if device.type == "cuda" else "reference", BackendContext(device, dtype))
+
+
+class Case:
+    """A cache of random pages, groups (sequences of each, prefix of each) and the sequences' own lengths."""
+
+    def __init__(self, device, dtype, groups, lengths, *, T=1, heads=4, kv_heads=2, D=64, page=16, order="places", seed=0,
+                 spread=1.0, extra=1):
+        rng = np.random.default_rng(seed)
+        self.device, self.dtype, self.page = device, dtype, page
+        self.T, self.heads, self.kv_heads, self.D = T, heads, kv_heads, D
+        self.lengths, self.prefixes = list(lengths), [p for _, p in groups] if groups else None
+        S = len(self.lengths)
+        self.starts = np.cumsum([0] + [n for n, _ in groups]) if groups else None
+        held = self.lengths + (self.prefixes or [])
+        need = [-(-n // page) for n in held]
+        P = sum(need) + 2
+        order_of = rng.permutation(P)
+        M, MP = max(need[:S], default=0) + extra, max(need[S:], default=0) + extra
+        tables = rng.integers(-3, P + 3, (len(held), max(M, MP)))  # (behind a sequence's pages: anything)
+        at = 0
+        for i, n in enumerate(need):
+            tables[i, :n] = order_of[at : at + n]
+            at += n
+        i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=device)  # noqa: E731
+        self.tables, self.prefix_tables = i32(tables)[:S, :M], i32(tables)[S:, :MP]
+        shape = (P, kv_heads, page, D) if order == "heads" else (P, page, kv_heads, D)
+        self.cache = [torch.tensor(rng.standard_normal(shape) * spread, dtype=torch.float32).to(dtype).to(device) for _ in range(2)]
+        if order == "heads":
+            self.cache = [t.transpose(1, 2) for t in self.cache]
+        self.q = torch.tensor(rng.standard_normal((S, T, heads, D)) * spread, dtype=torch.float32).to(dtype).to(device)
+        self.lengths_t = i32(self.lengths)
+        self.groups = {}
+        if groups:
+            self.groups = dict(prefix_lengths=i32(self.prefixes), max_prefix_pages=MP, group_starts=i32(self.starts))
+
+    def plan(self, b):
+        return b.plan(self.lengths_t, queries=self.T, heads=self.heads, kv_heads=self.kv_heads, head_dim=self.D,
+                      page_size=self.page, max_pages=self.tables.shape[1], **self.groups)
+
+    def attend(self, b, plan=None, scale=None):
+        return b.attend(self.q, *self.cache, self.tables, plan or self.plan(b), scale=scale,
+                        prefix_tables=self.prefix_tables if self.groups else None)
+
+    def want(self, scale=None):
+        S = len(self.lengths)
+        k, v = (t.double().cpu().numpy().reshape(-1, self.kv_heads, self.D) for t in self.cache)
+        tables, prefix_tables = self.tables.cpu().numpy(), self.prefix_tables.cpu().numpy()
+        pre, keys, values = [0] * S, [], []
+
+        def slots(row, n):
+            p = np.arange(n)
+            return row[p // self.page].astype(np.int64) * self.page + p % self.page
+
+        for s, n in enumerate(self.lengths):
+            at = slots(tables[s], n)
+            if self.groups:
+                g = int(np.searchsorted(self.starts, s, side="right")) - 1
+                pre[s] = self.prefixes[g]
+                at = np.concatenate([slots(prefix_tables[g], pre[s]), at])
+            keys.append(k[at])
+            values.append(v[at])
+        return paged_oracle.attend(self.q.double().cpu().numpy(), keys, values, self.lengths, pre, scale)
+
+    def check(self, scale=None, b=None):
+        got = self.attend(b or backend(self.device, self.dtype), scale=scale).double().cpu().numpy()
+        out, mass, size = self.want(scale)
+        n = max(self.lengths + [0]) + max(self.prefixes or [0])
+        step = torch.finfo(self.dtype).eps / 2
+        # The output's rounding; each weight's (fp16: half of 2^-24 at least, beside a sum of at least 2^-1, so that n of
+        # them add n 2^-25 times the largest value at most); scores' products summed in fp32, twice (weights and their
+        # sum); n weights and products summed in fp32, twice.
+        weight = step + 4 * (self.D + 16) * 2.0**-24 * size[..., None] + 2 * (n + 64) * 2.0**-24
+        tiny = n * 2.0**-24 * 8 * 2.0**-10 if self.dtype == F16 else 0.0
+        off = np.abs(got - out)
+        bound = step * np.abs(out) + weight * mass * 1.01 + tiny + 2.0**-25
+        assert np.isfinite(got).all()
+        assert np.all(off <= bound), (np.max(off - bound), np.argwhere(off > bound)[:5])
+        return got
+
+
+@pytest.mark.parametrize("D", [8, 64, 72, 80, 96, 128, 160, 192, 256])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_heads(device, dtype, D):
+    Case(device, dtype, [(2, 70), (1, 33)], [5, 130, 64], D=D, heads=6, kv_heads=2, seed=D).check()
+
+
+@pytest.mark.parametrize("heads", [(1, 1), (8, 1), (5, 5), (9, 3), (40, 2), (33, 1)], ids=str)
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_shared_key_heads(device, heads):
+    Case(device, BF16, [(3, 100), (2, 40)], [1, 17, 65, 129, 3], heads=heads[0], kv_heads=heads[1], T=2, seed=heads[0]).check()
+
+
+@pytest.mark.parametrize("page", [1, 2, 16, 64, 256, 4096])
+@pytest.mark.parametrize("order", ["places", "heads"])
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_pages(device, order, page):
+    Case(device, BF16, [(2, 200), (1, 63), (1, 65)], [1, 64, 66, 150], page=page, order=order, seed=page).check()
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_lengths_of_zero_and_one(device):
+    # groups without sequences, without a prefix, sequences without keys of their own: these give 0
+    c = Case(device, BF16, [(0, 50), (2, 0), (3, 1), (0, 0), (1, 64)], [0, 1, 0, 1, 2, 0], seed=1)
+    got = c.check()
+    assert (got[[0, 2, 5]] == 0).all()
+    c = Case(device, BF16, None, [0, 0], seed=2)
+    assert (c.check() == 0).all()
+    assert Case(device, BF16, None, [], seed=2).check().shape == (0, 1, 4, 64)
+
+
+@pytest.mark.parametrize("T", [2, 5, 33, 70])
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_new_tokens(device, T):
+    # causal among the new tokens; sequences shorter than them (padded on the left) have none before their first
+    lengths = [T, T + 1, 3, 0, T - 1, 64, 200]
+    got = Case(device, BF16, [(3, 31), (4, 0)], lengths, T=T, seed=T).check()
+    for s, n in enumerate(lengths):
+        assert (got[s, : max(0, T - n)] == 0).all()
+    Case(device, F16, None, lengths, T=T, heads=3, kv_heads=1, D=128, seed=T).check()
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_many_rows_of_a_group(device):
+    # rows past a workgroup's, in groups of unlike sizes
+    rng = np.random.default_rng(5)
+    Case(device, BF16, [(45, 130), (1, 500), (20, 64)], rng.integers(0, 40, 66).tolist(), heads=8, kv_heads=2, seed=6).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_long_keys_in_several_workgroups(D):
+    # one sequence's keys over the whole chip; a prefix and long own keys
+    Case(GPU, BF16, None, [20011], T=3, heads=8, kv_heads=4, D=D, seed=D).check()
+    Case(GPU, F16, [(3, 9001), (2, 777)], [1200, 0, 3001, 64, 1], heads=4, kv_heads=4, D=D, page=32, seed=D).check()
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_sharp_scores_and_a_scale(device):
+    # weights that differ by e^100 and more: maxima that move from tile to tile
+    Case(device, BF16, [(2, 300)], [100, 259], spread=4.0, D=128, seed=3).check()
+    Case(device, F16, [(2, 300)], [100, 259], D=32, seed=4).check(scale=2.5)
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_what_lies_behind_the_lengths_is_not_seen(device):
+    c = Case(device, BF16, [(2, 37)], [9, 30], seed=8)
+    want = c.check()
+    held = set()
+    for tables, lengths in ((c.tables, c.lengths), (c.prefix_tables, c.prefixes)):
+        for row, n in zip(tables.tolist(), lengths):
+            held |= {row[p // c.page] * c.page + p % c.page for p in range(n)}
+    other = torch.tensor([i for i in range(c.cache[0].shape[0] * c.page) if i not in held], device=device)
+    for bad in (math.nan, math.inf, -math.inf):
+        for t in c.cache:
+            t.view(-1, *t.shape[2:])[other] = bad
+        got = c.attend(backend(device, BF16)).double().cpu().numpy()
+        np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_keys_of_minus_infinity_and_rows_without_weight(device):
+    c = Case(device, BF16, None, [70, 3], heads=1, kv_heads=1, seed=9)
+    k = c.cache[0]
+    q0 = c.q.clone().abs_()
+    c.q.copy_(q0)
+    row = c.tables.tolist()
+    for p in (0, 5, 69):
+        k[row[0][p // 16], p % 16] = -math.inf  # (weights of 0)
+    for p in range(3):
+        k[row[1][0], p] = -math.inf  # (no weight at all: 0)
+    got = c.attend(backend(device, BF16)).double().cpu().numpy()
+    keep = [p for p in range(70) if p not in (0, 5, 69)]
+    at = np.array([row[0][p // 16] * 16 + p % 16 for p in keep])
+    kk, vv = (t.double().cpu().numpy().reshape(-1, 1, 64)[at] for t in c.cache)
+    out, mass, _ = paged_oracle.attend(c.q[:1].double().cpu().numpy(), [kk], [vv], [67])
+    assert np.all(np.abs(got[0] - out[0]) <= 2.0**-8 * (np.abs(out[0]) + 1.02 * mass[0]) + 2.0**-16)
+    assert (got[1] == 0).all()
+
+
+@pytest.mark.gpu
+def test_the_same_bits_every_time_in_graphs_and_on_other_streams():
+    rng = np.random.default_rng(11)
+    c = Case(GPU, BF16, [(30, 700), (3, 4000)], rng.integers(0, 300, 33).tolist(), heads=8, kv_heads=2, D=128, seed=11)
+    b = backend(GPU, BF16)
+    plan = c.plan(b)
+    want = c.attend(b, plan)
+    for _ in range(3):
+        assert torch.equal(c.attend(b), want)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams:  # two calls at once, of one plan
+        with torch.cuda.stream(s):
+            outs += [c.attend(b, plan) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    graphs = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                graphs.append((g, c.attend(b)))
+    c2 = Case(GPU, BF16, [(30, 650), (3, 3000)], rng.integers(0, 300, 33).tolist(), heads=8, kv_heads=2, D=128, seed=11)
+    for lengths, prefixes in ((c.lengths_t.clone(), c.groups["prefix_lengths"].clone()),
+                              (c.lengths_t // 2, c.groups["prefix_lengths"] - 50), (c2.lengths_t * 0 + 1, c2.groups["prefix_lengths"])):
+        c.lengths_t.copy_(lengths)  # (a plan that is captured is made anew from what the lengths have become)
+        c.groups["prefix_lengths"].copy_(prefixes)
+        now = c.attend(b)
+        torch.cuda.synchronize()
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, now) for _, o in graphs)
+
+
+@pytest.mark.gpu
+def test_queries_of_other_layouts():
+    c = Case(GPU, BF16, [(3, 50)], [9, 20, 70], T=2, heads=4, kv_heads=2, seed=12)
+    b = backend(GPU, BF16)
+    want = c.attend(b)
+    S, T, H, D = c.q.shape
+    wide = torch.zeros(S, T, H + 4, D + 8, dtype=BF16, device=GPU)
+    wide[:, :, :H, 8:].copy_(c.q)
+    odd = torch.zeros(S, T, H, D + 3, dtype=BF16, device=GPU)
+    odd[..., 1 : D + 1].copy_(c.q)
+    turned = c.q.transpose(1, 2).contiguous().transpose(1, 2)
+    for q in (wide[:, :, :H, 8:], odd[..., 1 : D + 1], turned):
+        c.q = q
+        assert torch.equal(c.attend(b), want)
+
+
+def test_refusals():
+    b = backend(torch.device("cpu"), BF16)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    good = dict(lengths=i32(2), queries=1, heads=4, kv_heads=2, head_dim=64, page_size=16, max_pages=3)
+    for bad, match in (({"queries": 0}, "queries"), ({"heads": 3}, "multiple"), ({"head_dim": 60}, "head_dim"),
+                       ({"head_dim": 264}, "head_dim"), ({"page_size": 24}, "power of two"), ({"max_pages": 0}, "max_pages"),
+                       ({"lengths": torch.zeros(2)}, "lengths"), ({"lengths": i32(2, 1)}, "lengths"), ({"kv_heads": 0}, "kv_heads"),
+                       ({"prefix_lengths": i32(1)}, "together"), ({"group_starts": i32(1)}, "together"),
+                       ({"prefix_lengths": i32(1), "group_starts": i32(1), "max_prefix_pages": 2}, "group_starts"),
+                       ({"prefix_lengths": i32(1), "group_starts": i32(2)}, "max_prefix_pages")):
+        with pytest.raises(ValueError, match=match):
+            b.plan(**{**good, **bad})
+    plan = b.plan(**good, prefix_lengths=i32(1), group_starts=i32(2), max_prefix_pages=2)
+    mk = lambda *s, dt=BF16: torch.zeros(*s, dtype=dt)  # noqa: E731
+    call = dict(q=mk(2, 1, 4, 64), k_pages=mk(5, 16, 2, 64), v_pages=mk(5, 16, 2, 64), tables=i32(2, 3), plan=plan,
+                prefix_tables=i32(1, 2))
+    b.attend(**call)
+    for bad, match in (({"q": mk(2, 4, 64)}, "q must be"), ({"q": mk(2, 1, 64, 4).transpose(2, 3)}, "unit stride"),
+                       ({"q": mk(2, 1, 4, 64).requires_grad_()}, "gradient"), ({"k_pages": mk(5, 16, 2, 64, dt=F16)}, "k_pages"),
+                       ({"k_pages": mk(5, 8, 2, 64), "v_pages": mk(5, 8, 2, 64)}, "positions"),
+                       ({"k_pages": mk(0, 16, 2, 64), "v_pages": mk(0, 16, 2, 64)}, "pages"),
+                       ({"tables": i32(2, 4)}, "tables"), ({"tables": i32(3, 2).T}, "tables"), ({"prefix_tables": None}, "prefix_tables"),
+                       ({"prefix_tables": i32(1, 3)}, "prefix_tables"), ({"scale": 0.0}, "scale"), ({"scale": math.nan}, "scale")):
+        with pytest.raises(ValueError, match=match):
+            b.attend(**{**call, **bad})

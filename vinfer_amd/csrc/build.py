@@ -1,5 +1,5 @@
 """Compile the HIP sources (gfx950 only): the sampler into ``vinfer_amd/libvsampler.so``, the operators
-around it into ``vinfer_amd/libvops.so``.
+around it into ``vinfer_amd/libvops.so``, the paged cache into ``vinfer_amd/libvpaged.so``.
 
 Run as ``python -m vinfer_amd.csrc.build``. The build is in-tree so the library travels with
 the source tree; there is no JIT cache.
@@ -20,6 +20,8 @@ LIB = PKG / "libvsampler.so"
 SOURCES = [PKG / "csrc" / "capi.hip"]
 OPS_LIB = PKG / "libvops.so"
 OPS_SOURCES = [PKG / "csrc" / "vops.hip"]
+PAGED_LIB = PKG / "libvpaged.so"
+PAGED_SOURCES = [PKG / "csrc" / "vpaged.hip"]
 
 # -ffp-contract=off: the penalty arithmetic rounds every operation on its own.
 # -fhip-fp32-correctly-rounded-divide-sqrt: x / T is IEEE division, as on the CPU.
@@ -41,6 +43,8 @@ FLAGS = [
 # The operators keep rows in registers across loops: constants that were kept in registers beside them would not fit
 # (the compiler moves each one's load out of the loop, fp64 polynomials' coefficients above all).
 OPS_FLAGS = [*FLAGS, "-mllvm", "-disable-machine-licm"]
+# The paged cache's products and sums are held in fp32 with one rounding fewer where the compiler fuses them.
+PAGED_FLAGS = [f for f in FLAGS if f != "-ffp-contract=off"]
 
 
 def hipcc() -> str:
@@ -69,8 +73,9 @@ def _compile(lib: Path, sources: list[Path], flags: list[str], verbose: bool) ->
 
 
 def build(verbose: bool = False) -> Path:
-    with ThreadPoolExecutor(2) as pool:
-        jobs = [pool.submit(_compile, *job, verbose) for job in ((LIB, SOURCES, FLAGS), (OPS_LIB, OPS_SOURCES, OPS_FLAGS))]
+    libraries = (LIB, SOURCES, FLAGS), (OPS_LIB, OPS_SOURCES, OPS_FLAGS), (PAGED_LIB, PAGED_SOURCES, PAGED_FLAGS)
+    with ThreadPoolExecutor(3) as pool:
+        jobs = [pool.submit(_compile, *job, verbose) for job in libraries]
     for job in jobs:
         job.result()
     return LIB
@@ -80,3 +85,4 @@ if __name__ == "__main__":
     build(verbose="-v" in sys.argv)
     print(LIB)
     print(OPS_LIB)
+    print(PAGED_LIB)

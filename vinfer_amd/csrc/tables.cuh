@@ -1,0 +1,209 @@
+// Page tables from the sequences' lengths: pages taken from a stack, tokens' slots, and pages given back.
+//
+// With len_s the sequences' lengths and c_s their new positions, sequence s needs
+//   need_s = ceil((len_s + c_s) / P) - ceil(len_s / P)
+// pages; the i-th page of the whole call (sequences in order) is the i-th from the stack's top, so two prefix sums
+// (of c and of need) give every page and every token its place. Bound by latency: one workgroup scans, takes the
+// pages and, where there are few tokens, writes them too; nothing waits between workgroups.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace vpg {
+
+constexpr int kTableThreads = 1024;
+
+struct Tables {
+  int32_t* tables;
+  int32_t* lengths;
+  int32_t* free_pages;
+  int32_t* free_count;
+  int S, M, pages, shift;
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
+// Exclusive prefix of x over the workgroup, and its total (every thread). `part`: a word a wave.
+template <class T>
+__device__ __forceinline__ T scan_exclusive(T x, T* part, T& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  T inc = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const T y = __shfl_up(inc, d);
+    if (lane >= d) inc += y;
+  }
+  __syncthreads();  // (part may still be read from an earlier scan)
+  if (lane == 63) part[wave] = inc;
+  __syncthreads();
+  T before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kTableThreads / 64; ++w) {
+    const T p = part[w];
+    all += p;
+    if (w < wave) before += p;
+  }
+  total = all;
+  return before + inc - x;
+}
+
+// The last of the n ascending starts that is <= i (starts[0] <= i).
+template <class T>
+__device__ __forceinline__ int find(const T* starts, int n, T i) {
+  int lo = 0;
+  for (int step = 1 << (31 - __clz(n)); step; step >>= 1)
+    if (lo + step < n && starts[lo + step] <= i) lo += step;
+  return lo;
+}
+
+// The token's slot and place; the tables' entries of this call are written.
+__device__ __forceinline__ void write_token(const Tables& t, int i, int s, int position, int32_t* slots,
+                                            int32_t* positions, int32_t* sequences) {
+  const int page = t.tables[static_cast<int64_t>(s) * t.M + (position >> t.shift)];
+  slots[i] = static_cast<int>((static_cast<unsigned>(page) << t.shift) + (position & ((1 << t.shift) - 1)));
+  positions[i] = position;
+  sequences[i] = s;
+}
+
+// SELF: this kernel writes the tokens. Else it leaves starts and bases for k_tokens: ws[0..S) a sequence's first token
+// (at most N), ws[S..2S) its length before, or -1 where its tokens are none.
+template <bool SELF>
+__global__ __launch_bounds__(kTableThreads) void k_extend(Tables t, const int32_t* __restrict__ counts, int N,
+                                                          int32_t* __restrict__ slots, int32_t* __restrict__ positions,
+                                                          int32_t* __restrict__ sequences, uint8_t* __restrict__ served,
+                                                          int32_t* __restrict__ ws) {
+  __shared__ int64_t part64[kTableThreads / 64];
+  __shared__ int part[kTableThreads / 64];
+  __shared__ int s_page[kTableThreads], s_have[kTableThreads], s_token[kTableThreads], s_base[kTableThreads];
+  const int tid = threadIdx.x;
+  const int P = 1 << t.shift;
+  const int64_t cap = min(static_cast<int64_t>(t.M) << t.shift, static_cast<int64_t>(INT32_MAX));
+  const int n_free = clampi(*t.free_count, 0, t.pages);
+  int64_t tokens_before = 0;
+  int pages_before = 0, taken = 0;
+  for (int base = 0; base < t.S; base += kTableThreads) {
+    const int s = base + tid;
+    int64_t len = 0, c = 0;
+    if (s < t.S) {
+      len = t.lengths[s];
+      len = len < 0 ? 0 : len > cap ? cap : len;
+      c = max(counts[s], 0);
+    }
+    int64_t all_tokens;
+    const int64_t start = tokens_before + scan_exclusive<int64_t>(c, part64, all_tokens);
+    const int64_t have = (len + P - 1) >> t.shift, want = (len + c + P - 1) >> t.shift;
+    const bool fits = len + c <= cap && start + c <= N;
+    const int need = fits ? static_cast<int>(want - have) : 0;
+    int all_pages;
+    const int first = scan_exclusive<int>(need, part, all_pages);  // (within this round)
+    const bool ok = fits && (need == 0 || pages_before + first + need <= n_free);
+    s_page[tid] = first;
+    s_have[tid] = ok ? static_cast<int>(have) : -1;
+    s_token[tid] = static_cast<int>(start > N ? N : start);
+    s_base[tid] = ok ? static_cast<int>(len) : -1;
+    if (s < t.S) {
+      served[s] = ok;
+      if (ok && c) t.lengths[s] = static_cast<int>(len + c);
+      if (!SELF) {
+        ws[s] = s_token[tid];
+        ws[t.S + s] = s_base[tid];
+      }
+    }
+    const int mine = ok ? need : 0;
+    int all_taken;
+    scan_exclusive<int>(mine, part, all_taken);  // (its barriers also publish the arrays)
+    taken += all_taken;
+    const int n = min(t.S - base, kTableThreads);
+    for (int i = tid; i < all_pages && pages_before + i < n_free; i += kTableThreads) {
+      const int k = find(s_page, n, i);
+      if (s_have[k] >= 0)
+        t.tables[static_cast<int64_t>(base + k) * t.M + s_have[k] + (i - s_page[k])] = t.free_pages[n_free - 1 - (pages_before + i)];
+    }
+    if (SELF) {
+      __syncthreads();  // (the tables' new entries, seen by this workgroup)
+      const int to = static_cast<int>(tokens_before + all_tokens > N ? N : tokens_before + all_tokens);
+      for (int i = static_cast<int>(tokens_before > N ? N : tokens_before) + tid; i < to; i += kTableThreads) {
+        const int k = find(s_token, n, i);
+        if (s_base[k] >= 0) {
+          write_token(t, i, base + k, s_base[k] + (i - s_token[k]), slots, positions, sequences);
+        } else {
+          slots[i] = positions[i] = sequences[i] = -1;
+        }
+      }
+    }
+    tokens_before += all_tokens;
+    pages_before += all_pages;
+    __syncthreads();
+  }
+  if (SELF)
+    for (int i = static_cast<int>(tokens_before > N ? N : tokens_before) + tid; i < N; i += kTableThreads)
+      slots[i] = positions[i] = sequences[i] = -1;
+  if (tid == 0) {
+    *t.free_count = n_free - taken;
+    if (!SELF) ws[2 * t.S] = static_cast<int>(tokens_before > N ? N : tokens_before);
+  }
+}
+
+__global__ __launch_bounds__(256) void k_tokens(Tables t, int N, int32_t* __restrict__ slots,
+                                                int32_t* __restrict__ positions, int32_t* __restrict__ sequences,
+                                                const int32_t* __restrict__ ws) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= N) return;
+  if (i < ws[2 * t.S]) {
+    const int s = find(ws, t.S, i);
+    if (ws[t.S + s] >= 0) return write_token(t, i, s, ws[t.S + s] + (i - ws[s]), slots, positions, sequences);
+  }
+  slots[i] = positions[i] = sequences[i] = -1;
+}
+
+__global__ __launch_bounds__(kTableThreads) void k_shrink(Tables t, const int32_t* __restrict__ to) {
+  __shared__ int part[kTableThreads / 64];
+  __shared__ int s_page[kTableThreads], s_keep[kTableThreads];
+  const int tid = threadIdx.x;
+  const int P = 1 << t.shift;
+  const int64_t cap = min(static_cast<int64_t>(t.M) << t.shift, static_cast<int64_t>(INT32_MAX));
+  const int n_free = clampi(*t.free_count, 0, t.pages);
+  auto cut = [&](int s, int& keep, int& drop) {  // the sequence's new length
+    int64_t len = t.lengths[s];
+    len = len < 0 ? 0 : len > cap ? cap : len;
+    const int64_t now = min(len, static_cast<int64_t>(max(to[s], 0)));
+    keep = static_cast<int>((now + P - 1) >> t.shift);
+    drop = static_cast<int>((len + P - 1) >> t.shift) - keep;
+    return static_cast<int>(now);
+  };
+  int total = 0;
+  if (t.S > kTableThreads) {  // the whole call's pages first: they are laid from the last one down
+    int sum = 0, keep, drop;
+    for (int s = tid; s < t.S; s += kTableThreads) {
+      cut(s, keep, drop);
+      sum += drop;
+    }
+    scan_exclusive<int>(sum, part, total);
+  }
+  int before = 0;
+  for (int base = 0; base < t.S; base += kTableThreads) {
+    const int s = base + tid;
+    int keep = 0, drop = 0, now = 0;
+    if (s < t.S) now = cut(s, keep, drop);
+    int all;
+    const int first = scan_exclusive<int>(drop, part, all);
+    if (t.S <= kTableThreads) total = all;
+    s_page[tid] = first;
+    s_keep[tid] = keep;
+    if (s < t.S) t.lengths[s] = now;
+    __syncthreads();
+    const int n = min(t.S - base, kTableThreads);
+    for (int i = tid; i < all; i += kTableThreads) {
+      const int k = find(s_page, n, i);
+      const int64_t at = static_cast<int64_t>(n_free) + total - 1 - (before + i);
+      if (at >= 0 && at < t.pages)  // (more pages than there are: tables that no call of extend wrote)
+        t.free_pages[at] = t.tables[static_cast<int64_t>(base + k) * t.M + s_keep[k] + (i - s_page[k])];
+    }
+    before += all;
+    __syncthreads();
+  }
+  if (tid == 0) *t.free_count = min(n_free + total, t.pages);
+}
+
+}  // namespace vpg
