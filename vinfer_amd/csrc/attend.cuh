@@ -1,16 +1,19 @@
 // Attention of sequences in groups that share a prefix, over pages.
 //
 // The rows that read a run of keys lie side by side: all of a group's (sequence, token, query head) rows of a key head
-// on its prefix, a sequence's (token, query head) rows on its own keys. A segment is up to kRows such rows on one run
-// of keys; per key head the segments' tiles of kKeys keys make one long line, all heads' lines are cut into as many
-// equal stretches as workgroups fit the chip, and each workgroup walks one stretch (the plan, made once a step). So
-// any mix of long and short keys, few and many rows, fills the chip evenly. Rows whose keys fall into several
-// stretches leave each one's maximum, sum and products (fp32), joined by a second kernel in the stretches' order.
+// on its prefix, a sequence's (token, query head) rows on its own keys. A segment is some of these rows on one run of
+// keys, in tiles. Two kinds are kept apart: wide segments (up to 128 rows where there are more than 32) are a
+// workgroup's, 32 rows a wave on one tile of 64 keys; narrow ones (up to 32 rows) are a wave's alone, in tiles of 32
+// keys. Per key head the segments' tiles make one long line; all heads' lines of a kind are cut into as many equal
+// stretches as workgroups (waves) fit the chip, and each walks its own (the plan, made once a step): any mix of long
+// and short keys, few and many rows, fills the chip evenly. Rows whose keys fall into several stretches leave each
+// one's maximum, sum and products (fp32), joined by a second kernel in the stretches' order.
 //
 // A tile: S^T = K Q^T by 32x32x16 matrix products (a lane holds one row's scores: maxima and sums stay in the lane
 // and its partner 32 lanes on), running maximum and sum, P rounded to the values' type, O^T += V^T P^T with V read
 // from LDS transposed, which brings its keys in the order in which the scores lie in a lane: P never leaves the
-// registers. Next tiles' keys and values come through registers into the other half of LDS while a tile is computed.
+// registers. The next tile's keys and values are on their way to registers while a tile is computed; their pages are
+// looked up a tile before that, by scalar loads (eight keys at a time).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -29,15 +32,15 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kRows = 128;  // of a segment: 32 a wave
+constexpr int kRows = 128;  // of a wide segment: 32 a wave
+constexpr int kNarrow = 32;  // of a narrow one
 constexpr int kWaves = 4;
-
-// Keys of a tile: as many as two halves of LDS hold with two workgroups a CU.
-constexpr int tile_keys(int head_dim) { return head_dim > 128 ? 32 : 64; }
+constexpr int kWideKeys = 64, kNarrowKeys = 32;  // of a tile
 
 struct Shape {
   int S, B, T, H, Hkv, D, shift, M, MP;
-  int G, rows, own_tiles, max_prefix, keys, wgs;  // query heads a key head; T G; a sequence's segments; the prefixes'
+  int G, rows, own_tiles, wgs;     // query heads a key head; T G; a sequence's segments; workgroups
+  int max_wide, max_narrow;        // segments there are room for
 };
 
 // A segment: `rows` rows from row0 of those that sequences from seq0 on make, on a run of keys.
@@ -48,39 +51,68 @@ struct alignas(16) Segment {
 };
 constexpr int kAlone = 1 << 30;  // in rows: no other segment has these rows
 
-struct Head {
-  int units, n_prefix, n_own, per_wg;  // tiles of a head's line; segments; tiles of a workgroup
+// What a row's joining needs: of its sequence's segment, and of its group's first.
+struct alignas(16) Place {
+  int keys, tiles, unit, index;  // keys 0: there are none
+};
+struct alignas(16) PrefixPlace {
+  int tiles, unit, index, row0;  // tiles 0: none; row0: the sequence's first row, or ~that where the group is wide
 };
 
-// The plan in memory, all of 4-byte words.
-struct Plan {
-  Head* head;
-  int2* start;      // [wgs]: a workgroup's first segment, and the tile in it
-  int* own;         // [S own_tiles]: segments of the sequences, -1 where there are no keys
-  int* group;       // [S]: a sequence's group, or -1
-  int* prefix;      // [B]: a group's first segment, or -1
-  Segment* segments;
+struct alignas(16) Start {  // of a stretch
+  int segment, tile, head, left;  // left: tiles in all
 };
-__host__ __device__ inline Plan plan_at(const Shape& s, void* p) {
+
+struct alignas(16) Lines {
+  int wide_units, n_wide, wide_per;        // tiles of a head's line, segments, tiles of a stretch
+  int narrow_units, n_narrow, narrow_per;
+  int n_narrow_prefix, n_narrow_own;
+};
+
+struct Plan {
+  Lines* lines;
+  Start *wide_start, *narrow_start;  // [wgs], [wgs kWaves]
+  Place* own;                        // [S own_tiles]
+  PrefixPlace* prefix;               // [S]
+  int4* group;                       // [B]: a group's prefix segments: tiles, unit, index, wide
+  Segment *wide, *narrow;
+};
+__host__ __device__ inline Plan plan_at(const Shape& s, void* p, size_t* bytes = nullptr) {
   char* c = static_cast<char*>(p);
-  auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    char* r = c + at;
+    at += (n + 255) & ~static_cast<size_t>(255);
+    return r;
+  };
   Plan r;
-  r.head = reinterpret_cast<Head*>(c);
-  size_t at = 256;
-  r.start = reinterpret_cast<int2*>(c + at);
-  at += up(static_cast<size_t>(s.wgs) * 8);
-  r.own = reinterpret_cast<int*>(c + at);
-  at += up(static_cast<size_t>(s.S) * s.own_tiles * 4);
-  r.group = reinterpret_cast<int*>(c + at);
-  at += up(static_cast<size_t>(s.S) * 4);
-  r.prefix = reinterpret_cast<int*>(c + at);
-  at += up(static_cast<size_t>(s.B) * 4);
-  r.segments = reinterpret_cast<Segment*>(c + at);
+  r.lines = reinterpret_cast<Lines*>(take(sizeof(Lines)));
+  r.wide_start = reinterpret_cast<Start*>(take(s.wgs * sizeof(Start)));
+  r.narrow_start = reinterpret_cast<Start*>(take(s.wgs * kWaves * sizeof(Start)));
+  r.own = reinterpret_cast<Place*>(take(static_cast<size_t>(s.S) * s.own_tiles * sizeof(Place)));
+  r.prefix = reinterpret_cast<PrefixPlace*>(take(s.S * sizeof(PrefixPlace)));
+  r.group = reinterpret_cast<int4*>(take(s.B * sizeof(int4)));
+  r.wide = reinterpret_cast<Segment*>(take(static_cast<size_t>(s.max_wide) * sizeof(Segment)));
+  r.narrow = reinterpret_cast<Segment*>(take(static_cast<size_t>(s.max_narrow) * sizeof(Segment)));
+  if (bytes) *bytes = at;
   return r;
 }
-inline size_t plan_bytes(const Shape& s) {
-  const Plan p = plan_at(s, nullptr);
-  return reinterpret_cast<size_t>(p.segments) + (static_cast<size_t>(s.max_prefix) + static_cast<size_t>(s.S) * s.own_tiles) * sizeof(Segment);
+
+// A line's stretches: those that begin within a segment are written by its thread.
+__device__ __forceinline__ void write_starts(const Segment* segments, int n, int units, int per, int heads, Start* out, int first) {
+  const int64_t all = static_cast<int64_t>(units) * heads;
+  for (int64_t item = first; item < static_cast<int64_t>(n) * heads; item += kTableThreads) {
+    const int h = static_cast<int>(item / n), j = static_cast<int>(item - static_cast<int64_t>(h) * n);
+    const int64_t from = static_cast<int64_t>(h) * units + segments[j].unit, to = from + segments[j].tiles;
+    for (int64_t w = (from + per - 1) / per; w * per < to; ++w) {
+      Start s;
+      s.segment = j;
+      s.tile = static_cast<int>(w * per - from);
+      s.head = h;
+      s.left = static_cast<int>(min(static_cast<int64_t>(per), all - w * per));
+      out[w] = s;
+    }
+  }
 }
 
 __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* __restrict__ lengths,
@@ -91,7 +123,8 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
   const int tid = threadIdx.x;
   const int64_t max_own = min(static_cast<int64_t>(z.M) << z.shift, static_cast<int64_t>(INT32_MAX) - 64);
   const int64_t max_prefix = min(static_cast<int64_t>(z.MP) << z.shift, static_cast<int64_t>(INT32_MAX) - 64);
-  int segments = 0, units = 0;
+  const bool own_narrow = z.rows <= kNarrow;
+  int sequences = 0, n_wide = 0, n_narrow = 0, wide_units = 0, narrow_units = 0;
   for (int base = 0; base < z.B; base += kTableThreads) {  // the groups' prefixes
     const int g = base + tid;
     int seq0 = 0, n = 0, len = 0, total;
@@ -100,16 +133,25 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
       n = max(clampi(group_starts[g + 1], 0, z.S) - seq0, 0);
       len = static_cast<int>(min(static_cast<int64_t>(max(prefix_lengths[g], 0)), max_prefix));
     }
+    const int before = sequences + scan_exclusive<int>(n, part, total);
+    sequences = min(sequences + total, z.S + 1);
+    if (before + static_cast<int64_t>(n) > z.S) n = 0;  // (group_starts that do not ascend)
     const int64_t rows = static_cast<int64_t>(n) * z.rows;
-    const int tiles = (len + z.keys - 1) / z.keys;
-    int mine = tiles ? static_cast<int>((rows + kRows - 1) / kRows) : 0;
-    const int first = segments + scan_exclusive<int>(mine, part, total);
-    segments += total;
-    if (first + mine > z.max_prefix) mine = 0;  // (group_starts that do not ascend)
-    const int unit = units + scan_exclusive<int>(mine * tiles, part, total);
-    units += total;
-    if (g < z.B) plan.prefix[g] = mine ? first : -1;
-    for (int i = 0; i < mine; ++i) {
+    const bool is_wide = rows > kNarrow;
+    const int keys = is_wide ? kWideKeys : kNarrowKeys, tiles = (len + keys - 1) / keys;
+    const int wide = tiles && is_wide ? static_cast<int>((rows + kRows - 1) / kRows) : 0;
+    const int narrow = tiles && rows && !is_wide;
+    const int first_wide = n_wide + scan_exclusive<int>(wide, part, total);
+    n_wide += total;
+    const int wide_unit = wide_units + scan_exclusive<int>(wide * tiles, part, total);
+    wide_units += total;
+    const int first_narrow = n_narrow + scan_exclusive<int>(narrow, part, total);
+    n_narrow += total;
+    const int narrow_unit = narrow_units + scan_exclusive<int>(narrow ? tiles : 0, part, total);
+    narrow_units += total;
+    if (g < z.B)
+      plan.group[g] = make_int4(wide || narrow ? tiles : 0, wide ? wide_unit : narrow_unit, wide ? first_wide : first_narrow, wide != 0);
+    for (int i = 0; i < wide + narrow; ++i) {
       Segment s;
       s.table = ~g;
       s.seq0 = seq0;
@@ -117,23 +159,33 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
       s.rows = static_cast<int>(min(rows - static_cast<int64_t>(i) * kRows, static_cast<int64_t>(kRows)));
       s.keys = len;
       s.tiles = tiles;
-      s.unit = unit + i * tiles;
-      s.index = first + i;
-      plan.segments[first + i] = s;
+      s.unit = wide ? wide_unit + i * tiles : narrow_unit;
+      s.index = wide ? first_wide + i : first_narrow;
+      if (wide) plan.wide[s.index] = s;
+      else plan.narrow[s.index] = s;
     }
   }
-  segments = min(segments, z.max_prefix);
-  const int n_prefix = segments;
+  const int n_narrow_prefix = n_narrow;
+  __syncthreads();
   for (int s = tid; s < z.S; s += kTableThreads) {
-    int g = -1;
+    PrefixPlace p{0, 0, 0, 0};
     if (z.B) {
-      g = find(group_starts, z.B, s);
-      if (s < group_starts[g] || s >= group_starts[g + 1]) g = -1;
+      const int g = find(group_starts, z.B, s), seq0 = max(group_starts[g], 0);
+      if (s >= seq0 && s < group_starts[g + 1]) {
+        const int4 q = plan.group[g];
+        p.tiles = q.x;
+        p.unit = q.y;
+        p.index = q.z;
+        p.row0 = (s - seq0) * z.rows;
+        if (q.w) p.row0 = ~p.row0;
+      }
     }
-    plan.group[s] = g;
+    plan.prefix[s] = p;
   }
   __syncthreads();
-  const int n_items = z.S * z.own_tiles;
+  const int n_items = z.S * z.own_tiles, keys = own_narrow ? kNarrowKeys : kWideKeys;
+  int& n_own = own_narrow ? n_narrow : n_wide;
+  int& units = own_narrow ? narrow_units : wide_units;
   int own = 0;
   for (int base = 0; base < n_items; base += kTableThreads) {  // the sequences' own keys
     const int item = base + tid;
@@ -144,41 +196,42 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
       rows = min(z.rows - row0, kRows);
       len = static_cast<int>(min(static_cast<int64_t>(max(lengths[s], 0)), max_own));
       const int seen = min(len, len - z.T + 1 + (row0 + rows - 1) / z.G);  // by the last row
-      tiles = seen > 0 ? (seen + z.keys - 1) / z.keys : 0;
+      tiles = seen > 0 ? (seen + keys - 1) / keys : 0;
     }
-    const int index = own + scan_exclusive<int>(tiles > 0, part, total);
+    const int at = scan_exclusive<int>(tiles > 0, part, total);
+    const int segment = n_own + at, index = own_narrow ? own + at : segment;
+    n_own += total;
     own += total;
     const int unit = units + scan_exclusive<int>(tiles, part, total);
     units += total;
-    if (item < n_items) plan.own[item] = tiles ? n_prefix + index : -1;
+    if (item < n_items) plan.own[item] = Place{tiles ? len : 0, tiles, unit, index};
     if (tiles) {
-      const int g = plan.group[s];
       Segment w;
       w.table = s;
       w.seq0 = s;
       w.row0 = row0;
-      w.rows = rows | (g < 0 || plan.prefix[g] < 0 ? kAlone : 0);
+      w.rows = rows | (plan.prefix[s].tiles ? 0 : kAlone);
       w.keys = len;
       w.tiles = tiles;
       w.unit = unit;
       w.index = index;
-      plan.segments[n_prefix + index] = w;
+      (own_narrow ? plan.narrow : plan.wide)[segment] = w;
     }
   }
-  const int64_t all = static_cast<int64_t>(units) * z.Hkv;
-  const int per_wg = static_cast<int>((all + z.wgs - 1) / z.wgs);
-  if (tid == 0) *plan.head = Head{units, n_prefix, own, per_wg};
+  auto per = [&](int units_, int stretches) {
+    return static_cast<int>(max((static_cast<int64_t>(units_) * z.Hkv + stretches - 1) / stretches, static_cast<int64_t>(1)));
+  };
+  const int wide_per = per(wide_units, z.wgs), narrow_per = per(narrow_units, z.wgs * kWaves);
+  if (tid == 0)
+    *plan.lines = Lines{wide_units, n_wide, wide_per, narrow_units, n_narrow, narrow_per, n_narrow_prefix, own_narrow ? own : 0};
+  // (stretches without tiles)
+  for (int w = tid; w < z.wgs; w += kTableThreads)
+    if (static_cast<int64_t>(w) * wide_per >= static_cast<int64_t>(wide_units) * z.Hkv) plan.wide_start[w] = Start{0, 0, 0, 0};
+  for (int w = tid; w < z.wgs * kWaves; w += kTableThreads)
+    if (static_cast<int64_t>(w) * narrow_per >= static_cast<int64_t>(narrow_units) * z.Hkv) plan.narrow_start[w] = Start{0, 0, 0, 0};
   __syncthreads();
-  for (int w = tid; w < z.wgs; w += kTableThreads) {
-    const int64_t u = static_cast<int64_t>(w) * per_wg;
-    if (u >= all) continue;
-    const int at = static_cast<int>(u % units);
-    int lo = 0;
-    const int n = n_prefix + own;
-    for (int step = 1 << (31 - __clz(n)); step; step >>= 1)
-      if (lo + step < n && plan.segments[lo + step].unit <= at) lo += step;
-    plan.start[w] = make_int2(lo, at - plan.segments[lo].unit);
-  }
+  write_starts(plan.wide, n_wide, wide_units, wide_per, z.Hkv, plan.wide_start, tid);
+  write_starts(plan.narrow, n_narrow, narrow_units, narrow_per, z.Hkv, plan.narrow_start, tid);
 }
 
 struct AttendArgs {
@@ -193,19 +246,21 @@ struct AttendArgs {
   int64_t table_stride, prefix_table_stride;
   void* out;
   void* plan;
-  // Partial results, by rows: those of segments that a workgroup began or ended within (two a workgroup, cut_rows
-  // each), then those of whole segments of sequences, own_rows each, and of prefixes, prefix_rows each.
+  // Partial results, by rows: those of segments that a stretch began or ended within (two a stretch, 128 and narrow_rows
+  // each), then those of whole segments.
   float* o;    // [..][D]
   float2* ml;  // maximum (in powers of 2) and sum
-  int64_t own_at, prefix_at;
-  int cut_rows, own_rows, prefix_rows;
+  int64_t narrow_cut_at, wide_at, prefix_at, own_at;
+  int narrow_rows, own_rows;
 };
 
-// Where the rows of segment g of head h are that stretch w has from `tile` on.
-__device__ __forceinline__ int64_t partial_row(const AttendArgs& a, const Head& head, const Segment& g, int h, int w, bool whole, bool from_start) {
-  if (!whole) return static_cast<int64_t>(2 * w + from_start) * a.cut_rows;
-  if (g.table < 0) return a.prefix_at + (static_cast<int64_t>(h) * head.n_prefix + g.index) * a.prefix_rows;
-  return a.own_at + (static_cast<int64_t>(h) * head.n_own + g.index) * a.own_rows;
+// Where the rows of a segment of head h are that stretch w has.
+__device__ __forceinline__ int64_t partial_row(const AttendArgs& a, const Lines& n, bool wide, bool prefix, int index, int h, int w,
+                                               bool whole, bool from_start) {
+  if (wide) return (whole ? a.wide_at : 0) + (whole ? static_cast<int64_t>(h) * n.n_wide + index : 2 * w + from_start) * kRows;
+  if (!whole) return a.narrow_cut_at + static_cast<int64_t>(2 * w + from_start) * a.narrow_rows;
+  return prefix ? a.prefix_at + (static_cast<int64_t>(h) * n.n_narrow_prefix + index) * a.narrow_rows
+                : a.own_at + (static_cast<int64_t>(h) * n.n_narrow_own + index) * a.own_rows;
 }
 
 // Workgroups of neighbouring stretches on one XCD: its L2 serves those that read the same keys.
@@ -226,171 +281,197 @@ struct Mma<_Float16> {
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
-// DP: the head's elements, rounded up to a multiple of 32.
-template <class T, int DP>
-__global__ __launch_bounds__(kWaves * 64, DP > 192 ? 1 : 2) void k_attend(AttendArgs a) {
+// What the plan and the tables hold, by scalar loads: nothing writes them while a kernel runs.
+template <class X>
+__device__ __forceinline__ X uniform(const X* p) {
+  static_assert(sizeof(X) % 4 == 0, "words");
+  typedef const __attribute__((address_space(4))) int* Words;
+  Words w = (Words)(reinterpret_cast<uintptr_t>(p));
+  X x;
+  int* to = reinterpret_cast<int*>(&x);
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(X) / 4; ++i) to[i] = w[i];
+  return x;
+}
+
+// What lanes of a wave wrote to LDS, read by its other lanes: a wave's accesses stay in order, the compiler has to know.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// A tile's layout in LDS. Keys' rows are 16 bytes longer: 16 keys' pieces lie in 16 different groups of banks. The values'
+// rows are 16 words on, modulo 32, so that four keys' 64 bytes (a transposed read of half a wave) fill the banks.
+template <int DP>
+struct Layout {
+  static constexpr int kStrideK = DP + 8, kStrideV = DP % 64 ? DP : DP + 32;
+  static constexpr int kPieces = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes of a key's 16-byte pieces
+  static constexpr int kAtOnce = 64 / kPieces;                        // keys of an access
+};
+
+// A segment's keys and values of a head on their way: KEYS of them by this wave.
+template <class T, int DP, int KEYS>
+struct Stage {
   typedef typename Mma<T>::V8 V8;
-  constexpr int kKeys = tile_keys(DP), CH = DP / 8, kThreads = kWaves * 64;
-  constexpr int kLoads = kKeys * CH / kThreads;  // 16-byte pieces of keys (and of values) that a thread brings
-  static_assert(kKeys * CH % kThreads == 0, "a tile is whole pieces of every thread");
-  // Rows 16 bytes longer: 16 keys' pieces lie in 16 different groups of banks. The values' rows are 16 words on, modulo
-  // 64, so that four keys' 64 bytes (a transposed read of half a wave) fill the banks.
-  constexpr int kStrideK = DP + 8, kStrideV = DP % 64 ? DP : DP + 32;
-  __shared__ __align__(16) T s_k[2][kKeys * kStrideK];
-  __shared__ __align__(16) T s_v[2][kKeys * kStrideV];
-  const Shape& z = a.z;
-  const Plan plan = plan_at(z, a.plan);
-  const Head head = *plan.head;
-  const int w = stretch_of(blockIdx.x, z.wgs);
-  const int64_t all = static_cast<int64_t>(head.units) * z.Hkv, u0 = static_cast<int64_t>(w) * head.per_wg;
-  if (u0 >= all) return;
-  int left = static_cast<int>(min(static_cast<int64_t>(head.per_wg), all - u0));
-  int h = static_cast<int>(u0 / head.units);
-  const int2 start = plan.start[w];
-  int seg = start.x, tile = start.y;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int col = lane & 31, half = lane >> 5;
-  const int n_segments = head.n_prefix + head.n_own;
+  typedef Layout<DP> L;
+  static constexpr int kLoads = KEYS / L::kAtOnce, kGroups = KEYS / 8, kVariants = 8 / L::kAtOnce;
+  V8 k[kLoads], v[kLoads];
+  int pages[kGroups];
+  const int32_t* table;
+  const T *k_head, *v_head;
+  int last;  // key
 
-  for (; left > 0; ++seg, tile = 0) {
-    if (seg == n_segments) {
-      seg = 0;
-      ++h;
-    }
-    const Segment g = plan.segments[seg];
-    const int n = min(left, g.tiles - tile);
-    left -= n;
-    const bool prefix = g.table < 0;
-    const int n_rows = g.rows & (kAlone - 1);
-    const bool busy = wave * 32 < n_rows;
-
-    // this lane's row: its queries, and the keys that it sees
-    const int r = wave * 32 + col;
-    const bool valid = r < n_rows;
-    V8 q[DP / 16];
-    int limit = 0;
-    if (busy) {
-      const int R = g.row0 + (valid ? r : 0);
-      const int in = R / z.rows, rest = R - in * z.rows, t = rest / z.G, gq = rest - t * z.G;
-      const T* from = static_cast<const T*>(a.q) + (g.seq0 + in) * a.q_stride + t * a.q_token + (h * z.G + gq) * a.q_head;
-      limit = prefix ? g.keys : min(g.keys, g.keys - z.T + t + 1);
+  __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& g, int h) {
+    table = g.table < 0 ? a.prefix_tables + static_cast<int64_t>(~g.table) * a.prefix_table_stride
+                        : a.tables + static_cast<int64_t>(g.table) * a.table_stride;
+    k_head = static_cast<const T*>(a.k) + h * a.head_stride;
+    v_head = static_cast<const T*>(a.v) + h * a.head_stride;
+    last = g.keys - 1;
+  }
+  // The pages of the keys from key0 on (keys past the last: the last eight once more).
+  __device__ __forceinline__ void look_up(const AttendArgs& a, int key0) {
+    if (a.z.shift < 3) return;
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        const int d = c * 16 + half * 8;
-        if (d < z.D) q[c] = *reinterpret_cast<const V8*>(from + d);
-        else q[c] = V8{};
-      }
-    }
-    const int least = prefix ? g.keys : min(g.keys, g.keys - z.T + 1 + (g.row0 + wave * 32) / z.G);  // of the wave's rows
-
-    const int32_t* table = prefix ? a.prefix_tables + static_cast<int64_t>(~g.table) * a.prefix_table_stride
-                                  : a.tables + static_cast<int64_t>(g.table) * a.table_stride;
-    const T* k_head = static_cast<const T*>(a.k) + h * a.head_stride;
-    const T* v_head = static_cast<const T*>(a.v) + h * a.head_stride;
-    V8 k_in[kLoads], v_in[kLoads];
-    auto fetch = [&](int tile_at) {
+    for (int g = 0; g < kGroups; ++g) pages[g] = uniform(table + (min(key0 + 8 * g, last & ~7) >> a.z.shift));
+  }
+  __device__ __forceinline__ void fetch(const AttendArgs& a, int key0) {
+    const int lane = threadIdx.x & 63, in = lane / L::kPieces, c = lane % L::kPieces;
+    const int mask = (1 << a.z.shift) - 1;
+    if (c * 8 >= a.z.D) return;
+    if (a.z.shift >= 3) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int piece = tid + i * kThreads, key = piece / CH, c = piece % CH;
-        const int j = min(tile_at * kKeys + key, g.keys - 1);  // (keys past the last are the last once more)
-        const int page = clampi(table[j >> z.shift], 0, a.pages - 1);
-        const int64_t at = page * a.page_stride + (j & ((1 << z.shift) - 1)) * a.place_stride + c * 8;
-        if (c * 8 < z.D) {
-          k_in[i] = *reinterpret_cast<const V8*>(k_head + at);
-          v_in[i] = *reinterpret_cast<const V8*>(v_head + at);
-        } else {
-          k_in[i] = V8{};
-          v_in[i] = V8{};
+      for (int g = 0; g < kGroups; ++g) {
+        const int first = min(key0 + 8 * g, last & ~7);
+        const int64_t at = clampi(pages[g], 0, a.pages - 1) * a.page_stride + (first & mask) * a.place_stride;
+        const char *kp = reinterpret_cast<const char*>(k_head + at), *vp = reinterpret_cast<const char*>(v_head + at);
+#pragma unroll
+        for (int i = 0; i < kVariants; ++i) {
+          const int key = min(i * L::kAtOnce + in, last - first);
+          const uint32_t off = (static_cast<uint32_t>(key) * static_cast<uint32_t>(a.place_stride) + c * 8) * 2;
+          k[g * kVariants + i] = *reinterpret_cast<const V8*>(kp + off);
+          v[g * kVariants + i] = *reinterpret_cast<const V8*>(vp + off);
         }
       }
-    };
-    auto put = [&](int b) {
+    } else {  // pages of fewer than eight keys
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int piece = tid + i * kThreads, key = piece / CH, c = piece % CH;
-        *reinterpret_cast<V8*>(&s_k[b][key * kStrideK + c * 8]) = k_in[i];
-        *reinterpret_cast<V8*>(&s_v[b][key * kStrideV + c * 8]) = v_in[i];
+        const int key = min(key0 + i * L::kAtOnce + in, last);
+        const int64_t at = clampi(table[key >> a.z.shift], 0, a.pages - 1) * a.page_stride + (key & mask) * a.place_stride + c * 8;
+        k[i] = *reinterpret_cast<const V8*>(k_head + at);
+        v[i] = *reinterpret_cast<const V8*>(v_head + at);
       }
-    };
+    }
+  }
+  __device__ __forceinline__ void put(const AttendArgs& a, T* s_k, T* s_v) {
+    const int lane = threadIdx.x & 63, in = lane / L::kPieces, c = lane % L::kPieces;
+    if (c * 8 >= a.z.D) return;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      *reinterpret_cast<V8*>(s_k + (i * L::kAtOnce + in) * L::kStrideK + c * 8) = k[i];
+      *reinterpret_cast<V8*>(s_v + (i * L::kAtOnce + in) * L::kStrideV + c * 8) = v[i];
+    }
+  }
+};
 
-    float m = -INFINITY, l = 0.0f;
-    f32x16 o[DP / 32];
+// A wave's 32 rows: a lane has row `lane % 32`, with its partner 32 lanes on.
+template <class T, int DP>
+struct Rows {
+  typedef typename Mma<T>::V8 V8;
+  typedef Layout<DP> L;
+  V8 q[DP / 16];
+  f32x16 o[DP / 32];
+  float m, l;
+  int limit;  // the keys before it are seen
+
+  __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& g, int h, int r, bool valid) {
+    const Shape& z = a.z;
+    const int half = (threadIdx.x & 63) >> 5;
+    const int R = g.row0 + (valid ? r : 0);
+    const int in = R / z.rows, rest = R - in * z.rows, t = rest / z.G, gq = rest - t * z.G;
+    const T* from = static_cast<const T*>(a.q) + (g.seq0 + in) * a.q_stride + t * a.q_token + (h * z.G + gq) * a.q_head;
+    limit = g.table < 0 ? g.keys : min(g.keys, g.keys - z.T + t + 1);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      const int d = c * 16 + half * 8;
+      if (d < z.D) q[c] = *reinterpret_cast<const V8*>(from + d);
+      else q[c] = V8{};
+    }
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
-    fetch(tile);
-    __syncthreads();  // (the segment before is read)
-    put(0);
-    if (n > 1) fetch(tile + 1);
-    __syncthreads();
-    for (int it = 0; it < n; ++it) {
-      const int b = it & 1, key0 = (tile + it) * kKeys;
-      if (busy) {
-        f32x16 s[kKeys / 32];
-        float most = -INFINITY;
+    m = -INFINITY;
+    l = 0.0f;
+  }
+
+  // BLOCKS of 32 keys from key0 on; the rows see those before `least` at least.
+  template <int BLOCKS>
+  __device__ __forceinline__ void tile(const T* s_k, const T* s_v, int key0, int least, float scale) {
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+    f32x16 s[BLOCKS];
+    float most = -INFINITY;
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 32; ++kk) {
-          s[kk] = f32x16{};
+    for (int b = 0; b < BLOCKS; ++b) {
+      s[b] = f32x16{};
 #pragma unroll
-          for (int c = 0; c < DP / 16; ++c) {
-            const V8 kv = *reinterpret_cast<const V8*>(&s_k[b][(kk * 32 + col) * kStrideK + c * 16 + half * 8]);
-            s[kk] = Mma<T>::mma(kv, q[c], s[kk]);
-          }
-        }
-        if (key0 + kKeys > least) {
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 32; ++kk)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (key0 + kk * 32 + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[kk][i] = -INFINITY;
-        }
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 32; ++kk)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) most = fmaxf(most, s[kk][i]);
-        most = fmaxf(most, other_half(most)) * a.scale;
-        if (__any(most > m)) {
-          const float now = fmaxf(m, most), by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
-          m = now;
-          l *= by;
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d) o[d] *= by;
-        }
-        const float from = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 32; ++kk) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            s[kk][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk][i], a.scale, -from));
-            l += s[kk][i];
-          }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            V8 p;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = static_cast<T>(s[kk][8 * c + i]);
-            const T* v0 = &s_v[b][(kk * 32 + c * 16 + 4 * half + (lane & 15) / 4) * kStrideV + (lane >> 4 & 1) * 16 + (lane & 3) * 4];
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) {
-              typedef __attribute__((address_space(3))) s16x4* Lds;
-              const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v0 + d * 32));
-              const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v0 + d * 32 + 8 * kStrideV));
-              const V8 vv = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-              o[d] = Mma<T>::mma(vv, p, o[d]);
-            }
-          }
-        }
+      for (int c = 0; c < DP / 16; ++c) {
+        const V8 kv = *reinterpret_cast<const V8*>(s_k + (b * 32 + col) * L::kStrideK + c * 16 + half * 8);
+        s[b] = Mma<T>::mma(kv, q[c], s[b]);
       }
-      if (it + 1 < n) {
-        put(b ^ 1);
-        if (it + 2 < n) fetch(tile + it + 2);
-      }
-      __syncthreads();
     }
+    if (key0 + BLOCKS * 32 > least) {
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (key0 + b * 32 + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[b][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][i]);
+    most = fmaxf(most, other_half(most)) * scale;
+    if (__any(most > m)) {
+      const float now = fmaxf(m, most), by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= by;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[d] *= by;
+    }
+    const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale, -from));
+        l += s[b][i];
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        V8 p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = static_cast<T>(s[b][8 * c + i]);
+        const T* v0 = s_v + (b * 32 + c * 16 + 4 * half + (lane & 15) / 4) * L::kStrideV + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          typedef __attribute__((address_space(3))) s16x4* Lds;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v0 + d * 32));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v0 + d * 32 + 8 * L::kStrideV));
+          const V8 vv = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          o[d] = Mma<T>::mma(vv, p, o[d]);
+        }
+      }
+    }
+  }
+
+  // The rows' outputs where no other stretch has any of them, else their part.
+  __device__ __forceinline__ void end(const AttendArgs& a, const Lines& lines, const Segment& g, bool wide, int h, int w, int r,
+                                      bool valid, bool whole, bool from_start) {
+    const Shape& z = a.z;
+    const int half = (threadIdx.x & 63) >> 5;
     l += other_half(l);
-    if (!valid || !busy) continue;
-    const int R = g.row0 + r;
-    if ((g.rows & kAlone) && n == g.tiles) {
-      const int t = R / z.G, gq = R - t * z.G;
+    if (!valid) return;
+    if (whole && (g.rows & kAlone)) {
+      const int R = g.row0 + r, t = R / z.G, gq = R - t * z.G;
       T* to = static_cast<T*>(a.out) + ((static_cast<int64_t>(g.seq0) * z.T + t) * z.H + h * z.G + gq) * z.D;
       const float by = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -406,9 +487,9 @@ __global__ __launch_bounds__(kWaves * 64, DP > 192 ? 1 : 2) void k_attend(Attend
             *reinterpret_cast<T4*>(to + at) = y;
           }
         }
-      continue;
+      return;
     }
-    const int64_t row = partial_row(a, head, g, h, w, n == g.tiles, tile == 0) + r;
+    const int64_t row = partial_row(a, lines, wide, g.table < 0, g.index, h, w, whole, from_start) + r;
     float* to = a.o + row * z.D;
     if (half == 0) a.ml[row] = make_float2(m, l);
 #pragma unroll
@@ -419,6 +500,127 @@ __global__ __launch_bounds__(kWaves * 64, DP > 192 ? 1 : 2) void k_attend(Attend
         if (at < z.D) *reinterpret_cast<f32x4*>(to + at) = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
       }
   }
+};
+
+// Heads of more elements than are there are filled up with zeros, once.
+template <class T, int DP, int KEYS>
+__device__ __forceinline__ void clear_rest(const AttendArgs& a, T* s_k, T* s_v, int first, int threads) {
+  typedef Layout<DP> L;
+  const int rest = (DP - a.z.D) / 8;
+  for (int i = first; i < KEYS * rest; i += threads) {
+    const int key = i / rest, c = i - key * rest;
+    *reinterpret_cast<typename Mma<T>::V8*>(s_k + key * L::kStrideK + a.z.D + c * 8) = {};
+    *reinterpret_cast<typename Mma<T>::V8*>(s_v + key * L::kStrideV + a.z.D + c * 8) = {};
+  }
+}
+
+// DP: the head's elements, rounded up to a width there is.
+template <class T, int DP>
+__global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(AttendArgs a) {
+  typedef Layout<DP> L;
+  constexpr int kWideK = kWideKeys * L::kStrideK, kWideV = kWideKeys * L::kStrideV;
+  constexpr int kWaveK = kNarrowKeys * L::kStrideK, kWaveV = kNarrowKeys * L::kStrideV;
+  constexpr int kWords = 2 * (kWideK + kWideV) > kWaves * (kWaveK + kWaveV) ? 2 * (kWideK + kWideV) : kWaves * (kWaveK + kWaveV);
+  __shared__ __align__(16) T lds[kWords];
+  const Shape& z = a.z;
+  const Plan plan = plan_at(z, a.plan);
+  const Lines lines = uniform(plan.lines);
+  const int group = stretch_of(blockIdx.x, z.wgs);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  {  // wide segments: the workgroup's
+    const Start start = uniform(plan.wide_start + group);
+    int left = start.left, h = start.head, seg = start.segment, tile = start.tile;
+    if (left > 0) {
+      T *s_k = lds, *s_v = lds + 2 * kWideK;
+      if (z.D < DP) {
+        clear_rest<T, DP, kWideKeys>(a, s_k, s_v, tid, kWaves * 64);
+        clear_rest<T, DP, kWideKeys>(a, s_k + kWideK, s_v + kWideV, tid, kWaves * 64);
+      }
+      constexpr int kShare = kWideKeys / kWaves;  // keys that a wave brings
+      T *put_k = s_k + wave * kShare * L::kStrideK, *put_v = s_v + wave * kShare * L::kStrideV;
+      for (; left > 0; ++seg, tile = 0) {
+        if (seg == lines.n_wide) {
+          seg = 0;
+          ++h;
+        }
+        const Segment g = uniform(plan.wide + seg);
+        const int n = min(left, g.tiles - tile), n_rows = g.rows & (kAlone - 1);
+        left -= n;
+        const int r = wave * 32 + (lane & 31);
+        const bool busy = wave * 32 < n_rows, valid = r < n_rows;
+        Stage<T, DP, kShare> in;
+        in.begin(a, g, h);
+        const int key0 = tile * kWideKeys, mine = key0 + wave * kShare;
+        in.look_up(a, mine);
+        in.fetch(a, mine);
+        in.look_up(a, mine + kWideKeys);
+        Rows<T, DP> rows;
+        if (busy) rows.begin(a, g, h, r, valid);
+        const int least = g.table < 0 ? g.keys : min(g.keys, g.keys - z.T + 1 + (g.row0 + wave * 32) / z.G);  // of the wave's rows
+        __syncthreads();  // (the segment before is read)
+        in.put(a, put_k, put_v);
+        if (n > 1) {
+          in.fetch(a, mine + kWideKeys);
+          in.look_up(a, mine + 2 * kWideKeys);
+        }
+        __syncthreads();
+        for (int it = 0; it < n; ++it) {
+          const int b = it & 1;
+          if (busy) rows.template tile<kWideKeys / 32>(s_k + b * kWideK, s_v + b * kWideV, key0 + it * kWideKeys, least, a.scale);
+          if (it + 1 < n) {
+            in.put(a, put_k + (b ^ 1) * kWideK, put_v + (b ^ 1) * kWideV);
+            if (it + 2 < n) {
+              in.fetch(a, mine + (it + 2) * kWideKeys);
+              in.look_up(a, mine + (it + 3) * kWideKeys);
+            }
+          }
+          __syncthreads();
+        }
+        if (busy) rows.end(a, lines, g, true, h, group, r, valid, n == g.tiles, tile == 0);
+      }
+    }
+  }
+  {  // narrow segments: each wave's
+    const int w = group * kWaves + wave;
+    const Start start = uniform(plan.narrow_start + w);
+    int left = start.left, h = start.head, seg = start.segment, tile = start.tile;
+    if (left > 0) {
+      T *s_k = lds + wave * (kWaveK + kWaveV), *s_v = s_k + kWaveK;
+      if (z.D < DP) clear_rest<T, DP, kNarrowKeys>(a, s_k, s_v, lane, 64);
+      for (; left > 0; ++seg, tile = 0) {
+        if (seg == lines.n_narrow) {
+          seg = 0;
+          ++h;
+        }
+        const Segment g = uniform(plan.narrow + seg);
+        const int n = min(left, g.tiles - tile), n_rows = g.rows & (kAlone - 1);
+        left -= n;
+        const int r = lane & 31;
+        const bool valid = r < n_rows;
+        Stage<T, DP, kNarrowKeys> in;
+        in.begin(a, g, h);
+        const int key0 = tile * kNarrowKeys;
+        in.look_up(a, key0);
+        in.fetch(a, key0);
+        in.look_up(a, key0 + kNarrowKeys);
+        Rows<T, DP> rows;
+        rows.begin(a, g, h, r, valid);
+        const int least = g.table < 0 ? g.keys : min(g.keys, g.keys - z.T + 1 + g.row0 / z.G);
+        for (int it = 0; it < n; ++it) {
+          wave_order();  // (the tile before is read)
+          in.put(a, s_k, s_v);
+          if (it + 1 < n) {
+            in.fetch(a, key0 + (it + 1) * kNarrowKeys);
+            in.look_up(a, key0 + (it + 2) * kNarrowKeys);
+          }
+          wave_order();
+          rows.template tile<1>(s_k, s_v, key0 + it * kNarrowKeys, least, a.scale);
+        }
+        rows.end(a, lines, g, false, h, w, r, valid, n == g.tiles, tile == 0);
+      }
+    }
+  }
 }
 
 // A wave joins a row's stretches: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
@@ -426,52 +628,52 @@ template <class T, int DP>
 __global__ __launch_bounds__(256) void k_join(AttendArgs a) {
   const Shape& z = a.z;
   const int lane = threadIdx.x & 63;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (id >= static_cast<int64_t>(z.S) * z.T * z.H) return;
   const int hq = static_cast<int>(id % z.H), st = static_cast<int>(id / z.H), t = st % z.T, s = st / z.T;
   const int h = hq / z.G, r = t * z.G + hq % z.G;
   const Plan plan = plan_at(z, a.plan);
-  const Head head = *plan.head;
+  const Lines lines = uniform(plan.lines);
+  const Place own = uniform(plan.own + static_cast<int64_t>(s) * z.own_tiles + r / kRows);
+  const PrefixPlace pre = uniform(plan.prefix + s);
   T* to = static_cast<T*>(a.out) + id * z.D;
-  constexpr int E = (DP + 63) / 64;
-  const int own = plan.own[s * z.own_tiles + r / kRows], grp = plan.group[s];
-  const int pre = grp < 0 ? -1 : plan.prefix[grp];
-  Segment g{};
-  if (own >= 0) g = plan.segments[own];
-  if (own < 0 || g.keys - z.T + t + 1 <= 0) {  // no token
-    for (int d = lane; d < z.D; d += 64) to[d] = static_cast<T>(0.0f);
-    return;
-  }
-  auto stretches = [&](const Segment& x, int& first) {
-    const int64_t u = static_cast<int64_t>(h) * head.units + x.unit;
-    first = static_cast<int>(u / head.per_wg);
-    return static_cast<int>((u + x.tiles - 1) / head.per_wg) - first + 1;
+  constexpr int E = DP > 128 ? 4 : DP > 64 ? 2 : 1;  // elements of a lane, side by side
+  typedef float V __attribute__((ext_vector_type(E)));
+  const bool mine = lane * E < z.D;
+  auto write = [&](V x) {
+    typedef T TV __attribute__((ext_vector_type(E)));
+    TV y;
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = static_cast<T>(x[e]);
+    if (mine) *reinterpret_cast<TV*>(to + lane * E) = y;
   };
-  int first_own, first_pre = 0, n_pre = 0, r_pre = 0;
-  const int n_own = stretches(g, first_own);
-  if (pre < 0 && n_own == 1) return;  // (written already)
-  Segment p{};
-  if (pre >= 0) {
-    const int R = (s - plan.segments[pre].seq0) * z.rows + r;
-    p = plan.segments[pre + R / kRows];
-    n_pre = stretches(p, first_pre);
-    r_pre = R % kRows;
-  }
+  if (own.keys - z.T + t + 1 <= 0) return write(V{});  // no token
+  const bool own_wide = z.rows > kNarrow, pre_wide = pre.row0 < 0;
+  auto stretches = [&](bool wide, int unit, int tiles, int& first) {
+    const int64_t u = static_cast<int64_t>(h) * (wide ? lines.wide_units : lines.narrow_units) + unit;
+    const int per = wide ? lines.wide_per : lines.narrow_per;
+    first = static_cast<int>(u / per);
+    return static_cast<int>((u + tiles - 1) / per) - first + 1;
+  };
+  int first_own, first_pre = 0, n_pre = 0;
+  const int n_own = stretches(own_wide, own.unit, own.tiles, first_own);
+  if (!pre.tiles && n_own == 1) return;  // (written already)
+  const int R = (pre_wide ? ~pre.row0 : pre.row0) + r, segment = pre_wide ? R / kRows : 0;
+  if (pre.tiles) n_pre = stretches(pre_wide, pre.unit + segment * pre.tiles, pre.tiles, first_pre);
   const int n = n_pre + n_own;
   auto row_of = [&](int i) {  // the prefix's stretches, then the sequence's own
-    const bool is_pre = i < n_pre;
-    if (!is_pre) i -= n_pre;
-    return is_pre ? partial_row(a, head, p, h, first_pre + i, n_pre == 1, i == 0) + r_pre
-                  : partial_row(a, head, g, h, first_own + i, n_own == 1, i == 0) + r % kRows;
+    if (i < n_pre)
+      return partial_row(a, lines, pre_wide, true, pre.index + segment, h, first_pre + i, n_pre == 1, i == 0) + (pre_wide ? R % kRows : R);
+    i -= n_pre;
+    return partial_row(a, lines, own_wide, false, own.index, h, first_own + i, n_own == 1, i == 0) + r % kRows;
   };
   float most = -INFINITY;
-  for (int i = lane; i < n; i += 64) {
-    most = fmaxf(most, a.ml[row_of(i)].x);
-  }
+  for (int i = lane; i < n; i += 64) most = fmaxf(most, a.ml[row_of(i)].x);
 #pragma unroll
   for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
   if (most == -INFINITY) most = 0.0f;
-  float total = 0.0f, o[E] = {};
+  float total = 0.0f;
+  V o = {};
   for (int base = 0; base < n; base += 64) {
     float by = 0.0f;
     if (base + lane < n) {
@@ -480,21 +682,20 @@ __global__ __launch_bounds__(256) void k_join(AttendArgs a) {
       total += by * ml.y;
     }
     const int m = min(n - base, 64);
-#pragma unroll 4
-    for (int i = 0; i < m; ++i) {
-      const float f = __shfl(by, i);
-      const float* from = a.o + row_of(base + i) * z.D;
+    for (int i = 0; i < m; i += 8) {
+      V x[8];
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (lane + 64 * e < z.D) o[e] += f * from[lane + 64 * e];
+      for (int j = 0; j < 8; ++j) {
+        x[j] = V{};
+        if (i + j < m && mine) x[j] = *reinterpret_cast<const V*>(a.o + row_of(base + i + j) * z.D + lane * E);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o += __shfl(by, min(i + j, 63)) * x[j];
     }
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
-  const float by = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (lane + 64 * e < z.D) to[lane + 64 * e] = static_cast<T>(o[e] * by);
+  write(o * (total == 0.0f ? 0.0f : 1.0f / total));
 }
 
 }  // namespace vpg

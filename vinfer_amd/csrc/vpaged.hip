@@ -112,7 +112,7 @@ vpg::Tables tables_of(const vpaged_tables* t) {
 
 constexpr int kCus = 256;
 
-// LDS holds two workgroups' tiles a CU for heads of up to 192 elements.
+// LDS and registers hold two workgroups a CU for heads of up to 128 elements.
 bool shape_of(const vpaged_shape* a, vpg::Shape& z) {
   if (!a || a->sequences < 0 || a->sequences > VPAGED_MAX_SEQUENCES || a->groups < 0 || a->groups > VPAGED_MAX_SEQUENCES ||
       a->queries < 1 || a->queries > VPAGED_MAX_QUERIES || a->kv_heads < 1 || a->heads < 1 || a->heads > VPAGED_MAX_HEADS ||
@@ -130,38 +130,48 @@ bool shape_of(const vpaged_shape* a, vpg::Shape& z) {
   z.MP = a->groups > 0 ? a->max_prefix_pages : 0;
   z.G = z.H / z.Hkv;
   const int64_t rows = static_cast<int64_t>(z.T) * z.G, own = (rows + vpg::kRows - 1) / vpg::kRows;
-  const int64_t prefix = z.B ? z.B + static_cast<int64_t>(z.S) * rows / vpg::kRows : 0;
-  z.keys = vpg::tile_keys(z.D);
-  auto tiles = [&](int64_t pages) { return ((pages << z.shift) + z.keys - 1) / z.keys; };
+  const bool own_narrow = rows <= vpg::kNarrow;
+  const int64_t wide = (z.B ? z.B + static_cast<int64_t>(z.S) * rows / vpg::kRows : 0) + (own_narrow ? 0 : z.S * own);
+  const int64_t narrow = z.B + (own_narrow ? z.S : 0);
   // (32 bits number a head's tiles and the segments' rows)
-  if (rows >= 1ll << 24 || (z.B && z.S * rows >= 1ll << 31) || z.S * own >= 1ll << 31 ||
-      static_cast<double>(prefix) * tiles(z.MP) + static_cast<double>(z.S) * own * tiles(z.M) >= 2147483648.0 * 1.0)
+  const int64_t pages = z.M > z.MP ? z.M : z.MP;
+  if (rows >= 1ll << 24 || z.S * rows >= 1ll << 31 || z.S * own >= 1ll << 31 ||
+      static_cast<double>(wide + narrow) * static_cast<double>((pages << z.shift) / vpg::kNarrowKeys + 1) >= 2147483648.0)
     return false;
   z.rows = static_cast<int>(rows);
   z.own_tiles = static_cast<int>(own);
-  z.max_prefix = static_cast<int>(prefix);
-  z.wgs = kCus * (z.D > 192 ? 1 : 2);
+  z.max_wide = static_cast<int>(wide);
+  z.max_narrow = static_cast<int>(narrow);
+  z.wgs = kCus * (z.D > 128 ? 1 : 2);
   return true;
 }
 
 struct AttendLayout {
-  int cut_rows, own_rows, prefix_rows;
-  int64_t own_at, prefix_at, rows;
+  int narrow_rows, own_rows;
+  int64_t narrow_cut_at, wide_at, prefix_at, own_at, rows;
   size_t ml, total;
 };
 AttendLayout attend_layout(const vpg::Shape& z) {
   AttendLayout L;
-  L.own_rows = z.rows < vpg::kRows ? z.rows : vpg::kRows;
-  const int64_t group = static_cast<int64_t>(z.S) * z.rows;  // (all sequences in one)
-  L.prefix_rows = !z.B ? 0 : group < vpg::kRows ? static_cast<int>(group) : vpg::kRows;
-  L.cut_rows = L.own_rows > L.prefix_rows ? L.own_rows : L.prefix_rows;
-  L.own_at = 2ll * z.wgs * L.cut_rows;
-  L.prefix_at = L.own_at + (z.B ? static_cast<int64_t>(z.S) * z.own_tiles * z.Hkv * L.own_rows : 0);
-  L.rows = L.prefix_at + static_cast<int64_t>(z.max_prefix) * z.Hkv * L.prefix_rows;
+  const int64_t group = z.B ? static_cast<int64_t>(z.S) * z.rows : z.rows;  // (all sequences in one)
+  L.narrow_rows = group < vpg::kNarrow ? static_cast<int>(group) : vpg::kNarrow;
+  L.own_rows = z.rows < vpg::kNarrow ? z.rows : vpg::kNarrow;
+  L.narrow_cut_at = z.max_wide ? 2ll * z.wgs * vpg::kRows : 0;
+  L.wide_at = L.narrow_cut_at + (z.max_narrow ? 2ll * z.wgs * vpg::kWaves * L.narrow_rows : 0);
+  // (whole segments leave parts only where there are prefixes)
+  L.prefix_at = L.wide_at + (z.B ? static_cast<int64_t>(z.max_wide) * z.Hkv * vpg::kRows : 0);
+  L.own_at = L.prefix_at + static_cast<int64_t>(z.B) * z.Hkv * L.narrow_rows;
+  L.rows = L.own_at + (z.B && z.rows <= vpg::kNarrow ? static_cast<int64_t>(z.S) * z.Hkv * L.own_rows : 0);
   L.ml = static_cast<size_t>(L.rows) * z.D * 4;
   L.ml = (L.ml + 255) & ~static_cast<size_t>(255);
   L.total = L.ml + static_cast<size_t>(L.rows) * 8;
   return L;
+}
+
+size_t plan_bytes(const vpg::Shape& z) {
+  size_t n;
+  vpg::plan_at(z, nullptr, &n);
+  return n;
 }
 
 const char* const kShapeRule =
@@ -300,17 +310,17 @@ int vpaged_rotate_store(const vpaged_rotate_args* a, void* stream) {
 
 size_t vpaged_plan_bytes(const vpaged_shape* shape) {
   vpg::Shape z;
-  return shape_of(shape, z) ? vpg::plan_bytes(z) : 0;
+  return shape_of(shape, z) ? plan_bytes(z) : 0;
 }
 
 int vpaged_plan(const vpaged_shape* shape, const int32_t* lengths, const int32_t* prefix_lengths, const int32_t* group_starts,
-                void* plan, size_t plan_bytes, void* stream) {
+                void* plan, size_t bytes, void* stream) {
   vpg::Shape z;
   if (!shape_of(shape, z)) return fail(VPAGED_E_ARG, "%s", kShapeRule);
   if (!z.S) return VPAGED_OK;
   if (!lengths || (z.B && (!prefix_lengths || !group_starts)))
     return fail(VPAGED_E_ARG, "lengths, and with groups prefix_lengths and group_starts, must be set");
-  if (int rc = check_memory("plan", plan, plan_bytes, vpg::plan_bytes(z))) return rc;
+  if (int rc = check_memory("plan", plan, bytes, plan_bytes(z))) return rc;
   if (int rc = check_current_device()) return rc;
   vpg::k_plan<<<1, vpg::kTableThreads, 0, static_cast<hipStream_t>(stream)>>>(z, lengths, prefix_lengths, group_starts, plan);
   return launched("vpaged_plan");
@@ -337,6 +347,8 @@ int vpaged_attend(const vpaged_attend_args* a, void* stream) {
       (reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_pages) | reinterpret_cast<uintptr_t>(a->v_pages) |
        reinterpret_cast<uintptr_t>(a->out)) % 16)
     return fail(VPAGED_E_ARG, "q, the pages and out must be 16-byte aligned, with strides of multiples of 8 elements");
+  if ((a->page_stride | a->place_stride | a->head_stride) < 0 || a->place_stride >= 1ll << 27)
+    return fail(VPAGED_E_ARG, "strides of the pages must be >= 0, place_stride below 2^27");
   if (a->table_stride < 0 || (d.z.B && a->prefix_table_stride < 0)) return fail(VPAGED_E_ARG, "table strides must be >= 0");
   const AttendLayout L = attend_layout(d.z);
   if (!a->plan || reinterpret_cast<uintptr_t>(a->plan) & 255u) return fail(VPAGED_E_WORKSPACE, "plan must be set and 256-byte aligned");
@@ -362,11 +374,12 @@ int vpaged_attend(const vpaged_attend_args* a, void* stream) {
   d.plan = const_cast<void*>(a->plan);
   d.o = static_cast<float*>(a->workspace);
   d.ml = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + L.ml);
-  d.own_at = L.own_at;
+  d.narrow_cut_at = L.narrow_cut_at;
+  d.wide_at = L.wide_at;
   d.prefix_at = L.prefix_at;
-  d.cut_rows = L.cut_rows;
+  d.own_at = L.own_at;
+  d.narrow_rows = L.narrow_rows;
   d.own_rows = L.own_rows;
-  d.prefix_rows = L.prefix_rows;
   return a->shape.dtype == VPAGED_BF16 ? attend<__bf16>(d, static_cast<hipStream_t>(stream))
                                        : attend<_Float16>(d, static_cast<hipStream_t>(stream));
 }
