@@ -40,6 +40,7 @@ enum vpaged_status {
 #define VPAGED_MAX_HEADS 1024
 #define VPAGED_MAX_SEQUENCES 65536
 #define VPAGED_MAX_QUERIES 65536
+#define VPAGED_MAX_TOKENS 1073741823 /* vpaged_extend */
 
 int vpaged_abi_version(void);
 

@@ -27,7 +27,7 @@ def test_symbols_version_and_limits_are_the_headers():
         assert hasattr(lib, n), n
     define = lambda n: int(re.search(rf"#define VPAGED_{n} (\d+)", text).group(1))  # noqa: E731
     assert lib.vpaged_abi_version() == _vpaged.ABI_VERSION == define("ABI_VERSION")
-    for n in ("MAX_PAGE_SIZE", "MAX_HEAD_DIM", "MAX_HEADS", "MAX_SEQUENCES", "MAX_QUERIES"):
+    for n in ("MAX_PAGE_SIZE", "MAX_HEAD_DIM", "MAX_HEADS", "MAX_SEQUENCES", "MAX_QUERIES", "MAX_TOKENS"):
         assert define(n) == getattr(_vpaged, n)
 
 
@@ -50,6 +50,19 @@ def test_structs_match_the_binding(tmp_path, name):
     subprocess.run([gcc, f"-I{HEADER.parent}", str(src), "-o", str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [getattr(struct, f).offset for f in fields] + [ctypes.sizeof(struct)]
+
+
+@pytest.mark.parametrize("name", STRUCTS)
+def test_packed_blocks_are_the_structs(name):
+    struct = STRUCTS[name]
+    pack = {"vpaged_tables": _vpaged.PACK_TABLES, "vpaged_rotate_args": _vpaged.PACK_ROTATE, "vpaged_shape": _vpaged.PACK_SHAPE,
+            "vpaged_attend_args": _vpaged.PACK_ATTEND}[name]
+    flat = [f for f, t in struct._fields_ for f in ([f] if t is not _vpaged.VpagedShape else [f"shape.{g}" for g, _ in t._fields_])]
+    values = [i + 1 for i in range(len(flat))]
+    block = struct.from_buffer_copy(pack.pack(*values))
+    assert ctypes.sizeof(struct) == pack.size
+    got = [getattr(block.shape, f[6:]) if f.startswith("shape.") else getattr(block, f) for f in flat]
+    assert got == values
 
 
 def shape(**changes):

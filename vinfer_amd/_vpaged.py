@@ -7,6 +7,7 @@ anything: if the library is missing, ``load()`` raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -23,6 +24,7 @@ MAX_HEAD_DIM = 256
 MAX_HEADS = 1024
 MAX_SEQUENCES = 65536
 MAX_QUERIES = 65536
+MAX_TOKENS = (1 << 30) - 1
 
 STATUS = {0: "ok", 1: "VPAGED_E_ARG", 2: "VPAGED_E_DTYPE", 3: "VPAGED_E_HIP", 4: "VPAGED_E_WORKSPACE", 5: "VPAGED_E_DEVICE"}
 
@@ -138,6 +140,14 @@ class VpagedAttendArgs(ctypes.Structure):
     ]
 
 
+# The same blocks as bytes (``struct`` formats, of their fields in order): packing one is several times as fast as filling
+# a ``Structure``. They begin at multiples of 16 bytes of a bytes object, whose address the library is given.
+PACK_TABLES = struct.Struct("4Q4i")
+PACK_ROTATE = struct.Struct("3Q6q3Q3q3Qf9i")
+PACK_SHAPE = struct.Struct("10i")
+PACK_ATTEND = struct.Struct("10iifQ3q2Q3q2Q2q4Q")
+
+
 class VpagedError(RuntimeError):
     """A failed library call; ``code`` is the VPAGED_E_* status."""
 
@@ -159,20 +169,20 @@ def load() -> ctypes.CDLL:
         if not LIB_PATH.exists():
             raise FileNotFoundError(f"{LIB_PATH} is not built; run `python -m vinfer_amd.csrc.build` (needs hipcc)")
         lib = ctypes.CDLL(str(LIB_PATH))
-        size, ptr = ctypes.c_size_t, ctypes.POINTER
+        size = ctypes.c_size_t
         lib.vpaged_abi_version.restype = ctypes.c_int
         version = lib.vpaged_abi_version()
         if version != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH} has ABI version {version}, expected {ABI_VERSION}")
         lib.vpaged_query.argtypes = [ctypes.c_int, ctypes.c_char_p, size]
         lib.vpaged_extend_workspace_bytes.argtypes = [_i32, _i32]
-        lib.vpaged_extend.argtypes = [ptr(VpagedTables), _p, _i32, _p, _p, _p, _p, _p, size, _p]
-        lib.vpaged_shrink.argtypes = [ptr(VpagedTables), _p, _p]
-        lib.vpaged_rotate_store.argtypes = [ptr(VpagedRotateArgs), _p]
-        lib.vpaged_plan_bytes.argtypes = [ptr(VpagedShape)]
-        lib.vpaged_plan.argtypes = [ptr(VpagedShape), _p, _p, _p, _p, size, _p]
-        lib.vpaged_attend_workspace_bytes.argtypes = [ptr(VpagedShape)]
-        lib.vpaged_attend.argtypes = [ptr(VpagedAttendArgs), _p]
+        lib.vpaged_extend.argtypes = [_p, _p, _i32, _p, _p, _p, _p, _p, size, _p]
+        lib.vpaged_shrink.argtypes = [_p, _p, _p]
+        lib.vpaged_rotate_store.argtypes = [_p, _p]
+        lib.vpaged_plan_bytes.argtypes = [_p]
+        lib.vpaged_plan.argtypes = [_p, _p, _p, _p, _p, size, _p]
+        lib.vpaged_attend_workspace_bytes.argtypes = [_p]
+        lib.vpaged_attend.argtypes = [_p, _p]
         for name in ("query", "extend", "shrink", "rotate_store", "plan", "attend"):
             getattr(lib, f"vpaged_{name}").restype = ctypes.c_int
         for name in ("extend_workspace_bytes", "plan_bytes", "attend_workspace_bytes"):

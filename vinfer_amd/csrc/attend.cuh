@@ -60,7 +60,8 @@ struct alignas(16) PrefixPlace {
 };
 
 struct alignas(16) Start {  // of a stretch
-  int segment, tile, head, left;  // left: tiles in all
+  int segment, tile, head, unused;
+  Segment first;  // the segment
 };
 
 struct alignas(16) Lines {
@@ -98,59 +99,81 @@ __host__ __device__ inline Plan plan_at(const Shape& s, void* p, size_t* bytes =
   return r;
 }
 
-// A line's stretches: those that begin within a segment are written by its thread.
-__device__ __forceinline__ void write_starts(const Segment* segments, int n, int units, int per, int heads, Start* out, int first) {
-  const int64_t all = static_cast<int64_t>(units) * heads;
-  for (int64_t item = first; item < static_cast<int64_t>(n) * heads; item += kTableThreads) {
-    const int h = static_cast<int>(item / n), j = static_cast<int>(item - static_cast<int64_t>(h) * n);
-    const int64_t from = static_cast<int64_t>(h) * units + segments[j].unit, to = from + segments[j].tiles;
-    for (int64_t w = (from + per - 1) / per; w * per < to; ++w) {
-      Start s;
-      s.segment = j;
-      s.tile = static_cast<int>(w * per - from);
-      s.head = h;
-      s.left = static_cast<int>(min(static_cast<int64_t>(per), all - w * per));
-      out[w] = s;
+constexpr int kHeld = 2048;  // segments and groups whose numbers a plan's making holds in LDS
+
+// Where a line's stretches begin. `unit`: the segments' first tiles.
+template <class Index>
+__device__ __forceinline__ void write_starts(const Segment* segments, const int* held, int n, int units, int per, int heads, Start* out) {
+  const Index all = static_cast<Index>(units) * heads;
+  for (Index w = threadIdx.x; w * per < all; w += kTableThreads) {
+    const Index u = w * per;
+    Start s;
+    s.head = static_cast<int>(u / units);
+    const int at = static_cast<int>(u - static_cast<Index>(s.head) * units);
+    int lo = 0;
+    if (n <= kHeld) {
+      lo = find(held, n, at);
+    } else {
+      for (int step = 1 << (31 - __clz(n)); step; step >>= 1)
+        if (lo + step < n && segments[lo + step].unit <= at) lo += step;
     }
+    s.segment = lo;
+    s.first = segments[lo];
+    s.tile = at - s.first.unit;
+    s.unused = 0;
+    out[w] = s;
   }
 }
 
 __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* __restrict__ lengths,
                                                         const int32_t* __restrict__ prefix_lengths,
                                                         const int32_t* __restrict__ group_starts, void* mem) {
-  __shared__ int part[kTableThreads / 64];
+  __shared__ unsigned part1[1][kTableThreads / 64], part4[4][kTableThreads / 64], part2[2][kTableThreads / 64];
+  __shared__ int s_wide[kHeld], s_narrow[kHeld], s_start[kHeld];
+  __shared__ int4 s_group[kHeld];
   const Plan plan = plan_at(z, mem);
   const int tid = threadIdx.x;
   const int64_t max_own = min(static_cast<int64_t>(z.M) << z.shift, static_cast<int64_t>(INT32_MAX) - 64);
   const int64_t max_prefix = min(static_cast<int64_t>(z.MP) << z.shift, static_cast<int64_t>(INT32_MAX) - 64);
-  const bool own_narrow = z.rows <= kNarrow;
+  const bool own_narrow = z.rows <= kNarrow, held = z.B < kHeld;
+  const int* starts = held ? s_start : group_starts;
+  int4* groups = held ? s_group : plan.group;
+  // (the first round's own lengths are on their way meanwhile)
+  const int n_items = z.S * z.own_tiles;
+  const int s_first = tid < n_items ? tid / z.own_tiles : 0;
+  const int len_first = tid < n_items ? lengths[s_first] : 0;
   int sequences = 0, n_wide = 0, n_narrow = 0, wide_units = 0, narrow_units = 0;
   for (int base = 0; base < z.B; base += kTableThreads) {  // the groups' prefixes
     const int g = base + tid;
-    int seq0 = 0, n = 0, len = 0, total;
+    int seq0 = 0, n = 0, len = 0;
     if (g < z.B) {
-      seq0 = clampi(group_starts[g], 0, z.S);
-      n = max(clampi(group_starts[g + 1], 0, z.S) - seq0, 0);
+      const int from = group_starts[g], to = group_starts[g + 1];
+      if (held) {
+        s_start[g] = from;
+        if (g == z.B - 1) s_start[z.B] = to;
+      }
+      seq0 = clampi(from, 0, z.S);
+      n = max(clampi(to, 0, z.S) - seq0, 0);
       len = static_cast<int>(min(static_cast<int64_t>(max(prefix_lengths[g], 0)), max_prefix));
     }
-    const int before = sequences + scan_exclusive<int>(n, part, total);
-    sequences = min(sequences + total, z.S + 1);
-    if (before + static_cast<int64_t>(n) > z.S) n = 0;  // (group_starts that do not ascend)
+    unsigned before[1] = {static_cast<unsigned>(n)}, total1[1];
+    scan_exclusive<1>(before, total1, part1, Add{});
+    if (sequences + static_cast<int64_t>(before[0]) + n > z.S) n = 0;  // (group_starts that do not ascend)
+    sequences = static_cast<int>(min(static_cast<unsigned>(sequences) + total1[0], static_cast<unsigned>(z.S) + 1));
     const int64_t rows = static_cast<int64_t>(n) * z.rows;
     const bool is_wide = rows > kNarrow;
     const int keys = is_wide ? kWideKeys : kNarrowKeys, tiles = (len + keys - 1) / keys;
     const int wide = tiles && is_wide ? static_cast<int>((rows + kRows - 1) / kRows) : 0;
     const int narrow = tiles && rows && !is_wide;
-    const int first_wide = n_wide + scan_exclusive<int>(wide, part, total);
-    n_wide += total;
-    const int wide_unit = wide_units + scan_exclusive<int>(wide * tiles, part, total);
-    wide_units += total;
-    const int first_narrow = n_narrow + scan_exclusive<int>(narrow, part, total);
-    n_narrow += total;
-    const int narrow_unit = narrow_units + scan_exclusive<int>(narrow ? tiles : 0, part, total);
-    narrow_units += total;
-    if (g < z.B)
-      plan.group[g] = make_int4(wide || narrow ? tiles : 0, wide ? wide_unit : narrow_unit, wide ? first_wide : first_narrow, wide != 0);
+    unsigned x[4] = {static_cast<unsigned>(wide), static_cast<unsigned>(wide) * tiles, static_cast<unsigned>(narrow),
+                     narrow ? static_cast<unsigned>(tiles) : 0u}, total[4];
+    scan_exclusive<4>(x, total, part4, Add{});
+    const int first_wide = n_wide + x[0], wide_unit = wide_units + x[1], first_narrow = n_narrow + x[2], narrow_unit = narrow_units + x[3];
+    n_wide += total[0];
+    wide_units += total[1];
+    n_narrow += total[2];
+    narrow_units += total[3];
+    if (g < z.B) groups[g] = make_int4(wide || narrow ? tiles : 0, wide ? wide_unit : narrow_unit, wide ? first_wide : first_narrow, wide != 0);
     for (int i = 0; i < wide + narrow; ++i) {
       Segment s;
       s.table = ~g;
@@ -161,77 +184,76 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
       s.tiles = tiles;
       s.unit = wide ? wide_unit + i * tiles : narrow_unit;
       s.index = wide ? first_wide + i : first_narrow;
-      if (wide) plan.wide[s.index] = s;
-      else plan.narrow[s.index] = s;
+      (wide ? plan.wide : plan.narrow)[s.index] = s;
+      if (s.index < kHeld) (wide ? s_wide : s_narrow)[s.index] = s.unit;
     }
   }
-  const int n_narrow_prefix = n_narrow;
+  const int n_narrow_prefix = n_narrow, keys = own_narrow ? kNarrowKeys : kWideKeys;
   __syncthreads();
-  for (int s = tid; s < z.S; s += kTableThreads) {
-    PrefixPlace p{0, 0, 0, 0};
-    if (z.B) {
-      const int g = find(group_starts, z.B, s), seq0 = max(group_starts[g], 0);
-      if (s >= seq0 && s < group_starts[g + 1]) {
-        const int4 q = plan.group[g];
-        p.tiles = q.x;
-        p.unit = q.y;
-        p.index = q.z;
-        p.row0 = (s - seq0) * z.rows;
-        if (q.w) p.row0 = ~p.row0;
-      }
-    }
-    plan.prefix[s] = p;
-  }
-  __syncthreads();
-  const int n_items = z.S * z.own_tiles, keys = own_narrow ? kNarrowKeys : kWideKeys;
-  int& n_own = own_narrow ? n_narrow : n_wide;
-  int& units = own_narrow ? narrow_units : wide_units;
-  int own = 0;
+  int n_own = own_narrow ? n_narrow : n_wide, units = own_narrow ? narrow_units : wide_units, own = 0;
   for (int base = 0; base < n_items; base += kTableThreads) {  // the sequences' own keys
     const int item = base + tid;
-    int s = 0, row0 = 0, rows = 0, len = 0, tiles = 0, total;
+    int s = 0, row0 = 0, rows = 0, len = 0, tiles = 0;
+    PrefixPlace p{0, 0, 0, 0};
     if (item < n_items) {
       s = item / z.own_tiles;
       row0 = (item - s * z.own_tiles) * kRows;
       rows = min(z.rows - row0, kRows);
-      len = static_cast<int>(min(static_cast<int64_t>(max(lengths[s], 0)), max_own));
+      len = static_cast<int>(min(static_cast<int64_t>(max(base ? lengths[s] : len_first, 0)), max_own));
       const int seen = min(len, len - z.T + 1 + (row0 + rows - 1) / z.G);  // by the last row
       tiles = seen > 0 ? (seen + keys - 1) / keys : 0;
+      if (z.B) {
+        const int g = find(starts, z.B, s), seq0 = max(starts[g], 0);
+        if (s >= seq0 && s < starts[g + 1]) {
+          const int4 q = groups[g];
+          p = PrefixPlace{q.x, q.y, q.z, q.w ? ~((s - seq0) * z.rows) : (s - seq0) * z.rows};
+        }
+      }
+      if (!row0) plan.prefix[s] = p;
     }
-    const int at = scan_exclusive<int>(tiles > 0, part, total);
-    const int segment = n_own + at, index = own_narrow ? own + at : segment;
-    n_own += total;
-    own += total;
-    const int unit = units + scan_exclusive<int>(tiles, part, total);
-    units += total;
+    unsigned x[2] = {tiles > 0, static_cast<unsigned>(tiles)}, total[2];
+    scan_exclusive<2>(x, total, part2, Add{});
+    const int at = x[0], segment = n_own + at, index = own_narrow ? own + at : segment, unit = units + x[1];
+    n_own += total[0];
+    own += total[0];
+    units += total[1];
     if (item < n_items) plan.own[item] = Place{tiles ? len : 0, tiles, unit, index};
     if (tiles) {
       Segment w;
       w.table = s;
       w.seq0 = s;
       w.row0 = row0;
-      w.rows = rows | (plan.prefix[s].tiles ? 0 : kAlone);
+      w.rows = rows | (p.tiles ? 0 : kAlone);
       w.keys = len;
       w.tiles = tiles;
       w.unit = unit;
       w.index = index;
       (own_narrow ? plan.narrow : plan.wide)[segment] = w;
+      if (segment < kHeld) (own_narrow ? s_narrow : s_wide)[segment] = unit;
     }
   }
+  if (own_narrow) {
+    n_narrow = n_own;
+    narrow_units = units;
+  } else {
+    n_wide = n_own;
+    wide_units = units;
+  }
   auto per = [&](int units_, int stretches) {
-    return static_cast<int>(max((static_cast<int64_t>(units_) * z.Hkv + stretches - 1) / stretches, static_cast<int64_t>(1)));
+    const int64_t all = static_cast<int64_t>(units_) * z.Hkv + stretches - 1;
+    return max(all >> 31 ? static_cast<int>(all / stretches) : static_cast<int>(all) / stretches, 1);
   };
   const int wide_per = per(wide_units, z.wgs), narrow_per = per(narrow_units, z.wgs * kWaves);
   if (tid == 0)
     *plan.lines = Lines{wide_units, n_wide, wide_per, narrow_units, n_narrow, narrow_per, n_narrow_prefix, own_narrow ? own : 0};
-  // (stretches without tiles)
-  for (int w = tid; w < z.wgs; w += kTableThreads)
-    if (static_cast<int64_t>(w) * wide_per >= static_cast<int64_t>(wide_units) * z.Hkv) plan.wide_start[w] = Start{0, 0, 0, 0};
-  for (int w = tid; w < z.wgs * kWaves; w += kTableThreads)
-    if (static_cast<int64_t>(w) * narrow_per >= static_cast<int64_t>(narrow_units) * z.Hkv) plan.narrow_start[w] = Start{0, 0, 0, 0};
   __syncthreads();
-  write_starts(plan.wide, n_wide, wide_units, wide_per, z.Hkv, plan.wide_start, tid);
-  write_starts(plan.narrow, n_narrow, narrow_units, narrow_per, z.Hkv, plan.narrow_start, tid);
+  auto write = [&](const Segment* segments, const int* unit, int n, int units_, int per_, Start* out) {
+    // (the last stretch begins before 2^31 tiles, and the next one's number is compared too)
+    if (static_cast<int64_t>(units_) * z.Hkv < 1ll << 30) write_starts<int>(segments, unit, n, units_, per_, z.Hkv, out);
+    else write_starts<int64_t>(segments, unit, n, units_, per_, z.Hkv, out);
+  };
+  write(plan.wide, s_wide, n_wide, wide_units, wide_per, plan.wide_start);
+  write(plan.narrow, s_narrow, n_narrow, narrow_units, narrow_per, plan.narrow_start);
 }
 
 struct AttendArgs {
@@ -528,9 +550,16 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
   const int group = stretch_of(blockIdx.x, z.wgs);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
+  const Start wide_start = uniform(plan.wide_start + group);
+  const Start narrow_start = uniform(plan.narrow_start + group * kWaves + wave);
+  auto tiles_of = [&](int units, int per, int w) {  // of a stretch
+    const int64_t left = static_cast<int64_t>(units) * z.Hkv - static_cast<int64_t>(w) * per;
+    return static_cast<int>(min(max(left, static_cast<int64_t>(0)), static_cast<int64_t>(per)));
+  };
+
   {  // wide segments: the workgroup's
-    const Start start = uniform(plan.wide_start + group);
-    int left = start.left, h = start.head, seg = start.segment, tile = start.tile;
+    int left = tiles_of(lines.wide_units, lines.wide_per, group), h = wide_start.head, seg = wide_start.segment, tile = wide_start.tile;
+    Segment g = wide_start.first;
     if (left > 0) {
       T *s_k = lds, *s_v = lds + 2 * kWideK;
       if (z.D < DP) {
@@ -539,12 +568,7 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
       }
       constexpr int kShare = kWideKeys / kWaves;  // keys that a wave brings
       T *put_k = s_k + wave * kShare * L::kStrideK, *put_v = s_v + wave * kShare * L::kStrideV;
-      for (; left > 0; ++seg, tile = 0) {
-        if (seg == lines.n_wide) {
-          seg = 0;
-          ++h;
-        }
-        const Segment g = uniform(plan.wide + seg);
+      for (;; tile = 0) {
         const int n = min(left, g.tiles - tile), n_rows = g.rows & (kAlone - 1);
         left -= n;
         const int r = wave * 32 + (lane & 31);
@@ -578,22 +602,23 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
           __syncthreads();
         }
         if (busy) rows.end(a, lines, g, true, h, group, r, valid, n == g.tiles, tile == 0);
+        if (left <= 0) break;
+        if (++seg == lines.n_wide) {
+          seg = 0;
+          ++h;
+        }
+        g = uniform(plan.wide + seg);
       }
     }
   }
   {  // narrow segments: each wave's
     const int w = group * kWaves + wave;
-    const Start start = uniform(plan.narrow_start + w);
-    int left = start.left, h = start.head, seg = start.segment, tile = start.tile;
+    int left = tiles_of(lines.narrow_units, lines.narrow_per, w), h = narrow_start.head, seg = narrow_start.segment, tile = narrow_start.tile;
+    Segment g = narrow_start.first;
     if (left > 0) {
       T *s_k = lds + wave * (kWaveK + kWaveV), *s_v = s_k + kWaveK;
       if (z.D < DP) clear_rest<T, DP, kNarrowKeys>(a, s_k, s_v, lane, 64);
-      for (; left > 0; ++seg, tile = 0) {
-        if (seg == lines.n_narrow) {
-          seg = 0;
-          ++h;
-        }
-        const Segment g = uniform(plan.narrow + seg);
+      for (;; tile = 0) {
         const int n = min(left, g.tiles - tile), n_rows = g.rows & (kAlone - 1);
         left -= n;
         const int r = lane & 31;
@@ -618,6 +643,12 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
           rows.template tile<1>(s_k, s_v, key0 + it * kNarrowKeys, least, a.scale);
         }
         rows.end(a, lines, g, false, h, w, r, valid, n == g.tiles, tile == 0);
+        if (left <= 0) break;
+        if (++seg == lines.n_narrow) {
+          seg = 0;
+          ++h;
+        }
+        g = uniform(plan.narrow + seg);
       }
     }
   }
@@ -628,15 +659,16 @@ template <class T, int DP>
 __global__ __launch_bounds__(256) void k_join(AttendArgs a) {
   const Shape& z = a.z;
   const int lane = threadIdx.x & 63;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (id >= static_cast<int64_t>(z.S) * z.T * z.H) return;
-  const int hq = static_cast<int>(id % z.H), st = static_cast<int>(id / z.H), t = st % z.T, s = st / z.T;
+  const unsigned id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (id >= static_cast<unsigned>(z.S) * z.T * z.H) return;
+  const unsigned st = id / static_cast<unsigned>(z.H);
+  const int hq = static_cast<int>(id - st * z.H), s = static_cast<int>(st / static_cast<unsigned>(z.T)), t = static_cast<int>(st) - s * z.T;
   const int h = hq / z.G, r = t * z.G + hq % z.G;
   const Plan plan = plan_at(z, a.plan);
   const Lines lines = uniform(plan.lines);
   const Place own = uniform(plan.own + static_cast<int64_t>(s) * z.own_tiles + r / kRows);
   const PrefixPlace pre = uniform(plan.prefix + s);
-  T* to = static_cast<T*>(a.out) + id * z.D;
+  T* to = static_cast<T*>(a.out) + static_cast<int64_t>(id) * z.D;
   constexpr int E = DP > 128 ? 4 : DP > 64 ? 2 : 1;  // elements of a lane, side by side
   typedef float V __attribute__((ext_vector_type(E)));
   const bool mine = lane * E < z.D;
@@ -650,10 +682,11 @@ __global__ __launch_bounds__(256) void k_join(AttendArgs a) {
   if (own.keys - z.T + t + 1 <= 0) return write(V{});  // no token
   const bool own_wide = z.rows > kNarrow, pre_wide = pre.row0 < 0;
   auto stretches = [&](bool wide, int unit, int tiles, int& first) {
-    const int64_t u = static_cast<int64_t>(h) * (wide ? lines.wide_units : lines.narrow_units) + unit;
-    const int per = wide ? lines.wide_per : lines.narrow_per;
-    first = static_cast<int>(u / per);
-    return static_cast<int>((u + tiles - 1) / per) - first + 1;
+    const uint64_t u = static_cast<uint64_t>(h) * (wide ? lines.wide_units : lines.narrow_units) + unit, last = u + tiles - 1;
+    const unsigned per = wide ? lines.wide_per : lines.narrow_per;
+    const bool small = last >> 32 == 0;
+    first = static_cast<int>(small ? static_cast<unsigned>(u) / per : u / per);
+    return static_cast<int>(small ? static_cast<unsigned>(last) / per : last / per) - first + 1;
   };
   int first_own, first_pre = 0, n_pre = 0;
   const int n_own = stretches(own_wide, own.unit, own.tiles, first_own);

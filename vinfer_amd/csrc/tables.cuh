@@ -24,29 +24,49 @@ struct Tables {
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
-// Exclusive prefix of x over the workgroup, and its total (every thread). `part`: a word a wave.
-template <class T>
-__device__ __forceinline__ T scan_exclusive(T x, T* part, T& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T inc = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T y = __shfl_up(inc, d);
-    if (lane >= d) inc += y;
-  }
-  __syncthreads();  // (part may still be read from an earlier scan)
-  if (lane == 63) part[wave] = inc;
-  __syncthreads();
-  T before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kTableThreads / 64; ++w) {
-    const T p = part[w];
-    all += p;
-    if (w < wave) before += p;
-  }
-  total = all;
-  return before + inc - x;
+// The inclusive prefix of x over a wave's lanes (`add` any associative sum whose zero is 0), by moves between lanes.
+template <class F>
+__device__ __forceinline__ unsigned scan_wave(unsigned x, F add) {
+#define VPG_STEP(ctrl, rows) x = add(x, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), ctrl, rows, 0xf, false)))
+  VPG_STEP(0x111, 0xf);  // one lane down a row of 16, two, four, eight
+  VPG_STEP(0x112, 0xf);
+  VPG_STEP(0x114, 0xf);
+  VPG_STEP(0x118, 0xf);
+  VPG_STEP(0x142, 0xa);  // each row's last lane to the next row
+  VPG_STEP(0x143, 0xc);  // lane 31 to the upper half
+#undef VPG_STEP
+  return x;
 }
+
+// Exclusive prefixes of K numbers over the workgroup, and their totals (every thread). `part`: K words a wave.
+template <int K, class F>
+__device__ __forceinline__ void scan_exclusive(unsigned (&x)[K], unsigned (&total)[K], unsigned (&part)[K][kTableThreads / 64], F add) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  unsigned inc[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) inc[k] = scan_wave(x[k], add);
+  __syncthreads();  // (part may still be read from an earlier scan)
+  if (lane == 63)
+#pragma unroll
+    for (int k = 0; k < K; ++k) part[k][wave] = inc[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    // (each row of 16 lanes has the waves' sums; a wave takes its own from the lane of its number)
+    const unsigned sums = scan_wave(lane < kTableThreads / 64 ? part[k][lane] : 0u, add);
+    total[k] = __builtin_amdgcn_readlane(sums, kTableThreads / 64 - 1);
+    const unsigned before = wave ? __builtin_amdgcn_readlane(sums, __builtin_amdgcn_readfirstlane(wave) - 1) : 0u;
+    const unsigned left = static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(inc[k]), 0x138, 0xf, 0xf, false));  // the lane below's
+    x[k] = add(before, lane ? left : 0u);
+  }
+}
+struct Add {
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return a + b; }
+};
+struct AddUpTo {  // (both at most cap <= 2^31)
+  unsigned cap;
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return min(a + b, cap); }
+};
 
 // The last of the n ascending starts that is <= i (starts[0] <= i).
 template <class T>
@@ -73,14 +93,14 @@ __global__ __launch_bounds__(kTableThreads) void k_extend(Tables t, const int32_
                                                           int32_t* __restrict__ slots, int32_t* __restrict__ positions,
                                                           int32_t* __restrict__ sequences, uint8_t* __restrict__ served,
                                                           int32_t* __restrict__ ws) {
-  __shared__ int64_t part64[kTableThreads / 64];
-  __shared__ int part[kTableThreads / 64];
+  __shared__ unsigned part[1][kTableThreads / 64];
   __shared__ int s_page[kTableThreads], s_have[kTableThreads], s_token[kTableThreads], s_base[kTableThreads];
   const int tid = threadIdx.x;
   const int P = 1 << t.shift;
   const int64_t cap = min(static_cast<int64_t>(t.M) << t.shift, static_cast<int64_t>(INT32_MAX));
   const int n_free = clampi(*t.free_count, 0, t.pages);
-  int64_t tokens_before = 0;
+  const unsigned none = static_cast<unsigned>(N) + 1;  // (what lies past the call's tokens)
+  unsigned tokens_before = 0;
   int pages_before = 0, taken = 0;
   for (int base = 0; base < t.S; base += kTableThreads) {
     const int s = base + tid;
@@ -90,17 +110,19 @@ __global__ __launch_bounds__(kTableThreads) void k_extend(Tables t, const int32_
       len = len < 0 ? 0 : len > cap ? cap : len;
       c = max(counts[s], 0);
     }
-    int64_t all_tokens;
-    const int64_t start = tokens_before + scan_exclusive<int64_t>(c, part64, all_tokens);
+    unsigned scan[1] = {static_cast<unsigned>(min(c, static_cast<int64_t>(none)))}, sum[1];
+    scan_exclusive<1>(scan, sum, part, AddUpTo{none});
+    const unsigned start = min(tokens_before + scan[0], none), tokens_after = min(tokens_before + sum[0], none);
     const int64_t have = (len + P - 1) >> t.shift, want = (len + c + P - 1) >> t.shift;
     const bool fits = len + c <= cap && start + c <= N;
     const int need = fits ? static_cast<int>(want - have) : 0;
-    int all_pages;
-    const int first = scan_exclusive<int>(need, part, all_pages);  // (within this round)
+    scan[0] = need;
+    scan_exclusive<1>(scan, sum, part, Add{});
+    const int first = scan[0], all_pages = sum[0];  // (within this round)
     const bool ok = fits && (need == 0 || pages_before + first + need <= n_free);
     s_page[tid] = first;
     s_have[tid] = ok ? static_cast<int>(have) : -1;
-    s_token[tid] = static_cast<int>(start > N ? N : start);
+    s_token[tid] = static_cast<int>(min(start, static_cast<unsigned>(N)));
     s_base[tid] = ok ? static_cast<int>(len) : -1;
     if (s < t.S) {
       served[s] = ok;
@@ -110,10 +132,9 @@ __global__ __launch_bounds__(kTableThreads) void k_extend(Tables t, const int32_
         ws[t.S + s] = s_base[tid];
       }
     }
-    const int mine = ok ? need : 0;
-    int all_taken;
-    scan_exclusive<int>(mine, part, all_taken);  // (its barriers also publish the arrays)
-    taken += all_taken;
+    scan[0] = ok ? need : 0;
+    scan_exclusive<1>(scan, sum, part, Add{});  // (its barriers also publish the arrays)
+    taken += static_cast<int>(sum[0]);
     const int n = min(t.S - base, kTableThreads);
     for (int i = tid; i < all_pages && pages_before + i < n_free; i += kTableThreads) {
       const int k = find(s_page, n, i);
@@ -122,8 +143,8 @@ __global__ __launch_bounds__(kTableThreads) void k_extend(Tables t, const int32_
     }
     if (SELF) {
       __syncthreads();  // (the tables' new entries, seen by this workgroup)
-      const int to = static_cast<int>(tokens_before + all_tokens > N ? N : tokens_before + all_tokens);
-      for (int i = static_cast<int>(tokens_before > N ? N : tokens_before) + tid; i < to; i += kTableThreads) {
+      const int to = static_cast<int>(min(tokens_after, static_cast<unsigned>(N)));
+      for (int i = static_cast<int>(min(tokens_before, static_cast<unsigned>(N))) + tid; i < to; i += kTableThreads) {
         const int k = find(s_token, n, i);
         if (s_base[k] >= 0) {
           write_token(t, i, base + k, s_base[k] + (i - s_token[k]), slots, positions, sequences);
@@ -132,16 +153,16 @@ __global__ __launch_bounds__(kTableThreads) void k_extend(Tables t, const int32_
         }
       }
     }
-    tokens_before += all_tokens;
+    tokens_before = tokens_after;
     pages_before += all_pages;
     __syncthreads();
   }
   if (SELF)
-    for (int i = static_cast<int>(tokens_before > N ? N : tokens_before) + tid; i < N; i += kTableThreads)
+    for (int i = static_cast<int>(min(tokens_before, static_cast<unsigned>(N))) + tid; i < N; i += kTableThreads)
       slots[i] = positions[i] = sequences[i] = -1;
   if (tid == 0) {
     *t.free_count = n_free - taken;
-    if (!SELF) ws[2 * t.S] = static_cast<int>(tokens_before > N ? N : tokens_before);
+    if (!SELF) ws[2 * t.S] = static_cast<int>(min(tokens_before, static_cast<unsigned>(N)));
   }
 }
 
@@ -158,7 +179,7 @@ __global__ __launch_bounds__(256) void k_tokens(Tables t, int N, int32_t* __rest
 }
 
 __global__ __launch_bounds__(kTableThreads) void k_shrink(Tables t, const int32_t* __restrict__ to) {
-  __shared__ int part[kTableThreads / 64];
+  __shared__ unsigned part[1][kTableThreads / 64];
   __shared__ int s_page[kTableThreads], s_keep[kTableThreads];
   const int tid = threadIdx.x;
   const int P = 1 << t.shift;
@@ -179,17 +200,20 @@ __global__ __launch_bounds__(kTableThreads) void k_shrink(Tables t, const int32_
       cut(s, keep, drop);
       sum += drop;
     }
-    scan_exclusive<int>(sum, part, total);
+    unsigned scan[1] = {static_cast<unsigned>(sum)}, all[1];
+    scan_exclusive<1>(scan, all, part, Add{});
+    total = static_cast<int>(all[0]);
   }
   int before = 0;
   for (int base = 0; base < t.S; base += kTableThreads) {
     const int s = base + tid;
     int keep = 0, drop = 0, now = 0;
     if (s < t.S) now = cut(s, keep, drop);
-    int all;
-    const int first = scan_exclusive<int>(drop, part, all);
+    unsigned scan[1] = {static_cast<unsigned>(drop)}, sum[1];
+    scan_exclusive<1>(scan, sum, part, Add{});
+    const int all = static_cast<int>(sum[0]);
     if (t.S <= kTableThreads) total = all;
-    s_page[tid] = first;
+    s_page[tid] = static_cast<int>(scan[0]);
     s_keep[tid] = keep;
     if (s < t.S) t.lengths[s] = now;
     __syncthreads();

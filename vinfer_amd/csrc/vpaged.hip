@@ -230,7 +230,7 @@ size_t vpaged_extend_workspace_bytes(int32_t sequences, int32_t tokens) {
 int vpaged_extend(const vpaged_tables* t, const int32_t* counts, int32_t tokens, int32_t* out_slots, int32_t* out_positions,
                   int32_t* out_sequences, uint8_t* out_served, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_tables(t)) return rc;
-  if (tokens < 0) return fail(VPAGED_E_ARG, "tokens must be >= 0, got %d", tokens);
+  if (tokens < 0 || tokens > VPAGED_MAX_TOKENS) return fail(VPAGED_E_ARG, "tokens must be in [0, %d], got %d", VPAGED_MAX_TOKENS, tokens);
   if (!t->sequences && !tokens) return VPAGED_OK;
   if ((t->sequences && (!counts || !out_served)) || (tokens && (!out_slots || !out_positions || !out_sequences)))
     return fail(VPAGED_E_ARG, "counts and the outputs must be set");
@@ -353,7 +353,7 @@ int vpaged_attend(const vpaged_attend_args* a, void* stream) {
   const AttendLayout L = attend_layout(d.z);
   if (!a->plan || reinterpret_cast<uintptr_t>(a->plan) & 255u) return fail(VPAGED_E_WORKSPACE, "plan must be set and 256-byte aligned");
   if (int rc = check_memory("workspace", a->workspace, a->workspace_bytes, L.total)) return rc;
-  if (static_cast<int64_t>(d.z.S) * d.z.T * d.z.H >= 1ll << 33) return fail(VPAGED_E_ARG, "more than 2^33 rows");
+  if (static_cast<int64_t>(d.z.S) * d.z.T * d.z.H >= 1ll << 31) return fail(VPAGED_E_ARG, "2^31 rows of outputs, or more");
   if (int rc = check_current_device()) return rc;
   d.pages = a->pages;
   d.scale = static_cast<float>(a->scale * 1.4426950408889634);

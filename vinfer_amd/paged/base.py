@@ -24,7 +24,7 @@ from vinfer_amd.registry import BackendRegistry
 DTYPES = {torch.bfloat16: _vpaged.VPAGED_BF16, torch.float16: _vpaged.VPAGED_F16}
 
 
-@dataclass(eq=False)
+@dataclass(eq=False, frozen=True)
 class PageTables:
     """What each sequence holds, and a stack of the pages that nobody holds, on one device (contiguous int32 tensors):
     ``tables [S, max_pages]``, ``lengths [S]``, ``free [pages]`` whose first ``free_count [1]`` entries are free, the
@@ -75,7 +75,7 @@ class Extension:
     served: torch.Tensor
 
 
-@dataclass(eq=False)
+@dataclass(eq=False, frozen=True)
 class Rotary:
     """How queries and keys are turned: pair j of a head's first ``2 * len(frequencies)`` elements by
     ``position * frequencies[j]`` (float64), ``magnitude`` times as long. Pairs are elements (j, j + len) or, where
@@ -185,8 +185,8 @@ def _words(name: str, t: torch.Tensor, n: int, device) -> None:
 
 def check_extend(pages: PageTables, counts, tokens: int) -> None:
     _words("counts", counts, pages.lengths.shape[0], pages.tables.device)
-    if not 0 <= tokens < 1 << 31 or (tokens and not counts.shape[0]):
-        raise ValueError(f"tokens must be in [0, 2^31), and 0 without sequences, got {tokens}")
+    if not 0 <= tokens <= _vpaged.MAX_TOKENS or (tokens and not counts.shape[0]):
+        raise ValueError(f"tokens must be in [0, {_vpaged.MAX_TOKENS}], and 0 without sequences, got {tokens}")
 
 
 def check_shrink(pages: PageTables, lengths) -> None:

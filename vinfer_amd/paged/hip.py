@@ -3,11 +3,13 @@
 Registered for device type ``"cuda"`` (ROCm PyTorch reports HIP devices as ``cuda``) and the dtypes bf16 and
 fp16. Every call enqueues its work on torch's current stream of its tensors' device and returns without
 synchronising; outputs, plans and workspaces are torch's, so calls may be captured into HIP graphs.
+
+A decode step makes these calls for few tokens, where their checks would take longer than their kernels: what a call
+says of shapes, layouts, types and devices is checked once, and what the library needs of it kept by all that was
+checked.
 """
 
 from __future__ import annotations
-
-import ctypes
 
 import torch
 
@@ -27,23 +29,19 @@ from vinfer_amd.paged.base import (
 )
 from vinfer_amd.registry import BackendContext
 
+_KNOWN = 4096  # calls of unlike shapes that a backend keeps in mind
+
 
 def _on_gpu(device) -> None:
     if device.type != "cuda":
         raise ValueError(f"the hip paged cache needs its tensors on a GPU, got {device}")
 
 
-def _dtype(t) -> int:
-    if t.dtype not in DTYPES:
-        raise ValueError(f"the hip paged cache supports bf16 and fp16, got {t.dtype}")
-    return DTYPES[t.dtype]
-
-
 class _Planned:
-    """A plan's memory, and the argument block that its layers share."""
+    """A plan's memory and stream, its shape packed, and its layers' workspace."""
 
-    def __init__(self, shape, memory, stream, workspace: int) -> None:
-        self.shape, self.memory, self.stream, self.workspace = shape, memory, stream, workspace
+    def __init__(self, key, shape, memory, stream, workspace) -> None:
+        self.key, self.shape, self.memory, self.stream, self.workspace = key, shape, memory, stream, workspace
 
 
 @PAGED.register("hip", devices={"cuda"}, dtypes=set(DTYPES), supports=lambda ctx: _vpaged.unsupported(ctx.device))
@@ -51,100 +49,132 @@ class HipPaged:
     def __init__(self, ctx: BackendContext) -> None:
         self.ctx = ctx
         self._lib = _vpaged.load()
-        self._need: dict[tuple, tuple] = {}  # a shape's block, and its plan's and workspace's bytes
+        self._known: dict[tuple, tuple] = {}
+
+    def _keep(self, key, value):
+        if len(self._known) >= _KNOWN:
+            self._known.clear()
+        self._known[key] = value
+        return value
+
+    def _check_dtype(self, t) -> None:
+        if t.dtype != self.ctx.dtype:
+            raise ValueError(f"this backend was made for {self.ctx.dtype}, got {t.dtype}")
 
     @staticmethod
-    def _tables(pages: PageTables) -> _vpaged.VpagedTables:
-        _on_gpu(pages.tables.device)
-        S, M = pages.tables.shape
-        return _vpaged.VpagedTables(pages.tables.data_ptr(), pages.lengths.data_ptr(), pages.free.data_ptr(),
-                                    pages.free_count.data_ptr(), S, M, pages.free.shape[0], pages.page_size)
+    def _tables(pages: PageTables) -> bytes:
+        t, free = pages.tables, pages.free
+        S, M = t.shape
+        return _vpaged.PACK_TABLES.pack(t.data_ptr(), pages.lengths.data_ptr(), free.data_ptr(), pages.free_count.data_ptr(),
+                                        S, M, free.shape[0], pages.page_size)
 
     def extend(self, pages: PageTables, counts: torch.Tensor, tokens: int) -> Extension:
         check_extend(pages, counts, tokens)
-        dev = pages.tables.device
-        t = self._tables(pages)
+        dev = counts.device
+        _on_gpu(dev)
         counts = counts.contiguous()
-        out = torch.empty(3, tokens, dtype=torch.int32, device=dev)
-        served = torch.empty(counts.shape, dtype=torch.bool, device=dev)
-        at, need = out.data_ptr(), self._lib.vpaged_extend_workspace_bytes(t.sequences, tokens)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _vpaged.call(self._lib.vpaged_extend, dev, ctypes.byref(t), counts.data_ptr(), tokens, at, at + 4 * tokens, at + 8 * tokens,
-                     served.data_ptr(), ws.data_ptr() if need else None, need)
-        return Extension(*out.unbind(0), served)
+        slots, positions, sequences = counts.new_empty(tokens), counts.new_empty(tokens), counts.new_empty(tokens)
+        served = counts.new_empty(counts.shape, dtype=torch.bool)
+        ws, need = None, self._lib.vpaged_extend_workspace_bytes(counts.shape[0], tokens)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)  # (torch aligns to 512 bytes)
+        _vpaged.call(self._lib.vpaged_extend, dev, self._tables(pages), counts.data_ptr(), tokens, slots.data_ptr(),
+                     positions.data_ptr(), sequences.data_ptr(), served.data_ptr(), ws.data_ptr() if need else None, need)
+        return Extension(slots, positions, sequences, served)
 
     def shrink(self, pages: PageTables, lengths: torch.Tensor) -> None:
         check_shrink(pages, lengths)
+        dev = lengths.device
+        _on_gpu(dev)
         lengths = lengths.contiguous()
-        _vpaged.call(self._lib.vpaged_shrink, pages.tables.device, ctypes.byref(self._tables(pages)), lengths.data_ptr())
+        _vpaged.call(self._lib.vpaged_shrink, dev, self._tables(pages), lengths.data_ptr())
 
     def rotate_store(self, q, k, v, positions, slots, k_pages, v_pages, rotary: Rotary) -> torch.Tensor:
-        check_rotate(q, k, v, positions, slots, k_pages, v_pages, rotary)
-        dev, dtype = q.device, _dtype(q)
-        _on_gpu(dev)
-        N, heads, D = q.shape
-        positions, slots = positions.contiguous(), slots.contiguous()
-        out = torch.empty(N, heads, D, dtype=q.dtype, device=dev)
-        (qn, qh, _), (kn, kh, _), (vn, vh, _), (pn, pp, ph, _) = q.stride(), k.stride(), v.stride(), k_pages.stride()
         f = rotary.frequencies
-        a = _vpaged.VpagedRotateArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), qn, kn, vn, qh, kh, vh, out.data_ptr(),
-                                     k_pages.data_ptr(), v_pages.data_ptr(), pn, pp, ph, positions.data_ptr(),
-                                     slots.data_ptr(), f.data_ptr(), rotary.magnitude, dtype, N, heads, k.shape[1], D,
-                                     2 * f.shape[0], rotary.interleaved, k_pages.shape[0], k_pages.shape[1])
-        _vpaged.call(self._lib.vpaged_rotate_store, dev, ctypes.byref(a))
+        key = ("rotate", torch.is_grad_enabled(), q.requires_grad, k.requires_grad, v.requires_grad, rotary.interleaved,
+               rotary.magnitude, f.shape, q.shape, k.shape, v.shape, positions.shape, slots.shape, k_pages.shape, v_pages.shape,
+               q.stride(), k.stride(), v.stride(), k_pages.stride(), v_pages.stride(), q.dtype, k.dtype, v.dtype,
+               positions.dtype, slots.dtype, k_pages.dtype, v_pages.dtype, q.get_device(), k.get_device(), v.get_device(),
+               positions.get_device(), slots.get_device(), k_pages.get_device(), v_pages.get_device(), f.get_device())
+        known = self._known.get(key)
+        if known is None:
+            check_rotate(q, k, v, positions, slots, k_pages, v_pages, rotary)
+            _on_gpu(q.device)
+            self._check_dtype(q)
+            N, heads, D = q.shape
+            known = self._keep(key, (
+                q.device, (N, heads, D), tuple(x for t in (q, k, v) for x in t.stride()[:1]) + tuple(t.stride(1) for t in (q, k, v)),
+                k_pages.stride()[:3], (rotary.magnitude, DTYPES[q.dtype], N, heads, k.shape[1], D, 2 * f.shape[0],
+                                       int(rotary.interleaved), k_pages.shape[0], k_pages.shape[1])))
+        dev, shape, strides, page_strides, rest = known
+        positions, slots = positions.contiguous(), slots.contiguous()
+        out = q.new_empty(shape)
+        a = _vpaged.PACK_ROTATE.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides, out.data_ptr(), k_pages.data_ptr(),
+                                     v_pages.data_ptr(), *page_strides, positions.data_ptr(), slots.data_ptr(), f.data_ptr(), *rest)
+        _vpaged.call(self._lib.vpaged_rotate_store, dev, a)
         return out
 
     def plan(self, lengths, *, queries, heads, kv_heads, head_dim, page_size, max_pages, prefix_lengths=None,
              max_prefix_pages=0, group_starts=None) -> AttentionPlan:
-        check_plan(lengths, queries, heads, kv_heads, head_dim, page_size, max_pages, prefix_lengths, max_prefix_pages,
-                   group_starts)
-        dev = lengths.device
-        _on_gpu(dev)
-        S, B = lengths.shape[0], 0 if prefix_lengths is None else prefix_lengths.shape[0]
-        if not B:
-            max_prefix_pages = 0
-        key = S, B, queries, heads, kv_heads, head_dim, page_size, max_pages, max_prefix_pages
-        known = self._need.get(key)
-        if known is None:
-            shape = _vpaged.VpagedShape(DTYPES[self.ctx.dtype], *key)
-            known = shape, self._lib.vpaged_plan_bytes(shape), self._lib.vpaged_attend_workspace_bytes(shape)
-            if not known[1]:
-                raise ValueError(f"a shape of more tiles or rows than 32 bits number: {key}")
-            if len(self._need) > 4096:
-                self._need.clear()
-            self._need[key] = known
-        shape, need, workspace = known
-        memory = torch.empty(need, dtype=torch.uint8, device=dev)  # (torch aligns to 512 bytes)
+        groups = prefix_lengths is not None and group_starts is not None
+        key = ("plan", queries, heads, kv_heads, head_dim, page_size, max_pages, max_prefix_pages, lengths.shape, lengths.dtype,
+               lengths.get_device(), *((prefix_lengths.shape, prefix_lengths.dtype, prefix_lengths.get_device(), group_starts.shape,
+                                        group_starts.dtype, group_starts.get_device()) if groups else ()))
+        known = self._known.get(key)
+        if known is None or groups != (prefix_lengths is not None or group_starts is not None):
+            check_plan(lengths, queries, heads, kv_heads, head_dim, page_size, max_pages, prefix_lengths, max_prefix_pages,
+                       group_starts)
+            _on_gpu(lengths.device)
+            S, B = lengths.shape[0], prefix_lengths.shape[0] if groups else 0
+            shape = DTYPES[self.ctx.dtype], S, B, queries, heads, kv_heads, head_dim, page_size, max_pages, max_prefix_pages if B else 0
+            block = _vpaged.PACK_SHAPE.pack(*shape)
+            need = self._lib.vpaged_plan_bytes(block)
+            if not need:
+                raise ValueError(f"a shape of more tiles or rows than 32 bits number: {S} sequences of {queries} x {heads} queries "
+                                 f"on {max_pages} pages, {B} prefixes of {max_prefix_pages}, of {page_size} positions")
+            known = self._keep(key, (lengths.device, shape, block, need, self._lib.vpaged_attend_workspace_bytes(block)))
+        dev, shape, block, need, workspace = known
+        memory = torch.empty(need, dtype=torch.uint8, device=dev)
         lengths = lengths.contiguous()
-        if B:
+        pre = starts = None
+        if groups:
             prefix_lengths, group_starts = prefix_lengths.contiguous(), group_starts.contiguous()
-        _vpaged.call(self._lib.vpaged_plan, dev, ctypes.byref(shape), lengths.data_ptr(), prefix_lengths.data_ptr() if B else None,
-                     group_starts.data_ptr() if B else None, memory.data_ptr(), need)
-        return AttentionPlan(S, B, queries, heads, kv_heads, head_dim, page_size, max_pages, max_prefix_pages, dev,
-                             _Planned(shape, memory, torch._C._cuda_getCurrentRawStream(dev.index), workspace))
+            pre, starts = prefix_lengths.data_ptr(), group_starts.data_ptr()
+        _vpaged.call(self._lib.vpaged_plan, dev, block, lengths.data_ptr(), pre, starts, memory.data_ptr(), need)
+        return AttentionPlan(*shape[1:], dev, _Planned(shape, block, memory, torch._C._cuda_getCurrentRawStream(dev.index), workspace))
 
     def attend(self, q, k_pages, v_pages, tables, plan: AttentionPlan, *, prefix_tables=None, scale=None) -> torch.Tensor:
-        check_attend(q, k_pages, v_pages, tables, plan, prefix_tables, scale)
-        dev, data = q.device, plan.data
-        if q.dtype != self.ctx.dtype:
-            raise ValueError(f"this backend was made for {self.ctx.dtype}, got {q.dtype}")
-        sn, st, sh, _ = q.stride()
-        if (sn | st | sh) & 7 or q.data_ptr() & 15:
+        data, pre = plan.data, prefix_tables
+        key = ("attend", data.key, scale, torch.is_grad_enabled(), q.requires_grad, q.shape, k_pages.shape, v_pages.shape, tables.shape,
+               q.stride(), k_pages.stride(), v_pages.stride(), tables.stride(), q.dtype, k_pages.dtype, v_pages.dtype, tables.dtype,
+               q.get_device(), k_pages.get_device(), v_pages.get_device(), tables.get_device(), plan.device.index,
+               *((pre.shape, pre.stride(), pre.dtype, pre.get_device()) if pre is not None else ()))
+        known = self._known.get(key)
+        if known is None:
+            check_attend(q, k_pages, v_pages, tables, plan, pre, scale)
+            self._check_dtype(q)
+            strides = k_pages.stride()[:3]
+            if any(x & 7 for x in strides) or strides[1] >= 1 << 27:
+                raise ValueError(f"the cache's strides must be multiples of 8 elements (positions' below 2^27), got {strides}")
+            known = self._keep(key, (q.device, any(x & 7 for x in q.stride()[:3]), q.stride()[:3], strides,
+                                     (*data.key, k_pages.shape[0], plan.head_dim**-0.5 if scale is None else scale),
+                                     (tables.stride(0), pre.stride(0) if plan.groups else 0)))
+        dev, odd, q_strides, strides, first, table_strides = known
+        kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+        if (kp | vp) & 15:
+            raise ValueError("the cache must be 16-byte aligned")
+        if odd or q.data_ptr() & 15:
             q = q.contiguous()
-            sn, st, sh, _ = q.stride()
-        pn, pp, ph, _ = k_pages.stride()
-        if (pn | pp | ph) & 7 or (k_pages.data_ptr() | v_pages.data_ptr()) & 15:
-            raise ValueError("the cache must be 16-byte aligned, with strides of multiples of 8 elements")
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        if torch._C._cuda_getCurrentRawStream(dev.index) != data.stream:
-            data.memory.record_stream(torch.cuda.current_stream(dev))
+            q_strides = q.stride()[:3]
+        out = q.new_empty(q.shape)
         ws = torch.empty(data.workspace, dtype=torch.uint8, device=dev)
-        pre, pre_stride = (prefix_tables.data_ptr(), prefix_tables.stride(0)) if plan.groups else (None, 0)
-        a = _vpaged.VpagedAttendArgs(data.shape, k_pages.shape[0], plan.head_dim**-0.5 if scale is None else scale,
-                                     q.data_ptr(), sn, st, sh, k_pages.data_ptr(), v_pages.data_ptr(), pn, pp, ph,
-                                     tables.data_ptr(), pre, tables.stride(0), pre_stride, out.data_ptr(),
-                                     data.memory.data_ptr(), ws.data_ptr(), data.workspace)
-        _vpaged.call(self._lib.vpaged_attend, dev, ctypes.byref(a))
+        memory = data.memory
+        if torch._C._cuda_getCurrentRawStream(dev.index) != data.stream:
+            memory.record_stream(torch.cuda.current_stream(dev))
+        a = _vpaged.PACK_ATTEND.pack(*first, q.data_ptr(), *q_strides, kp, vp, *strides, tables.data_ptr(),
+                                     pre.data_ptr() if plan.groups else 0, *table_strides, out.data_ptr(), memory.data_ptr(),
+                                     ws.data_ptr(), data.workspace)
+        _vpaged.call(self._lib.vpaged_attend, dev, a)
         return out
 
 
