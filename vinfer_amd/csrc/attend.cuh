@@ -288,20 +288,42 @@ __device__ __forceinline__ int64_t partial_row(const AttendArgs& a, const Lines&
 // Workgroups of neighbouring stretches on one XCD: its L2 serves those that read the same keys.
 __device__ __forceinline__ int stretch_of(int block, int wgs) { return (block & 7) * (wgs >> 3) + (block >> 3); }
 
+// f(0), .., f(N - 1), each with its number as a constant: registers are told apart by numbers that the compiler knows.
+template <int I>
+struct Number {
+  static constexpr int value = I;
+};
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(Number<I>{});
+    each<N, I + 1>(f);
+  }
+}
+
 template <class T>
 struct Mma;
 template <>
 struct Mma<__bf16> {
   typedef bf16x8 V8;
   static __device__ __forceinline__ f32x16 mma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ float add_pair(int x, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), bf16x2{1.0f, 1.0f}, sum, false);
+  }
 };
 template <>
 struct Mma<_Float16> {
   typedef f16x8 V8;
   static __device__ __forceinline__ f32x16 mma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ float add_pair(int x, float sum) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), f16x2{1.0f, 1.0f}, sum, false);
+  }
 };
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+__device__ __forceinline__ float other_half(float x) {  // the partner's, 32 lanes on
+  const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  return __builtin_bit_cast(float, (threadIdx.x & 32) ? both[0] : both[1]);
+}
 
 // What the plan and the tables hold, by scalar loads: nothing writes them while a kernel runs.
 template <class X>
@@ -332,17 +354,25 @@ struct Layout {
   static constexpr int kAtOnce = 64 / kPieces;                        // keys of an access
 };
 
-// A segment's keys and values of a head on their way: KEYS of them by this wave.
-template <class T, int DP, int KEYS>
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// A segment's keys and values of a head on their way: KEYS of them by this wave, eight at a time from their page (a
+// scalar base, the lanes' offsets the same for all; what a lane has not of a head's elements lies past the range: 0).
+// SMALL: pages of fewer than eight keys (a place of its own for each key of each lane).
+template <class T, int DP, int KEYS, bool SMALL>
 struct Stage {
   typedef typename Mma<T>::V8 V8;
   typedef Layout<DP> L;
   static constexpr int kLoads = KEYS / L::kAtOnce, kGroups = KEYS / 8, kVariants = 8 / L::kAtOnce;
+  static constexpr uint32_t kRange = 0x80000000u;
   V8 k[kLoads], v[kLoads];
-  int pages[kGroups];
+  uint32_t offset[kVariants];
   const int32_t* table;
   const T *k_head, *v_head;
   int last;  // key
+  struct Pages {
+    int page[kGroups];
+  };
 
   __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& g, int h) {
     table = g.table < 0 ? a.prefix_tables + static_cast<int64_t>(~g.table) * a.prefix_table_stride
@@ -350,50 +380,64 @@ struct Stage {
     k_head = static_cast<const T*>(a.k) + h * a.head_stride;
     v_head = static_cast<const T*>(a.v) + h * a.head_stride;
     last = g.keys - 1;
+    const int lane = threadIdx.x & 63, in = lane / L::kPieces, c = lane % L::kPieces;
+#pragma unroll
+    for (int i = 0; i < kVariants; ++i) offset[i] = place(a, i * L::kAtOnce + in, c);
+  }
+  static __device__ __forceinline__ uint32_t place(const AttendArgs& a, int key, int c) {
+    return c * 8 < a.z.D ? (static_cast<uint32_t>(key) * static_cast<uint32_t>(a.place_stride) + c * 8) * 2 : kRange;
   }
   // The pages of the keys from key0 on (keys past the last: the last eight once more).
-  __device__ __forceinline__ void look_up(const AttendArgs& a, int key0) {
-    if (a.z.shift < 3) return;
+  __device__ __forceinline__ Pages look_up(const AttendArgs& a, int key0) const {
+    Pages p;
+    if (SMALL) return p;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) pages[g] = uniform(table + (min(key0 + 8 * g, last & ~7) >> a.z.shift));
+    for (int g = 0; g < kGroups; ++g) p.page[g] = uniform(table + (min(key0 + 8 * g, last & ~7) >> a.z.shift));
+    return p;
   }
-  __device__ __forceinline__ void fetch(const AttendArgs& a, int key0) {
+  static __device__ __forceinline__ V8 load(const T* base, uint32_t off) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, kRange, 0x00027000);
+    return __builtin_bit_cast(V8, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+  }
+  // x[..] = what the keys from key0 on have at `head`: the keys themselves or their values.
+  __device__ __forceinline__ void fetch(V8 (&x)[kLoads], const T* head, const Pages& p, const AttendArgs& a, int key0) const {
     const int lane = threadIdx.x & 63, in = lane / L::kPieces, c = lane % L::kPieces;
     const int mask = (1 << a.z.shift) - 1;
-    if (c * 8 >= a.z.D) return;
-    if (a.z.shift >= 3) {
+    if constexpr (!SMALL) {
+      if (key0 + KEYS <= last + 1) {
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const int first = min(key0 + 8 * g, last & ~7);
-        const int64_t at = clampi(pages[g], 0, a.pages - 1) * a.page_stride + (first & mask) * a.place_stride;
-        const char *kp = reinterpret_cast<const char*>(k_head + at), *vp = reinterpret_cast<const char*>(v_head + at);
+        for (int g = 0; g < kGroups; ++g) {
+          const T* base = head + clampi(p.page[g], 0, a.pages - 1) * a.page_stride + ((key0 + 8 * g) & mask) * a.place_stride;
 #pragma unroll
-        for (int i = 0; i < kVariants; ++i) {
-          const int key = min(i * L::kAtOnce + in, last - first);
-          const uint32_t off = (static_cast<uint32_t>(key) * static_cast<uint32_t>(a.place_stride) + c * 8) * 2;
-          k[g * kVariants + i] = *reinterpret_cast<const V8*>(kp + off);
-          v[g * kVariants + i] = *reinterpret_cast<const V8*>(vp + off);
+          for (int i = 0; i < kVariants; ++i) x[g * kVariants + i] = load(base, offset[i]);
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const int first = min(key0 + 8 * g, last & ~7);
+          const T* base = head + clampi(p.page[g], 0, a.pages - 1) * a.page_stride + (first & mask) * a.place_stride;
+#pragma unroll
+          for (int i = 0; i < kVariants; ++i) x[g * kVariants + i] = load(base, place(a, min(i * L::kAtOnce + in, last - first), c));
         }
       }
-    } else {  // pages of fewer than eight keys
+    } else {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int key = min(key0 + i * L::kAtOnce + in, last);
-        const int64_t at = clampi(table[key >> a.z.shift], 0, a.pages - 1) * a.page_stride + (key & mask) * a.place_stride + c * 8;
-        k[i] = *reinterpret_cast<const V8*>(k_head + at);
-        v[i] = *reinterpret_cast<const V8*>(v_head + at);
+        const T* at = head + clampi(table[key >> a.z.shift], 0, a.pages - 1) * a.page_stride + (key & mask) * a.place_stride + c * 8;
+        x[i] = c * 8 < a.z.D ? *reinterpret_cast<const V8*>(at) : V8{};
       }
     }
   }
-  __device__ __forceinline__ void put(const AttendArgs& a, T* s_k, T* s_v) {
+  template <int STRIDE>
+  __device__ __forceinline__ void put(const V8 (&x)[kLoads], T* to) const {
     const int lane = threadIdx.x & 63, in = lane / L::kPieces, c = lane % L::kPieces;
-    if (c * 8 >= a.z.D) return;
+    if (DP % (L::kPieces * 8) != 0 && c * 8 >= DP) return;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      *reinterpret_cast<V8*>(s_k + (i * L::kAtOnce + in) * L::kStrideK + c * 8) = k[i];
-      *reinterpret_cast<V8*>(s_v + (i * L::kAtOnce + in) * L::kStrideV + c * 8) = v[i];
-    }
+    for (int i = 0; i < kLoads; ++i) *reinterpret_cast<V8*>(to + (i * L::kAtOnce + in) * STRIDE + c * 8) = x[i];
   }
+  __device__ __forceinline__ void put_keys(T* s_k) const { put<L::kStrideK>(k, s_k); }
+  __device__ __forceinline__ void put_values(T* s_v) const { put<L::kStrideV>(v, s_v); }
 };
 
 // A wave's 32 rows: a lane has row `lane % 32`, with its partner 32 lanes on.
@@ -419,70 +463,125 @@ struct Rows {
       if (d < z.D) q[c] = *reinterpret_cast<const V8*>(from + d);
       else q[c] = V8{};
     }
+    // (here, not in the tiles' loop, where the wait would be one for the next tile's loads too)
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) asm volatile("" : "+v"(q[c]));
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
     m = -INFINITY;
     l = 0.0f;
   }
 
-  // BLOCKS of 32 keys from key0 on; the rows see those before `least` at least.
-  template <int BLOCKS>
-  __device__ __forceinline__ void tile(const T* s_k, const T* s_v, int key0, int least, float scale) {
-    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    f32x16 s[BLOCKS];
-    float most = -INFINITY;
+  // Operands of the products: 32 keys' elements 16 c and on; 16 keys' (of a block of 32, `c`) elements 32 d and on.
+  static __device__ __forceinline__ V8 key_part(const T* s_k, int c) {
+    const int lane = threadIdx.x & 63;
+    return *reinterpret_cast<const V8*>(s_k + (lane & 31) * L::kStrideK + (lane >> 5) * 8 + c * 16);
+  }
+  static __device__ __forceinline__ V8 value_part(const T* s_v, int c, int d) {
+    typedef __attribute__((address_space(3))) s16x4* Lds;
+    const int lane = threadIdx.x & 63;
+    const T* at = s_v + (4 * (lane >> 5) + (lane & 15) / 4 + c * 16) * L::kStrideV + (lane >> 4 & 1) * 16 + (lane & 3) * 4 + d * 32;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 8 * L::kStrideV));
+    return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+
+  // A pair of weights is worked out here (the compiler would put it behind all products, next to its use) and summed, as
+  // rounded.
+  __device__ __forceinline__ void pin_pair(V8& w, int i) {
+    i32x4 x = __builtin_bit_cast(i32x4, w);
+    int y = x[i];
+    asm volatile("" : "+v"(y));
+    x[i] = y;
+    w = __builtin_bit_cast(V8, x);
+    l = Mma<T>::add_pair(y, l);
+  }
+
+  // A block of 32 keys in a pipeline of three: the next block's scores (QK), this block's weights, and the products of
+  // the last block's weights and values (PV). Matrix and vector instructions are independent of each other and
+  // alternate.
+  //
+  // The order of the reads of LDS and of the products is the one written here (kOrder lets only scalar and vector
+  // arithmetic move past it): left to itself the compiler reads a product's operand right before it and waits. Reads
+  // are kAhead products ahead.
+  template <bool QK, bool PV>
+  __device__ __forceinline__ void step(f32x16& s, V8 (&p)[2], const T* s_k, const T* s_v, int key0, int least, float scale) {
+    constexpr int kOrder = 0, kAhead = 4, DT = DP / 32, N = (QK ? DP / 16 : 0) + (PV ? 2 * DT : 0);
+    const int half = (threadIdx.x & 63) >> 5;
+    // (the scores' products, each of which waits for the one before, alternate with the values', which do not)
+    auto part = [&](auto f) {
+      constexpr int i = QK && PV ? f.value / 2 : f.value;
+      if constexpr (QK && !(PV && f.value % 2)) return key_part(s_k, i);
+      else return value_part(s_v, i / DT, i % DT);
+    };
+    V8 parts[kAhead];
+    each<(N < kAhead ? N : kAhead)>([&](auto f) { parts[f.value] = part(f); });
+    __builtin_amdgcn_sched_barrier(kOrder);
+    if (key0 + 32 > least) {
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) {
-      s[b] = f32x16{};
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        const V8 kv = *reinterpret_cast<const V8*>(s_k + (b * 32 + col) * L::kStrideK + c * 16 + half * 8);
-        s[b] = Mma<T>::mma(kv, q[c], s[b]);
-      }
+      for (int i = 0; i < 16; ++i)
+        if (key0 + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[i] = -INFINITY;
     }
-    if (key0 + BLOCKS * 32 > least) {
+    float most = s[0];
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (key0 + b * 32 + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[b][i] = -INFINITY;
-    }
-#pragma unroll
-    for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][i]);
+    for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
     most = fmaxf(most, other_half(most)) * scale;
-    if (__any(most > m)) {
-      const float now = fmaxf(m, most), by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+    // (weights of up to 2^8 instead of 1: the sums are fp32, and hardly a block moves the maximum by more)
+    const bool up = __any(most > m + 8.0f);
+    float by = 1.0f;
+    if (up) {
+      const float now = fmaxf(m, most);
+      by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       m = now;
       l *= by;
-#pragma unroll
-      for (int d = 0; d < DP / 32; ++d) o[d] *= by;
     }
     const float from = m == -INFINITY ? 0.0f : m;
+    f32x16 next{};
+    V8 w[2];
+    auto weights = [&](auto from_pair, auto to_pair) {
+      each<to_pair.value - from_pair.value>([&](auto j) {
+        constexpr int i = from_pair.value + j.value;
+        w[i / 4][i % 4 * 2] = static_cast<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], scale, -from)));
+        w[i / 4][i % 4 * 2 + 1] = static_cast<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], scale, -from)));
+        pin_pair(w[i / 4], i % 4);
+      });
+    };
+    each<N>([&](auto f) {
+      __builtin_amdgcn_sched_barrier(kOrder);
+      constexpr int i = QK && PV ? f.value / 2 : f.value;
+      if constexpr (QK && !(PV && f.value % 2)) next = Mma<T>::mma(parts[f.value % kAhead], q[i], next);
+      else o[i % DT] = Mma<T>::mma(parts[f.value % kAhead], p[i / DT], o[i % DT]);
+      if constexpr (f.value + kAhead < N) parts[f.value % kAhead] = part(Number<f.value + kAhead>{});
+      weights(Number<8 * f.value / N>{}, Number<8 * (f.value + 1) / N>{});
+    });
+    if constexpr (N == 0) weights(Number<0>{}, Number<8>{});
+    __builtin_amdgcn_sched_barrier(kOrder);
+    if (up) {
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale, -from));
-        l += s[b][i];
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        V8 p;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = static_cast<T>(s[b][8 * c + i]);
-        const T* v0 = s_v + (b * 32 + c * 16 + 4 * half + (lane & 15) / 4) * L::kStrideV + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          typedef __attribute__((address_space(3))) s16x4* Lds;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v0 + d * 32));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v0 + d * 32 + 8 * L::kStrideV));
-          const V8 vv = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-          o[d] = Mma<T>::mma(vv, p, o[d]);
-        }
-      }
+      for (int d = 0; d < DT; ++d) o[d] *= by;
     }
+    p[0] = w[0];
+    p[1] = w[1];
+    if (QK) s = next;
+  }
+  __device__ __forceinline__ void first_scores(f32x16& s, const T* s_k) {
+    s = f32x16{};
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) s = Mma<T>::mma(key_part(s_k, c), q[c], s);
+  }
+  __device__ __forceinline__ void last_values(const V8 (&p)[2], const T* s_v) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[d] = Mma<T>::mma(value_part(s_v, c, d), p[c], o[d]);
+  }
+  // A block alone.
+  __device__ __forceinline__ void block(const T* s_k, const T* s_v, int key0, int least, float scale) {
+    f32x16 s;
+    V8 p[2];
+    first_scores(s, s_k);
+    step<false, false>(s, p, s_k, s_v, key0, least, scale);
+    last_values(p, s_v);
   }
 
   // The rows' outputs where no other stretch has any of them, else their part.
@@ -524,22 +623,11 @@ struct Rows {
   }
 };
 
-// Heads of more elements than are there are filled up with zeros, once.
-template <class T, int DP, int KEYS>
-__device__ __forceinline__ void clear_rest(const AttendArgs& a, T* s_k, T* s_v, int first, int threads) {
-  typedef Layout<DP> L;
-  const int rest = (DP - a.z.D) / 8;
-  for (int i = first; i < KEYS * rest; i += threads) {
-    const int key = i / rest, c = i - key * rest;
-    *reinterpret_cast<typename Mma<T>::V8*>(s_k + key * L::kStrideK + a.z.D + c * 8) = {};
-    *reinterpret_cast<typename Mma<T>::V8*>(s_v + key * L::kStrideV + a.z.D + c * 8) = {};
-  }
-}
-
 // DP: the head's elements, rounded up to a width there is.
-template <class T, int DP>
+template <class T, int DP, bool SMALL>
 __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(AttendArgs a) {
   typedef Layout<DP> L;
+  typedef typename Mma<T>::V8 V8;
   constexpr int kWideK = kWideKeys * L::kStrideK, kWideV = kWideKeys * L::kStrideV;
   constexpr int kWaveK = kNarrowKeys * L::kStrideK, kWaveV = kNarrowKeys * L::kStrideV;
   constexpr int kWords = 2 * (kWideK + kWideV) > kWaves * (kWaveK + kWaveV) ? 2 * (kWideK + kWideV) : kWaves * (kWaveK + kWaveV);
@@ -547,25 +635,21 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
   const Shape& z = a.z;
   const Plan plan = plan_at(z, a.plan);
   const Lines lines = uniform(plan.lines);
-  const int group = stretch_of(blockIdx.x, z.wgs);
+  // 256 workgroups (one a CU) for wide segments, 256 for narrow ones, and so on: where there are both, a CU has one that
+  // computes beside one that waits for memory. (Workgroups for both in turn take 30 registers more, which are not there.)
+  const int block = blockIdx.x, group = stretch_of((block >> 9) * 256 + (block & 255), z.wgs);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-  const Start wide_start = uniform(plan.wide_start + group);
-  const Start narrow_start = uniform(plan.narrow_start + group * kWaves + wave);
   auto tiles_of = [&](int units, int per, int w) {  // of a stretch
     const int64_t left = static_cast<int64_t>(units) * z.Hkv - static_cast<int64_t>(w) * per;
     return static_cast<int>(min(max(left, static_cast<int64_t>(0)), static_cast<int64_t>(per)));
   };
 
-  {  // wide segments: the workgroup's
-    int left = tiles_of(lines.wide_units, lines.wide_per, group), h = wide_start.head, seg = wide_start.segment, tile = wide_start.tile;
-    Segment g = wide_start.first;
+  if (!(block & 256)) {  // wide segments: the workgroup's
+    const Start start = uniform(plan.wide_start + group);
+    int left = tiles_of(lines.wide_units, lines.wide_per, group), h = start.head, seg = start.segment, tile = start.tile;
+    Segment g = start.first;
     if (left > 0) {
       T *s_k = lds, *s_v = lds + 2 * kWideK;
-      if (z.D < DP) {
-        clear_rest<T, DP, kWideKeys>(a, s_k, s_v, tid, kWaves * 64);
-        clear_rest<T, DP, kWideKeys>(a, s_k + kWideK, s_v + kWideV, tid, kWaves * 64);
-      }
       constexpr int kShare = kWideKeys / kWaves;  // keys that a wave brings
       T *put_k = s_k + wave * kShare * L::kStrideK, *put_v = s_v + wave * kShare * L::kStrideV;
       for (;; tile = 0) {
@@ -573,33 +657,53 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
         left -= n;
         const int r = wave * 32 + (lane & 31);
         const bool busy = wave * 32 < n_rows, valid = r < n_rows;
-        Stage<T, DP, kShare> in;
+        Stage<T, DP, kShare, SMALL> in;
+        typedef typename Stage<T, DP, kShare, SMALL>::Pages Pages;
         in.begin(a, g, h);
         const int key0 = tile * kWideKeys, mine = key0 + wave * kShare;
-        in.look_up(a, mine);
-        in.fetch(a, mine);
-        in.look_up(a, mine + kWideKeys);
+        // Keys of tile t + 1 and values of tile t go to LDS between the two blocks of tile t: what they take the place of
+        // was read before the barrier in tile t - 1.
+        const Pages pages = in.look_up(a, mine);
+        in.fetch(in.k, in.k_head, pages, a, mine);
+        in.fetch(in.v, in.v_head, pages, a, mine);
+        Pages ahead = in.look_up(a, mine + kWideKeys);
         Rows<T, DP> rows;
         if (busy) rows.begin(a, g, h, r, valid);
         const int least = g.table < 0 ? g.keys : min(g.keys, g.keys - z.T + 1 + (g.row0 + wave * 32) / z.G);  // of the wave's rows
         __syncthreads();  // (the segment before is read)
-        in.put(a, put_k, put_v);
-        if (n > 1) {
-          in.fetch(a, mine + kWideKeys);
-          in.look_up(a, mine + 2 * kWideKeys);
-        }
+        in.put_keys(put_k);
+        if (n > 1) in.fetch(in.k, in.k_head, ahead, a, mine + kWideKeys);
         __syncthreads();
-        for (int it = 0; it < n; ++it) {
-          const int b = it & 1;
-          if (busy) rows.template tile<kWideKeys / 32>(s_k + b * kWideK, s_v + b * kWideV, key0 + it * kWideKeys, least, a.scale);
-          if (it + 1 < n) {
-            in.put(a, put_k + (b ^ 1) * kWideK, put_v + (b ^ 1) * kWideV);
-            if (it + 2 < n) {
-              in.fetch(a, mine + (it + 2) * kWideKeys);
-              in.look_up(a, mine + (it + 3) * kWideKeys);
-            }
+        auto keys_of = [&](int t) { return s_k + (t & 1) * kWideK; };
+        auto values_of = [&](int t) { return s_v + (t & 1) * kWideV; };
+        auto middle = [&](int t) {
+          in.put_values(put_v + (t & 1) * kWideV);
+          if (t + 1 < n) {
+            in.put_keys(put_k + ((t + 1) & 1) * kWideK);
+            const Pages next = in.look_up(a, mine + (t + 2) * kWideKeys);
+            in.fetch(in.v, in.v_head, ahead, a, mine + (t + 1) * kWideKeys);
+            in.fetch(in.k, in.k_head, next, a, mine + (t + 2) * kWideKeys);  // (behind the last tile: its last keys again)
+            ahead = next;
           }
           __syncthreads();
+        };
+        constexpr int kSecondK = 32 * L::kStrideK, kSecondV = 32 * L::kStrideV;
+        if (busy) {
+          f32x16 s;
+          V8 p[2];
+          rows.first_scores(s, s_k);
+          rows.template step<true, false>(s, p, s_k + kSecondK, s_v, key0, least, a.scale);
+          middle(0);
+          for (int t = 0; t + 1 < n; ++t) {
+            const int key = key0 + t * kWideKeys;
+            rows.template step<true, true>(s, p, keys_of(t + 1), values_of(t), key + 32, least, a.scale);
+            rows.template step<true, true>(s, p, keys_of(t + 1) + kSecondK, values_of(t) + kSecondV, key + 64, least, a.scale);
+            middle(t + 1);
+          }
+          rows.template step<false, true>(s, p, s_k, values_of(n - 1), key0 + (n - 1) * kWideKeys + 32, least, a.scale);
+          rows.last_values(p, values_of(n - 1) + kSecondV);
+        } else {
+          for (int t = 0; t < n; ++t) middle(t);
         }
         if (busy) rows.end(a, lines, g, true, h, group, r, valid, n == g.tiles, tile == 0);
         if (left <= 0) break;
@@ -611,36 +715,41 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
       }
     }
   }
-  {  // narrow segments: each wave's
+  else {  // narrow segments: each wave's
     const int w = group * kWaves + wave;
-    int left = tiles_of(lines.narrow_units, lines.narrow_per, w), h = narrow_start.head, seg = narrow_start.segment, tile = narrow_start.tile;
-    Segment g = narrow_start.first;
+    const Start start = uniform(plan.narrow_start + w);
+    int left = tiles_of(lines.narrow_units, lines.narrow_per, w), h = start.head, seg = start.segment, tile = start.tile;
+    Segment g = start.first;
     if (left > 0) {
       T *s_k = lds + wave * (kWaveK + kWaveV), *s_v = s_k + kWaveK;
-      if (z.D < DP) clear_rest<T, DP, kNarrowKeys>(a, s_k, s_v, lane, 64);
       for (;; tile = 0) {
         const int n = min(left, g.tiles - tile), n_rows = g.rows & (kAlone - 1);
         left -= n;
         const int r = lane & 31;
         const bool valid = r < n_rows;
-        Stage<T, DP, kNarrowKeys> in;
+        Stage<T, DP, kNarrowKeys, SMALL> in;
+        typedef typename Stage<T, DP, kNarrowKeys, SMALL>::Pages Pages;
         in.begin(a, g, h);
         const int key0 = tile * kNarrowKeys;
-        in.look_up(a, key0);
-        in.fetch(a, key0);
-        in.look_up(a, key0 + kNarrowKeys);
+        const Pages pages = in.look_up(a, key0);
+        in.fetch(in.k, in.k_head, pages, a, key0);
+        in.fetch(in.v, in.v_head, pages, a, key0);
+        Pages ahead = in.look_up(a, key0 + kNarrowKeys);
         Rows<T, DP> rows;
         rows.begin(a, g, h, r, valid);
         const int least = g.table < 0 ? g.keys : min(g.keys, g.keys - z.T + 1 + g.row0 / z.G);
         for (int it = 0; it < n; ++it) {
+          const int key = key0 + it * kNarrowKeys;
           wave_order();  // (the tile before is read)
-          in.put(a, s_k, s_v);
+          in.put_keys(s_k);
+          in.put_values(s_v);
           if (it + 1 < n) {
-            in.fetch(a, key0 + (it + 1) * kNarrowKeys);
-            in.look_up(a, key0 + (it + 2) * kNarrowKeys);
+            in.fetch(in.k, in.k_head, ahead, a, key + kNarrowKeys);
+            in.fetch(in.v, in.v_head, ahead, a, key + kNarrowKeys);
+            ahead = in.look_up(a, key + 2 * kNarrowKeys);
           }
           wave_order();
-          rows.template tile<1>(s_k, s_v, key0 + it * kNarrowKeys, least, a.scale);
+          rows.block(s_k, s_v, key, least, a.scale);
         }
         rows.end(a, lines, g, false, h, w, r, valid, n == g.tiles, tile == 0);
         if (left <= 0) break;

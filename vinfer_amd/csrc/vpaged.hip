@@ -197,7 +197,9 @@ int attend(const vpg::AttendArgs& d, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(d.z.S) * d.z.T * d.z.H;
   with_width(d.z.D, [&](auto w) {
     constexpr int DP = decltype(w)::value;
-    vpg::k_attend<T, DP><<<dim3(d.z.wgs), dim3(vpg::kWaves * 64), 0, stream>>>(d);
+    const dim3 grid(2 * d.z.wgs), block(vpg::kWaves * 64);
+    if (d.z.shift < 3) vpg::k_attend<T, DP, true><<<grid, block, 0, stream>>>(d);
+    else vpg::k_attend<T, DP, false><<<grid, block, 0, stream>>>(d);
     vpg::k_join<T, DP><<<dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream>>>(d);
   });
   return launched("vpaged_attend");
