@@ -13,7 +13,7 @@
 // and its partner 32 lanes on), running maximum and sum, P rounded to the values' type, O^T += V^T P^T with V read
 // from LDS transposed, which brings its keys in the order in which the scores lie in a lane: P never leaves the
 // registers. The next tile's keys and values are on their way to registers while a tile is computed; their pages are
-// looked up a tile before that, by scalar loads (eight keys at a time).
+// looked up a tile before that, by scalar loads.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -36,6 +36,7 @@ constexpr int kRows = 128;  // of a wide segment: 32 a wave
 constexpr int kNarrow = 32;  // of a narrow one
 constexpr int kWaves = 4;
 constexpr int kWideKeys = 64, kNarrowKeys = 32;  // of a tile
+constexpr int kRun = 16;                         // keys that a page is looked up for
 
 struct Shape {
   int S, B, T, H, Hkv, D, shift, M, MP;
@@ -60,7 +61,7 @@ struct alignas(16) PrefixPlace {
 };
 
 struct alignas(16) Start {  // of a stretch
-  int segment, tile, head, unused;
+  int segment, tile, head, lead;  // lead: places before the tile
   Segment first;  // the segment
 };
 
@@ -99,6 +100,10 @@ __host__ __device__ inline Plan plan_at(const Shape& s, void* p, size_t* bytes =
   return r;
 }
 
+// A segment costs its tiles and what its beginning takes (its queries' and first keys' way from memory, its results'):
+// about as long as the next two tiles' at full bandwidth. A line has this many places before each segment's first tile.
+constexpr int kLead = 2;
+
 constexpr int kHeld = 2048;  // segments and groups whose numbers a plan's making holds in LDS
 
 // Where a line's stretches begin. `unit`: the segments' first tiles.
@@ -112,15 +117,15 @@ __device__ __forceinline__ void write_starts(const Segment* segments, const int*
     const int at = static_cast<int>(u - static_cast<Index>(s.head) * units);
     int lo = 0;
     if (n <= kHeld) {
-      lo = find(held, n, at);
+      lo = find(held, n, at + kLead);
     } else {
       for (int step = 1 << (31 - __clz(n)); step; step >>= 1)
-        if (lo + step < n && segments[lo + step].unit <= at) lo += step;
+        if (lo + step < n && segments[lo + step].unit <= at + kLead) lo += step;
     }
     s.segment = lo;
     s.first = segments[lo];
-    s.tile = at - s.first.unit;
-    s.unused = 0;
+    s.tile = max(at - s.first.unit, 0);
+    s.lead = max(s.first.unit - at, 0);
     out[w] = s;
   }
 }
@@ -165,10 +170,11 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
     const int keys = is_wide ? kWideKeys : kNarrowKeys, tiles = (len + keys - 1) / keys;
     const int wide = tiles && is_wide ? static_cast<int>((rows + kRows - 1) / kRows) : 0;
     const int narrow = tiles && rows && !is_wide;
-    unsigned x[4] = {static_cast<unsigned>(wide), static_cast<unsigned>(wide) * tiles, static_cast<unsigned>(narrow),
-                     narrow ? static_cast<unsigned>(tiles) : 0u}, total[4];
+    unsigned x[4] = {static_cast<unsigned>(wide), static_cast<unsigned>(wide) * (tiles + kLead), static_cast<unsigned>(narrow),
+                     narrow ? static_cast<unsigned>(tiles + kLead) : 0u}, total[4];
     scan_exclusive<4>(x, total, part4, Add{});
-    const int first_wide = n_wide + x[0], wide_unit = wide_units + x[1], first_narrow = n_narrow + x[2], narrow_unit = narrow_units + x[3];
+    const int first_wide = n_wide + x[0], wide_unit = wide_units + x[1] + kLead, first_narrow = n_narrow + x[2];
+    const int narrow_unit = narrow_units + x[3] + kLead;
     n_wide += total[0];
     wide_units += total[1];
     n_narrow += total[2];
@@ -182,7 +188,7 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
       s.rows = static_cast<int>(min(rows - static_cast<int64_t>(i) * kRows, static_cast<int64_t>(kRows)));
       s.keys = len;
       s.tiles = tiles;
-      s.unit = wide ? wide_unit + i * tiles : narrow_unit;
+      s.unit = wide ? wide_unit + i * (tiles + kLead) : narrow_unit;
       s.index = wide ? first_wide + i : first_narrow;
       (wide ? plan.wide : plan.narrow)[s.index] = s;
       if (s.index < kHeld) (wide ? s_wide : s_narrow)[s.index] = s.unit;
@@ -211,9 +217,9 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
       }
       if (!row0) plan.prefix[s] = p;
     }
-    unsigned x[2] = {tiles > 0, static_cast<unsigned>(tiles)}, total[2];
+    unsigned x[2] = {tiles > 0, tiles ? static_cast<unsigned>(tiles + kLead) : 0u}, total[2];
     scan_exclusive<2>(x, total, part2, Add{});
-    const int at = x[0], segment = n_own + at, index = own_narrow ? own + at : segment, unit = units + x[1];
+    const int at = x[0], segment = n_own + at, index = own_narrow ? own + at : segment, unit = units + x[1] + kLead;
     n_own += total[0];
     own += total[0];
     units += total[1];
@@ -263,7 +269,8 @@ struct AttendArgs {
   const void* q;
   int64_t q_stride, q_token, q_head;
   const void *k, *v;
-  int64_t page_stride, place_stride, head_stride;
+  uint32_t page_bytes, place_bytes;
+  int64_t head_stride;
   const int32_t *tables, *prefix_tables;
   int64_t table_stride, prefix_table_stride;
   void* out;
@@ -356,14 +363,14 @@ struct Layout {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// A segment's keys and values of a head on their way: KEYS of them by this wave, eight at a time from their page (a
-// scalar base, the lanes' offsets the same for all; what a lane has not of a head's elements lies past the range: 0).
-// SMALL: pages of fewer than eight keys (a place of its own for each key of each lane).
+// A segment's keys and values of a head on their way: KEYS of them by this wave, 16 at a time from their page (a scalar
+// base, the lanes' offsets the same for all; what a lane has not of a head's elements lies past the range: 0).
+// SMALL: pages of fewer than 16 keys (a place of its own for each key of each lane).
 template <class T, int DP, int KEYS, bool SMALL>
 struct Stage {
   typedef typename Mma<T>::V8 V8;
   typedef Layout<DP> L;
-  static constexpr int kLoads = KEYS / L::kAtOnce, kGroups = KEYS / 8, kVariants = 8 / L::kAtOnce;
+  static constexpr int kLoads = KEYS / L::kAtOnce, kGroups = KEYS / kRun, kVariants = kRun / L::kAtOnce;
   static constexpr uint32_t kRange = 0x80000000u;
   V8 k[kLoads], v[kLoads];
   uint32_t offset[kVariants];
@@ -371,7 +378,7 @@ struct Stage {
   const T *k_head, *v_head;
   int last;  // key
   struct Pages {
-    int page[kGroups];
+    uint64_t at[kGroups];  // bytes from a head's first page
   };
 
   __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& g, int h) {
@@ -385,46 +392,49 @@ struct Stage {
     for (int i = 0; i < kVariants; ++i) offset[i] = place(a, i * L::kAtOnce + in, c);
   }
   static __device__ __forceinline__ uint32_t place(const AttendArgs& a, int key, int c) {
-    return c * 8 < a.z.D ? (static_cast<uint32_t>(key) * static_cast<uint32_t>(a.place_stride) + c * 8) * 2 : kRange;
+    return c * 8 < a.z.D ? static_cast<uint32_t>(key) * a.place_bytes + c * 16 : kRange;
   }
-  // The pages of the keys from key0 on (keys past the last: the last eight once more).
+  // Where the keys from key0 on lie (keys past the last: the last run once more).
   __device__ __forceinline__ Pages look_up(const AttendArgs& a, int key0) const {
     Pages p;
     if (SMALL) return p;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) p.page[g] = uniform(table + (min(key0 + 8 * g, last & ~7) >> a.z.shift));
+    for (int g = 0; g < kGroups; ++g) {
+      const int first = min(key0 + kRun * g, last & ~(kRun - 1));
+      const unsigned page = clampi(uniform(table + (first >> a.z.shift)), 0, a.pages - 1);
+      p.at[g] = static_cast<uint64_t>(page) * a.page_bytes + static_cast<unsigned>(first & ((1 << a.z.shift) - 1)) * a.place_bytes;
+    }
     return p;
   }
-  static __device__ __forceinline__ V8 load(const T* base, uint32_t off) {
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, kRange, 0x00027000);
+  static __device__ __forceinline__ V8 load(const T* base, uint64_t at, uint32_t off) {
+    char* p = const_cast<char*>(reinterpret_cast<const char*>(base)) + at;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(p, 0, kRange, 0x00027000);
     return __builtin_bit_cast(V8, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
   }
   // x[..] = what the keys from key0 on have at `head`: the keys themselves or their values.
   __device__ __forceinline__ void fetch(V8 (&x)[kLoads], const T* head, const Pages& p, const AttendArgs& a, int key0) const {
     const int lane = threadIdx.x & 63, in = lane / L::kPieces, c = lane % L::kPieces;
-    const int mask = (1 << a.z.shift) - 1;
     if constexpr (!SMALL) {
       if (key0 + KEYS <= last + 1) {
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const T* base = head + clampi(p.page[g], 0, a.pages - 1) * a.page_stride + ((key0 + 8 * g) & mask) * a.place_stride;
+        for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-          for (int i = 0; i < kVariants; ++i) x[g * kVariants + i] = load(base, offset[i]);
-        }
+          for (int i = 0; i < kVariants; ++i) x[g * kVariants + i] = load(head, p.at[g], offset[i]);
       } else {
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-          const int first = min(key0 + 8 * g, last & ~7);
-          const T* base = head + clampi(p.page[g], 0, a.pages - 1) * a.page_stride + (first & mask) * a.place_stride;
+          const int first = min(key0 + kRun * g, last & ~(kRun - 1));
 #pragma unroll
-          for (int i = 0; i < kVariants; ++i) x[g * kVariants + i] = load(base, place(a, min(i * L::kAtOnce + in, last - first), c));
+          for (int i = 0; i < kVariants; ++i) x[g * kVariants + i] = load(head, p.at[g], place(a, min(i * L::kAtOnce + in, last - first), c));
         }
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int key = min(key0 + i * L::kAtOnce + in, last);
-        const T* at = head + clampi(table[key >> a.z.shift], 0, a.pages - 1) * a.page_stride + (key & mask) * a.place_stride + c * 8;
+        const unsigned page = clampi(table[key >> a.z.shift], 0, a.pages - 1);
+        const char* at = reinterpret_cast<const char*>(head) + static_cast<uint64_t>(page) * a.page_bytes +
+                         static_cast<unsigned>(key & ((1 << a.z.shift) - 1)) * a.place_bytes + c * 16;
         x[i] = c * 8 < a.z.D ? *reinterpret_cast<const V8*>(at) : V8{};
       }
     }
@@ -639,20 +649,24 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
   // computes beside one that waits for memory. (Workgroups for both in turn take 30 registers more, which are not there.)
   const int block = blockIdx.x, group = stretch_of((block >> 9) * 256 + (block & 255), z.wgs);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  auto tiles_of = [&](int units, int per, int w) {  // of a stretch
+  auto places_of = [&](int units, int per, int w) {  // of a stretch
     const int64_t left = static_cast<int64_t>(units) * z.Hkv - static_cast<int64_t>(w) * per;
     return static_cast<int>(min(max(left, static_cast<int64_t>(0)), static_cast<int64_t>(per)));
   };
 
   if (!(block & 256)) {  // wide segments: the workgroup's
     const Start start = uniform(plan.wide_start + group);
-    int left = tiles_of(lines.wide_units, lines.wide_per, group), h = start.head, seg = start.segment, tile = start.tile;
+    // (a stretch behind the line has no places, and its start holds nothing)
+    const int places = places_of(lines.wide_units, lines.wide_per, group);
+    int left = places ? places - start.lead : 0, h = start.head, seg = start.segment, tile = start.tile;
     Segment g = start.first;
     if (left > 0) {
       T *s_k = lds, *s_v = lds + 2 * kWideK;
       constexpr int kShare = kWideKeys / kWaves;  // keys that a wave brings
       T *put_k = s_k + wave * kShare * L::kStrideK, *put_v = s_v + wave * kShare * L::kStrideV;
       for (;; tile = 0) {
+        const int next = seg + 1 == lines.n_wide ? 0 : seg + 1;
+        const Segment following = uniform(plan.wide + next);
         const int n = min(left, g.tiles - tile), n_rows = g.rows & (kAlone - 1);
         left -= n;
         const int r = wave * 32 + (lane & 31);
@@ -706,23 +720,26 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
           for (int t = 0; t < n; ++t) middle(t);
         }
         if (busy) rows.end(a, lines, g, true, h, group, r, valid, n == g.tiles, tile == 0);
+        left -= kLead;
         if (left <= 0) break;
-        if (++seg == lines.n_wide) {
-          seg = 0;
-          ++h;
-        }
-        g = uniform(plan.wide + seg);
+        if (!next) ++h;
+        seg = next;
+        g = following;
       }
     }
   }
   else {  // narrow segments: each wave's
     const int w = group * kWaves + wave;
     const Start start = uniform(plan.narrow_start + w);
-    int left = tiles_of(lines.narrow_units, lines.narrow_per, w), h = start.head, seg = start.segment, tile = start.tile;
+    // (a stretch behind the line has no places, and its start holds nothing)
+    const int places = places_of(lines.narrow_units, lines.narrow_per, w);
+    int left = places ? places - start.lead : 0, h = start.head, seg = start.segment, tile = start.tile;
     Segment g = start.first;
     if (left > 0) {
       T *s_k = lds + wave * (kWaveK + kWaveV), *s_v = s_k + kWaveK;
       for (;; tile = 0) {
+        const int next = seg + 1 == lines.n_narrow ? 0 : seg + 1;
+        const Segment following = uniform(plan.narrow + next);
         const int n = min(left, g.tiles - tile), n_rows = g.rows & (kAlone - 1);
         left -= n;
         const int r = lane & 31;
@@ -752,12 +769,11 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
           rows.block(s_k, s_v, key, least, a.scale);
         }
         rows.end(a, lines, g, false, h, w, r, valid, n == g.tiles, tile == 0);
+        left -= kLead;
         if (left <= 0) break;
-        if (++seg == lines.n_narrow) {
-          seg = 0;
-          ++h;
-        }
-        g = uniform(plan.narrow + seg);
+        if (!next) ++h;
+        seg = next;
+        g = following;
       }
     }
   }
@@ -801,7 +817,7 @@ __global__ __launch_bounds__(256) void k_join(AttendArgs a) {
   const int n_own = stretches(own_wide, own.unit, own.tiles, first_own);
   if (!pre.tiles && n_own == 1) return;  // (written already)
   const int R = (pre_wide ? ~pre.row0 : pre.row0) + r, segment = pre_wide ? R / kRows : 0;
-  if (pre.tiles) n_pre = stretches(pre_wide, pre.unit + segment * pre.tiles, pre.tiles, first_pre);
+  if (pre.tiles) n_pre = stretches(pre_wide, pre.unit + segment * (pre.tiles + kLead), pre.tiles, first_pre);
   const int n = n_pre + n_own;
   auto row_of = [&](int i) {  // the prefix's stretches, then the sequence's own
     if (i < n_pre)
@@ -809,6 +825,29 @@ __global__ __launch_bounds__(256) void k_join(AttendArgs a) {
     i -= n_pre;
     return partial_row(a, lines, own_wide, false, own.index, h, first_own + i, n_own == 1, i == 0) + r % kRows;
   };
+  if (n <= 8) {  // all at once: what each stretch says of the row by scalar loads
+    V x[8];
+    float2 ml[8];
+    each<8>([&](auto i) {
+      x[i.value] = V{};
+      ml[i.value] = make_float2(-INFINITY, 0.0f);
+      if (i.value < n) {
+        const int64_t row = row_of(i.value);
+        ml[i.value] = uniform(a.ml + row);
+        if (mine) x[i.value] = *reinterpret_cast<const V*>(a.o + row * z.D + lane * E);
+      }
+    });
+    float most = -INFINITY, total = 0.0f;
+    each<8>([&](auto i) { most = fmaxf(most, ml[i.value].x); });
+    if (most == -INFINITY) most = 0.0f;
+    V o = {};
+    each<8>([&](auto i) {
+      const float by = ml[i.value].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[i.value].x - most);
+      total += by * ml[i.value].y;
+      o += by * x[i.value];
+    });
+    return write(o * (total == 0.0f ? 0.0f : 1.0f / total));
+  }
   float most = -INFINITY;
   for (int i = lane; i < n; i += 64) most = fmaxf(most, a.ml[row_of(i)].x);
 #pragma unroll

@@ -136,7 +136,7 @@ bool shape_of(const vpaged_shape* a, vpg::Shape& z) {
   // (32 bits number a head's tiles and the segments' rows)
   const int64_t pages = z.M > z.MP ? z.M : z.MP;
   if (rows >= 1ll << 24 || z.S * rows >= 1ll << 31 || z.S * own >= 1ll << 31 ||
-      static_cast<double>(wide + narrow) * static_cast<double>((pages << z.shift) / vpg::kNarrowKeys + 1) >= 2147483648.0)
+      static_cast<double>(wide + narrow) * static_cast<double>((pages << z.shift) / vpg::kNarrowKeys + 1 + vpg::kLead) >= 2147483648.0)
     return false;
   z.rows = static_cast<int>(rows);
   z.own_tiles = static_cast<int>(own);
@@ -198,7 +198,7 @@ int attend(const vpg::AttendArgs& d, hipStream_t stream) {
   with_width(d.z.D, [&](auto w) {
     constexpr int DP = decltype(w)::value;
     const dim3 grid(2 * d.z.wgs), block(vpg::kWaves * 64);
-    if (d.z.shift < 3) vpg::k_attend<T, DP, true><<<grid, block, 0, stream>>>(d);
+    if ((1 << d.z.shift) < vpg::kRun) vpg::k_attend<T, DP, true><<<grid, block, 0, stream>>>(d);
     else vpg::k_attend<T, DP, false><<<grid, block, 0, stream>>>(d);
     vpg::k_join<T, DP><<<dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream>>>(d);
   });
@@ -349,8 +349,10 @@ int vpaged_attend(const vpaged_attend_args* a, void* stream) {
       (reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_pages) | reinterpret_cast<uintptr_t>(a->v_pages) |
        reinterpret_cast<uintptr_t>(a->out)) % 16)
     return fail(VPAGED_E_ARG, "q, the pages and out must be 16-byte aligned, with strides of multiples of 8 elements");
-  if ((a->page_stride | a->place_stride | a->head_stride) < 0 || a->place_stride >= 1ll << 27)
-    return fail(VPAGED_E_ARG, "strides of the pages must be >= 0, place_stride below 2^27");
+  // (offsets within a page, and a page's bytes, in 32 bits)
+  if ((a->page_stride | a->place_stride | a->head_stride) < 0 || a->page_stride >= 1ll << 31 ||
+      a->place_stride * (a->shape.page_size > vpg::kRun ? a->shape.page_size : vpg::kRun) >= 1ll << 30)
+    return fail(VPAGED_E_ARG, "strides of the pages must be >= 0, page_stride below 2^31, a page's positions below 2^30 elements");
   if (a->table_stride < 0 || (d.z.B && a->prefix_table_stride < 0)) return fail(VPAGED_E_ARG, "table strides must be >= 0");
   const AttendLayout L = attend_layout(d.z);
   if (!a->plan || reinterpret_cast<uintptr_t>(a->plan) & 255u) return fail(VPAGED_E_WORKSPACE, "plan must be set and 256-byte aligned");
@@ -365,8 +367,8 @@ int vpaged_attend(const vpaged_attend_args* a, void* stream) {
   d.q_head = a->q_head_stride;
   d.k = a->k_pages;
   d.v = a->v_pages;
-  d.page_stride = a->page_stride;
-  d.place_stride = a->place_stride;
+  d.page_bytes = static_cast<uint32_t>(a->page_stride * 2);
+  d.place_bytes = static_cast<uint32_t>(a->place_stride * 2);
   d.head_stride = a->head_stride;
   d.tables = a->tables;
   d.prefix_tables = a->prefix_tables;

@@ -154,8 +154,9 @@ class HipPaged:
             check_attend(q, k_pages, v_pages, tables, plan, pre, scale)
             self._check_dtype(q)
             strides = k_pages.stride()[:3]
-            if any(x & 7 for x in strides) or strides[1] >= 1 << 27:
-                raise ValueError(f"the cache's strides must be multiples of 8 elements (positions' below 2^27), got {strides}")
+            if any(x & 7 for x in strides) or strides[0] >= 1 << 31 or strides[1] * max(plan.page_size, 16) >= 1 << 30:
+                raise ValueError(f"the cache's strides must be multiples of 8 elements, pages less than 2^31 elements apart and "
+                                 f"a page's positions within 2^30, got {strides}")
             known = self._keep(key, (q.device, any(x & 7 for x in q.stride()[:3]), q.stride()[:3], strides,
                                      (*data.key, k_pages.shape[0], plan.head_dim**-0.5 if scale is None else scale),
                                      (tables.stride(0), pre.stride(0) if plan.groups else 0)))
