@@ -104,6 +104,7 @@ __host__ __device__ inline Plan plan_at(const Shape& s, void* p, size_t* bytes =
 // about as long as the next two tiles' at full bandwidth. A line has this many places before each segment's first tile.
 constexpr int kLead = 2;
 
+constexpr int kLeast = 2;  // tiles of a narrow stretch at least: joining more of them takes longer than a tile more
 constexpr int kHeld = 2048;  // segments and groups whose numbers a plan's making holds in LDS
 
 // Where a line's stretches begin. `unit`: the segments' first tiles.
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
     const int64_t all = static_cast<int64_t>(units_) * z.Hkv + stretches - 1;
     return max(all >> 31 ? static_cast<int>(all / stretches) : static_cast<int>(all) / stretches, 1);
   };
-  const int wide_per = per(wide_units, z.wgs), narrow_per = per(narrow_units, z.wgs * kWaves);
+  const int wide_per = per(wide_units, z.wgs), narrow_per = max(per(narrow_units, z.wgs * kWaves), kLeast);
   if (tid == 0)
     *plan.lines = Lines{wide_units, n_wide, wide_per, narrow_units, n_narrow, narrow_per, n_narrow_prefix, own_narrow ? own : 0};
   __syncthreads();
@@ -779,12 +780,13 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
   }
 }
 
-// A wave joins a row's stretches: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
-template <class T, int DP>
-__global__ __launch_bounds__(256) void k_join(AttendArgs a) {
+// WAVES waves join a row's stretches: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. (Where there are few rows, one
+// has many stretches: 16 waves take them at once.)
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void k_join(AttendArgs a) {
   const Shape& z = a.z;
-  const int lane = threadIdx.x & 63;
-  const unsigned id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = WAVES == 1 ? 0 : wave;
+  const unsigned id = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
   if (id >= static_cast<unsigned>(z.S) * z.T * z.H) return;
   const unsigned st = id / static_cast<unsigned>(z.H);
   const int hq = static_cast<int>(id - st * z.H), s = static_cast<int>(st / static_cast<unsigned>(z.T)), t = static_cast<int>(st) - s * z.T;
@@ -802,7 +804,7 @@ __global__ __launch_bounds__(256) void k_join(AttendArgs a) {
     TV y;
 #pragma unroll
     for (int e = 0; e < E; ++e) y[e] = static_cast<T>(x[e]);
-    if (mine) *reinterpret_cast<TV*>(to + lane * E) = y;
+    if (mine && !share) *reinterpret_cast<TV*>(to + lane * E) = y;
   };
   if (own.keys - z.T + t + 1 <= 0) return write(V{});  // no token
   const bool own_wide = z.rows > kNarrow, pre_wide = pre.row0 < 0;
@@ -826,6 +828,7 @@ __global__ __launch_bounds__(256) void k_join(AttendArgs a) {
     return partial_row(a, lines, own_wide, false, own.index, h, first_own + i, n_own == 1, i == 0) + r % kRows;
   };
   if (n <= 8) {  // all at once: what each stretch says of the row by scalar loads
+    if (share) return;
     V x[8];
     float2 ml[8];
     each<8>([&](auto i) {
@@ -848,34 +851,56 @@ __global__ __launch_bounds__(256) void k_join(AttendArgs a) {
     });
     return write(o * (total == 0.0f ? 0.0f : 1.0f / total));
   }
+  const int each_wave = (n + WAVES - 1) / WAVES, begin = share * each_wave, end = min(begin + each_wave, n);
   float most = -INFINITY;
-  for (int i = lane; i < n; i += 64) most = fmaxf(most, a.ml[row_of(i)].x);
+  for (int i = begin + lane; i < end; i += 64) most = fmaxf(most, a.ml[row_of(i)].x);
 #pragma unroll
   for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-  if (most == -INFINITY) most = 0.0f;
+  const float from = most == -INFINITY ? 0.0f : most;
   float total = 0.0f;
   V o = {};
-  for (int base = 0; base < n; base += 64) {
+  for (int base = begin; base < end; base += 64) {
     float by = 0.0f;
-    if (base + lane < n) {
+    if (base + lane < end) {
       const float2 ml = a.ml[row_of(base + lane)];
-      by = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - most);
+      by = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - from);
       total += by * ml.y;
     }
-    const int m = min(n - base, 64);
-    for (int i = 0; i < m; i += 8) {
-      V x[8];
+    const int m = min(end - base, 64);
+    for (int i = 0; i < m; i += 16) {
+      V x[16];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 16; ++j) {
         x[j] = V{};
         if (i + j < m && mine) x[j] = *reinterpret_cast<const V*>(a.o + row_of(base + i + j) * z.D + lane * E);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o += __shfl(by, min(i + j, 63)) * x[j];
+      for (int j = 0; j < 16; ++j) o += __shfl(by, min(i + j, 63)) * x[j];
     }
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
+  if constexpr (WAVES > 1) {
+    __shared__ V s_o[WAVES][64];
+    __shared__ float2 s_ml[WAVES];
+    s_o[wave][lane] = o;
+    if (!lane) s_ml[wave] = make_float2(most, total);
+    __syncthreads();
+    if (share) return;
+    float all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all = fmaxf(all, s_ml[w].x);
+    if (all == -INFINITY) all = 0.0f;
+    total = 0.0f;
+    o = V{};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float2 ml = s_ml[w];
+      const float by = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - all);
+      total += by * ml.y;
+      o += by * s_o[w][lane];
+    }
+  }
   write(o * (total == 0.0f ? 0.0f : 1.0f / total));
 }
 

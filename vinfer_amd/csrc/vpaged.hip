@@ -192,6 +192,9 @@ void with_width(int D, F f) {
   else f(Width<256>{});
 }
 
+// Up to this many rows of outputs (a sequence's token's head each) 16 waves join one: the longest has few others beside it.
+constexpr int kFewRows = 512;
+
 template <class T>
 int attend(const vpg::AttendArgs& d, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(d.z.S) * d.z.T * d.z.H;
@@ -200,7 +203,8 @@ int attend(const vpg::AttendArgs& d, hipStream_t stream) {
     const dim3 grid(2 * d.z.wgs), block(vpg::kWaves * 64);
     if ((1 << d.z.shift) < vpg::kRun) vpg::k_attend<T, DP, true><<<grid, block, 0, stream>>>(d);
     else vpg::k_attend<T, DP, false><<<grid, block, 0, stream>>>(d);
-    vpg::k_join<T, DP><<<dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream>>>(d);
+    if (rows <= kFewRows) vpg::k_join<T, DP, 16><<<dim3(static_cast<unsigned>(rows)), dim3(1024), 0, stream>>>(d);
+    else vpg::k_join<T, DP, 1><<<dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream>>>(d);
   });
   return launched("vpaged_attend");
 }
