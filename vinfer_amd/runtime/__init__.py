@@ -1,7 +1,8 @@
-"""Callers of the sampler: the continuous-batching decode loop and beam search."""
+"""Callers of the operators: the continuous-batching decode loop, beam search, and the paged cache of their models."""
 
 from vinfer_amd.runtime.batch import BatchDecoder, DecodeModel, SpeculativeDecoder, Step, TextStream, check_request
 from vinfer_amd.runtime.beam import BeamModel, Hypothesis, beam_search
+from vinfer_amd.runtime.paged import CacheStep, SharedPromptCache
 
-__all__ = ["BatchDecoder", "BeamModel", "DecodeModel", "Hypothesis", "SpeculativeDecoder", "Step", "TextStream",
-           "beam_search", "check_request"]
+__all__ = ["BatchDecoder", "BeamModel", "CacheStep", "DecodeModel", "Hypothesis", "SharedPromptCache", "SpeculativeDecoder",
+           "Step", "TextStream", "beam_search", "check_request"]

@@ -26,7 +26,9 @@ from vinfer_amd.sampler.beams import BeamState
 
 
 class BeamModel(Protocol):
-    """A decode model whose slots' states can be moved: ``DecodeModel``'s two calls, and the states."""
+    """A decode model whose slots' states can be moved: ``DecodeModel``'s two calls, and the states. With
+    ``shared_prompts = True`` the states hold a beam's continuation alone (``SharedPromptCache``: the model keeps a
+    request's prompt for all of its beams), and their lengths count from the prompt's end."""
 
     device: torch.device
 
@@ -70,8 +72,9 @@ def beam_search(model: BeamModel, sampler: SamplerBackend, prompts: Sequence[Seq
 
     rows = torch.stack([model.prefill(b * W, torch.as_tensor(p, device=dev)) for b, p in enumerate(prompts)])
     logits = rows[:, None].expand(B, W, rows.shape[-1])
+    held = torch.zeros_like(lengths) if getattr(model, "shared_prompts", False) else lengths  # of the states' positions
     if states is not None:  # (every beam starts from its request's prompt)
-        states.launch(torch.zeros(B, W, dtype=torch.int32, device=dev), lengths)
+        states.launch(torch.zeros(B, W, dtype=torch.int32, device=dev), held)
     scores = torch.full((B, W), -math.inf, device=dev)
     scores[:, 0] = 0.0
     finished = torch.zeros(B, W, dtype=torch.bool, device=dev)
@@ -88,7 +91,7 @@ def beam_search(model: BeamModel, sampler: SamplerBackend, prompts: Sequence[Seq
         if step + 1 == max_tokens or (step + 1) % check_every == 0 and bool(finished.all()):
             break
         if states is not None:
-            states.launch(beams, lengths + step)
+            states.launch(beams, held + step)
         positions = (lengths + step).repeat_interleave(W)
         logits = model.decode(slots, tokens.clamp(min=0).reshape(-1).long(), positions.long()).view(B, W, -1)
 
