@@ -210,12 +210,13 @@ int attend(const vpg::AttendArgs& d, hipStream_t stream) {
 }
 
 template <class T>
-void rotate(const vpg::RotateArgs& r, bool vectors, bool interleaved, dim3 grid, hipStream_t stream) {
+void rotate(const vpg::RotateArgs& r, bool vectors, vpg::Pairs pairs, dim3 grid, hipStream_t stream) {
   const dim3 block(vpg::kRotateThreads);
-  if (vectors && interleaved) vpg::k_rotate<T, 8, true><<<grid, block, 0, stream>>>(r);
-  else if (vectors) vpg::k_rotate<T, 8, false><<<grid, block, 0, stream>>>(r);
-  else if (interleaved) vpg::k_rotate<T, 1, true><<<grid, block, 0, stream>>>(r);
-  else vpg::k_rotate<T, 1, false><<<grid, block, 0, stream>>>(r);
+  if (vectors && pairs == vpg::kAdjacent) vpg::k_rotate<T, 8, vpg::kAdjacent><<<grid, block, 0, stream>>>(r);
+  else if (vectors && pairs == vpg::kExchanged) vpg::k_rotate<T, 8, vpg::kExchanged><<<grid, block, 0, stream>>>(r);
+  else if (vectors) vpg::k_rotate<T, 8, vpg::kHalves><<<grid, block, 0, stream>>>(r);
+  else if (pairs == vpg::kAdjacent) vpg::k_rotate<T, 1, vpg::kAdjacent><<<grid, block, 0, stream>>>(r);
+  else vpg::k_rotate<T, 1, vpg::kHalves><<<grid, block, 0, stream>>>(r);
 }
 
 }  // namespace
@@ -288,7 +289,7 @@ int vpaged_rotate_store(const vpaged_rotate_args* a, void* stream) {
   vpg::RotateArgs r{a->q, a->k, a->v, a->q_stride, a->k_stride, a->v_stride, a->q_head_stride, a->k_head_stride, a->v_head_stride,
                     a->out_q, a->k_pages, a->v_pages, a->page_stride, a->place_stride, a->head_stride, a->positions, a->slots,
                     a->frequencies, a->magnitude, a->tokens, a->heads, a->kv_heads, a->head_dim, a->dim,
-                    static_cast<int64_t>(a->pages) * a->page_size, log2_of(a->page_size), 0, 0, {}, {}};
+                    static_cast<int64_t>(a->pages) * a->page_size, log2_of(a->page_size), 0, {}, {}};
   // 16-byte accesses where every head's row begins and ends on one, and halves' pairs are eight apart in both.
   int64_t all = a->head_dim | (a->interleaved ? 0 : half);
   if (a->heads) all |= a->q_stride | a->q_head_stride;
@@ -297,20 +298,21 @@ int vpaged_rotate_store(const vpaged_rotate_args* a, void* stream) {
                        reinterpret_cast<uintptr_t>(a->out_q) | reinterpret_cast<uintptr_t>(a->k_pages) | reinterpret_cast<uintptr_t>(a->v_pages);
   const bool vectors = all % 8 == 0 && at % 16 == 0;
   const int E = vectors ? 8 : 1;
-  const int per_head = (a->interleaved ? a->head_dim : a->head_dim - half) / E;
+  const vpg::Pairs pairs = a->interleaved ? vpg::kAdjacent
+                           : vectors && half && power_of_two(a->head_dim) ? vpg::kExchanged
+                                                                         : vpg::kHalves;
+  const int per_head = (pairs == vpg::kHalves ? a->head_dim - half : a->head_dim) / E;
   r.per_head = div_by(per_head);
   r.tail = div_by(a->head_dim / E);
   r.items = (a->heads + a->kv_heads) * per_head + a->kv_heads * (a->head_dim / E);
-  // Few tokens: a workgroup each, their heads over several; many: a workgroup takes four, whose angles fill its threads.
-  r.tokens = a->tokens >= 4 * 4 * kCus ? vpg::kRotateTokens : 1;
-  const int64_t x = (static_cast<int64_t>(a->tokens) + r.tokens - 1) / r.tokens;
-  const int64_t rounds = (r.items + vpg::kRotateThreads - 1) / vpg::kRotateThreads;
-  int64_t y = x >= 4 * kCus ? 1 : (4 * kCus + x - 1) / x;
+  // A workgroup a token; where those are few, a token's items over several.
+  const int rounds = (r.items + vpg::kRotateThreads - 1) / vpg::kRotateThreads;
+  int y = a->tokens >= 4 * kCus ? 1 : (4 * kCus + a->tokens - 1) / a->tokens;
   if (y > rounds) y = rounds;
-  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(y));
+  const dim3 grid(static_cast<unsigned>(a->tokens), static_cast<unsigned>(y));
   const auto s = static_cast<hipStream_t>(stream);
-  if (a->dtype == VPAGED_BF16) rotate<__bf16>(r, vectors, a->interleaved, grid, s);
-  else rotate<_Float16>(r, vectors, a->interleaved, grid, s);
+  if (a->dtype == VPAGED_BF16) rotate<__bf16>(r, vectors, pairs, grid, s);
+  else rotate<_Float16>(r, vectors, pairs, grid, s);
   return launched("vpaged_rotate_store");
 }
 
