@@ -116,7 +116,8 @@ int vpaged_rotate_store(const vpaged_rotate_args* args, void* stream);
 /* Sequences s of `queries` new tokens each, in groups: group g's are [group_starts[g], group_starts[g + 1]), and they
  * share a prefix of prefix_lengths[g] positions. lengths[s] are a sequence's own positions behind it, its new tokens
  * the last of them: token t sees the prefix and own positions up to lengths[s] - queries + t. Where that is below 0
- * there is no such token, and its outputs are 0. Lengths outside what the tables hold are taken as the nearest inside;
+ * there is no such token, and its outputs are 0. What lies behind a sequence's length is not seen, whatever it holds; a
+ * value that is not finite at a sequence's own position reaches all of the call's new tokens. Lengths outside what the tables hold are taken as the nearest inside;
  * group_starts ascend from 0 to sequences.
  *   out[s][t][h] = sum_j softmax_j(scale q[s][t][h] . k[j][h / (heads / kv_heads)]) v[j][h / (heads / kv_heads)] */
 typedef struct vpaged_shape {

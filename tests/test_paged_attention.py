@@ -278,3 +278,32 @@ def test_refusals():
                        ({"prefix_tables": i32(1, 3)}, "prefix_tables"), ({"scale": 0.0}, "scale"), ({"scale": math.nan}, "scale")):
         with pytest.raises(ValueError, match=match):
             b.attend(**{**call, **bad})
+
+
+@pytest.mark.gpu
+def test_a_plan_of_another_backend_is_refused():
+    c = Case(torch.device("cpu"), BF16, None, [9], seed=13)
+    plan = c.plan(backend(c.device, BF16))
+    with pytest.raises(ValueError, match="another backend"):
+        c.attend(backend(GPU, BF16), plan)
+
+
+@pytest.mark.gpu
+def test_a_cache_past_32_bits():
+    # pages whose bytes lie past 2^32 from the first one's, as keys and as a place to store them
+    P, page, D = 300000, 16, 256
+    cache = [torch.empty(P, page, 2, D, dtype=BF16, device=GPU) for _ in range(2)]  # 4.9 GB each
+    tables = torch.tensor([[P - 1, 5, P - 7, 262144]], dtype=torch.int32, device=GPU)
+    g = torch.Generator().manual_seed(1)
+    small = [torch.randn(4, page, 2, D, generator=g).to(BF16) for _ in range(2)]
+    for t, x in zip(cache, small):
+        t[tables[0].long()] = x.to(GPU)
+    q = torch.randn(1, 1, 4, D, generator=g).to(BF16)
+    b = backend(GPU, BF16)
+    plan = b.plan(torch.tensor([61], dtype=torch.int32, device=GPU), queries=1, heads=4, kv_heads=2, head_dim=D, page_size=page, max_pages=4)
+    got = b.attend(q.to(GPU), *cache, tables, plan)
+    near = [torch.zeros(4, page, 2, D, dtype=BF16, device=GPU) for _ in range(2)]
+    for t, x in zip(near, small):
+        t.copy_(x)
+    want = b.attend(q.to(GPU), *near, torch.arange(4, dtype=torch.int32, device=GPU)[None], plan)
+    assert torch.equal(got, want)

@@ -131,7 +131,9 @@ bool shape_of(const vpaged_shape* a, vpg::Shape& z) {
   z.G = z.H / z.Hkv;
   const int64_t rows = static_cast<int64_t>(z.T) * z.G, own = (rows + vpg::kRows - 1) / vpg::kRows;
   const bool own_narrow = rows <= vpg::kNarrow;
-  const int64_t wide = (z.B ? z.B + static_cast<int64_t>(z.S) * rows / vpg::kRows : 0) + (own_narrow ? 0 : z.S * own);
+  // (a wide group has more than kNarrow rows)
+  const int64_t all = static_cast<int64_t>(z.S) * rows, groups = all / (vpg::kNarrow + 1);
+  const int64_t wide = (z.B ? (z.B < groups ? z.B : groups) + all / vpg::kRows : 0) + (own_narrow ? 0 : z.S * own);
   const int64_t narrow = z.B + (own_narrow ? z.S : 0);
   // (32 bits number a head's tiles and the segments' rows)
   const int64_t pages = z.M > z.MP ? z.M : z.MP;

@@ -166,7 +166,8 @@ class PagedBackend(Protocol):
         """Attention ``[S, queries, heads, head_dim]``: token t of sequence s sees its group's prefix and the own
         positions up to ``lengths[s] - queries + t``; where that is below 0 there is no such token (a batch padded on
         the left, a finished sequence), and its output is 0. Query heads share key heads in order. ``scale`` (positive)
-        defaults to ``head_dim ** -0.5``. An entry of a table outside the cache is taken as the nearest page."""
+        defaults to ``head_dim ** -0.5``. What lies behind the lengths is not seen, whatever it holds; a value that is not
+        finite at an own position reaches all of the sequence's new tokens of the call. An entry of a table outside the cache is taken as the nearest page."""
         ...
 
 

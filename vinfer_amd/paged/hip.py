@@ -145,6 +145,8 @@ class HipPaged:
 
     def attend(self, q, k_pages, v_pages, tables, plan: AttentionPlan, *, prefix_tables=None, scale=None) -> torch.Tensor:
         data, pre = plan.data, prefix_tables
+        if not isinstance(data, _Planned):
+            raise ValueError("the plan is another backend's")
         key = ("attend", data.key, scale, torch.is_grad_enabled(), q.requires_grad, q.shape, k_pages.shape, v_pages.shape, tables.shape,
                q.stride(), k_pages.stride(), v_pages.stride(), tables.stride(), q.dtype, k_pages.dtype, v_pages.dtype, tables.dtype,
                q.get_device(), k_pages.get_device(), v_pages.get_device(), tables.get_device(), plan.device.index,
