@@ -14,6 +14,11 @@
 // from LDS transposed, which brings its keys in the order in which the scores lie in a lane: P never leaves the
 // registers. The next tile's keys and values are on their way to registers while a tile is computed; their pages are
 // looked up a tile before that, by scalar loads.
+//
+// Bound by HBM where rows are few: 4 sequences of 100000 positions with 5 tokens each (64 query, 8 key heads of 128, 1.15
+// GB) 207 us, 5.5 TB/s; 64 requests of 4 beams behind up to 8192 positions (1.2 GB) 241 us, 5.0 TB/s. By matrix and vector
+// instructions where a prefix has many: 192 sequences behind 32768 positions 103 GFLOP in 155 us, 660 TFLOP/s (heads of 256
+// 640, of 64 590). By chains of loads where there is little of both: 4 beams behind 1000 positions 12 us and 6 to join.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -131,6 +136,8 @@ __device__ __forceinline__ void write_starts(const Segment* segments, const int*
   }
 }
 
+// One workgroup: the groups' segments, then the sequences' own, then the stretches' beginnings; prefix sums and searches in
+// LDS. A chain of loads and barriers: 7 us for one request, 16 for 256 sequences in 64 groups.
 __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* __restrict__ lengths,
                                                         const int32_t* __restrict__ prefix_lengths,
                                                         const int32_t* __restrict__ group_starts, void* mem) {
@@ -354,7 +361,7 @@ __device__ __forceinline__ void wave_order() {
 }
 
 // A tile's layout in LDS. Keys' rows are 16 bytes longer: 16 keys' pieces lie in 16 different groups of banks. The values'
-// rows are 16 words on, modulo 32, so that four keys' 64 bytes (a transposed read of half a wave) fill the banks.
+// rows are 16 or 48 words on, modulo 64, so that four keys' 64 bytes (a transposed read of half a wave) fill the banks.
 template <int DP>
 struct Layout {
   static constexpr int kStrideK = DP + 8, kStrideV = DP % 64 ? DP : DP + 32;
@@ -728,8 +735,7 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
         g = following;
       }
     }
-  }
-  else {  // narrow segments: each wave's
+  } else {  // narrow segments: each wave's
     const int w = group * kWaves + wave;
     const Start start = uniform(plan.narrow_start + w);
     // (a stretch behind the line has no places, and its start holds nothing)
@@ -781,7 +787,8 @@ __global__ __launch_bounds__(kWaves * 64, DP > 128 ? 1 : 2) void k_attend(Attend
 }
 
 // WAVES waves join a row's stretches: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. (Where there are few rows, one
-// has many stretches: 16 waves take them at once.)
+// has many stretches: 16 waves take them at once. A sequence of 30000 positions, 8 key heads: attention and joining 65 us with
+// one wave a row, 33 with 16.) Bound by its three loads one behind the other: 6 us for 128 rows, 13 for 8192.
 template <class T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void k_join(AttendArgs a) {
   const Shape& z = a.z;

@@ -4,8 +4,8 @@
 //   y1 = m (x1 cos a - x2 sin a), y2 = m (x2 cos a + x1 sin a)
 // a is taken in 64 bits and brought to turns there (a / 2 pi less its nearest whole number), so that its sine and
 // cosine are right to fp32 at any position. Each element is read and written once, products and sums are fp32, and
-// the result is rounded once to the elements' type. Bound by HBM for many tokens, by latency for few: the angles of a
-// workgroup's tokens are worked out once, in LDS, for all heads.
+// the result is rounded once to the elements' type. Bound by HBM for many tokens (16384 of 48 heads of 128, 403 MB: 75 us, 5.4
+// TB/s, as a copy), by latency for few (4 tokens 3 us): a token's angles are worked out once, in LDS, for all heads.
 #pragma once
 
 #include <hip/hip_runtime.h>
