@@ -24,6 +24,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "stretches.cuh"
 #include "tables.cuh"
 
 namespace vpg {
@@ -114,13 +115,12 @@ constexpr int kHeld = 2048;  // segments and groups whose numbers a plan's makin
 
 // Where a line's stretches begin. `unit`: the segments' first tiles.
 template <class Index>
-__device__ __forceinline__ void write_starts(const Segment* segments, const int* held, int n, int units, int per, int heads, Start* out) {
-  const Index all = static_cast<Index>(units) * heads;
-  for (Index w = threadIdx.x; w * per < all; w += kTableThreads) {
-    const Index u = w * per;
+__device__ __forceinline__ void write_starts(const Segment* segments, const int* held, int n, const Stretches& line, Start* out) {
+  for (int w = threadIdx.x; begins<Index>(line, w); w += kTableThreads) {
+    const Index u = static_cast<Index>(w) * line.per;
     Start s;
-    s.head = static_cast<int>(u / units);
-    const int at = static_cast<int>(u - static_cast<Index>(s.head) * units);
+    s.head = static_cast<int>(u / line.units);
+    const int at = static_cast<int>(u - static_cast<Index>(s.head) * line.units);
     int lo = 0;
     if (n <= kHeld) {
       lo = find(held, n, at + kLead);
@@ -253,21 +253,16 @@ __global__ __launch_bounds__(kTableThreads) void k_plan(Shape z, const int32_t* 
     n_wide = n_own;
     wide_units = units;
   }
-  auto per = [&](int units_, int stretches) {
-    const int64_t all = static_cast<int64_t>(units_) * z.Hkv + stretches - 1;
-    return max(all >> 31 ? static_cast<int>(all / stretches) : static_cast<int>(all) / stretches, 1);
-  };
-  const int wide_per = per(wide_units, z.wgs), narrow_per = max(per(narrow_units, z.wgs * kWaves), kLeast);
+  const Stretches wide_line = cut(wide_units, z.Hkv, z.wgs, 1), narrow_line = cut(narrow_units, z.Hkv, z.wgs * kWaves, kLeast);
   if (tid == 0)
-    *plan.lines = Lines{wide_units, n_wide, wide_per, narrow_units, n_narrow, narrow_per, n_narrow_prefix, own_narrow ? own : 0};
+    *plan.lines = Lines{wide_units, n_wide, wide_line.per, narrow_units, n_narrow, narrow_line.per, n_narrow_prefix, own_narrow ? own : 0};
   __syncthreads();
-  auto write = [&](const Segment* segments, const int* unit, int n, int units_, int per_, Start* out) {
-    // (the last stretch begins before 2^31 tiles, and the next one's number is compared too)
-    if (static_cast<int64_t>(units_) * z.Hkv < 1ll << 30) write_starts<int>(segments, unit, n, units_, per_, z.Hkv, out);
-    else write_starts<int64_t>(segments, unit, n, units_, per_, z.Hkv, out);
+  auto write = [&](const Segment* segments, const int* unit, int n, const Stretches& line, Start* out) {
+    if (small(line)) write_starts<int>(segments, unit, n, line, out);
+    else write_starts<int64_t>(segments, unit, n, line, out);
   };
-  write(plan.wide, s_wide, n_wide, wide_units, wide_per, plan.wide_start);
-  write(plan.narrow, s_narrow, n_narrow, narrow_units, narrow_per, plan.narrow_start);
+  write(plan.wide, s_wide, n_wide, wide_line, plan.wide_start);
+  write(plan.narrow, s_narrow, n_narrow, narrow_line, plan.narrow_start);
 }
 
 struct AttendArgs {
