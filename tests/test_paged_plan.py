@@ -94,3 +94,13 @@ def test_lines_of_half_a_billion_tiles(D, heads, length):
     behind = 64 + (12 * wgs + 63) // 64 * 64
     assert (starts[len(u) :] == -7).all()
     assert (got[behind : behind + 12 * 4 * wgs] == -7).all()  # (no narrow segment: their starts stay)
+
+
+def test_stretches_of_2_31_tiles_are_refused():
+    # 512 segments of 65536 x 1 rows on 1024 key heads: more than 2^31 tiles for each of the 256 workgroups of wide heads
+    lib = _vpaged.load()
+    shape = lambda pages, D=256: ctypes.byref(_vpaged.VpagedShape(0, 1, 0, 65536, 1024, 1024, D, 4096, pages, 0))  # noqa: E731
+    for D, least in ((256, 8192), (128, 16384)):
+        # (pages * 4096 / 32 + 3 tiles of 512 segments and a head each)
+        assert 512 * (least * 128 + 3) * 1024 >= (2**31 - 1) * (256 if D > 128 else 512) > 512 * ((least - 1) * 128 + 3) * 1024
+        assert lib.vpaged_plan_bytes(shape(least, D)) == 0 < lib.vpaged_plan_bytes(shape(least - 1, D))

@@ -135,16 +135,17 @@ bool shape_of(const vpaged_shape* a, vpg::Shape& z) {
   const int64_t all = static_cast<int64_t>(z.S) * rows, groups = all / (vpg::kNarrow + 1);
   const int64_t wide = (z.B ? (z.B < groups ? z.B : groups) + all / vpg::kRows : 0) + (own_narrow ? 0 : z.S * own);
   const int64_t narrow = z.B + (own_narrow ? z.S : 0);
-  // (32 bits number a head's tiles and the segments' rows)
+  z.wgs = kCus * (z.D > 128 ? 1 : 2);
+  // (32 bits number a head's tiles, a stretch's of all heads' tiles, and the segments' rows)
   const int64_t pages = z.M > z.MP ? z.M : z.MP;
-  if (rows >= 1ll << 24 || z.S * rows >= 1ll << 31 || z.S * own >= 1ll << 31 ||
-      static_cast<double>(wide + narrow) * static_cast<double>((pages << z.shift) / vpg::kNarrowKeys + 1 + vpg::kLead) >= 2147483648.0)
+  const double tiles = static_cast<double>(wide + narrow) * static_cast<double>((pages << z.shift) / vpg::kNarrowKeys + 1 + vpg::kLead);
+  if (rows >= 1ll << 24 || z.S * rows >= 1ll << 31 || z.S * own >= 1ll << 31 || tiles >= 2147483648.0 ||
+      tiles * z.Hkv >= 2147483647.0 * z.wgs)
     return false;
   z.rows = static_cast<int>(rows);
   z.own_tiles = static_cast<int>(own);
   z.max_wide = static_cast<int>(wide);
   z.max_narrow = static_cast<int>(narrow);
-  z.wgs = kCus * (z.D > 128 ? 1 : 2);
   return true;
 }
 
@@ -178,7 +179,8 @@ size_t plan_bytes(const vpg::Shape& z) {
 
 const char* const kShapeRule =
     "the shape is refused: sequences and groups in [0, 65536], queries in [1, 65536], heads a multiple of kv_heads up to 1024, head_dim a "
-    "multiple of 8 in [8, 256], page_size a power of two up to 4096, tables of at least a page, fewer than 2^31 tiles and rows";
+    "multiple of 8 in [8, 256], page_size a power of two up to 4096, tables of at least a page, fewer than 2^31 rows and tiles of a head, and "
+    "of all heads' tiles fewer than 2^31 for each of 256 workgroups";
 
 // f(a tag whose ::value is the head's elements rounded up) for a head of D
 template <int N>
