@@ -139,7 +139,7 @@ int vpaged_plan(const vpaged_shape* shape, const int32_t* lengths, const int32_t
                 const int32_t* group_starts, void* plan, size_t plan_bytes, void* stream);
 
 typedef struct vpaged_attend_args {
-  vpaged_shape shape; /* the plan's */
+  vpaged_shape shape; /* the plan's, with the type of q, the pages and out (a plan knows none) */
   int32_t pages;      /* of the cache; a table's entry outside them is taken as the nearest inside */
   float scale;
   const void* q; /* sequence s, token t, head h at s * q_stride + t * q_token_stride + h * q_head_stride */

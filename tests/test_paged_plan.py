@@ -13,6 +13,8 @@ import pytest
 import torch
 
 from vinfer_amd import _vpaged
+from vinfer_amd.paged import PAGED
+from vinfer_amd.registry import BackendContext
 
 GPU = torch.device("cuda", 0)
 CSRC = Path(_vpaged.__file__).resolve().parent / "csrc"
@@ -104,3 +106,19 @@ def test_stretches_of_2_31_tiles_are_refused():
         # (pages * 4096 / 32 + 3 tiles of 512 segments and a head each)
         assert 512 * (least * 128 + 3) * 1024 >= (2**31 - 1) * (256 if D > 128 else 512) > 512 * ((least - 1) * 128 + 3) * 1024
         assert lib.vpaged_plan_bytes(shape(least, D)) == 0 < lib.vpaged_plan_bytes(shape(least - 1, D))
+
+
+@pytest.mark.gpu
+def test_a_plan_serves_layers_of_either_type():
+    types = torch.bfloat16, torch.float16
+    backends = [PAGED.resolve("hip", BackendContext(GPU, t)) for t in types]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=GPU)  # noqa: E731
+    plans = [b.plan(i32([40, 7, 65]), queries=1, heads=4, kv_heads=2, head_dim=64, page_size=16, max_pages=5, prefix_lengths=i32([50]),
+                    group_starts=i32([0, 3]), max_prefix_pages=4) for b in backends]
+    tables, prefix_tables = i32(np.arange(15).reshape(3, 5)), i32([[15, 16, 17, 18]])
+    for t, b, own in zip(types, backends, plans):
+        q, k, v = (torch.randn(*s, device=GPU).to(t) for s in ((3, 1, 4, 64), (19, 16, 2, 64), (19, 16, 2, 64)))
+        got = [b.attend(q, k, v, tables, p, prefix_tables=prefix_tables) for p in plans]
+        assert torch.equal(got[0], got[1])
+        with pytest.raises(ValueError, match="made for"):
+            backends[t == types[0]].attend(q, k, v, tables, own, prefix_tables=prefix_tables)

@@ -115,8 +115,8 @@ def rotary_frequencies(dim: int, *, base: float = 10000.0, stretch: float = 1.0,
 
 @dataclass(eq=False)
 class AttentionPlan:
-    """``plan``'s result, for the attention of one step: opaque but for the shape that it was made for. Layers share
-    it; calls on other streams must be ordered behind its making by the caller."""
+    """``plan``'s result, for the attention of one step: opaque but for the shape that it was made for, which has no type.
+    Layers share it; calls on other streams must be ordered behind its making by the caller."""
 
     sequences: int
     groups: int

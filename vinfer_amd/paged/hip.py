@@ -38,10 +38,10 @@ def _on_gpu(device) -> None:
 
 
 class _Planned:
-    """A plan's memory and stream, its shape packed, and its layers' workspace."""
+    """A plan's memory and stream, its shape (any type's: the kernels that make it know none), and its layers' workspace."""
 
-    def __init__(self, key, shape, memory, stream, workspace) -> None:
-        self.key, self.shape, self.memory, self.stream, self.workspace = key, shape, memory, stream, workspace
+    def __init__(self, shape, memory, stream, workspace) -> None:
+        self.shape, self.memory, self.stream, self.workspace = shape, memory, stream, workspace
 
 
 @PAGED.register("hip", devices={"cuda"}, dtypes=set(DTYPES), supports=lambda ctx: _vpaged.unsupported(ctx.device))
@@ -126,8 +126,8 @@ class HipPaged:
                        group_starts)
             _on_gpu(lengths.device)
             S, B = lengths.shape[0], prefix_lengths.shape[0] if groups else 0
-            shape = DTYPES[self.ctx.dtype], S, B, queries, heads, kv_heads, head_dim, page_size, max_pages, max_prefix_pages if B else 0
-            block = _vpaged.PACK_SHAPE.pack(*shape)
+            shape = S, B, queries, heads, kv_heads, head_dim, page_size, max_pages, max_prefix_pages if B else 0
+            block = _vpaged.PACK_SHAPE.pack(DTYPES[self.ctx.dtype], *shape)
             need = self._lib.vpaged_plan_bytes(block)
             if not need:
                 raise ValueError(f"a shape of more tiles or rows than 32 bits number: {S} sequences of {queries} x {heads} queries "
@@ -141,13 +141,13 @@ class HipPaged:
             prefix_lengths, group_starts = prefix_lengths.contiguous(), group_starts.contiguous()
             pre, starts = prefix_lengths.data_ptr(), group_starts.data_ptr()
         _vpaged.call(self._lib.vpaged_plan, dev, block, lengths.data_ptr(), pre, starts, memory.data_ptr(), need)
-        return AttentionPlan(*shape[1:], dev, _Planned(shape, block, memory, torch._C._cuda_getCurrentRawStream(dev.index), workspace))
+        return AttentionPlan(*shape, dev, _Planned(shape, memory, torch._C._cuda_getCurrentRawStream(dev.index), workspace))
 
     def attend(self, q, k_pages, v_pages, tables, plan: AttentionPlan, *, prefix_tables=None, scale=None) -> torch.Tensor:
         data, pre = plan.data, prefix_tables
         if not isinstance(data, _Planned):
             raise ValueError("the plan is another backend's")
-        key = ("attend", data.key, scale, torch.is_grad_enabled(), q.requires_grad, q.shape, k_pages.shape, v_pages.shape, tables.shape,
+        key = ("attend", data.shape, scale, torch.is_grad_enabled(), q.requires_grad, q.shape, k_pages.shape, v_pages.shape, tables.shape,
                q.stride(), k_pages.stride(), v_pages.stride(), tables.stride(), q.dtype, k_pages.dtype, v_pages.dtype, tables.dtype,
                q.get_device(), k_pages.get_device(), v_pages.get_device(), tables.get_device(), plan.device.index,
                *((pre.shape, pre.stride(), pre.dtype, pre.get_device()) if pre is not None else ()))
@@ -160,7 +160,7 @@ class HipPaged:
                 raise ValueError(f"the cache's strides must be multiples of 8 elements, pages less than 2^31 elements apart and "
                                  f"a page's positions within 2^30, got {strides}")
             known = self._keep(key, (q.device, any(x & 7 for x in q.stride()[:3]), q.stride()[:3], strides,
-                                     (*data.key, k_pages.shape[0], plan.head_dim**-0.5 if scale is None else scale),
+                                     (DTYPES[q.dtype], *data.shape, k_pages.shape[0], plan.head_dim**-0.5 if scale is None else scale),
                                      (tables.stride(0), pre.stride(0) if plan.groups else 0)))
         dev, odd, q_strides, strides, first, table_strides = known
         kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
