@@ -307,3 +307,26 @@ def test_a_cache_past_32_bits():
         t.copy_(x)
     want = b.attend(q.to(GPU), *near, torch.arange(4, dtype=torch.int32, device=GPU)[None], plan)
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_grid_s_dimension_has_threads():
+    # 2^26 rows of outputs, all but the last two tokens' of each sequence without a token
+    S, T, H, D, lengths = 16, 65536, 64, 8, [2, 1] * 8
+    g = torch.Generator().manual_seed(21)
+    one, k, v = (torch.randn(*s, generator=g).to(BF16).to(GPU) for s in ((S, 1, H, D), (S, 16, H, D), (S, 16, H, D)))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=GPU)  # noqa: E731
+    b = backend(GPU, BF16)
+    plan = b.plan(i32(lengths), queries=T, heads=H, kv_heads=H, head_dim=D, page_size=16, max_pages=1)
+    torch.full((S, T, H, D), math.nan, dtype=BF16, device=GPU)  # (what the outputs' memory held)
+    got = b.attend(one.expand(S, T, H, D), k, v, i32(range(S))[:, None], plan)
+    x, kk, vv = one[:, 0].double(), k[:, :2].double(), v[:, :2].double()
+    z = (x[:, None] * kk).sum(3) * D**-0.5  # [S, keys, H]
+    first, both = vv[:, 0], (torch.softmax(z, 1)[..., None] * vv).sum(1)
+    n = torch.tensor(lengths, device=GPU)[:, None, None]
+    # one or two weights and the output rounded, each by half a step
+    near = lambda a, want: bool(((a.double() - want).abs() <= 2.0**-8 * (want.abs() + 1.02 * vv.abs().amax(1)) + 2.0**-20).all())  # noqa: E731
+    assert near(got[:, T - 1], torch.where(n == 2, both, first))
+    assert near(got[:, T - 2], torch.where(n == 2, first, 0.0))
+    for s in range(S):
+        assert int(torch.count_nonzero(got[s, : T - 2])) == 0

@@ -165,3 +165,24 @@ def test_refusals():
             Rotary(bad)
     with pytest.raises(ValueError, match="magnitude"):
         Rotary(rotary_frequencies(8), magnitude=math.inf)
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_a_grid_s_dimension_has_threads():
+    # 2^24 tokens and some, against the same tokens in two calls
+    N, cut, D = (1 << 24) + 5, 9_000_001, 8
+    r = Rotary(rotary_frequencies(D, device=GPU))
+    b = backend(GPU)
+    q = torch.randn(N, 1, D, device=GPU).to(BF16)
+    k, v = q.flip(0), -q
+    positions = torch.arange(N, dtype=torch.int32, device=GPU)
+    slots = positions.flip(0).contiguous()
+    shape = (N + 15) // 16, 16, 1, D
+    both = []
+    for parts in (((0, N),), ((0, cut), (cut, N))):
+        k_pages, v_pages = (torch.zeros(shape, dtype=BF16, device=GPU) for _ in range(2))
+        out = [b.rotate_store(q[i:j], k[i:j], v[i:j], positions[i:j], slots[i:j], k_pages, v_pages, r) for i, j in parts]
+        both.append((torch.cat(out), k_pages, v_pages))
+    for x, y in zip(*both):
+        assert torch.equal(x, y)
+    assert int(torch.count_nonzero(both[0][0][-1])) > 0

@@ -196,6 +196,14 @@ void with_width(int D, F f) {
   else f(Width<256>{});
 }
 
+// n workgroups over x and `over`, a grid's other dimension: a launch has fewer than 2^32 threads in one.
+constexpr int64_t kGridX = 1 << 20;
+dim3 grid_of(int64_t n, unsigned dim3::*over) {
+  dim3 grid(static_cast<unsigned>(n < kGridX ? n : kGridX));
+  grid.*over = static_cast<unsigned>((n + kGridX - 1) / kGridX);
+  return grid;
+}
+
 // Up to this many rows of outputs (a sequence's token's head each) 16 waves join one: the longest has few others beside it.
 constexpr int kFewRows = 512;
 
@@ -208,7 +216,7 @@ int attend(const vpg::AttendArgs& d, hipStream_t stream) {
     if ((1 << d.z.shift) < vpg::kRun) vpg::k_attend<T, DP, true><<<grid, block, 0, stream>>>(d);
     else vpg::k_attend<T, DP, false><<<grid, block, 0, stream>>>(d);
     if (rows <= kFewRows) vpg::k_join<T, DP, 16><<<dim3(static_cast<unsigned>(rows)), dim3(1024), 0, stream>>>(d);
-    else vpg::k_join<T, DP, 1><<<dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream>>>(d);
+    else vpg::k_join<T, DP, 1><<<grid_of((rows + 3) / 4, &dim3::y), dim3(256), 0, stream>>>(d);
   });
   return launched("vpaged_attend");
 }
@@ -313,7 +321,8 @@ int vpaged_rotate_store(const vpaged_rotate_args* a, void* stream) {
   const int rounds = (r.items + vpg::kRotateThreads - 1) / vpg::kRotateThreads;
   int y = a->tokens >= 4 * kCus ? 1 : (4 * kCus + a->tokens - 1) / a->tokens;
   if (y > rounds) y = rounds;
-  const dim3 grid(static_cast<unsigned>(a->tokens), static_cast<unsigned>(y));
+  dim3 grid = grid_of(a->tokens, &dim3::z);
+  grid.y = static_cast<unsigned>(y);
   const auto s = static_cast<hipStream_t>(stream);
   if (a->dtype == VPAGED_BF16) rotate<__bf16>(r, vectors, pairs, grid, s);
   else rotate<_Float16>(r, vectors, pairs, grid, s);
