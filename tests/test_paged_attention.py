@@ -330,3 +330,30 @@ def test_more_rows_than_a_grid_s_dimension_has_threads():
     assert near(got[:, T - 2], torch.where(n == 2, first, 0.0))
     for s in range(S):
         assert int(torch.count_nonzero(got[s, : T - 2])) == 0
+
+
+@pytest.mark.gpu
+def test_queries_and_caches_whose_layout_torch_calls_contiguous():
+    # rows at odd addresses, and odd strides of dimensions of one element
+    b = backend(GPU, BF16)
+    for lengths, T, D, page, kv_heads, extra in (([9, 20, 70], 2, 64, 16, 2, 1), ([33], 3, 72, 64, 1, 0)):
+        c = Case(GPU, BF16, None, lengths, T=T, heads=4, kv_heads=kv_heads, D=D, page=page, extra=extra, seed=14)
+        want = c.attend(b)
+        n, shape, q = c.q.numel(), c.q.shape, c.q
+        for skip in (1, 4):
+            c.q = torch.zeros(n + skip, dtype=BF16, device=GPU)[skip:].view(shape).copy_(q)
+            assert c.q.is_contiguous() and c.q.data_ptr() % 16
+            assert torch.equal(c.attend(b), want)
+        if len(lengths) > 1:
+            continue
+        for odd in (n + 1, 3):
+            c.q = torch.zeros(n, dtype=BF16, device=GPU).as_strided(shape, (odd, *q.stride()[1:])).copy_(q)
+            assert c.q.is_contiguous()
+            assert torch.equal(c.attend(b), want)
+        # one page, one key head
+        table = c.tables[:, :1].clone()
+        held = [t[int(table[0, 0])] for t in c.cache]
+        c.tables = torch.zeros_like(table)
+        for odd in (1, 5):
+            c.cache = [torch.zeros(page * D, dtype=BF16, device=GPU).as_strided((1, page, 1, D), (odd, D, odd, 1)).copy_(t[None]) for t in held]
+            assert torch.equal(c.attend(b), want)

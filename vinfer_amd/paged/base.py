@@ -167,7 +167,10 @@ class PagedBackend(Protocol):
         positions up to ``lengths[s] - queries + t``; where that is below 0 there is no such token (a batch padded on
         the left, a finished sequence), and its output is 0. Query heads share key heads in order. ``scale`` (positive)
         defaults to ``head_dim ** -0.5``. What lies behind the lengths is not seen, whatever it holds; a value that is not
-        finite at an own position reaches all of the sequence's new tokens of the call. An entry of a table outside the cache is taken as the nearest page."""
+        finite at an own position reaches all of the sequence's new tokens of the call. An entry of a table outside the
+        cache is taken as the nearest page. The ``hip`` backend takes ``q`` of any layout with unit stride along its
+        heads' elements, and caches of 16-byte aligned rows: strides of multiples of 8 elements, pages less than 2^31
+        elements apart, a page's positions (16 at least) within 2^30."""
         ...
 
 

@@ -37,6 +37,11 @@ def _on_gpu(device) -> None:
         raise ValueError(f"the hip paged cache needs its tensors on a GPU, got {device}")
 
 
+def _strides(t, n: int) -> tuple[int, ...]:
+    """The first n strides, 0 in dimensions of one element (torch keeps any number there)."""
+    return tuple(st if size > 1 else 0 for st, size in zip(t.stride()[:n], t.shape))
+
+
 class _Planned:
     """A plan's memory and stream, its shape (any type's: the kernels that make it know none), and its layers' workspace."""
 
@@ -155,11 +160,12 @@ class HipPaged:
         if known is None:
             check_attend(q, k_pages, v_pages, tables, plan, pre, scale)
             self._check_dtype(q)
-            strides = k_pages.stride()[:3]
+            strides = _strides(k_pages, 3)
             if any(x & 7 for x in strides) or strides[0] >= 1 << 31 or strides[1] * max(plan.page_size, 16) >= 1 << 30:
                 raise ValueError(f"the cache's strides must be multiples of 8 elements, pages less than 2^31 elements apart and "
                                  f"a page's positions within 2^30, got {strides}")
-            known = self._keep(key, (q.device, any(x & 7 for x in q.stride()[:3]), q.stride()[:3], strides,
+            q_strides = _strides(q, 3)
+            known = self._keep(key, (q.device, any(x & 7 for x in q_strides), q_strides, strides,
                                      (DTYPES[q.dtype], *data.shape, k_pages.shape[0], plan.head_dim**-0.5 if scale is None else scale),
                                      (tables.stride(0), pre.stride(0) if plan.groups else 0)))
         dev, odd, q_strides, strides, first, table_strides = known
@@ -167,8 +173,8 @@ class HipPaged:
         if (kp | vp) & 15:
             raise ValueError("the cache must be 16-byte aligned")
         if odd or q.data_ptr() & 15:
-            q = q.contiguous()
-            q_strides = q.stride()[:3]
+            q = q.clone(memory_format=torch.contiguous_format)  # (contiguous() keeps what lies at an odd address)
+            q_strides = _strides(q, 3)
         out = q.new_empty(q.shape)
         ws = torch.empty(data.workspace, dtype=torch.uint8, device=dev)
         memory = data.memory
