@@ -357,3 +357,23 @@ def test_queries_and_caches_whose_layout_torch_calls_contiguous():
         for odd in (1, 5):
             c.cache = [torch.zeros(page * D, dtype=BF16, device=GPU).as_strided((1, page, 1, D), (odd, D, odd, 1)).copy_(t[None]) for t in held]
             assert torch.equal(c.attend(b), want)
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_derivatives_are_refused(device):
+    c = Case(device, BF16, None, [9, 20], seed=15)
+    b = backend(device, BF16)
+    plan = c.plan(b)
+    want = c.attend(b, plan)  # (what was checked once is checked again where a tensor asks for more)
+    tensors = {"q": c.q, "k_pages": c.cache[0], "v_pages": c.cache[1]}
+    call = lambda t: b.attend(t["q"], t["k_pages"], t["v_pages"], c.tables, plan)  # noqa: E731
+    for name, t in tensors.items():
+        asking = {**tensors, name: t.clone().requires_grad_()}
+        with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+            call(asking)
+        with torch.no_grad():
+            assert torch.equal(call(asking), want)
+        with torch.autograd.forward_ad.dual_level():
+            assert torch.equal(call(tensors), want)
+            with pytest.raises(ValueError, match=f"{name} has a tangent"):
+                call({**tensors, name: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))})

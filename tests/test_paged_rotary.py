@@ -186,3 +186,24 @@ def test_more_tokens_than_a_grid_s_dimension_has_threads():
     for x, y in zip(*both):
         assert torch.equal(x, y)
     assert int(torch.count_nonzero(both[0][0][-1])) > 0
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_derivatives_are_refused(device):
+    b = backend(device)
+    mk = lambda *s: torch.randn(*s).to(BF16).to(device)  # noqa: E731
+    tensors = {"q": mk(3, 4, 8), "k": mk(3, 2, 8), "v": mk(3, 2, 8), "k_pages": mk(2, 16, 2, 8), "v_pages": mk(2, 16, 2, 8),
+               "frequencies": rotary_frequencies(8, device=device)}
+    words = torch.arange(3, dtype=torch.int32, device=device)
+
+    def call(t):
+        return b.rotate_store(t["q"], t["k"], t["v"], words, words, t["k_pages"], t["v_pages"], Rotary(t["frequencies"]))
+
+    want = call(tensors)  # (what was checked once is checked again where a tensor asks for more)
+    for name, t in tensors.items():
+        with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+            call({**tensors, name: t.clone().requires_grad_()})
+        with torch.autograd.forward_ad.dual_level():
+            assert torch.equal(call(tensors), want)
+            with pytest.raises(ValueError, match=f"{name} has a tangent"):
+                call({**tensors, name: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))})

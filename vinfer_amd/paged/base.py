@@ -17,6 +17,7 @@ from dataclasses import dataclass
 from typing import Protocol
 
 import torch
+from torch.autograd import forward_ad
 
 from vinfer_amd import _vpaged
 from vinfer_amd.registry import BackendRegistry
@@ -132,6 +133,9 @@ class AttentionPlan:
 
 
 class PagedBackend(Protocol):
+    """Serving operators: none has a derivative, and arguments that ask for one (a gradient where those are enabled, a
+    tangent of forward mode) are refused."""
+
     def extend(self, pages: PageTables, counts: torch.Tensor, tokens: int) -> Extension:
         """Sequence s grows by ``counts[s]`` positions (int32; below 0: 0), the sequences in their order taking the
         pages they need. A sequence is served whole or not at all: not where its table would be too short, where its
@@ -187,6 +191,20 @@ def _words(name: str, t: torch.Tensor, n: int, device) -> None:
         raise ValueError(f"{name} must be an int32 [{n}] tensor on {device}")
 
 
+def differentiated() -> bool:
+    """Whether a forward-mode level is entered, within which tensors may carry tangents (else there is nothing to ask)."""
+    return forward_ad._current_level >= 0
+
+
+def check_constants(what: str, **tensors) -> None:
+    """``ValueError`` for an argument that asks for a derivative, in either mode: ``what`` has none."""
+    for name, t in tensors.items():
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient: {what} has none")
+        if differentiated() and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} has a tangent: {what} has no forward-mode derivative")
+
+
 def check_extend(pages: PageTables, counts, tokens: int) -> None:
     _words("counts", counts, pages.lengths.shape[0], pages.tables.device)
     if not 0 <= tokens <= _vpaged.MAX_TOKENS or (tokens and not counts.shape[0]):
@@ -223,8 +241,7 @@ def check_rotate(q, k, v, positions, slots, k_pages, v_pages, rotary: Rotary) ->
             raise ValueError(f"q, k and v must be of one type on one device, got {t.dtype} on {t.device} for {name}")
         if t.stride(2) != 1 and D > 1 and t.numel():
             raise ValueError(f"{name} must have unit stride along its heads' elements")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} requires a gradient: rotate_store has none")
+    check_constants("rotate_store", q=q, k=k, v=v, k_pages=k_pages, v_pages=v_pages, frequencies=rotary.frequencies)
     _words("positions", positions, N, q.device)
     _words("slots", slots, N, q.device)
     check_cache(k_pages, v_pages, k.shape[1], D, q)
@@ -264,8 +281,7 @@ def check_attend(q, k_pages, v_pages, tables, plan: AttentionPlan, prefix_tables
                          f"planned, got {tuple(q.shape)} on {q.device}")
     if q.stride(3) != 1 and q.numel():
         raise ValueError("q must have unit stride along its heads' elements")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise ValueError("q requires a gradient: attend has none")
+    check_constants("attend", q=q, k_pages=k_pages, v_pages=v_pages)
     check_cache(k_pages, v_pages, plan.kv_heads, plan.head_dim, q)
     if k_pages.shape[1] != plan.page_size or (k_pages.shape[0] < 1 and plan.sequences):
         raise ValueError(f"the cache must have pages, of the plan's {plan.page_size} positions, got {tuple(k_pages.shape)}")

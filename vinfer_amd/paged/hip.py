@@ -26,6 +26,7 @@ from vinfer_amd.paged.base import (
     check_plan,
     check_rotate,
     check_shrink,
+    differentiated,
 )
 from vinfer_amd.registry import BackendContext
 
@@ -96,13 +97,14 @@ class HipPaged:
 
     def rotate_store(self, q, k, v, positions, slots, k_pages, v_pages, rotary: Rotary) -> torch.Tensor:
         f = rotary.frequencies
-        key = ("rotate", torch.is_grad_enabled(), q.requires_grad, k.requires_grad, v.requires_grad, rotary.interleaved,
-               rotary.magnitude, f.shape, q.shape, k.shape, v.shape, positions.shape, slots.shape, k_pages.shape, v_pages.shape,
-               q.stride(), k.stride(), v.stride(), k_pages.stride(), v_pages.stride(), q.dtype, k.dtype, v.dtype,
-               positions.dtype, slots.dtype, k_pages.dtype, v_pages.dtype, q.get_device(), k.get_device(), v.get_device(),
-               positions.get_device(), slots.get_device(), k_pages.get_device(), v_pages.get_device(), f.get_device())
+        key = ("rotate", torch.is_grad_enabled(), q.requires_grad, k.requires_grad, v.requires_grad, k_pages.requires_grad,
+               v_pages.requires_grad, f.requires_grad, rotary.interleaved, rotary.magnitude, f.shape, q.shape, k.shape, v.shape,
+               positions.shape, slots.shape, k_pages.shape, v_pages.shape, q.stride(), k.stride(), v.stride(), k_pages.stride(),
+               v_pages.stride(), q.dtype, k.dtype, v.dtype, positions.dtype, slots.dtype, k_pages.dtype, v_pages.dtype,
+               q.get_device(), k.get_device(), v.get_device(), positions.get_device(), slots.get_device(), k_pages.get_device(),
+               v_pages.get_device(), f.get_device())
         known = self._known.get(key)
-        if known is None:
+        if known is None or differentiated():
             check_rotate(q, k, v, positions, slots, k_pages, v_pages, rotary)
             _on_gpu(q.device)
             self._check_dtype(q)
@@ -152,12 +154,13 @@ class HipPaged:
         data, pre = plan.data, prefix_tables
         if not isinstance(data, _Planned):
             raise ValueError("the plan is another backend's")
-        key = ("attend", data.shape, scale, torch.is_grad_enabled(), q.requires_grad, q.shape, k_pages.shape, v_pages.shape, tables.shape,
-               q.stride(), k_pages.stride(), v_pages.stride(), tables.stride(), q.dtype, k_pages.dtype, v_pages.dtype, tables.dtype,
-               q.get_device(), k_pages.get_device(), v_pages.get_device(), tables.get_device(), plan.device.index,
+        key = ("attend", data.shape, scale, torch.is_grad_enabled(), q.requires_grad, k_pages.requires_grad, v_pages.requires_grad,
+               q.shape, k_pages.shape, v_pages.shape, tables.shape, q.stride(), k_pages.stride(), v_pages.stride(), tables.stride(),
+               q.dtype, k_pages.dtype, v_pages.dtype, tables.dtype, q.get_device(), k_pages.get_device(), v_pages.get_device(),
+               tables.get_device(), plan.device.index,
                *((pre.shape, pre.stride(), pre.dtype, pre.get_device()) if pre is not None else ()))
         known = self._known.get(key)
-        if known is None:
+        if known is None or differentiated():
             check_attend(q, k_pages, v_pages, tables, plan, pre, scale)
             self._check_dtype(q)
             strides = _strides(k_pages, 3)
