@@ -243,3 +243,16 @@ def test_the_example_searches(device, capsys):
     found = main(["--device", device.type, "--vocab", "500", "--tokens", "5"])
     assert all(len(h) == 4 and all(len(x.tokens) <= 5 for x in h) for h in found)
     assert "39 tokens:" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_a_search_longer_than_the_cache_is_refused(device):
+    # (pages of 16: the room is what was asked for, not what its pages hold)
+    sampler = resolve(SAMPLER, device)
+    search = lambda room, tokens: beam_search(  # noqa: E731
+        AttentionLM(97, requests=2, beams=2, max_tokens=room, device=device, seed=3), sampler, [[1, 2, 3], [7]], width=2, max_tokens=tokens)
+    for room, tokens in ((4, 10), (4, 6), (16, 18)):
+        with pytest.raises(ValueError, match="room for"):
+            search(room, tokens)
+    for room, tokens in ((4, 5), (1, 2), (1, 1)):  # (the last token is not decoded)
+        assert [[h.tokens for h in x] for x in search(room, tokens)] == [[h.tokens for h in x] for x in search(40, tokens)]

@@ -28,7 +28,8 @@ from vinfer_amd.sampler.beams import BeamState
 class BeamModel(Protocol):
     """A decode model whose slots' states can be moved: ``DecodeModel``'s two calls, and the states. With
     ``shared_prompts = True`` the states hold a beam's continuation alone (``SharedPromptCache``: the model keeps a
-    request's prompt for all of its beams), and their lengths count from the prompt's end."""
+    request's prompt for all of its beams), and their lengths count from the prompt's end: a search is refused where
+    they have no room for what it may decode."""
 
     device: torch.device
 
@@ -63,7 +64,12 @@ def beam_search(model: BeamModel, sampler: SamplerBackend, prompts: Sequence[Seq
     B, W, dev = len(prompts), width, model.device
     lengths = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device=dev)
     history = torch.zeros(B * W, max_tokens, dtype=torch.int32, device=dev)
+    shared = getattr(model, "shared_prompts", False)
     model_states = list(model.beam_states(B * W))
+    for s in model_states if shared else ():  # (the last token that is drawn is not decoded)
+        if s.length_dim is not None and s.tensor.shape[s.length_dim] < max_tokens - 1:
+            raise ValueError(f"a search of {max_tokens} tokens decodes {max_tokens - 1}, the model's states have room for "
+                             f"{s.tensor.shape[s.length_dim]}")
     states = sampler.prepare_reorder(model_states, B, W) if model_states else None
     histories = sampler.prepare_reorder([BeamState(history)], B, W)
     eos = torch.tensor(sorted(set(eos_token_ids)), dtype=torch.int32, device=dev)
@@ -72,7 +78,7 @@ def beam_search(model: BeamModel, sampler: SamplerBackend, prompts: Sequence[Seq
 
     rows = torch.stack([model.prefill(b * W, torch.as_tensor(p, device=dev)) for b, p in enumerate(prompts)])
     logits = rows[:, None].expand(B, W, rows.shape[-1])
-    held = torch.zeros_like(lengths) if getattr(model, "shared_prompts", False) else lengths  # of the states' positions
+    held = torch.zeros_like(lengths) if shared else lengths  # of the states' positions
     if states is not None:  # (every beam starts from its request's prompt)
         states.launch(torch.zeros(B, W, dtype=torch.int32, device=dev), held)
     scores = torch.full((B, W), -math.inf, device=dev)

@@ -98,7 +98,8 @@ class SharedPromptCache:
 
     def decode(self, slots: torch.Tensor, positions: torch.Tensor) -> CacheStep:
         """The step of one token at ``positions`` (in its prompt and continuation) for each of ``slots``: of a cache of
-        several beams all of its slots in their order, of one beam any slots, each once."""
+        several beams all of its slots in their order, of one beam any slots, each once. A token past its continuation's
+        ``max_tokens`` places is none (only the device knows): nothing is stored and its attention is 0."""
         n = slots.shape[0]
         if self.beams > 1 and n != self.requests * self.beams:
             raise ValueError(f"a step of beams takes all {self.requests * self.beams} slots, got {n}")
@@ -122,10 +123,11 @@ class SharedPromptCache:
                                  page_size=self.page_size, max_pages=tables.shape[1], **groups)
 
     def beam_states(self) -> list[BeamState]:
-        """The continuations, as ``prepare_reorder`` takes them: with lengths of tokens behind the prompt."""
+        """The continuations, as ``prepare_reorder`` takes them: ``max_tokens`` long, with lengths of tokens behind the
+        prompt."""
         slots = self.requests * self.beams
-        return [BeamState(t[:, self.prompt_pages :].unflatten(1, (slots, -1)).flatten(2, 3), slot_dim=1, length_dim=2)
-                for t in (self.keys, self.values)]
+        return [BeamState(t[:, self.prompt_pages :].unflatten(1, (slots, -1)).flatten(2, 3)[:, :, : self.max_tokens], slot_dim=1,
+                          length_dim=2) for t in (self.keys, self.values)]
 
 
 __all__ = ["CacheStep", "SharedPromptCache"]
