@@ -256,3 +256,13 @@ def test_a_search_longer_than_the_cache_is_refused(device):
             search(room, tokens)
     for room, tokens in ((4, 5), (1, 2), (1, 1)):  # (the last token is not decoded)
         assert [[h.tokens for h in x] for x in search(room, tokens)] == [[h.tokens for h in x] for x in search(40, tokens)]
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_a_search_of_another_width_is_refused(device):
+    # as many slots, but another request's: slot 4 is the third request of two beams, the second of four
+    sampler = resolve(SAMPLER, device)
+    for requests, beams, width in ((4, 2, 4), (4, 2, 1), (2, 4, 2), (4, 1, 2)):
+        model = AttentionLM(97, requests=requests, beams=beams, device=device, seed=3)
+        with pytest.raises(ValueError, match=f"for {beams} beams"):
+            beam_search(model, sampler, [[1, 2, 3]] * (requests * beams // width), width=width, max_tokens=3)

@@ -123,11 +123,11 @@ class SharedPromptCache:
                                  page_size=self.page_size, max_pages=tables.shape[1], **groups)
 
     def beam_states(self) -> list[BeamState]:
-        """The continuations, as ``prepare_reorder`` takes them: ``max_tokens`` long, with lengths of tokens behind the
-        prompt."""
+        """The continuations, as ``prepare_reorder`` takes them, for this cache's number of beams: ``max_tokens`` long,
+        with lengths of tokens behind the prompt."""
         slots = self.requests * self.beams
         return [BeamState(t[:, self.prompt_pages :].unflatten(1, (slots, -1)).flatten(2, 3)[:, :, : self.max_tokens], slot_dim=1,
-                          length_dim=2) for t in (self.keys, self.values)]
+                          length_dim=2, beams=self.beams) for t in (self.keys, self.values)]
 
 
 __all__ = ["CacheStep", "SharedPromptCache"]

@@ -25,11 +25,12 @@ class BeamState:
     """One tensor of states that a search's beams carry: ``slot_dim`` indexes the ``requests * beams`` slots
     (request b's beam w in slot ``b * beams + w``); with ``length_dim`` (a cache's or a history's positions)
     only a request's first positions count. Any dtype, any strides without overlap, and no memory that another state
-    of the same plan holds."""
+    of the same plan holds. ``beams``: the only number of them that the slots are laid out for, if there is one."""
 
     tensor: torch.Tensor
     slot_dim: int = 0
     length_dim: int | None = None
+    beams: int | None = None
 
 
 # ---- checks ---------------------------------------------------------------------------------------------
@@ -94,6 +95,8 @@ def check_states(states: Sequence[BeamState], requests: int, beams: int) -> torc
             raise ValueError(f"state {i} requires a gradient: states are reordered in place")
         if not 0 <= s.slot_dim < t.dim() or t.shape[s.slot_dim] != requests * beams:
             raise ValueError(f"state {i}: dimension {s.slot_dim} of {tuple(t.shape)} must hold the {requests * beams} slots")
+        if s.beams is not None and s.beams != beams:
+            raise ValueError(f"state {i} is laid out for {s.beams} beams a request, got {beams}")
         if s.length_dim is not None and (not 0 <= s.length_dim < t.dim() or s.length_dim == s.slot_dim):
             raise ValueError(f"state {i}: length_dim {s.length_dim} is not another dimension of {tuple(t.shape)}")
         if t.numel() == 0:
