@@ -11,7 +11,7 @@ from oracle import paged_oracle
 from vinfer_amd.examples.shared_prompt_search import AttentionLM, main
 from vinfer_amd.paged import PAGED, PageTables, Rotary, rotary_frequencies
 from vinfer_amd.registry import BackendContext
-from vinfer_amd.runtime import BatchDecoder, SharedPromptCache, beam_search
+from vinfer_amd.runtime import BatchDecoder, SharedPromptCache, SpeculativeDecoder, beam_search
 from vinfer_amd.sampler import SAMPLER
 from vinfer_amd.sampling import SamplingParams
 
@@ -266,3 +266,23 @@ def test_a_search_of_another_width_is_refused(device):
         model = AttentionLM(97, requests=requests, beams=beams, device=device, seed=3)
         with pytest.raises(ValueError, match=f"for {beams} beams"):
             beam_search(model, sampler, [[1, 2, 3]] * (requests * beams // width), width=width, max_tokens=3)
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_the_decode_loop_refuses_requests_past_the_cache(device):
+    sampler = resolve(SAMPLER, device)
+
+    def run(room, tokens):
+        loop = BatchDecoder(AttentionLM(97, requests=1, beams=1, max_tokens=room, device=device, seed=2), sampler, num_slots=1, max_seq_len=64)
+        loop.submit([1, 2, 3], SamplingParams(temperature=0.0, max_tokens=tokens))
+        return [s.token_id for s in loop.run()[0]]
+
+    with pytest.raises(ValueError, match="room for 4"):
+        run(4, 6)
+    assert run(4, 5) == run(40, 5)
+    model, other = (AttentionLM(97, requests=1, beams=1, max_tokens=n, device=device) for n in (8, 40))
+    for target, draft in ((model, other), (other, model)):
+        loop = SpeculativeDecoder(target, sampler, draft_model=draft, num_draft=3, num_slots=1, max_seq_len=64)
+        with pytest.raises(ValueError, match="room for 8"):
+            loop.submit([1, 2, 3], SamplingParams(temperature=0.0, max_tokens=7))
+        loop.submit([1, 2, 3], SamplingParams(temperature=0.0, max_tokens=6))

@@ -39,6 +39,7 @@ class AttentionLM:
             PAGED.resolve(name, BackendContext(self.device, dtype)), layers=layers, requests=requests, beams=beams, heads=heads,
             kv_heads=kv_heads, head_dim=head_dim, prompt_pages=requests * -(-max_prompt // 16), max_prompt=max_prompt,
             max_tokens=max_tokens, rotary=Rotary(rotary_frequencies(head_dim, device=self.device)), dtype=dtype, device=self.device)
+        self.max_new_tokens = max_tokens
 
     def _hidden(self, step, tokens):
         x = self.emb[tokens]

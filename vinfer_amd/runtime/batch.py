@@ -84,10 +84,10 @@ class Step:
     top_logprobs: list[tuple[int, float]] | None = None
 
 
-def check_request(prompt_len: int, params: SamplingParams, max_seq_len: int) -> None:
+def check_request(prompt_len: int, params: SamplingParams, max_seq_len: int, max_new_tokens: int | None = None) -> None:
     """Raise ``ValueError`` if a request cannot run in ``max_seq_len`` positions (the rule of
     generate.py:91-103: the last sampled token is never fed back, so a request needs
-    ``prompt_len + max_tokens - 1`` positions)."""
+    ``prompt_len + max_tokens - 1`` positions), of which a model has room for ``max_new_tokens`` behind a prompt."""
     if prompt_len == 0:
         raise ValueError("empty prompt")
     needed = prompt_len + params.max_tokens - 1
@@ -96,6 +96,9 @@ def check_request(prompt_len: int, params: SamplingParams, max_seq_len: int) -> 
             f"prompt ({prompt_len}) + max_tokens ({params.max_tokens}) needs {needed} positions, "
             f"more than max_seq_len ({max_seq_len})"
         )
+    if max_new_tokens is not None and params.max_tokens - 1 > max_new_tokens:
+        raise ValueError(f"max_tokens ({params.max_tokens}) needs {params.max_tokens - 1} positions behind the prompt, the model has "
+                         f"room for {max_new_tokens}")
 
 
 class DecodeModel(Protocol):
@@ -106,7 +109,8 @@ class DecodeModel(Protocol):
     ``decode_into(slots, tokens, positions, out)``, ``decode`` writing its logits into ``out``
     (the captured loop then needs no copy of them; ``out`` may be a row-strided view), and
     ``stateless = True`` when its slots keep no state (a speculative loop then does not feed it
-    tokens whose logits it does not use)."""
+    tokens whose logits it does not use), and ``max_new_tokens``, the positions that its slots have room for
+    behind a prompt (a request that may need more is refused)."""
 
     device: torch.device
 
@@ -295,7 +299,7 @@ class BatchDecoder:
     # ---- requests ------------------------------------------------------------------------------
     def submit(self, prompt_ids: list[int], params: SamplingParams) -> int:
         """Queue a request; returns its id. Raises ``ValueError`` if it can never run."""
-        check_request(len(prompt_ids), params, self.max_seq_len)
+        check_request(len(prompt_ids), params, self.max_seq_len, getattr(self.model, "max_new_tokens", None))
         if params.seed is None:
             params = dataclasses.replace(params, seed=self._rng.getrandbits(63))
         stop_ids = frozenset(params.stop_token_ids) | (frozenset() if params.ignore_eos else self.eos_token_ids)
@@ -725,8 +729,9 @@ class SpeculativeDecoder(BatchDecoder):
         if param_field(params, "logprobs"):
             raise ValueError("speculative decoding reports no log-probabilities")
         # positions up to prompt + max_tokens - 1 + num_draft are scored (the last block's drafts)
-        check_request(len(prompt_ids), dataclasses.replace(params, max_tokens=params.max_tokens + self.num_draft),
-                      self.max_seq_len)
+        for model in (self.model, self.draft_model):
+            check_request(len(prompt_ids), dataclasses.replace(params, max_tokens=params.max_tokens + self.num_draft),
+                          self.max_seq_len, getattr(model, "max_new_tokens", None))
         return super().submit(prompt_ids, params)
 
     def step(self) -> list[tuple[int, Step]]:

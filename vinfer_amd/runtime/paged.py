@@ -11,6 +11,7 @@ continuations alone (``beam_states``), and a request's beams start without a cop
 
     class Model:
         shared_prompts = True
+        max_new_tokens = property(lambda self: cache.max_tokens)
         def prefill(self, slot, prompt_ids): step = cache.prefill(slot, len(prompt_ids)); ... step.attend(layer, q, k, v)
         def decode(self, slots, tokens, positions): step = cache.decode(slots, positions); ... step.attend(layer, q, k, v)
         def release(self, slot): cache.release(slot)
