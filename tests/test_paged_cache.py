@@ -286,3 +286,23 @@ def test_the_decode_loop_refuses_requests_past_the_cache(device):
         with pytest.raises(ValueError, match="room for 8"):
             loop.submit([1, 2, 3], SamplingParams(temperature=0.0, max_tokens=7))
         loop.submit([1, 2, 3], SamplingParams(temperature=0.0, max_tokens=6))
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_a_prompt_that_cannot_be_planned_holds_nothing(device, monkeypatch):
+    with pytest.raises(ValueError, match="max_prompt must be at most 65536"):
+        make_cache(device, 1, 1, max_prompt=65537)
+    make_cache(device, 1, 1, max_prompt=65536)
+    cache = make_cache(device, 2, 2)
+    cache.prefill(0, 100)
+
+    def refused(*a, **k):
+        raise ValueError("a shape of more tiles")
+
+    with monkeypatch.context() as m:
+        m.setattr(cache.backend, "plan", refused)
+        with pytest.raises(ValueError, match="more tiles"):
+            cache.prefill(2, 300)
+    assert cache.prompts.lengths.tolist() == [100, 0] and int(cache.prompts.free_count) == 40 - 7
+    cache.prefill(2, 300)
+    assert cache.prompts.lengths.tolist() == [100, 300] and int(cache.prompts.free_count) == 40 - 7 - 19

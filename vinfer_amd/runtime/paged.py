@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import torch
 
+from vinfer_amd import _vpaged
 from vinfer_amd.paged import AttentionPlan, PagedBackend, PageTables, Rotary
 from vinfer_amd.sampler.beams import BeamState
 
@@ -46,7 +47,7 @@ class CacheStep:
 
 
 class SharedPromptCache:
-    """``requests`` prompts in ``prompt_pages`` pages together (each of up to ``max_prompt`` positions), and ``max_tokens``
+    """``requests`` prompts in ``prompt_pages`` pages together (each of up to ``max_prompt`` positions, 65536 at most), and ``max_tokens``
     positions for each of their ``beams`` continuations."""
 
     def __init__(self, backend: PagedBackend, *, layers: int, requests: int, beams: int, heads: int, kv_heads: int, head_dim: int,
@@ -54,6 +55,8 @@ class SharedPromptCache:
                  device="cuda", scale: float | None = None) -> None:
         if min(layers, requests, beams, prompt_pages, max_prompt, max_tokens) < 1:
             raise ValueError("layers, requests, beams, prompt_pages, max_prompt and max_tokens must be positive")
+        if max_prompt > _vpaged.MAX_QUERIES:  # (a prompt is one step's new tokens)
+            raise ValueError(f"max_prompt must be at most {_vpaged.MAX_QUERIES}, got {max_prompt}")
         self.backend, self.rotary, self.scale = backend, rotary, scale
         self.requests, self.beams, self.max_prompt, self.max_tokens = requests, beams, max_prompt, max_tokens
         self.heads, self.kv_heads, self.head_dim, self.page_size = heads, kv_heads, head_dim, page_size
@@ -86,7 +89,7 @@ class SharedPromptCache:
 
     def prefill(self, slot: int, tokens: int) -> CacheStep:
         """The step of a prompt of ``tokens`` tokens, which takes the place of the one that ``slot``'s request had.
-        ``RuntimeError`` if there are too few pages left (and nothing is held then)."""
+        ``RuntimeError`` if there are too few pages left. Nothing is held for the request where this raises."""
         request = self._request(slot)
         if not 1 <= tokens <= self.max_prompt:
             raise ValueError(f"a prompt must have 1 to {self.max_prompt} tokens, got {tokens}")
@@ -95,7 +98,12 @@ class SharedPromptCache:
         if not bool(e.served[request]):
             raise RuntimeError(f"no pages for a prompt of {tokens} tokens: {int(self.prompts.free_count)} are free")
         lengths, tables = self.prompts.lengths[request : request + 1], self.prompts.tables[request : request + 1]
-        return CacheStep(self, e.positions, e.slots, self._plan(lengths, tokens, tables), tables, None)
+        try:
+            plan = self._plan(lengths, tokens, tables)
+        except BaseException:
+            self.release(slot)
+            raise
+        return CacheStep(self, e.positions, e.slots, plan, tables, None)
 
     def decode(self, slots: torch.Tensor, positions: torch.Tensor) -> CacheStep:
         """The step of one token at ``positions`` (in its prompt and continuation) for each of ``slots``: of a cache of
