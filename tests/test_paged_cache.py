@@ -11,7 +11,7 @@ from oracle import paged_oracle
 from vinfer_amd.examples.shared_prompt_search import AttentionLM, main
 from vinfer_amd.paged import PAGED, PageTables, Rotary, rotary_frequencies
 from vinfer_amd.registry import BackendContext
-from vinfer_amd.runtime import BatchDecoder, SharedPromptCache, SpeculativeDecoder, beam_search
+from vinfer_amd.runtime import BatchDecoder, NoRoom, SharedPromptCache, SpeculativeDecoder, beam_search
 from vinfer_amd.sampler import SAMPLER
 from vinfer_amd.sampling import SamplingParams
 
@@ -306,3 +306,63 @@ def test_a_prompt_that_cannot_be_planned_holds_nothing(device, monkeypatch):
     assert cache.prompts.lengths.tolist() == [100, 0] and int(cache.prompts.free_count) == 40 - 7
     cache.prefill(2, 300)
     assert cache.prompts.lengths.tolist() == [100, 300] and int(cache.prompts.free_count) == 40 - 7 - 19
+
+
+@pytest.mark.parametrize("graphs", [False, pytest.param(True, marks=pytest.mark.gpu)], ids=["eager", "graphs"])
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_the_decode_loop_waits_for_pages(device, graphs):
+    # prompts of two pages each, three or six pages free: a prompt waits until others end, and no token changes
+    if graphs and device.type == "cpu":
+        pytest.skip("graphs need a GPU")
+    sampler = resolve(SAMPLER, device)
+    prompts = [list(range(1 + i, 20 + i)) for i in range(5)]
+
+    def run(free):
+        model = AttentionLM(97, requests=3, beams=1, max_prompt=32, max_tokens=12, device=device, seed=2)
+        model.cache.prompts.free_count.fill_(free)  # (the others: held elsewhere)
+        loop = BatchDecoder(model, sampler, num_slots=3, max_seq_len=64, graphs=graphs, graph_after=1)
+        ids = [loop.submit(p, SamplingParams(temperature=0.0, max_tokens=5 + i % 3 * 3)) for i, p in enumerate(prompts)]
+        done = loop.run()
+        assert int(model.cache.prompts.free_count) == free and loop._free == [2, 1, 0]
+        return [[s.token_id for s in done[i]] for i in ids]
+
+    want = run(6)
+    assert [len(x) for x in want] == [5, 8, 11, 5, 8]
+    assert run(3) == want and run(2) == want
+    model = AttentionLM(97, requests=3, beams=1, max_prompt=64, device=device, seed=2)
+    model.cache.prompts.free_count.fill_(2)
+    loop = BatchDecoder(model, sampler, num_slots=3, max_seq_len=64, graphs=graphs)
+    loop.submit([1] * 40, SamplingParams(temperature=0.0, max_tokens=2))
+    rid = loop.submit([1], SamplingParams(temperature=0.0, max_tokens=2))
+    with pytest.raises(NoRoom, match="no pages"):  # (none is running whose end would make room)
+        loop.step()
+    assert len(loop.run()[rid]) == 2 and loop._free == [2, 1, 0]
+
+
+def test_a_prefill_that_raises_costs_the_others_nothing():
+    sampler = resolve(SAMPLER, torch.device("cpu"))
+
+    class Failing(AttentionLM):
+        def prefill(self, slot, prompt_ids):
+            if int(prompt_ids[0]) == 96:
+                raise OSError("the prompt cannot be read")
+            return super().prefill(slot, prompt_ids)
+
+    def run(prompts):
+        loop = BatchDecoder(Failing(97, requests=3, beams=1, max_tokens=12, seed=2), sampler, num_slots=3, max_seq_len=64)
+        ids = [loop.submit(p, SamplingParams(temperature=0.0, max_tokens=4)) for p in prompts]
+        done, errors = {}, 0
+        for _ in range(40):
+            if not loop.busy:
+                break
+            try:
+                for rid, s in loop.step():
+                    done.setdefault(rid, []).append(s.token_id)
+            except OSError:
+                errors += 1
+        assert not loop.busy and loop._free == [2, 1, 0]
+        return [done.get(i) for i in ids], errors
+
+    fine, errors = run([[1, 2], [3], [5, 6, 7]])
+    assert errors == 0
+    assert run([[1, 2], [96], [3], [96, 1], [5, 6, 7]]) == ([fine[0], None, fine[1], None, fine[2]], 2)

@@ -101,6 +101,10 @@ def check_request(prompt_len: int, params: SamplingParams, max_seq_len: int, max
                          f"room for {max_new_tokens}")
 
 
+class NoRoom(RuntimeError):
+    """Raised by a model's ``prefill`` where a prompt has no room as long as others hold theirs (pages of a cache)."""
+
+
 class DecodeModel(Protocol):
     """What the loop needs of a model: a prefill into a slot and a batched one-token step. A
     model may also define ``release(slot)``, called when a slot's request ends (where a state
@@ -116,7 +120,8 @@ class DecodeModel(Protocol):
 
     def prefill(self, slot: int, prompt_ids: torch.Tensor) -> torch.Tensor:
         """Run ``prompt_ids`` (int64 ``[P]``) into ``slot``; the logits ``[V]`` of its last
-        position."""
+        position. ``NoRoom`` if others must end first: the request waits for that (and is dropped, with the error, where
+        none is running)."""
         ...
 
     def decode(self, slots: torch.Tensor, tokens: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
@@ -343,10 +348,10 @@ class BatchDecoder:
         if self._inflight is not None:
             return self._step_inflight()
         groups = []
+        admitted = self._admit()  # (before the pending logits are taken: a prefill may raise)
         if self._pending is not None:
             groups.append(self._pending)
             self._pending = None
-        admitted = self._admit()
         if admitted is not None:
             groups.append(admitted)
         if not groups:
@@ -582,7 +587,10 @@ class BatchDecoder:
         if release is not None:
             release(s.slot)
 
-    def _admit(self) -> tuple[list[_Seq], torch.Tensor] | None:
+    def _admit(self, drawn: bool = False) -> tuple[list[_Seq], torch.Tensor] | None:
+        """Prefill the waiting requests that have a slot and room. One whose prefill raises is dropped with the error, but
+        waits on where it found no room beside others, and is tried again where the step has something to return (the
+        requests admitted before it; ``drawn`` tokens, for one without room)."""
         seqs, rows = [], []
         dev = self.model.device
         while self._waiting and self._free:
@@ -595,7 +603,14 @@ class BatchDecoder:
                 base = s.slot * self._hist_row
                 self.hist[base : base + len(s.prompt)] = prompt.to(torch.int32).to(dev)
                 self._hist_len[s.slot] = len(s.prompt)
-            rows.append(self.model.prefill(s.slot, prompt.to(dev)).reshape(-1))
+            try:
+                rows.append(self.model.prefill(s.slot, prompt.to(dev)).reshape(-1))
+            except Exception as e:
+                self._free.append(s.slot)
+                if not seqs and not (isinstance(e, NoRoom) and (self._running or drawn)):
+                    raise
+                self._waiting.appendleft(s)
+                break
             self._running[s.rid] = s
             seqs.append(s)
         return (seqs, torch.stack(rows)) if seqs else None
@@ -743,7 +758,7 @@ class SpeculativeDecoder(BatchDecoder):
             self._ready = []
             if spec:
                 out += self._speculate(spec)
-        admitted = self._admit()
+        admitted = self._admit(bool(out))
         if admitted is not None:
             seqs, logits = admitted
             for s in seqs:

@@ -26,6 +26,7 @@ import torch
 
 from vinfer_amd import _vpaged
 from vinfer_amd.paged import AttentionPlan, PagedBackend, PageTables, Rotary
+from vinfer_amd.runtime.batch import NoRoom
 from vinfer_amd.sampler.beams import BeamState
 
 
@@ -47,8 +48,8 @@ class CacheStep:
 
 
 class SharedPromptCache:
-    """``requests`` prompts in ``prompt_pages`` pages together (each of up to ``max_prompt`` positions, 65536 at most), and ``max_tokens``
-    positions for each of their ``beams`` continuations."""
+    """``requests`` prompts in ``prompt_pages`` pages together (each of up to ``max_prompt`` positions, 65536 at most), and
+    ``max_tokens`` positions for each of their ``beams`` continuations."""
 
     def __init__(self, backend: PagedBackend, *, layers: int, requests: int, beams: int, heads: int, kv_heads: int, head_dim: int,
                  prompt_pages: int, max_prompt: int, max_tokens: int, rotary: Rotary, page_size: int = 16, dtype=torch.bfloat16,
@@ -89,14 +90,14 @@ class SharedPromptCache:
 
     def prefill(self, slot: int, tokens: int) -> CacheStep:
         """The step of a prompt of ``tokens`` tokens, which takes the place of the one that ``slot``'s request had.
-        ``RuntimeError`` if there are too few pages left. Nothing is held for the request where this raises."""
+        ``NoRoom`` (a ``RuntimeError``) if there are too few pages left. Nothing is held for the request where this raises."""
         request = self._request(slot)
         if not 1 <= tokens <= self.max_prompt:
             raise ValueError(f"a prompt must have 1 to {self.max_prompt} tokens, got {tokens}")
         self.release(slot)
         e = self.backend.extend(self.prompts, self._one(request, tokens), tokens)
         if not bool(e.served[request]):
-            raise RuntimeError(f"no pages for a prompt of {tokens} tokens: {int(self.prompts.free_count)} are free")
+            raise NoRoom(f"no pages for a prompt of {tokens} tokens: {int(self.prompts.free_count)} are free")
         lengths, tables = self.prompts.lengths[request : request + 1], self.prompts.tables[request : request + 1]
         try:
             plan = self._plan(lengths, tokens, tables)
