@@ -377,3 +377,39 @@ def test_derivatives_are_refused(device):
             assert torch.equal(call(tensors), want)
             with pytest.raises(ValueError, match=f"{name} has a tangent"):
                 call({**tensors, name: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))})
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_scores_far_from_zero(device, dtype):
+    # scores n 2^b, n whole numbers of 8 bits: where one is the largest its value comes out, where two are their mean. (All
+    # other weights are e^(-2^b) at most; a score times log2 e is off by up to 2^(b - 18) where it is rounded.)
+    for b, sign, groups, lengths, T, page in ((25, 1, None, [1, 200, 77], 1, 16), (30, -1, None, [130, 5], 2, 16), (30, 1, [(3, 300), (1, 0)], [1, 70, 3, 9], 1, 16),
+                                             (34, -1, [(45, 90)], [3] * 45, 1, 8), (28, -1, None, [9000], 1, 64)):
+        half = min(b // 2, 14) if dtype == F16 else b // 2
+        if dtype == F16 and b - half > 7:  # (255 2^7 is what fp16 holds of a key; the rest is the scale's)
+            up = 7
+        else:
+            up = b - half
+        c = Case(device, dtype, groups, lengths, T=T, heads=2, kv_heads=1, D=64, page=page, seed=b)
+        k, v = c.cache
+        rng = np.random.default_rng(b)
+        n = torch.tensor(rng.integers(128, 255, k.shape[:2]), dtype=torch.float64)
+        for s in range(len(lengths)):  # one or two own keys of each sequence are the largest
+            row = c.tables[s].tolist()
+            at = list(range(lengths[s]))[: 2 - s % 2]
+            for p in at:
+                n[row[p // page], p % page] = 255 if sign > 0 else 127
+        k.zero_()
+        k[..., 0, 0] = (sign * n * 2.0**up).to(dtype).to(device)
+        c.q.zero_()
+        c.q[..., 0] = 2.0**half
+        got = c.attend(backend(device, dtype), scale=2.0 ** (b - half - up)).double().cpu()
+        for s in range(len(lengths)):
+            row = c.tables[s].tolist()
+            for t in range(T):
+                last = lengths[s] - T + t + 1
+                at = list(range(min(last, 2 - s % 2)))
+                want = torch.stack([v[row[p // page], p % page, 0] for p in at]).double().cpu().mean(0)
+                off = (got[s, t] - want).abs()
+                assert bool((off <= torch.finfo(dtype).eps / 2 * want.abs() * 1.01 + 2.0**-24).all()), (b, s, t, off.max())

@@ -335,6 +335,11 @@ __device__ __forceinline__ float other_half(float x) {  // the partner's, 32 lan
   return __builtin_bit_cast(float, (threadIdx.x & 32) ? both[0] : both[1]);
 }
 
+__device__ __forceinline__ float rounded_apart(float x, float scale, float from) {  // x scale, rounded, less `from`
+#pragma clang fp contract(off)
+  return x * scale - from;
+}
+
 // What the plan and the tables hold, by scalar loads: nothing writes them while a kernel runs.
 template <class X>
 __device__ __forceinline__ X uniform(const X* p) {
@@ -462,6 +467,11 @@ struct Rows {
   f32x16 o[DP / 32];
   float m, l;
   int limit;  // the keys before it are seen
+  bool far;   // a maximum of the wave's rows is past kFar
+  // Scores' differences from the maximum are taken in one step, s scale - m, from the exact product: it is off by what rounding
+  // the maximum's own product left, at most 1/2 up to here, and by the same for all keys. Past it that factor would leave
+  // the weights' type (fp16 from 2^27, fp32 from 2^31), and the product is rounded first.
+  static constexpr float kFar = 0x1p24f;
 
   __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& g, int h, int r, bool valid) {
     const Shape& z = a.z;
@@ -483,6 +493,7 @@ struct Rows {
     for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
     m = -INFINITY;
     l = 0.0f;
+    far = false;
   }
 
   // Operands of the products: 32 keys' elements 16 c and on; 16 keys' (of a block of 32, `c`) elements 32 d and on.
@@ -542,13 +553,19 @@ struct Rows {
     // (weights of up to 2^8 instead of 1: the sums are fp32, and hardly a block moves the maximum by more)
     const bool up = __any(most > m + 8.0f);
     float by = 1.0f;
-    if (up) {
-      const float now = fmaxf(m, most);
+    if (up || far) {
+      const float now = up ? fmaxf(m, most) : m;
       by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       m = now;
       l *= by;
+      far = __any(fabsf(m) > kFar && m != -INFINITY);
+      if (far) {
+        const float back = 1.0f / scale, from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = rounded_apart(s[i], scale, from) * back;
+      }
     }
-    const float from = m == -INFINITY ? 0.0f : m;
+    const float from = far || m == -INFINITY ? 0.0f : m;
     f32x16 next{};
     V8 w[2];
     auto weights = [&](auto from_pair, auto to_pair) {
