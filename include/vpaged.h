@@ -141,7 +141,7 @@ int vpaged_plan(const vpaged_shape* shape, const int32_t* lengths, const int32_t
 typedef struct vpaged_attend_args {
   vpaged_shape shape; /* the plan's, with the type of q, the pages and out (a plan knows none) */
   int32_t pages;      /* of the cache; a table's entry outside them is taken as the nearest inside */
-  float scale;
+  float scale;        /* 2^-126 .. 2^64; scores are fp32, and those past it infinite */
   const void* q; /* sequence s, token t, head h at s * q_stride + t * q_token_stride + h * q_head_stride */
   int64_t q_stride, q_token_stride, q_head_stride; /* elements, multiples of 8, as all strides of q and pages */
   const void* k_pages; /* as in vpaged_rotate_args, 16-byte aligned */

@@ -413,3 +413,17 @@ def test_scores_far_from_zero(device, dtype):
                 want = torch.stack([v[row[p // page], p % page, 0] for p in at]).double().cpu().mean(0)
                 off = (got[s, t] - want).abs()
                 assert bool((off <= torch.finfo(dtype).eps / 2 * want.abs() * 1.01 + 2.0**-24).all()), (b, s, t, off.max())
+
+
+@pytest.mark.parametrize("device", DEVICES, ids=str)
+def test_scales_that_fp32_does_not_hold_are_refused(device):
+    c = Case(device, BF16, None, [1, 3], seed=16)
+    b = backend(device, BF16)
+    for scale in (1e300, 2.0**127, 2.0**64 * 1.01, 2.0**-127, 1e-300):
+        with pytest.raises(ValueError, match="scale"):
+            c.attend(b, scale=scale)
+    one = torch.stack([c.cache[1][int(t[0]), 0] for t in c.tables.cpu()]).repeat_interleave(2, 1)  # (a single key's value)
+    assert torch.equal(c.attend(b, scale=2.0**64)[0, 0], one[0])
+    got = c.attend(b, scale=2.0**-126)[1, 0].double().cpu()  # (equal weights)
+    v = torch.stack([c.cache[1][int(c.tables[1, 0]), p] for p in range(3)]).repeat_interleave(2, 1).double().cpu()
+    assert bool(((got - v.mean(0)).abs() <= 2.0**-8 * (v.mean(0).abs() + 1.02 * v.abs().mean(0)) + 2.0**-20).all())

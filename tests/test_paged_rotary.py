@@ -207,3 +207,9 @@ def test_derivatives_are_refused(device):
             assert torch.equal(call(tensors), want)
             with pytest.raises(ValueError, match=f"{name} has a tangent"):
                 call({**tensors, name: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))})
+
+
+def test_magnitudes_that_fp32_does_not_hold_are_refused():
+    for magnitude in (1e39, -1e300, math.nan):
+        with pytest.raises(ValueError, match="magnitude"):
+            Rotary(rotary_frequencies(8), magnitude=magnitude)

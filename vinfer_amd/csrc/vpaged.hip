@@ -358,7 +358,8 @@ int vpaged_attend(const vpaged_attend_args* a, void* stream) {
     return fail(VPAGED_E_DTYPE, "unsupported dtype %d (VPAGED_BF16=0, VPAGED_F16=1)", a->shape.dtype);
   vpg::AttendArgs d{};
   if (!shape_of(&a->shape, d.z)) return fail(VPAGED_E_ARG, "%s", kShapeRule);
-  if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return fail(VPAGED_E_ARG, "scale must be positive and finite, got %g", a->scale);
+  // (normal; scores are fp32)
+  if (!(a->scale >= 0x1p-126f && a->scale <= 0x1p64f)) return fail(VPAGED_E_ARG, "scale must be in [2^-126, 2^64], got %g", a->scale);
   if (!d.z.S) return VPAGED_OK;
   if (a->pages < 1 || static_cast<int64_t>(a->pages) * a->shape.page_size >= 1ll << 31)
     return fail(VPAGED_E_ARG, "pages must be >= 1 and pages * page_size < 2^31, got %d", a->pages);

@@ -92,8 +92,8 @@ class Rotary:
             raise ValueError("frequencies must be a contiguous float64 tensor of one dimension")
         if 2 * f.shape[0] > _vpaged.MAX_HEAD_DIM:
             raise ValueError(f"at most {_vpaged.MAX_HEAD_DIM // 2} frequencies, got {f.shape[0]}")
-        if not math.isfinite(self.magnitude):
-            raise ValueError(f"magnitude must be finite, got {self.magnitude}")
+        if not abs(self.magnitude) <= torch.finfo(torch.float32).max:
+            raise ValueError(f"magnitude must be finite in fp32, got {self.magnitude}")
 
 
 def rotary_frequencies(dim: int, *, base: float = 10000.0, stretch: float = 1.0, trained: int | None = None,
@@ -169,8 +169,8 @@ class PagedBackend(Protocol):
                plan: AttentionPlan, *, prefix_tables: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
         """Attention ``[S, queries, heads, head_dim]``: token t of sequence s sees its group's prefix and the own
         positions up to ``lengths[s] - queries + t``; where that is below 0 there is no such token (a batch padded on
-        the left, a finished sequence), and its output is 0. Query heads share key heads in order. ``scale`` (positive)
-        defaults to ``head_dim ** -0.5``. What lies behind the lengths is not seen, whatever it holds; a value that is not
+        the left, a finished sequence), and its output is 0. Query heads share key heads in order. ``scale`` (in fp32,
+        2^-126 to 2^64) defaults to ``head_dim ** -0.5``. What lies behind the lengths is not seen, whatever it holds; a value that is not
         finite at an own position reaches all of the sequence's new tokens of the call. An entry of a table outside the
         cache is taken as the nearest page. The ``hip`` backend takes ``q`` of any layout with unit stride along its
         heads' elements, and caches of 16-byte aligned rows: strides of multiples of 8 elements, pages less than 2^31
@@ -291,8 +291,8 @@ def check_attend(q, k_pages, v_pages, tables, plan: AttentionPlan, prefix_tables
             continue
         if t is None or t.dtype != torch.int32 or t.shape != (n, m) or t.device != q.device or (t.stride(1) != 1 and m > 1):
             raise ValueError(f"{name} must be an int32 [{n}, {m}] tensor with unit stride along its pages on {q.device}")
-    if scale is not None and not (math.isfinite(scale) and scale > 0.0):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if scale is not None and not 2.0**-126 <= scale <= 2.0**64:
+        raise ValueError(f"scale must be in [2^-126, 2^64], got {scale}")
 
 
 PAGED: BackendRegistry[PagedBackend] = BackendRegistry("paged")
