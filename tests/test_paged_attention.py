@@ -427,3 +427,48 @@ def test_scales_that_fp32_does_not_hold_are_refused(device):
     got = c.attend(b, scale=2.0**-126)[1, 0].double().cpu()  # (equal weights)
     v = torch.stack([c.cache[1][int(c.tables[1, 0]), p] for p in range(3)]).repeat_interleave(2, 1).double().cpu()
     assert bool(((got - v.mean(0)).abs() <= 2.0**-8 * (v.mean(0).abs() + 1.02 * v.abs().mean(0)) + 2.0**-20).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["alone", "many groups", "wide", "prompts"])
+def test_more_sequences_than_a_plan_s_threads(kind):
+    # past 1024 sequences and groups a plan goes round, past 2048 segments and 2047 groups it searches in memory
+    rng = np.random.default_rng(22)
+    if kind == "alone":
+        S, groups, shape = 2500, None, {}
+    elif kind == "many groups":  # of no, one and several sequences
+        sizes = [(0, 1, 1, 3, 1)[i % 5] for i in range(2200)]
+        groups, S, shape = [(n, int(rng.integers(0, 60))) for n in sizes], sum(sizes), {}
+    elif kind == "wide":  # more than 32 rows a group and a sequence
+        groups, S, shape = [(1 + i % 2, int(rng.integers(0, 90))) for i in range(900)], 1350, dict(heads=33, kv_heads=1)
+    else:  # several segments a sequence
+        S, groups, shape = 300, [(300, 70)], dict(T=40, heads=8, kv_heads=1, page=64)
+    assert groups is None or sum(n for n, _ in groups) == S
+    Case(GPU, BF16, groups, rng.integers(0, 80, S).tolist(), **{**dict(heads=2, kv_heads=2, D=8), **shape}, seed=22).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+def test_many_weights_far_below_the_largest(dtype):
+    # one key of weight 1, the others' 2^-17, 2^-20 and 2^-25: numbers that fp16 holds below its smallest normal one, 2^-14
+    # (2^-25 rounds to 0)
+    n, D = 30000, 64
+    c = Case(GPU, dtype, None, [n], heads=2, kv_heads=1, D=D, seed=23)
+    k, v = c.cache
+    page_of = c.tables[0].long()
+    v.abs_()
+    c.q.fill_(1.0)
+    for low, mass in ((17, n * 2.0**-17), (20, n * 2.0**-20), (25, n * 2.0**-25)):
+        k.zero_()
+        k[page_of[0], 0, 0, 0] = low  # (scale ln 2: powers of 2)
+        got = c.attend(backend(GPU, dtype), scale=math.log(2.0)).double()[0, 0]
+        flat = v[page_of].flatten(0, 1)[:n, 0].double()
+        first, rest = flat[0], flat[1:].sum(0) * 2.0**-low
+        want = (first + rest) / (1.0 + (n - 1) * 2.0**-low)
+        # a score of `low` and its product with log2 e in fp32, each a few steps; the first weight 1 to 2^-20, the others one
+        # rounding (fp16: up to 2^-25 each); sums of n in fp32
+        step = torch.finfo(dtype).eps / 2
+        lost = (n - 1) * 2.0**-25 if dtype == F16 and low > 20 else 0.0
+        off = (got - want).abs()
+        bound = step * want + (step + 2.0**-18 + n * 2.0**-24) * mass * 8 + lost * (want + flat.max(0).values) + 2.0**-18 * want
+        assert bool((off <= bound).all()), (low, float((off - bound).max()))
