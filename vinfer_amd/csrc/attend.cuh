@@ -805,7 +805,7 @@ template <class T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void k_join(AttendArgs a) {
   const Shape& z = a.z;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = WAVES == 1 ? 0 : wave;
-  const unsigned id = WAVES == 1 ? (blockIdx.y * gridDim.x + blockIdx.x) * 4 + wave : blockIdx.x;
+  const unsigned id = WAVES == 1 ? (blockIdx.y * kGridX + blockIdx.x) * 4 + wave : blockIdx.x;
   if (id >= static_cast<unsigned>(z.S) * z.T * z.H) return;
   const unsigned st = id / static_cast<unsigned>(z.H);
   const int hq = static_cast<int>(id - st * z.H), s = static_cast<int>(st / static_cast<unsigned>(z.T)), t = static_cast<int>(st) - s * z.T;

@@ -52,15 +52,14 @@ enum Pairs {
   kAdjacent     // (2j, 2j + 1)
 };
 
-// A workgroup takes a token, over x and z (and, where there are few, some of its items: gridDim.y of them share it). E: elements of an
+// A workgroup takes a token (and, where there are few, some of its items: gridDim.y of them share it). E: elements of an
 // access, 8 (all addresses are multiples of 16 bytes, and halves' pairs lie in whole vectors) or 1. An item is E elements of
 // a head, but with kHalves, of queries and keys, E pairs of the turned part, or E elements of the rest.
 template <class T, int E, Pairs PAIRS>
 __global__ __launch_bounds__(kRotateThreads) void k_rotate(RotateArgs a) {
   __shared__ float2 s_turn[128];
   const int tid = threadIdx.x, half = a.dim / 2;
-  const int64_t token = static_cast<int64_t>(blockIdx.z) * gridDim.x + blockIdx.x;
-  if (token >= a.N) return;
+  const int64_t token = blockIdx.x;
   const int pos = a.positions[token], place = a.slots[token];
   for (int j = tid; j < half; j += kRotateThreads) {
     const double turns = pos * a.freq[j] * 0.15915494309189533577;

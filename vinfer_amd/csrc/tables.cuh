@@ -14,6 +14,9 @@
 namespace vpg {
 
 constexpr int kTableThreads = 1024;
+// Workgroups over a grid's first dimension (a launch has fewer than 2^32 threads in one): more go on in another, or in another
+// launch where that is rare and the kernel short (a second dimension in k_rotate costs 4 tokens' 3.15 us 0.24).
+constexpr int kGridX = 1 << 20;
 
 struct Tables {
   int32_t* tables;

@@ -196,27 +196,20 @@ void with_width(int D, F f) {
   else f(Width<256>{});
 }
 
-// n workgroups over x and `over`, a grid's other dimension: a launch has fewer than 2^32 threads in one.
-constexpr int64_t kGridX = 1 << 20;
-dim3 grid_of(int64_t n, unsigned dim3::*over) {
-  dim3 grid(static_cast<unsigned>(n < kGridX ? n : kGridX));
-  grid.*over = static_cast<unsigned>((n + kGridX - 1) / kGridX);
-  return grid;
-}
-
 // Up to this many rows of outputs (a sequence's token's head each) 16 waves join one: the longest has few others beside it.
 constexpr int kFewRows = 512;
 
 template <class T>
 int attend(const vpg::AttendArgs& d, hipStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(d.z.S) * d.z.T * d.z.H;
+  const int64_t rows = static_cast<int64_t>(d.z.S) * d.z.T * d.z.H, fours = (rows + 3) / 4;
+  const dim3 join(static_cast<unsigned>(fours < vpg::kGridX ? fours : vpg::kGridX), static_cast<unsigned>((fours + vpg::kGridX - 1) / vpg::kGridX));
   with_width(d.z.D, [&](auto w) {
     constexpr int DP = decltype(w)::value;
     const dim3 grid(2 * d.z.wgs), block(vpg::kWaves * 64);
     if ((1 << d.z.shift) < vpg::kRun) vpg::k_attend<T, DP, true><<<grid, block, 0, stream>>>(d);
     else vpg::k_attend<T, DP, false><<<grid, block, 0, stream>>>(d);
     if (rows <= kFewRows) vpg::k_join<T, DP, 16><<<dim3(static_cast<unsigned>(rows)), dim3(1024), 0, stream>>>(d);
-    else vpg::k_join<T, DP, 1><<<grid_of((rows + 3) / 4, &dim3::y), dim3(256), 0, stream>>>(d);
+    else vpg::k_join<T, DP, 1><<<join, dim3(256), 0, stream>>>(d);
   });
   return launched("vpaged_attend");
 }
@@ -321,11 +314,23 @@ int vpaged_rotate_store(const vpaged_rotate_args* a, void* stream) {
   const int rounds = (r.items + vpg::kRotateThreads - 1) / vpg::kRotateThreads;
   int y = a->tokens >= 4 * kCus ? 1 : (4 * kCus + a->tokens - 1) / a->tokens;
   if (y > rounds) y = rounds;
-  dim3 grid = grid_of(a->tokens, &dim3::z);
-  grid.y = static_cast<unsigned>(y);
   const auto s = static_cast<hipStream_t>(stream);
-  if (a->dtype == VPAGED_BF16) rotate<__bf16>(r, vectors, pairs, grid, s);
-  else rotate<_Float16>(r, vectors, pairs, grid, s);
+  for (int left = a->tokens; left > 0; left -= vpg::kGridX) {
+    r.N = left < vpg::kGridX ? left : vpg::kGridX;
+    const dim3 grid(static_cast<unsigned>(r.N), static_cast<unsigned>(y));
+    if (a->dtype == VPAGED_BF16) rotate<__bf16>(r, vectors, pairs, grid, s);
+    else rotate<_Float16>(r, vectors, pairs, grid, s);
+    // (elements of two bytes; a power of two of them keeps the alignment)
+    const auto on = [&](const void* p, int64_t stride) { return static_cast<const char*>(p) + 2 * stride * vpg::kGridX; };
+    if (left > vpg::kGridX) {
+      r.q = on(r.q, r.q_stride);
+      r.k = on(r.k, r.k_stride);
+      r.v = on(r.v, r.v_stride);
+      r.out_q = static_cast<char*>(r.out_q) + 2 * static_cast<int64_t>(r.heads) * r.D * vpg::kGridX;
+      r.positions += vpg::kGridX;
+      r.slots += vpg::kGridX;
+    }
+  }
   return launched("vpaged_rotate_store");
 }
 
