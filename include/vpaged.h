@@ -65,8 +65,8 @@ typedef struct vpaged_tables {
 /* Each sequence s grows by counts[s] positions (below 0: 0), the sequences in their order taking the pages that they
  * need. A sequence is served whole or not at all: not where its table would be too short, where its tokens lie past
  * `tokens`, or where the pages that it and those before it need are more than are free; served[s] says so (1 where it
- * asks for nothing). The sequences' tokens lie one after the other, counts[s] of each: slots, positions and sequence
- * of the i-th, or -1 where there is none or its sequence is not served. */
+ * asks for nothing, but 0 for all behind tokens that lie past `tokens`). The sequences' tokens lie one after the other,
+ * counts[s] of each: slots, positions and sequence of the i-th, or -1 where there is none or its sequence is not served. */
 size_t vpaged_extend_workspace_bytes(int32_t sequences, int32_t tokens);
 int vpaged_extend(const vpaged_tables* t, const int32_t* counts, int32_t tokens, int32_t* out_slots,
                   int32_t* out_positions, int32_t* out_sequences, uint8_t* out_served, void* workspace,
@@ -117,8 +117,9 @@ int vpaged_rotate_store(const vpaged_rotate_args* args, void* stream);
  * share a prefix of prefix_lengths[g] positions. lengths[s] are a sequence's own positions behind it, its new tokens
  * the last of them: token t sees the prefix and own positions up to lengths[s] - queries + t. Where that is below 0
  * there is no such token, and its outputs are 0. What lies behind a sequence's length is not seen, whatever it holds; a
- * value that is not finite at a sequence's own position reaches all of the call's new tokens. Lengths outside what the tables hold are taken as the nearest inside;
- * group_starts ascend from 0 to sequences.
+ * value that is not finite at a sequence's own position reaches all of the call's new tokens. Scores are fp32, weights
+ * rounded to the values' type. Lengths outside what the tables hold are taken as the nearest inside; group_starts ascend
+ * from 0 to sequences.
  *   out[s][t][h] = sum_j softmax_j(scale q[s][t][h] . k[j][h / (heads / kv_heads)]) v[j][h / (heads / kv_heads)] */
 typedef struct vpaged_shape {
   int32_t dtype;
@@ -133,7 +134,9 @@ typedef struct vpaged_shape {
   int32_t max_prefix_pages; /* of the groups' */
 } vpaged_shape;
 
-/* A step's plan, from the lengths on the device: which keys each workgroup takes. Layers of one shape share it. */
+/* A step's plan, from the lengths on the device: which keys each workgroup takes. Layers of one shape share it, of
+ * either type. A shape is refused (0 bytes) whose tiles of a head, or of all heads for each of 256 workgroups (512 for heads
+ * of up to 128), or rows are 2^31 and more. */
 size_t vpaged_plan_bytes(const vpaged_shape* shape); /* 0: a shape that is refused */
 int vpaged_plan(const vpaged_shape* shape, const int32_t* lengths, const int32_t* prefix_lengths,
                 const int32_t* group_starts, void* plan, size_t plan_bytes, void* stream);

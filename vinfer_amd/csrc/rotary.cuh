@@ -3,9 +3,11 @@
 // Pair (x1, x2) of a token at position p turns by a = p f_j:
 //   y1 = m (x1 cos a - x2 sin a), y2 = m (x2 cos a + x1 sin a)
 // a is taken in 64 bits and brought to turns there (a / 2 pi less its nearest whole number), so that its sine and
-// cosine are right to fp32 at any position. Each element is read and written once, products and sums are fp32, and
-// the result is rounded once to the elements' type. Bound by HBM for many tokens (16384 of 48 heads of 128, 403 MB: 75 us, 5.4
-// TB/s, as a copy), by latency for few (4 tokens 3 us): a token's angles are worked out once, in LDS, for all heads.
+// cosine are right to fp32 up to position 2^28 (then a's own rounding, a 2^-53, shows). Each element is read and written
+// once, products and sums are fp32, and the result is rounded once to the elements' type. Bound by HBM for many tokens (16384 of 48 heads of 128, 403 MB: 74 us, 5.4
+// TB/s, as a copy, pairs of either kind; rows at odd addresses, an element at a time, 163 in halves and 241 in pairs; heads of 192
+// in halves, which are not exchanged, 139, 4.3 TB/s), by latency for few (4 tokens 3 us): a token's angles are worked
+// out once, in LDS, for all heads.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -48,7 +50,7 @@ constexpr int kRotateThreads = 256;
 enum Pairs {
   kHalves,      // (j, j + dim / 2): it takes E of each half
   kExchanged,   // the same, from the lane that has the other half: whole heads lie in a wave, eight elements a lane. All
-                // lanes' accesses are one run then: 16384 tokens of 48 heads of 128 77 us, against 89
+                // lanes' accesses are one run then: 16384 tokens of 48 heads of 128 74 us, against 89
   kAdjacent     // (2j, 2j + 1)
 };
 

@@ -139,8 +139,9 @@ class PagedBackend(Protocol):
     def extend(self, pages: PageTables, counts: torch.Tensor, tokens: int) -> Extension:
         """Sequence s grows by ``counts[s]`` positions (int32; below 0: 0), the sequences in their order taking the
         pages they need. A sequence is served whole or not at all: not where its table would be too short, where its
-        tokens lie past ``tokens``, or where the pages that it and those before it need are more than are free. The
-        sequences' tokens lie one after the other, ``tokens`` places in all."""
+        tokens lie past ``tokens``, or where the pages that it and those before it need are more than are free. One that
+        asks for nothing is served, but none behind tokens that lie past ``tokens`` is. The sequences' tokens lie one
+        after the other, ``tokens`` places in all."""
         ...
 
     def shrink(self, pages: PageTables, lengths: torch.Tensor) -> None:
@@ -170,9 +171,9 @@ class PagedBackend(Protocol):
         """Attention ``[S, queries, heads, head_dim]``: token t of sequence s sees its group's prefix and the own
         positions up to ``lengths[s] - queries + t``; where that is below 0 there is no such token (a batch padded on
         the left, a finished sequence), and its output is 0. Query heads share key heads in order. ``scale`` (in fp32,
-        2^-126 to 2^64) defaults to ``head_dim ** -0.5``. What lies behind the lengths is not seen, whatever it holds; a value that is not
-        finite at an own position reaches all of the sequence's new tokens of the call. An entry of a table outside the
-        cache is taken as the nearest page. The ``hip`` backend takes ``q`` of any layout with unit stride along its
+        2^-126 to 2^64) defaults to ``head_dim ** -0.5``. What lies behind the lengths is not seen, whatever it holds; a
+        value that is not finite at an own position reaches all of the sequence's new tokens of the call. An entry of a
+        table outside the cache is taken as the nearest page. Scores are fp32, weights rounded to the values' type. The ``hip`` backend takes ``q`` of any layout with unit stride along its
         heads' elements, and caches of 16-byte aligned rows: strides of multiples of 8 elements, pages less than 2^31
         elements apart, a page's positions (16 at least) within 2^30."""
         ...
